@@ -20,7 +20,9 @@ QMAX_EXACT = 1
 SEL_CHUNK_SHIFT = 8
 FLAG_OUT_GATE, FLAG_DENSE, FLAG_DGATE, FLAG_RAGGED = 1, 2, 4, 8
 SELECT_SCRATCH_BYTES = 32 << 20   # FBSA_SELECT_SCRATCH_BYTES
+EVICT_IN_PLACE = 1
 
+_i64x2 = ctypes.c_int64 * 2
 _i64x3 = ctypes.c_int64 * 3
 
 
@@ -70,6 +72,37 @@ class QmaxDesc(ctypes.Structure):
     ]
 
 
+class AppendDesc(ctypes.Structure):
+    """Mirror of ``fbsa_append_desc``."""
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("flags", ctypes.c_int32),
+        ("B", ctypes.c_int64), ("H", ctypes.c_int64), ("T", ctypes.c_int64), ("S", ctypes.c_int64), ("D", ctypes.c_int64),
+        ("sk", _i64x3), ("sv", _i64x3), ("skn", _i64x3), ("svn", _i64x3), ("sw", _i64x2),
+    ]
+
+
+class CacheDesc(ctypes.Structure):
+    """Mirror of ``fbsa_cache_desc``."""
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("flags", ctypes.c_int32),
+        ("B", ctypes.c_int64), ("Hq", ctypes.c_int64), ("Hkv", ctypes.c_int64), ("T", ctypes.c_int64),
+        ("S", ctypes.c_int64), ("P", ctypes.c_int64), ("D", ctypes.c_int64),
+        ("scale", ctypes.c_float), ("reserved", ctypes.c_int32),
+        ("sq", _i64x3), ("sk", _i64x3), ("sv", _i64x3), ("so", _i64x3), ("sog", _i64x3),
+        ("skp", _i64x2), ("svp", _i64x2), ("sw", _i64x2), ("swo", _i64x2),
+    ]
+
+
+class EvictDesc(ctypes.Structure):
+    """Mirror of ``fbsa_evict_desc``."""
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("flags", ctypes.c_int32),
+        ("B", ctypes.c_int64), ("H", ctypes.c_int64), ("S", ctypes.c_int64), ("SO", ctypes.c_int64), ("D", ctypes.c_int64),
+        ("budget", ctypes.c_int64), ("recent", ctypes.c_int64), ("sink", ctypes.c_int64),
+        ("sk", _i64x3), ("sv", _i64x3), ("sko", _i64x3), ("svo", _i64x3), ("sw", _i64x2), ("swo", _i64x2),
+    ]
+
+
 _vp = ctypes.c_void_p
 # name -> (restype, argtypes); every symbol declared in include/fbsa.h
 SIGNATURES = {
@@ -99,6 +132,10 @@ SIGNATURES = {
     "fbsa_bwd_dq": (ctypes.c_int, [ctypes.POINTER(AttnDesc)] + [_vp] * 9 + [ctypes.c_size_t, _vp]),
     "fbsa_bwd_dkdv": (ctypes.c_int, [ctypes.POINTER(AttnDesc)] + [_vp] * 8 + [ctypes.c_size_t, _vp]),
     "fbsa_bwd": (ctypes.c_int, [ctypes.POINTER(AttnDesc)] + [_vp] * 15 + [ctypes.c_size_t, _vp]),
+    "fbsa_cache_append": (ctypes.c_int, [ctypes.POINTER(AppendDesc)] + [_vp] * 8),
+    "fbsa_cache_attn_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(CacheDesc)]),
+    "fbsa_cache_attn": (ctypes.c_int, [ctypes.POINTER(CacheDesc)] + [_vp] * 13 + [ctypes.c_size_t, _vp]),
+    "fbsa_cache_evict": (ctypes.c_int, [ctypes.POINTER(EvictDesc)] + [_vp] * 10),
 }
 
 _lib = None

@@ -333,6 +333,86 @@ int fbsa_bwd(const fbsa_attn_desc *d, const void *q, const void *k, const void *
              const void *out_gate, void *dq, void *dk, void *dv, float *dgate, void *dout_gate,
              void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- caches (serving) -------------------------------------------------
+ * A cache holds the keys and values of B sequences: k, v (B, H, S, D) of
+ * capacity S, strides {b, h, row} in elements (multiples of 16 bytes, D
+ * contiguous), sequence b's rows being [0, lens[b]). lens, start and count are
+ * int32 arrays of B entries in device memory, read by the kernels, so a
+ * captured graph follows them; lens outside [0, S] and count outside [0, T]
+ * are clamped. Rows at or past lens[b] are neither read nor written (by
+ * fbsa_cache_append: rows outside the ones it is given). D is a multiple of 8 up to
+ * 256. No counterpart in the reference, whose attention is over whole prompts. */
+
+/* New rows behind each sequence: k[b, h, start[b] + t] = k_new[b, h, t] and v
+ * alike for t < count[b] (NULL: T), weight (nullable, fp32 (B, H, S), rows
+ * contiguous) zeroed there. Rows that would fall outside [0, S) are dropped. */
+typedef struct fbsa_append_desc {
+  int32_t dtype, flags;                     /* flags: 0 */
+  int64_t B, H, T, S, D;
+  int64_t sk[3], sv[3], skn[3], svn[3];     /* k, v, k_new, v_new: {b, h, row} */
+  int64_t sw[2];                            /* weight: {b, h} */
+} fbsa_append_desc;
+
+int fbsa_cache_append(const fbsa_append_desc *d, void *k, void *v, const void *k_new, const void *v_new,
+                      const int32_t *start, const int32_t *count, float *weight, void *stream);
+
+/* Attention of the newest tokens over their caches, optionally behind a prefix
+ * that every sequence shares: k_prefix, v_prefix (Hkv, P, D), strides {h, row},
+ * P = 0 for none. q (B, Hq, T, D); query head h reads KV head h / (Hq / Hkv).
+ * Query t < count[b] (NULL: T) is the token of row lens[b] - count[b] + t: it
+ * sees the whole prefix and its sequence's rows up to and including that one
+ * (lens counts the new tokens, which are already in the cache). It writes
+ *   o[b, h, t]   = softmax(scale q.k) v [* sigmoid(out_gate)], (B, Hq, T, D)
+ *   lse[b, h, t] = the softmax's natural-log normaliser, (B, Hq, T) contiguous
+ *                  fp32, nullable
+ * a query that sees nothing, or t >= count[b]: o = 0, lse = -inf. With
+ * out_weight (fp32 (B, Hkv, S), rows contiguous) every own row s < lens[b]
+ * has out_weight = weight (NULL: 0) + the probability that the sequence's
+ * queries of the KV head's group gave it; weight may be out_weight. Softmax,
+ * sums and weights are fp32. The split of the keys follows from the sizes, and
+ * parts are joined in a fixed order: results are bitwise repeatable.
+ * The workspace is 256-byte aligned; fbsa_cache_attn_workspace_bytes returns 0
+ * (with fbsa_last_error set) for a descriptor that fbsa_cache_attn refuses. */
+typedef struct fbsa_cache_desc {
+  int32_t dtype, flags;                     /* flags: 0 */
+  int64_t B, Hq, Hkv, T, S, P, D;
+  float scale;
+  int32_t reserved;
+  int64_t sq[3], sk[3], sv[3], so[3], sog[3];  /* q, k, v, o, out_gate: {b, h, row} */
+  int64_t skp[2], svp[2];                   /* prefix: {h, row} */
+  int64_t sw[2], swo[2];                    /* weight, out_weight: {b, h} */
+} fbsa_cache_desc;
+
+size_t fbsa_cache_attn_workspace_bytes(const fbsa_cache_desc *d);
+int fbsa_cache_attn(const fbsa_cache_desc *d, const void *q, const void *k, const void *v, const int32_t *lens,
+                    const int32_t *count, const void *k_prefix, const void *v_prefix, const void *out_gate,
+                    void *o, float *lse, const float *weight, float *out_weight, void *workspace,
+                    size_t workspace_bytes, void *stream);
+
+/* Cuts every sequence to at most `budget` rows per (sequence, head). A sequence
+ * of n <= budget rows keeps them all; a longer one keeps its first `sink` rows,
+ * its last `recent` rows and, of those between, the budget - sink - recent of
+ * greatest weight (ties to the lower row; NaN ranks as -inf). Kept rows keep
+ * their order. index (B, H, min(budget, S)) contiguous int32 is the row each
+ * kept one had, -1 past the last; new_lens[b] = min(lens[b], budget). Rows, and
+ * their weights, go to k_out, v_out (B, H, SO, D) and w_out (B, H, SO), SO >=
+ * min(budget, S), whose rows past new_lens[b] are left as they were; none of
+ * them may overlap k, v or weight, except with FBSA_EVICT_IN_PLACE, where they
+ * are k, v and weight themselves (same pointers, strides and SO = S). lens and
+ * new_lens may be the same array in neither case. */
+enum { FBSA_EVICT_IN_PLACE = 1 };
+
+typedef struct fbsa_evict_desc {
+  int32_t dtype, flags;
+  int64_t B, H, S, SO, D, budget, recent, sink;
+  int64_t sk[3], sv[3], sko[3], svo[3];     /* k, v, k_out, v_out: {b, h, row} */
+  int64_t sw[2], swo[2];                    /* weight, w_out: {b, h} */
+} fbsa_evict_desc;
+
+int fbsa_cache_evict(const fbsa_evict_desc *d, const void *k, const void *v, const float *weight,
+                     const int32_t *lens, void *k_out, void *v_out, float *w_out, int32_t *index,
+                     int32_t *new_lens, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
