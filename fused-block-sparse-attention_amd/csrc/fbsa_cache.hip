@@ -36,12 +36,16 @@ struct CacheArgs {
   int64_t sq[3], sk[3], sv[3], so[3], sog[3], skp[2], svp[2], sw[2], swo[2];
   int32_t B, Hq, Hkv, T, S, P, D, G;
   int32_t TG;                // rows per (sequence, KV head): T * G
-  int32_t rt_own, rt_pre;    // 16-row tiles of a (sequence, KV head); of a KV head's prefix rows
+  int32_t tr_own, tr_pre;    // rows of a tile
+  int32_t rt_own, rt_pre;    // tiles of a (sequence, KV head); of a KV head's prefix rows
   int32_t np_own, np_pre;    // shares of a tile's keys
+  int32_t few_own, few_pre;  // tiles of 16 rows, a wave each
+  int32_t direct;            // a tile's one share is its whole answer: no parts
   float scale2;              // scale * log2(e)
-  float *part;               // [slot][16][DP] unnormalised O
-  float2 *stat;              // [slot][16] row maximum (log2 domain), row sum
+  float *part;               // [tile, share][row] unnormalised O (DP floats): prefix tiles, then own
+  float2 *stat;              // [tile, share][row] row maximum (log2 domain), row sum
   float *lse2;               // [B][Hkv][TG] log2-domain lse, -inf for rows that see nothing
+  float *sc;                 // [B][Hkv][TG][S rounded up to 32] log2-domain scores (few_own, with weights)
 };
 
 // keys per chunk: 32, 16 for fp32 at d >= 128 (registers)
@@ -114,16 +118,45 @@ template <typename T, int DP> struct TilePlan {
   }
 };
 
+// o[d .. d + 3] = acc * inv [* sigmoid(gate)] of a row
+template <typename T> __device__ __forceinline__ void store_row(const CacheArgs &a, const RowInfo &ri, f32x4 acc, float inv, int d) {
+  if (d >= a.D) return;
+  T *orow = (T *)a.o + ri.b * a.so[0] + ri.hq * a.so[1] + ri.t * a.so[2] + d;
+  float y[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) y[r] = acc[r] * inv;
+  if (a.og) {
+    const T *og = (const T *)a.og + ri.b * a.sog[0] + ri.hq * a.sog[1] + ri.t * a.sog[2] + d;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) y[r] *= 1.f / (1.f + __expf(-to_f32<T>(og[r])));
+  }
+  if constexpr (sizeof(T) == 4) {
+    *(f32x4 *)orow = f32x4{y[0], y[1], y[2], y[3]};
+  } else {
+    s16x4 pk;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) pk[r] = bits16<T>((T)y[r]);
+    *(s16x4 *)orow = pk;
+  }
+}
+
+// first row of the own tiles' parts
+__device__ __forceinline__ int64_t own_slot(const CacheArgs &a) { return (int64_t)a.Hkv * a.rt_pre * a.np_pre * a.tr_pre; }
+__device__ __forceinline__ int64_t score_row(const CacheArgs &a, int b, int hk, int rho) {
+  return (((int64_t)b * a.Hkv + hk) * a.TG + rho) * (((int64_t)a.S + 31) / 32 * 32);
+}
+
 template <typename T, int DP> __global__ __launch_bounds__(64) void cache_part_kernel(CacheArgs a) {
   using C = CacheCfg<T, DP>;
   constexpr int KC = C::KC, NM = KC / 16;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x, g = lane >> 4, p = lane & 15;
-  const uint32_t npre = (uint32_t)a.Hkv * a.np_pre * a.rt_pre;
+  const uint32_t npre = a.few_pre ? (uint32_t)a.Hkv * a.np_pre * a.rt_pre : 0;
   uint32_t id = blockIdx.x;
   const bool pre = id < npre;
   RowInfo ri;
-  int64_t slot;
+  float *score = nullptr;  // this row's scores, where the weights are taken from them
+  int64_t slot;  // the tile's first row among the parts
   int split, np, keys;
   const char *kb, *vb;
   int64_t kstep, vstep;
@@ -136,7 +169,7 @@ template <typename T, int DP> __global__ __launch_bounds__(64) void cache_part_k
     ri = row_info(a, (int)(x / a.TG), hk, (int)(x % a.TG));
     ri.valid = ri.valid && rho < rows;
     ri.lim = a.P;
-    slot = ((int64_t)hk * a.rt_pre + tile) * np + split;
+    slot = (((int64_t)hk * a.rt_pre + tile) * np + split) * 16;
     kstep = a.skp[1] * C::ES;
     vstep = a.svp[1] * C::ES;
     kb = (const char *)a.kp + hk * a.skp[0] * C::ES;
@@ -147,7 +180,8 @@ template <typename T, int DP> __global__ __launch_bounds__(64) void cache_part_k
     split = id / a.rt_own % a.np_own;
     np = a.np_own;
     ri = row_info(a, b, hk, tile * 16 + p);
-    slot = (int64_t)a.Hkv * a.rt_pre * a.np_pre + (((int64_t)b * a.Hkv + hk) * a.rt_own + tile) * np + split;
+    if (a.sc) score = a.sc + score_row(a, b, hk, ri.valid ? p : 0);
+    slot = own_slot(a) + (((int64_t)b * a.Hkv + hk) * a.rt_own + tile) * np * 16 + split * 16;
     kstep = a.sk[2] * C::ES;
     vstep = a.sv[2] * C::ES;
     kb = (const char *)a.k + (b * a.sk[0] + hk * a.sk[1]) * C::ES;
@@ -206,6 +240,10 @@ template <typename T, int DP> __global__ __launch_bounds__(64) void cache_part_k
         for (int r = 0; r < 4; ++r)
           if (16 * m + r >= lm) s[m][r] = -INFINITY;
     }
+    if (score && ri.valid) {
+#pragma unroll
+      for (int m = 0; m < NM; ++m) *(f32x4 *)(score + (int64_t)c * KC + 16 * m + 4 * g) = s[m];
+    }
     float mx = -INFINITY;
 #pragma unroll
     for (int m = 0; m < NM; ++m) mx = fmaxf(mx, fmaxf(fmaxf(s[m][0], s[m][1]), fmaxf(s[m][2], s[m][3])));
@@ -234,61 +272,140 @@ template <typename T, int DP> __global__ __launch_bounds__(64) void cache_part_k
 
   float lt = l_run + shfl_xor_f(l_run, 16);
   lt += shfl_xor_f(lt, 32);
-  if (g == 0) a.stat[slot * 16 + p] = float2{m_run, lt};
+  if (g == 0) a.stat[slot + p] = float2{m_run, lt};
   if (ri.valid && lt != 0.f) {  // (a NaN sum is kept)
-    float *dst = a.part + (slot * 16 + p) * DP;
+    float *dst = a.part + (slot + p) * DP;
 #pragma unroll
     for (int t = 0; t < DP / 16; ++t) *(f32x4 *)(dst + 16 * t + 4 * g) = oacc[t];
   }
 }
 
-template <typename T, int DP> __global__ __launch_bounds__(256) void cache_combine_kernel(CacheArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= (int64_t)a.B * a.Hkv * a.TG) return;
-  const int rho = (int)(row % a.TG), hk = (int)(row / a.TG % a.Hkv), b = (int)(row / a.TG / a.Hkv);
-  const RowInfo ri = row_info(a, b, hk, rho);
+// A row's parts: number i of its prefix tile's shares, then of its own tile's.
+struct RowParts {
+  int64_t pre0, own0;
+  int npre, n;
+  __device__ __forceinline__ int64_t at(const CacheArgs &a, int i) const {
+    return i < npre ? pre0 + (int64_t)i * a.tr_pre : own0 + (int64_t)(i - npre) * a.tr_own;
+  }
+};
+__device__ __forceinline__ RowParts row_parts(const CacheArgs &a, int b, int hk, int rho) {
+  RowParts r;
   const int64_t rp = (int64_t)b * a.TG + rho;
-  const int64_t pre0 = ((int64_t)hk * a.rt_pre + rp / 16) * a.np_pre * 16 + rp % 16;
-  const int64_t own0 = (int64_t)a.Hkv * a.rt_pre * a.np_pre * 16 +
-                       (((int64_t)b * a.Hkv + hk) * a.rt_own + rho / 16) * a.np_own * 16 + rho % 16;
-  const int n = ri.valid ? a.np_pre + a.np_own : 0;
-  auto place = [&](int i) { return i < a.np_pre ? pre0 + (int64_t)i * 16 : own0 + (int64_t)(i - a.np_pre) * 16; };
+  r.npre = a.np_pre;
+  r.n = a.np_pre + a.np_own;
+  r.pre0 = a.np_pre ? ((int64_t)hk * a.rt_pre + rp / a.tr_pre) * a.np_pre * a.tr_pre + rp % a.tr_pre : 0;
+  r.own0 = own_slot(a) + (((int64_t)b * a.Hkv + hk) * a.rt_own + rho / a.tr_own) * a.np_own * a.tr_own + rho % a.tr_own;
+  return r;
+}
+
+constexpr int kMaxShares = 512;    // np_own + np_pre
+constexpr int kWeightKeys = 1024;  // keys of a weight workgroup
+
+// Workgroups [0, rows): a row each. Groups of DP / 4 threads take every NG-th
+// part, a float4 a thread, and are added in order at the end.
+// Workgroups past them (a.sc): kWeightKeys keys of a (sequence, KV head): each row's
+// lse from its parts' statistics, then weight + sum over rows of exp2(score - lse).
+template <typename T, int DP> __global__ __launch_bounds__(256) void cache_combine_kernel(CacheArgs a) {
+  constexpr int LG = DP / 4, NG = 256 / LG;
+  __shared__ float s_f[kMaxShares];
+  __shared__ f32x4 s_acc[256];
+  __shared__ float s_red[8];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t rows = (int64_t)a.B * a.Hkv * a.TG;
+  if (blockIdx.x >= rows) {
+    const int per = (a.S + kWeightKeys - 1) / kWeightKeys;
+    const int64_t u = blockIdx.x - rows;
+    const int key0 = (int)(u % per) * kWeightKeys, hk = (int)(u / per % a.Hkv), b = (int)(u / per / a.Hkv);
+    const int n = seq_len(a, b), c = seq_count(a, b);
+    if (key0 >= n) return;
+    __shared__ float s_lse[16];
+    const int real = min(c * a.G, a.TG);  // rows of real queries
+    for (int rho = wave; rho < real; rho += 4) {
+      const RowParts rp = row_parts(a, b, hk, rho);
+      float m = -INFINITY, l = 0.f;
+      for (int i = lane; i < rp.n; i += 64) m = fmaxf(m, a.stat[rp.at(a, i)].x);
+#pragma unroll
+      for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, shfl_xor_f(m, x));
+      const float ref = m == -INFINITY ? 0.f : m;
+      for (int i = lane; i < rp.n; i += 64) {
+        const float2 st = a.stat[rp.at(a, i)];
+        if (st.y != 0.f) l += __builtin_amdgcn_exp2f(st.x - ref) * st.y;
+      }
+#pragma unroll
+      for (int x = 1; x < 64; x <<= 1) l += shfl_xor_f(l, x);
+      if (lane == 0) s_lse[rho] = l == 0.f ? -INFINITY : m + __log2f(l);
+    }
+    __syncthreads();
+    const float *sc = a.sc + score_row(a, b, hk, 0);
+    const int64_t step = score_row(a, 0, 0, 1);
+    // four keys a thread, four rows' scores in flight (rows of scores are whole multiples of 32)
+    static_assert(kWeightKeys == 4 * 256, "four keys to a thread");
+    const int key = key0 + 4 * tid;
+    if (key >= n) return;
+    f32x4 w = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int r0 = 0; r0 < real; r0 += 4) {
+      f32x4 x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = *(const f32x4 *)(sc + (r0 + j < real ? r0 + j : r0) * step + key);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float l2 = r0 + j < real ? s_lse[r0 + j] : -INFINITY;
+        // (a row's scores are written up to the last key that a row of its tile sees)
+        const int64_t lim = (int64_t)n - c + (r0 + j) / a.G + 1;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (key + e < lim && l2 != -INFINITY) w[e] += __builtin_amdgcn_exp2f(x[j][e] - l2);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (key + e < n) {
+        const float w0 = a.w ? a.w[b * a.sw[0] + hk * a.sw[1] + key + e] : 0.f;
+        a.wo[b * a.swo[0] + hk * a.swo[1] + key + e] = w0 + w[e];
+      }
+    return;
+  }
+  const int rho = (int)(blockIdx.x % a.TG), hk = (int)(blockIdx.x / a.TG % a.Hkv), b = (int)(blockIdx.x / a.TG / a.Hkv);
+  const RowInfo ri = row_info(a, b, hk, rho);
+  const RowParts rp = row_parts(a, b, hk, rho);
+  const int n = ri.valid ? rp.n : 0;
   float m = -INFINITY;
-  for (int i = lane; i < n; i += 64) m = fmaxf(m, a.stat[place(i)].x);
+  for (int i = tid; i < n; i += 256) m = fmaxf(m, a.stat[rp.at(a, i)].x);
 #pragma unroll
   for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, shfl_xor_f(m, x));
+  if (lane == 0) s_red[wave] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
   const float ref = m == -INFINITY ? 0.f : m;
-  constexpr int NE = DP / 64 ? DP / 64 : 1;
-  float l = 0.f, acc[NE];
-#pragma unroll
-  for (int e = 0; e < NE; ++e) acc[e] = 0.f;
-  for (int i = 0; i < n; ++i) {
-    const int64_t at = place(i);
-    const float2 st = a.stat[at];
-    if (st.y == 0.f) continue;
-    const float f = __builtin_amdgcn_exp2f(st.x - ref);
-    l += f * st.y;
-    if (lane * NE < DP)
-#pragma unroll
-      for (int e = 0; e < NE; ++e) acc[e] += f * a.part[at * DP + lane * NE + e];
+  float l = 0.f;
+  for (int i = tid; i < n; i += 256) {
+    const float2 st = a.stat[rp.at(a, i)];
+    const float f = st.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(st.x - ref);
+    if (st.y != 0.f) l += f * st.y;
+    s_f[i] = st.y == 0.f ? -1.f : f;  // (a part of no keys has no O)
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  T *orow = (T *)a.o + b * a.so[0] + ri.hq * a.so[1] + ri.t * a.so[2];
-  const T *og = a.og ? (const T *)a.og + b * a.sog[0] + ri.hq * a.sog[1] + ri.t * a.sog[2] : nullptr;
 #pragma unroll
-  for (int e = 0; e < NE; ++e) {
-    const int d = lane * NE + e;
-    if (d < a.D) {
-      float y = acc[e] * inv;
-      if (og) y *= 1.f / (1.f + __expf(-to_f32<T>(og[d])));
-      orow[d] = from_f32<T>(y);
-    }
+  for (int x = 1; x < 64; x <<= 1) l += shfl_xor_f(l, x);
+  if (lane == 0) s_red[4 + wave] = l;
+  __syncthreads();
+  l = (s_red[4] + s_red[5]) + (s_red[6] + s_red[7]);
+  const int gi = tid / LG, e = tid % LG;
+  f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i = gi; i < n; i += NG) {
+    const float f = s_f[i];
+    if (f != -1.f) acc += f * *(const f32x4 *)(a.part + rp.at(a, i) * DP + 4 * e);
   }
-  if (lane == 0) {
+  s_acc[tid] = acc;
+  __syncthreads();
+  if (tid < LG) {
+    for (int j = 1; j < NG; ++j) acc += s_acc[j * LG + tid];
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    store_row<T>(a, ri, acc, inv, 4 * tid);
+  }
+  if (tid == 0) {
     const float l2 = l == 0.f ? -INFINITY : m + __log2f(l);
     if (a.lse) a.lse[((int64_t)b * a.Hq + ri.hq) * a.T + ri.t] = l2 * kLn2;
-    if (a.wo) a.lse2[row] = l2;
+    if (a.lse2) a.lse2[blockIdx.x] = l2;
   }
 }
 
@@ -349,8 +466,9 @@ static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 // Tiles and shares of a call, from its sizes alone (lengths are on the device:
 // the capacity stands for them).
 struct CachePlan {
-  int64_t rt_own, rt_pre, np_own, np_pre, slots, DP;
-  size_t stat, part, lse2, total;
+  int64_t tr_own, tr_pre, rt_own, rt_pre, np_own, np_pre, rows, DP;
+  bool few_own, few_pre, direct;
+  size_t stat, part, lse2, sc, total;
 };
 static CachePlan cache_plan(const fbsa_cache_desc *d) {
   CachePlan p;
@@ -358,45 +476,52 @@ static CachePlan cache_plan(const fbsa_cache_desc *d) {
   p.DP = d->D <= 32 ? 32 : d->D <= 64 ? 64 : d->D <= 128 ? 128 : 256;
   const int64_t KC = d->dtype == FBSA_F32 && p.DP >= 128 ? 16 : 32;
   constexpr int64_t kWaves = 1024;  // four waves to a CU
-  p.rt_own = cdiv(TG, 16);
-  p.rt_pre = d->P ? cdiv(d->B * TG, 16) : 0;
+  p.few_own = p.few_pre = true;
+  p.direct = false;
+  p.tr_own = p.tr_pre = 16;
+  p.rt_own = cdiv(TG, p.tr_own);
+  p.rt_pre = d->P ? cdiv(d->B * TG, p.tr_pre) : 0;
   auto shares = [&](int64_t tiles, int64_t keys) {
     const int64_t want = cdiv(kWaves, tiles), most = cdiv(keys, 4 * KC);
-    return want < most ? want : most;
+    const int64_t n = want < most ? want : most;
+    return n < kMaxShares / 2 ? n : kMaxShares / 2;
   };
   p.np_own = shares(d->B * d->Hkv * p.rt_own, d->S);
   p.np_pre = d->P ? shares(d->Hkv * p.rt_pre, d->P) : 0;
-  p.slots = d->B * d->Hkv * p.rt_own * p.np_own + d->Hkv * p.rt_pre * p.np_pre;
+  p.rows = d->B * d->Hkv * p.rt_own * p.np_own * p.tr_own + d->Hkv * p.rt_pre * p.np_pre * p.tr_pre;
   p.stat = 0;
-  p.part = up256((size_t)p.slots * 16 * 8);
-  p.lse2 = p.part + up256((size_t)p.slots * 16 * p.DP * 4);
-  p.total = p.lse2 + up256((size_t)(d->B * d->Hkv * TG) * 4);
+  p.part = up256((size_t)p.rows * 8);
+  p.lse2 = p.part + up256((size_t)p.rows * p.DP * 4);
+  p.sc = p.lse2 + up256((size_t)(d->B * d->Hkv * TG) * 4);
+  p.total = p.sc + (d->flags & FBSA_CACHE_WEIGHT && p.rt_own == 1 ? up256((size_t)(d->B * d->Hkv * TG) * cdiv(d->S, 32) * 128) : 0);
   return p;
 }
 
-template <typename T, int DP> static int launch_cache(const CacheArgs &a, const CachePlan &pl, hipStream_t s) {
+template <typename T, int DP> static int launch_cache(const CacheArgs &a, hipStream_t s) {
   using C = CacheCfg<T, DP>;
   const size_t lds = (size_t)C::NST * 2 * C::TILE;
   int e = lds_optin((const void *)cache_part_kernel<T, DP>, lds, "hipFuncSetAttribute(cache_part)");
   if (e) return e;
-  const int64_t parts = pl.slots, rows = (int64_t)a.B * a.Hkv * a.TG;
+  const int64_t rows = (int64_t)a.B * a.Hkv * a.TG;
+  const int64_t parts = (int64_t)a.B * a.Hkv * a.rt_own * a.np_own + (int64_t)a.Hkv * a.rt_pre * a.np_pre;
   hipLaunchKernelGGL((cache_part_kernel<T, DP>), dim3((unsigned)parts), dim3(64), lds, s, a);
   if ((e = hip_check(hipGetLastError(), "cache_part_kernel launch"))) return e;
-  hipLaunchKernelGGL((cache_combine_kernel<T, DP>), dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, s, a);
+  const int64_t wgs = a.sc ? (int64_t)a.B * a.Hkv * cdiv(a.S, kWeightKeys) : 0;
+  hipLaunchKernelGGL((cache_combine_kernel<T, DP>), dim3((unsigned)(rows + wgs)), dim3(256), 0, s, a);
   if ((e = hip_check(hipGetLastError(), "cache_combine_kernel launch"))) return e;
-  if (a.wo) {
+  if (a.wo && !a.sc) {
     hipLaunchKernelGGL((cache_weight_kernel<T, DP>), dim3((unsigned)cdiv(a.S, C::KC), (unsigned)(a.B * a.Hkv)), dim3(64), C::TILE, s, a);
     e = hip_check(hipGetLastError(), "cache_weight_kernel launch");
   }
   return e;
 }
 
-template <typename T> static int dispatch_cache(const CacheArgs &a, const CachePlan &pl, hipStream_t s) {
-  switch (pl.DP) {
-    case 32: return launch_cache<T, 32>(a, pl, s);
-    case 64: return launch_cache<T, 64>(a, pl, s);
-    case 128: return launch_cache<T, 128>(a, pl, s);
-    default: return launch_cache<T, 256>(a, pl, s);
+template <typename T> static int dispatch_cache(const CacheArgs &a, int64_t DP, hipStream_t s) {
+  switch (DP) {
+    case 32: return launch_cache<T, 32>(a, s);
+    case 64: return launch_cache<T, 64>(a, s);
+    case 128: return launch_cache<T, 128>(a, s);
+    default: return launch_cache<T, 256>(a, s);
   }
 }
 
@@ -406,7 +531,7 @@ static int check_cache(const fbsa_cache_desc *d) {
   static const char *fn = "fbsa_cache_attn";
   if (!d) return fail(FBSA_EINVAL, "%s: null descriptor", fn);
   if (d->dtype < FBSA_F32 || d->dtype > FBSA_F16) return fail(FBSA_EINVAL, "%s: bad dtype %d", fn, d->dtype);
-  if (d->flags) return fail(FBSA_EINVAL, "%s: unknown flags 0x%x", fn, d->flags);
+  if (d->flags & ~FBSA_CACHE_WEIGHT) return fail(FBSA_EINVAL, "%s: unknown flags 0x%x", fn, d->flags);
   if (d->B < 1 || d->Hq < 1 || d->Hkv < 1 || d->T < 1 || d->S < 1 || d->P < 0)
     return fail(FBSA_EINVAL, "%s: sizes must be positive (B=%lld Hq=%lld Hkv=%lld T=%lld S=%lld P=%lld)", fn, (long long)d->B,
                 (long long)d->Hq, (long long)d->Hkv, (long long)d->T, (long long)d->S, (long long)d->P);
@@ -429,7 +554,8 @@ static int check_cache(const fbsa_cache_desc *d) {
   const int64_t rs[4] = {d->sk[2], d->sv[2], d->P ? d->skp[1] : 0, d->P ? d->svp[1] : 0};
   for (int64_t r : rs)
     if (r * es >= 1LL << 26) return fail(FBSA_EUNSUPPORTED, "%s: a row stride of %lld elements is 64 MiB or more", fn, (long long)r);
-  if (cache_plan(d).slots > lim) return fail(FBSA_EUNSUPPORTED, "%s: grid too large", fn);
+  const CachePlan pl = cache_plan(d);
+  if (pl.rows > lim || d->B * d->Hkv * (d->T * (d->Hq / d->Hkv) + cdiv(d->S, kWeightKeys)) > lim) return fail(FBSA_EUNSUPPORTED, "%s: grid too large", fn);
   return FBSA_OK;
 }
 
@@ -449,6 +575,8 @@ int fbsa_cache_attn(const fbsa_cache_desc *d, const void *q, const void *k, cons
   if (!q || !k || !v || !lens || !o || (d->P && (!k_prefix || !v_prefix)))
     return fail(FBSA_EINVAL, "fbsa_cache_attn: null tensor pointer");
   if (weight && !out_weight) return fail(FBSA_EINVAL, "fbsa_cache_attn: weight without out_weight");
+  if (!out_weight != !(d->flags & FBSA_CACHE_WEIGHT))
+    return fail(FBSA_EINVAL, "fbsa_cache_attn: out_weight and FBSA_CACHE_WEIGHT go together");
   const int64_t es = d->dtype == FBSA_F32 ? 4 : 2;
   if (!aligned_to(q, 16) || !aligned_to(k, 16) || !aligned_to(v, 16) || !aligned_to(o, 16) ||
       (d->P && (!aligned_to(k_prefix, 16) || !aligned_to(v_prefix, 16))))
@@ -469,14 +597,18 @@ int fbsa_cache_attn(const fbsa_cache_desc *d, const void *q, const void *k, cons
   }
   a.B = (int)d->B; a.Hq = (int)d->Hq; a.Hkv = (int)d->Hkv; a.T = (int)d->T; a.S = (int)d->S; a.P = (int)d->P; a.D = (int)d->D;
   a.G = (int)(d->Hq / d->Hkv); a.TG = a.T * a.G;
+  a.tr_own = (int)pl.tr_own; a.tr_pre = (int)pl.tr_pre;
   a.rt_own = (int)pl.rt_own; a.rt_pre = (int)pl.rt_pre; a.np_own = (int)pl.np_own; a.np_pre = (int)pl.np_pre;
+  a.few_own = pl.few_own; a.few_pre = pl.few_pre; a.direct = pl.direct;
   a.scale2 = d->scale * kLog2e;
   char *ws = (char *)workspace;
-  a.stat = (float2 *)(ws + pl.stat); a.part = (float *)(ws + pl.part); a.lse2 = (float *)(ws + pl.lse2);
+  a.stat = (float2 *)(ws + pl.stat); a.part = (float *)(ws + pl.part);
+  if (out_weight && pl.rt_own == 1) a.sc = (float *)(ws + pl.sc);
+  else if (out_weight) a.lse2 = (float *)(ws + pl.lse2);
   switch (d->dtype) {
-    case FBSA_BF16: return dispatch_cache<bf16>(a, pl, (hipStream_t)stream);
-    case FBSA_F16: return dispatch_cache<f16>(a, pl, (hipStream_t)stream);
-    default: return dispatch_cache<float>(a, pl, (hipStream_t)stream);
+    case FBSA_BF16: return dispatch_cache<bf16>(a, pl.DP, (hipStream_t)stream);
+    case FBSA_F16: return dispatch_cache<f16>(a, pl.DP, (hipStream_t)stream);
+    default: return dispatch_cache<float>(a, pl.DP, (hipStream_t)stream);
   }
 }
 

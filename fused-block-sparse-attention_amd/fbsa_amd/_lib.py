@@ -21,6 +21,7 @@ SEL_CHUNK_SHIFT = 8
 FLAG_OUT_GATE, FLAG_DENSE, FLAG_DGATE, FLAG_RAGGED = 1, 2, 4, 8
 SELECT_SCRATCH_BYTES = 32 << 20   # FBSA_SELECT_SCRATCH_BYTES
 EVICT_IN_PLACE = 1
+CACHE_WEIGHT = 1
 
 _i64x2 = ctypes.c_int64 * 2
 _i64x3 = ctypes.c_int64 * 3

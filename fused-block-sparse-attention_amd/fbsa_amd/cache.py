@@ -175,6 +175,7 @@ def _attend(what, q, kp, vp, k, v, lens, count, scale, out_gate, weight, out_wei
     if weight is not None:
         d.sw[:] = _strides(weight, 2)
     if out_weight is not None:
+        d.flags = _lib.CACHE_WEIGHT
         d.swo[:] = _strides(out_weight, 2)
     lib = _lib.load()
     with torch.cuda.device(q.device):

@@ -371,10 +371,13 @@ int fbsa_cache_append(const fbsa_append_desc *d, void *k, void *v, const void *k
  * queries of the KV head's group gave it; weight may be out_weight. Softmax,
  * sums and weights are fp32. The split of the keys follows from the sizes, and
  * parts are joined in a fixed order: results are bitwise repeatable.
- * The workspace is 256-byte aligned; fbsa_cache_attn_workspace_bytes returns 0
- * (with fbsa_last_error set) for a descriptor that fbsa_cache_attn refuses. */
+ * FBSA_CACHE_WEIGHT in flags says that out_weight is given. The workspace is
+ * 256-byte aligned; fbsa_cache_attn_workspace_bytes returns 0 (with
+ * fbsa_last_error set) for a descriptor that fbsa_cache_attn refuses. */
+enum { FBSA_CACHE_WEIGHT = 1 };
+
 typedef struct fbsa_cache_desc {
-  int32_t dtype, flags;                     /* flags: 0 */
+  int32_t dtype, flags;
   int64_t B, Hq, Hkv, T, S, P, D;
   float scale;
   int32_t reserved;

@@ -33,7 +33,7 @@ def test_struct_layouts():
 
 
 @pytest.mark.parametrize("kw,needle", [
-    ({"dtype": 5}, "dtype"), ({"flags": 1}, "flags"), ({"T": 0}, "positive"), ({"S": 0}, "positive"), ({"P": -1}, "positive"),
+    ({"dtype": 5}, "dtype"), ({"flags": 2}, "flags"), ({"T": 0}, "positive"), ({"S": 0}, "positive"), ({"P": -1}, "positive"),
     ({"Hkv": 3}, "multiple"), ({"D": 60}, "head dim"), ({"D": 264}, "head dim"), ({"scale": float("nan")}, "scale"),
     ({"S": 1 << 31}, "32-bit"), ({"B": 40000}, "grid"), ({"sk": (8192, 4096, 63)}, "stride"), ({"sv": (8192, -64, 64)}, "stride"),
     ({"sk": (0, 0, 1 << 26)}, "64 MiB"), ({"P": 8, "skp": (512, 60)}, "k_prefix"),
@@ -53,6 +53,8 @@ def test_attention_pointers_and_workspace():
     assert _call(d, q=None) == _lib.EINVAL and _call(d, lens=None) == _lib.EINVAL
     assert _call(d, q=DUMMY + 8) == _lib.EINVAL and b"aligned" in lib.fbsa_last_error()
     assert _call(d, weight=DUMMY) == _lib.EINVAL and b"out_weight" in lib.fbsa_last_error()
+    assert _call(d, out_weight=DUMMY) == _lib.EINVAL and b"FBSA_CACHE_WEIGHT" in lib.fbsa_last_error()
+    assert _call(_attn(flags=_lib.CACHE_WEIGHT)) == _lib.EINVAL
     assert _call(d, ws=None) == _lib.EWORKSPACE and _call(d, nbytes=need - 1) == _lib.EWORKSPACE
     assert _call(d, ws=DUMMY + 128, nbytes=need) == _lib.EINVAL
     assert _call(_attn(P=16, skp=(1024, 64), svp=(1024, 64))) == _lib.EINVAL  # a prefix of no tensors
