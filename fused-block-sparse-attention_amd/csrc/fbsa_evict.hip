@@ -4,9 +4,9 @@
 // Eviction keeps, of a (sequence, head) with n > budget rows, the first `sink`,
 // the last `recent` and the K = budget - sink - recent greatest weights between.
 // Weights become unsigned keys of the same order; the K-th greatest is found by
-// a radix select, a byte a pass, and one ordered pass over the rows then writes
+// a radix select in three digits, and one ordered pass over the rows then writes
 // the kept rows' numbers and weights (ties to the lower row: of the rows that
-// equal the K-th greatest the first are kept). A second kernel moves the rows.
+// equal the K-th greatest the first are kept). Another kernel moves the rows.
 #include "fbsa_common.h"
 #include "fbsa_internal.h"
 
@@ -63,9 +63,47 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// The K-th greatest key is found digit by digit: 11, 11 and 10 bits.
+constexpr int kBins = 2048;
+__device__ __forceinline__ int digit_shift(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
+__device__ __forceinline__ int digit_bits(int pass) { return pass == 2 ? 10 : 11; }
+
+// The bin of the need-th greatest key, and how many of that bin are needed, from
+// a histogram in LDS; NT threads, each NB = kBins / NT bins in descending order.
+struct Pick {
+  uint32_t bin, need;
+};
+template <int NT> __device__ __forceinline__ Pick pick_bin(const uint32_t *hist, uint32_t need, uint32_t *s_wave, Pick *s_pick) {
+  constexpr int NB = kBins / NT, NW = NT / 64;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  uint32_t c[NB], sum = 0;
+#pragma unroll
+  for (int j = 0; j < NB; ++j) sum += c[j] = hist[kBins - 1 - NB * tid - j];
+  uint32_t before = sum;
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) {
+    const uint32_t y = __shfl_up(before, x, 64);
+    if (lane >= x) before += y;
+  }
+  if (lane == 63) s_wave[wave] = before;
+  before -= sum;
+  __syncthreads();
+  for (int v = 0; v < NW; ++v)
+    if (v < wave) before += s_wave[v];
+#pragma unroll
+  for (int j = 0; j < NB; ++j) {
+    if (before < need && need <= before + c[j]) *s_pick = Pick{(uint32_t)(kBins - 1 - NB * tid - j), need - before};
+    before += c[j];
+  }
+  __syncthreads();
+  return *s_pick;
+}
+
 constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64;
 
-__global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) {
+// A workgroup per (sequence, head) whose weights stay in registers, R a thread:
+// rows tid + 1024 r.
+template <int R> __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int h = blockIdx.x % a.H, b = blockIdx.x / a.H;
   const int n = evict_len(a, b);
@@ -76,75 +114,356 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
   if (h == 0 && tid == 0) a.new_lens[b] = kept;
   for (int i = kept + tid; i < a.ni; i += kSelThreads) index[i] = -1;
 
-  __shared__ uint32_t hist[256];
-  __shared__ uint32_t s_prefix, s_need;
-  __shared__ int s_def[kSelWaves], s_eq[kSelWaves];
-  const int lo = a.sink, hi = n - a.recent;       // rows that the weight decides about (n > budget)
-  uint32_t need = n > a.budget ? (uint32_t)(a.budget - a.recent - a.sink) : 0, prefix = 0;
-  if (need) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
+  __shared__ uint32_t hist[kBins];
+  __shared__ uint32_t s_wave[kSelWaves];
+  __shared__ Pick s_pick;
+  __shared__ int s_cnt[R][kSelWaves];  // rows kept for certain and rows that equal the K-th, packed
+  float x[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) x[r] = tid + r * kSelThreads < n ? w[tid + r * kSelThreads] : 0.f;
+  const int lo = a.sink, hi = n - a.recent;  // rows that the weight decides about (n > budget)
+  const bool all = n <= a.budget;
+  uint32_t need = all ? 0 : (uint32_t)(a.budget - a.recent - a.sink), prefix = 0;
+  const bool mid = need > 0;
+  if (mid) {
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = digit_shift(pass), bits = digit_bits(pass);
+      for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
       __syncthreads();
-      for (int i = lo + tid; i < hi; i += kSelThreads) {
-        const uint32_t key = weight_key(w[i]);
-        if (shift == 24 || (key >> (shift + 8)) == prefix) atomicAdd(&hist[key >> shift & 255], 1u);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const int i = tid + r * kSelThreads;
+        const uint32_t key = weight_key(x[r]);
+        if (i >= lo && i < hi && (pass == 0 || key >> (shift + bits) == prefix)) atomicAdd(&hist[key >> shift & ((1u << bits) - 1)], 1u);
       }
       __syncthreads();
-      if (wave == 0) {
-        // lane l holds bins 255 - 4l - j, j = 0..3: counts in descending key order
-        uint32_t c[4], sum = 0;
-        for (int j = 0; j < 4; ++j) sum += c[j] = hist[255 - 4 * lane - j];
-        uint32_t before = sum;
-        for (int x = 1; x < 64; x <<= 1) {
-          const uint32_t y = __shfl_up(before, x, 64);
-          if (lane >= x) before += y;
-        }
-        before -= sum;
-        for (int j = 0; j < 4; ++j) {
-          if (before < need && need <= before + c[j]) {
-            s_prefix = prefix << 8 | (uint32_t)(255 - 4 * lane - j);
-            s_need = need - before;
-          }
-          before += c[j];
-        }
-      }
+      const Pick pk = pick_bin<kSelThreads>(hist, need, s_wave, &s_pick);
+      prefix = prefix << bits | pk.bin;
+      need = pk.need;
       __syncthreads();
-      prefix = s_prefix;
-      need = s_need;
     }
   }
   // rows above the K-th greatest key are kept, and the first `need` that equal it
-  int ndef = 0, neq = 0;  // of the rows before this step's
-  const bool all = n <= a.budget, mid = !all && a.budget > a.recent + a.sink;
-  for (int base = 0; base < n; base += kSelThreads) {
-    const int i = base + tid;
-    bool def = false, eq = false;
-    float x = 0.f;
-    if (i < n) {
-      x = w[i];
-      if (all || i < lo || i >= hi) def = true;
-      else if (mid) {
-        const uint32_t key = weight_key(x);
-        def = key > prefix;
-        eq = key == prefix;
-      }
+  const uint64_t below = (1ull << lane) - 1;
+  auto rank = [&](int r, bool &def, bool &eq) {  // (formed twice: held, they cost registers that R = 32 has not)
+    const int i = tid + r * kSelThreads;
+    const uint32_t key = weight_key(x[r]);
+    const bool free_ = i >= lo && i < hi && !all;
+    def = i < n && (!free_ || (mid && key > prefix));
+    eq = i < n && free_ && mid && key == prefix;
+  };
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    bool def, eq;
+    rank(r, def, eq);
+    const int d = __popcll(__ballot(def)), e = __popcll(__ballot(eq));
+    if (lane == 0) s_cnt[r][wave] = d | e << 16;
+  }
+  wait_vmcnt<0>();  // (in place: this wave's weights are here before any wave writes one)
+  __syncthreads();
+  if (wave == 0) {  // counts to the sums before them, in row order
+    constexpr int PL = (R * kSelWaves + 63) / 64;
+    int *cnt = &s_cnt[0][0], c[PL], sum = 0;
+#pragma unroll
+    for (int j = 0; j < PL; ++j) {
+      const int u = lane * PL + j;
+      c[j] = u < R * kSelWaves ? cnt[u] : 0;
+      sum += c[j];
     }
-    const uint64_t md = __ballot(def), me = __ballot(eq), below = (1ull << lane) - 1;
-    if (lane == 0) { s_def[wave] = __popcll(md); s_eq[wave] = __popcll(me); }
-    __syncthreads();
-    int d0 = ndef + __popcll(md & below), e0 = neq + __popcll(me & below);
-    for (int v = 0; v < kSelWaves; ++v) {
-      if (v < wave) { d0 += s_def[v]; e0 += s_eq[v]; }
-      ndef += s_def[v];
-      neq += s_eq[v];
+    int before = sum;
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) {
+      const int y = __shfl_up(before, x, 64);
+      if (lane >= x) before += y;
     }
+    before -= sum;
+#pragma unroll
+    for (int j = 0; j < PL; ++j) {
+      const int u = lane * PL + j;
+      if (u < R * kSelWaves) cnt[u] = before;
+      before += c[j];
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const uint32_t c = (uint32_t)s_cnt[r][wave];
+    bool def, eq;
+    rank(r, def, eq);
+    const int d0 = (int)(c & 0xffff) + __popcll(__ballot(def) & below);
+    const int e0 = (int)(c >> 16) + __popcll(__ballot(eq) & below);
     if (def || (eq && e0 < (int)need)) {
       const int at = d0 + (e0 < (int)need ? e0 : (int)need);
-      index[at] = i;
-      wo[at] = x;  // (in place: at <= i, and every row up to this step's last has been read)
+      index[at] = tid + r * kSelThreads;
+      wo[at] = x[r];
     }
-    __syncthreads();
   }
+}
+
+// Longer rows: chunks of kChunk weights, a workgroup each, in four steps over a
+// workspace. hist: the first digit's histogram of the row. cand: the chunk's keys
+// that share the K-th greatest's first digit, in order, and how many lie above.
+// rank (a workgroup per row): the other two digits among those, and each chunk's
+// place in the output. place: kept rows' numbers and weights.
+constexpr int kChunkR = 8, kChunk = kSelThreads * kChunkR;
+struct EvictWs {
+  uint32_t *hist;   // [row][kBins]
+  uint32_t *cand;   // [row][chunk][kChunk]
+  float *copy;      // [row][chunk][kChunk]: the weights, where they are moved in place
+  uint2 *count;     // [row][chunk]: keys above the first digit, keys of it
+  uint2 *start;     // [row][chunk]: kept for certain before the chunk, equal to the K-th before it
+  uint2 *pick;      // [row]: the K-th greatest key, and how many equal to it are kept
+  int nch;
+};
+
+__global__ __launch_bounds__(256) void evict_zero_kernel(uint32_t *x, int64_t n) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i < n) x[i] = 0;
+}
+
+// what the steps need to know of a row: the range that the weight decides about
+// and how many of it are kept; `mid` false: nothing to rank
+struct EvictRow {
+  int b, h, n, lo, hi;
+  uint32_t need;
+  bool all, mid;
+};
+__device__ __forceinline__ EvictRow evict_row(const EvictArgs &a, int row) {
+  EvictRow r;
+  r.h = row % a.H;
+  r.b = row / a.H;
+  r.n = evict_len(a, r.b);
+  r.lo = a.sink;
+  r.hi = r.n - a.recent;
+  r.all = r.n <= a.budget;
+  r.need = r.all ? 0 : (uint32_t)(a.budget - a.recent - a.sink);
+  r.mid = r.need > 0;
+  return r;
+}
+
+__global__ __launch_bounds__(kSelThreads) void evict_hist_kernel(EvictArgs a, EvictWs ws) {
+  const EvictRow er = evict_row(a, blockIdx.y);
+  const int64_t base = (int64_t)blockIdx.x * kChunk;
+  const float *w = a.w + er.b * a.sw[0] + er.h * a.sw[1];
+  if (blockIdx.x == 0) {
+    const int kept = er.n < a.budget ? er.n : a.budget;
+    if (er.h == 0 && threadIdx.x == 0) a.new_lens[er.b] = kept;
+  }
+  const int kept = er.n < a.budget ? er.n : a.budget;
+  for (int r = 0; r < kChunkR; ++r) {
+    const int64_t i = base + threadIdx.x + r * kSelThreads;
+    if (i >= kept && i < a.ni) a.index[(int64_t)blockIdx.y * a.ni + i] = -1;
+  }
+  if (base >= er.n) return;
+  __shared__ uint32_t hist[kBins];
+  for (int i = threadIdx.x; i < kBins; i += kSelThreads) hist[i] = 0;
+  float x[kChunkR];
+#pragma unroll
+  for (int r = 0; r < kChunkR; ++r) {
+    const int64_t i = base + threadIdx.x + r * kSelThreads;
+    x[r] = i < er.n ? w[i] : 0.f;
+    if (ws.copy && i < er.n) ws.copy[(int64_t)blockIdx.y * ws.nch * kChunk + i] = x[r];
+  }
+  if (!er.mid) return;
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kChunkR; ++r) {
+    const int64_t i = base + threadIdx.x + r * kSelThreads;
+    if (i >= er.lo && i < er.hi) atomicAdd(&hist[weight_key(x[r]) >> digit_shift(0)], 1u);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kBins; i += kSelThreads)
+    if (hist[i]) atomicAdd(&ws.hist[(int64_t)blockIdx.y * kBins + i], hist[i]);  // (whole numbers: any order gives the same)
+}
+
+__global__ __launch_bounds__(kSelThreads) void evict_cand_kernel(EvictArgs a, EvictWs ws) {
+  const EvictRow er = evict_row(a, blockIdx.y);
+  const int64_t base = (int64_t)blockIdx.x * kChunk;
+  if (!er.mid || base >= er.n) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ uint32_t hist[kBins], s_wave[kSelWaves];
+  __shared__ Pick s_pick;
+  __shared__ int s_cnt[kChunkR][kSelWaves];
+  const float *w = a.w + er.b * a.sw[0] + er.h * a.sw[1];
+  float x[kChunkR];
+#pragma unroll
+  for (int r = 0; r < kChunkR; ++r) {
+    const int64_t i = base + tid + r * kSelThreads;
+    x[r] = i < er.n ? w[i] : 0.f;
+  }
+  for (int i = tid; i < kBins; i += kSelThreads) hist[i] = ws.hist[(int64_t)blockIdx.y * kBins + i];
+  __syncthreads();
+  const Pick pk = pick_bin<kSelThreads>(hist, er.need, s_wave, &s_pick);
+  bool in[kChunkR];
+#pragma unroll
+  for (int r = 0; r < kChunkR; ++r) {
+    const int64_t i = base + tid + r * kSelThreads;
+    const uint32_t top = weight_key(x[r]) >> digit_shift(0);
+    const bool free_ = i >= er.lo && i < er.hi;
+    in[r] = free_ && top == pk.bin;
+    const int above = __popcll(__ballot(free_ && top > pk.bin)), c = __popcll(__ballot(in[r]));
+    if (lane == 0) s_cnt[r][wave] = c | above << 16;
+  }
+  __syncthreads();
+  uint32_t *dst = ws.cand + ((int64_t)blockIdx.y * ws.nch + blockIdx.x) * kChunk;
+  int before = 0;
+#pragma unroll
+  for (int r = 0; r < kChunkR; ++r) {
+    int at = 0;
+    for (int v = 0; v < kSelWaves; ++v) {
+      if (v == wave) at = before & 0xffff;
+      before += s_cnt[r][v];
+    }
+    at += __popcll(__ballot(in[r]) & ((1ull << lane) - 1));
+    if (in[r]) dst[at] = weight_key(x[r]);
+  }
+  if (tid == 0) ws.count[(int64_t)blockIdx.y * ws.nch + blockIdx.x] = uint2{(uint32_t)before >> 16, (uint32_t)before & 0xffff};
+  if (tid == 0 && blockIdx.x == 0) ws.pick[blockIdx.y] = uint2{pk.bin, pk.need};
+}
+
+__global__ __launch_bounds__(kSelThreads) void evict_rank_kernel(EvictArgs a, EvictWs ws) {
+  const EvictRow er = evict_row(a, blockIdx.x);
+  if (er.all) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int nch = (int)(((int64_t)er.n + kChunk - 1) / kChunk);
+  const uint2 *count = ws.count + (int64_t)blockIdx.x * ws.nch;
+  uint2 *start = ws.start + (int64_t)blockIdx.x * ws.nch;
+  const uint32_t *cand = ws.cand + (int64_t)blockIdx.x * ws.nch * kChunk;
+  __shared__ uint32_t hist[kBins], s_wave[kSelWaves];
+  __shared__ Pick s_pick;
+  uint32_t prefix = 0, need = 0;
+  if (er.mid) {
+    prefix = ws.pick[blockIdx.x].x;
+    need = ws.pick[blockIdx.x].y;
+    for (int pass = 1; pass < 3; ++pass) {
+      const int shift = digit_shift(pass), bits = digit_bits(pass);
+      for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
+      __syncthreads();
+      for (int c = wave; c < nch; c += kSelWaves) {  // a wave per chunk
+        const int m = (int)count[c].y;
+        for (int i = lane; i < m; i += 64) {
+          const uint32_t key = cand[(int64_t)c * kChunk + i];
+          if (key >> (shift + bits) == prefix) atomicAdd(&hist[key >> shift & ((1u << bits) - 1)], 1u);
+        }
+      }
+      __syncthreads();
+      const Pick pk = pick_bin<kSelThreads>(hist, need, s_wave, &s_pick);
+      prefix = prefix << bits | pk.bin;
+      need = pk.need;
+      __syncthreads();
+    }
+  }
+  // each chunk's rows kept for certain and equal to the K-th, then their sums before it
+  for (int c = wave; c < nch; c += kSelWaves) {
+    uint32_t d = 0, e = 0;
+    const int m = er.mid ? (int)count[c].y : 0;
+    for (int i0 = 0; i0 < m; i0 += 64) {
+      const uint32_t key = i0 + lane < m ? cand[(int64_t)c * kChunk + i0 + lane] : 0;
+      d += __popcll(__ballot(i0 + lane < m && key > prefix));
+      e += __popcll(__ballot(i0 + lane < m && key == prefix));
+    }
+    const int64_t r0 = (int64_t)c * kChunk, r1 = r0 + kChunk < er.n ? r0 + kChunk : er.n;
+    const int64_t sink = r0 < er.lo ? (r1 < er.lo ? r1 : er.lo) - r0 : 0, tail = r1 > er.hi ? r1 - (r0 > er.hi ? r0 : er.hi) : 0;
+    if (lane == 0) start[c] = uint2{(er.mid ? count[c].x : 0) + d + (uint32_t)(sink + tail), e};
+  }
+  __syncthreads();
+  if (wave == 0) {
+    uint32_t d0 = 0, e0 = 0;
+    for (int c0 = 0; c0 < nch; c0 += 64) {
+      const int c = c0 + lane;
+      const uint2 x = c < nch ? start[c] : uint2{0, 0};
+      uint32_t d = x.x, e = x.y;
+#pragma unroll
+      for (int y = 1; y < 64; y <<= 1) {
+        const uint32_t dd = __shfl_up(d, y, 64), ee = __shfl_up(e, y, 64);
+        if (lane >= y) { d += dd; e += ee; }
+      }
+      if (c < nch) start[c] = uint2{d0 + d - x.x, e0 + e - x.y};
+      d0 += __shfl(d, 63, 64);
+      e0 += __shfl(e, 63, 64);
+    }
+    if (lane == 0) ws.pick[blockIdx.x] = uint2{prefix, need};
+  }
+}
+
+__global__ __launch_bounds__(kSelThreads) void evict_place_kernel(EvictArgs a, EvictWs ws) {
+  const EvictRow er = evict_row(a, blockIdx.y);
+  const int64_t base = (int64_t)blockIdx.x * kChunk;
+  if (base >= er.n) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const float *w = ws.copy ? ws.copy + (int64_t)blockIdx.y * ws.nch * kChunk : a.w + er.b * a.sw[0] + er.h * a.sw[1];
+  float *wo = a.wo + er.b * a.swo[0] + er.h * a.swo[1];
+  int32_t *index = a.index + (int64_t)blockIdx.y * a.ni;
+  if (er.all) {
+    for (int r = 0; r < kChunkR; ++r) {
+      const int64_t i = base + tid + r * kSelThreads;
+      if (i < er.n) {
+        index[i] = (int32_t)i;
+        wo[i] = w[i];
+      }
+    }
+    return;
+  }
+  __shared__ int s_cnt[kChunkR][kSelWaves];
+  const uint2 st = ws.start[(int64_t)blockIdx.y * ws.nch + blockIdx.x], pk = ws.pick[blockIdx.y];
+  float x[kChunkR];
+  bool def[kChunkR], eq[kChunkR];
+#pragma unroll
+  for (int r = 0; r < kChunkR; ++r) {
+    const int64_t i = base + tid + r * kSelThreads;
+    x[r] = i < er.n ? w[i] : 0.f;
+  }
+#pragma unroll
+  for (int r = 0; r < kChunkR; ++r) {
+    const int64_t i = base + tid + r * kSelThreads;
+    const uint32_t key = weight_key(x[r]);
+    const bool free_ = i >= er.lo && i < er.hi;
+    def[r] = i < er.n && (!free_ || (er.mid && key > pk.x));
+    eq[r] = free_ && er.mid && key == pk.x;
+    const int d = __popcll(__ballot(def[r])), e = __popcll(__ballot(eq[r]));
+    if (lane == 0) s_cnt[r][wave] = d | e << 16;
+  }
+  __syncthreads();
+  const uint64_t below = (1ull << lane) - 1;
+  int before = 0;
+#pragma unroll
+  for (int r = 0; r < kChunkR; ++r) {
+    int at = 0;
+    for (int v = 0; v < kSelWaves; ++v) {
+      if (v == wave) at = before;
+      before += s_cnt[r][v];
+    }
+    const uint32_t d0 = st.x + ((uint32_t)at & 0xffff) + __popcll(__ballot(def[r]) & below);
+    const uint32_t e0 = st.y + ((uint32_t)at >> 16) + __popcll(__ballot(eq[r]) & below);
+    if (def[r] || (eq[r] && e0 < pk.y)) {
+      const uint32_t o = d0 + (e0 < pk.y ? e0 : pk.y);
+      index[o] = (int32_t)(base + tid + r * kSelThreads);
+      wo[o] = x[r];
+    }
+  }
+}
+
+// Rows of up to this many weights: one workgroup, weights in registers. Longer
+// ones: the steps above, whose five launches cost more than they save below it.
+constexpr int64_t kOneGroup = 32768;
+
+struct EvictPlan {
+  int64_t nch;
+  size_t hist, count, start, pick, cand, copy, total;
+};
+static EvictPlan evict_plan(const fbsa_evict_desc *d) {
+  EvictPlan p = {};
+  if (d->S <= kOneGroup) return p;
+  const size_t rows = (size_t)(d->B * d->H);
+  p.nch = (d->S + kChunk - 1) / kChunk;
+  p.hist = 0;
+  p.count = p.hist + rows * kBins * 4;
+  p.start = p.count + rows * p.nch * 8;
+  p.pick = p.start + rows * p.nch * 8;
+  p.cand = (p.pick + rows * 8 + 255) / 256 * 256;
+  p.copy = p.cand + rows * p.nch * kChunk * 4;
+  p.total = p.copy + (d->flags & FBSA_EVICT_IN_PLACE ? rows * p.nch * kChunk * 4 : 0);
+  return p;
 }
 
 // rows to other buffers: a 16-byte chunk of a key row and of its value row per thread
@@ -249,15 +568,13 @@ int fbsa_cache_append(const fbsa_append_desc *d, void *k, void *v, const void *k
   return hip_check(hipGetLastError(), "cache_append_kernel launch");
 }
 
-int fbsa_cache_evict(const fbsa_evict_desc *d, const void *k, const void *v, const float *weight, const int32_t *lens, void *k_out,
-                     void *v_out, float *w_out, int32_t *index, int32_t *new_lens, void *stream) {
+static int check_evict(const fbsa_evict_desc *d) {
   static const char *fn = "fbsa_cache_evict";
   if (!d) return fail(FBSA_EINVAL, "%s: null descriptor", fn);
   const int64_t(*const st[])[3] = {&d->sk, &d->sv, &d->sko, &d->svo};
   static const char *const name[] = {"k", "v", "k_out", "v_out"};
-  int e = check_rows(fn, d->dtype, d->D, st, name, 4);
+  const int e = check_rows(fn, d->dtype, d->D, st, name, 4);
   if (e) return e;
-  const bool inplace = d->flags & FBSA_EVICT_IN_PLACE;
   if (d->flags & ~FBSA_EVICT_IN_PLACE) return fail(FBSA_EINVAL, "%s: unknown flags 0x%x", fn, d->flags);
   if (d->B < 1 || d->H < 1 || d->S < 1 || d->budget < 1)
     return fail(FBSA_EINVAL, "%s: sizes must be positive (B=%lld H=%lld S=%lld budget=%lld)", fn, (long long)d->B, (long long)d->H,
@@ -269,6 +586,20 @@ int fbsa_cache_evict(const fbsa_evict_desc *d, const void *k, const void *v, con
   if (d->SO < ni) return fail(FBSA_EINVAL, "%s: output capacity %lld is below %lld", fn, (long long)d->SO, (long long)ni);
   if (d->S > kMaxRows || d->budget > kMaxRows || d->B > 65535 || d->H > 65535 || d->B * d->H > 65535)
     return fail(FBSA_EUNSUPPORTED, "%s: sizes exceed the grid or 32-bit row indices", fn);
+  return FBSA_OK;
+}
+
+size_t fbsa_cache_evict_workspace_bytes(const fbsa_evict_desc *d) { return check_evict(d) ? 0 : evict_plan(d).total; }
+
+int fbsa_cache_evict(const fbsa_evict_desc *d, const void *k, const void *v, const float *weight, const int32_t *lens, void *k_out,
+                     void *v_out, float *w_out, int32_t *index, int32_t *new_lens, void *workspace, size_t workspace_bytes,
+                     void *stream) {
+  static const char *fn = "fbsa_cache_evict";
+  int e = check_evict(d);
+  if (e) return e;
+  const bool inplace = d->flags & FBSA_EVICT_IN_PLACE;
+  const EvictPlan pl = evict_plan(d);
+  const int64_t ni = d->budget < d->S ? d->budget : d->S;
   if (!k || !v || !weight || !lens || !k_out || !v_out || !w_out || !index || !new_lens)
     return fail(FBSA_EINVAL, "%s: null tensor pointer", fn);
   if (!aligned_to(k, 16) || !aligned_to(v, 16) || !aligned_to(k_out, 16) || !aligned_to(v_out, 16) || !aligned_to(weight, 4) ||
@@ -282,6 +613,9 @@ int fbsa_cache_evict(const fbsa_evict_desc *d, const void *k, const void *v, con
   } else if (k == k_out || v == v_out || weight == w_out) {
     return fail(FBSA_EINVAL, "%s: outputs overlap inputs (FBSA_EVICT_IN_PLACE evicts in place)", fn);
   }
+  if (pl.total && (!workspace || workspace_bytes < pl.total))
+    return fail(FBSA_EWORKSPACE, "%s: workspace of %zu bytes, %zu needed", fn, workspace ? workspace_bytes : 0, pl.total);
+  if (pl.total && !aligned_to(workspace, 256)) return fail(FBSA_EINVAL, "%s: workspace must be 256-byte aligned", fn);
   const int64_t es = d->dtype == FBSA_F32 ? 4 : 2, cpr = d->D * es / 16;
   EvictArgs a = {};
   a.k = (const char *)k; a.v = (const char *)v; a.ko = (char *)k_out; a.vo = (char *)v_out; a.w = weight; a.wo = w_out;
@@ -294,8 +628,26 @@ int fbsa_cache_evict(const fbsa_evict_desc *d, const void *k, const void *v, con
   a.ni = (int)ni; a.cpr = (int)cpr;
   const hipStream_t s = (hipStream_t)stream;
   const unsigned rows = (unsigned)(d->B * d->H);
-  hipLaunchKernelGGL(evict_select_kernel, dim3(rows), dim3(kSelThreads), 0, s, a);
-  if ((e = hip_check(hipGetLastError(), "evict_select_kernel launch"))) return e;
+  if (d->S <= kOneGroup) {
+    const dim3 grid(rows), wg(kSelThreads);
+    if (d->S <= 2 * kSelThreads) hipLaunchKernelGGL(evict_select_kernel<2>, grid, wg, 0, s, a);
+    else if (d->S <= 8 * kSelThreads) hipLaunchKernelGGL(evict_select_kernel<8>, grid, wg, 0, s, a);
+    else if (d->S <= 16 * kSelThreads) hipLaunchKernelGGL(evict_select_kernel<16>, grid, wg, 0, s, a);
+    else hipLaunchKernelGGL(evict_select_kernel<32>, grid, wg, 0, s, a);
+    if ((e = hip_check(hipGetLastError(), "evict_select_kernel launch"))) return e;
+  } else {
+    char *p = (char *)workspace;
+    EvictWs ws = {(uint32_t *)(p + pl.hist), (uint32_t *)(p + pl.cand), inplace ? (float *)(p + pl.copy) : nullptr, (uint2 *)(p + pl.count),
+                  (uint2 *)(p + pl.start), (uint2 *)(p + pl.pick), (int)pl.nch};
+    const dim3 grid((unsigned)pl.nch, rows), wg(kSelThreads);
+    const int64_t nz = (int64_t)rows * kBins;
+    hipLaunchKernelGGL(evict_zero_kernel, dim3((unsigned)((nz + 255) / 256)), dim3(256), 0, s, ws.hist, nz);
+    hipLaunchKernelGGL(evict_hist_kernel, grid, wg, 0, s, a, ws);
+    hipLaunchKernelGGL(evict_cand_kernel, grid, wg, 0, s, a, ws);
+    hipLaunchKernelGGL(evict_rank_kernel, dim3(rows), wg, 0, s, a, ws);
+    hipLaunchKernelGGL(evict_place_kernel, grid, wg, 0, s, a, ws);
+    if ((e = hip_check(hipGetLastError(), "evict kernels launch"))) return e;
+  }
   if (inplace)
     hipLaunchKernelGGL(evict_move_kernel, dim3((unsigned)((cpr + 3) / 4), 2, rows), dim3(256), 0, s, a);
   else

@@ -136,7 +136,8 @@ SIGNATURES = {
     "fbsa_cache_append": (ctypes.c_int, [ctypes.POINTER(AppendDesc)] + [_vp] * 8),
     "fbsa_cache_attn_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(CacheDesc)]),
     "fbsa_cache_attn": (ctypes.c_int, [ctypes.POINTER(CacheDesc)] + [_vp] * 13 + [ctypes.c_size_t, _vp]),
-    "fbsa_cache_evict": (ctypes.c_int, [ctypes.POINTER(EvictDesc)] + [_vp] * 10),
+    "fbsa_cache_evict_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(EvictDesc)]),
+    "fbsa_cache_evict": (ctypes.c_int, [ctypes.POINTER(EvictDesc)] + [_vp] * 10 + [ctypes.c_size_t, _vp]),
 }
 
 _lib = None

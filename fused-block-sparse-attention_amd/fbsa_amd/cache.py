@@ -274,9 +274,12 @@ def evict(k, v, weight, lens, budget, *, recent=0, sink=0, out=None):
     d.B, d.H, d.S, d.SO, d.D, d.budget, d.recent, d.sink = B, H, S, SO, D, budget, recent, sink
     d.sk[:], d.sv[:], d.sko[:], d.svo[:] = _strides(k, 3), _strides(v, 3), _strides(ko, 3), _strides(vo, 3)
     d.sw[:], d.swo[:] = _strides(weight, 2), _strides(wo, 2)
+    lib = _lib.load()
     with torch.cuda.device(k.device):
-        _lib.check(_lib.load().fbsa_cache_evict(d, _ptr(k), _ptr(v), _ptr(weight), _ptr(lens), _ptr(ko), _ptr(vo), _ptr(wo),
-                                                _ptr(index), _ptr(new_lens), _stream()), "fbsa_cache_evict")
+        nbytes = lib.fbsa_cache_evict_workspace_bytes(d)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=k.device) if nbytes else None
+        _lib.check(lib.fbsa_cache_evict(d, _ptr(k), _ptr(v), _ptr(weight), _ptr(lens), _ptr(ko), _ptr(vo), _ptr(wo), _ptr(index),
+                                        _ptr(new_lens), _ptr(ws), nbytes, _stream()), "fbsa_cache_evict")
     return index, new_lens
 
 

@@ -402,7 +402,10 @@ int fbsa_cache_attn(const fbsa_cache_desc *d, const void *q, const void *k, cons
  * min(budget, S), whose rows past new_lens[b] are left as they were; none of
  * them may overlap k, v or weight, except with FBSA_EVICT_IN_PLACE, where they
  * are k, v and weight themselves (same pointers, strides and SO = S). lens and
- * new_lens may be the same array in neither case. */
+ * new_lens may be the same array in neither case. The workspace (256-byte aligned)
+ * may be NULL where fbsa_cache_evict_workspace_bytes returns 0, as it does for
+ * capacities up to 32768 (and, with fbsa_last_error set, for a descriptor that
+ * fbsa_cache_evict refuses). */
 enum { FBSA_EVICT_IN_PLACE = 1 };
 
 typedef struct fbsa_evict_desc {
@@ -412,9 +415,10 @@ typedef struct fbsa_evict_desc {
   int64_t sw[2], swo[2];                    /* weight, w_out: {b, h} */
 } fbsa_evict_desc;
 
+size_t fbsa_cache_evict_workspace_bytes(const fbsa_evict_desc *d);
 int fbsa_cache_evict(const fbsa_evict_desc *d, const void *k, const void *v, const float *weight,
                      const int32_t *lens, void *k_out, void *v_out, float *w_out, int32_t *index,
-                     int32_t *new_lens, void *stream);
+                     int32_t *new_lens, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -82,15 +82,21 @@ def _evict(**kw):
 ])
 def test_evict_descriptor(kw, needle):
     p = [DUMMY * i for i in range(1, 9)]
-    assert _lib.load().fbsa_cache_evict(_evict(**kw), *p[:4], *p[4:], DUMMY * 9, None) in (_lib.EINVAL, _lib.EUNSUPPORTED)
+    assert _lib.load().fbsa_cache_evict(_evict(**kw), *p[:4], *p[4:], DUMMY * 9, None, 0, None) in (_lib.EINVAL, _lib.EUNSUPPORTED)
     assert needle in _lib.load().fbsa_last_error().decode()
 
 
 def test_evict_pointers():
     lib, p = _lib.load(), [DUMMY * i for i in range(1, 10)]
-    assert lib.fbsa_cache_evict(_evict(), *p[:3], None, *p[4:], None) == _lib.EINVAL
-    assert lib.fbsa_cache_evict(_evict(), *p[:4], p[0], *p[5:], None) == _lib.EINVAL and b"overlap" in lib.fbsa_last_error()
-    assert lib.fbsa_cache_evict(_evict(), *p[:8], p[3], None) == _lib.EINVAL and b"new_lens" in lib.fbsa_last_error()
+    assert lib.fbsa_cache_evict(_evict(), *p[:3], None, *p[4:], None, 0, None) == _lib.EINVAL
+    assert lib.fbsa_cache_evict(_evict(), *p[:4], p[0], *p[5:], None, 0, None) == _lib.EINVAL and b"overlap" in lib.fbsa_last_error()
+    assert lib.fbsa_cache_evict(_evict(), *p[:8], p[3], None, 0, None) == _lib.EINVAL and b"new_lens" in lib.fbsa_last_error()
+    assert lib.fbsa_cache_evict_workspace_bytes(_evict()) == 0
+    d = _evict(S=40000)
+    need = lib.fbsa_cache_evict_workspace_bytes(d)
+    assert need > 0 and lib.fbsa_cache_evict(d, *p, DUMMY, need - 1, None) == _lib.EWORKSPACE
+    assert lib.fbsa_cache_evict(d, *p, None, 0, None) == _lib.EWORKSPACE
+    assert lib.fbsa_cache_evict(d, *p, DUMMY + 16, need, None) == _lib.EINVAL
 
 
 @pytest.mark.parametrize("kw,needle", [({"T": 0}, "positive"), ({"D": 12}, "head dim"), ({"flags": 1}, "flags"),

@@ -250,8 +250,16 @@ def test_evict_types_and_widths(inplace, dt, D):
 
 
 @pytest.mark.parametrize("inplace", [False, True])
-def test_evict_long(inplace):
-    _evict_case("bf16", 1, 2, 70001, 32, [70001], 20000, 512, 4, "ties", inplace)
+@pytest.mark.parametrize("kind", ["random", "ties", "equal", "odd"])
+@pytest.mark.parametrize("budget,recent,sink", [(20000, 512, 4), (9000, 8500, 500), (69999, 0, 0), (8, 0, 8)])
+def test_evict_long(inplace, kind, budget, recent, sink):
+    _evict_case("bf16", 3, 2, 70001, 16, [70001, 33000, 8192], budget, recent, sink, kind, inplace)
+
+
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("S", [2048, 8192, 16384, 32768])
+def test_evict_at_each_register_count(inplace, S):
+    _evict_case("fp16", 2, 1, S, 16, [S, S - 1], S // 3, 100, 4, "ties", inplace)
 
 
 def test_evict_lengths_past_the_capacity():
