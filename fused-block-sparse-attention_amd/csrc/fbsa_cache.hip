@@ -16,13 +16,18 @@
 //            softmax in the log2 domain; leaves unnormalised fp32 O, row
 //            maximum and row sum
 //   combine  a row's parts joined in a fixed order; O, lse
-//   weight   a wave per 32 keys over all rows, p recomputed from the final lse
+//   tile     many rows: a workgroup per (64- or 128-row tile, share of the keys)
+//   weight   a workgroup per 128 keys over many rows, scores formed again
 // Lengths are read on the device; nothing depends on launch order.
 #include <math.h>
 
 #include "fbsa_common.h"
 #include "fbsa_internal.h"
 #include "fbsa_tiles.h"
+
+#ifndef FBSA_CT_NW
+#define FBSA_CT_NW 8
+#endif
 
 namespace fbsa {
 
@@ -41,9 +46,11 @@ struct CacheArgs {
   int32_t np_own, np_pre;    // shares of a tile's keys
   int32_t few_own, few_pre;  // tiles of 16 rows, a wave each
   int32_t direct;            // a tile's one share is its whole answer: no parts
-  float scale2;              // scale * log2(e)
+  float scale2;              // |scale| * log2(e); the sign is the query's (zero: queries of zeros, scale 1)
+  uint32_t qand, qxor;       // applied to the query's words
   float *part;               // [tile, share][row] unnormalised O (DP floats): prefix tiles, then own
   float2 *stat;              // [tile, share][row] row maximum (log2 domain), row sum
+  float *wpart;              // [row share][B][Hkv][S] weights, where the rows are shared out
   float *lse2;               // [B][Hkv][TG] log2-domain lse, -inf for rows that see nothing
   float *sc;                 // [B][Hkv][TG][S rounded up to 32] log2-domain scores (few_own, with weights)
 };
@@ -56,7 +63,6 @@ template <typename T, int DP> struct CacheCfg {
   static constexpr int TILE = KC * DP * ES;
   static constexpr int LPT = KC * CPR / 64;  // 16-byte loads per lane and tile
   static constexpr int NST = 2;
-  static_assert(LPT * 64 == KC * CPR, "tile must be whole wave-loads");
 };
 
 // Row rho of a (sequence, KV head): token rho / G, head rho % G. The keys it
@@ -84,39 +90,100 @@ __device__ __forceinline__ RowInfo row_info(const CacheArgs &a, int b, int hk, i
 }
 
 template <typename T, int DP>
-__device__ __forceinline__ void load_frag(RowFrag<T, DP> &fr, const T *row, int g, int D) {
+__device__ __forceinline__ void load_frag(RowFrag<T, DP> &fr, const T *row, int g, const CacheArgs &a) {
   // (elements past the head dim are zeros: the tile's columns there hold copies of the row's last chunk)
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int ks = 0; ks < DP / 4; ++ks) fr.f[ks] = 4 * ks + g < D ? ((const float *)row)[4 * ks + g] : 0.f;
+    for (int ks = 0; ks < DP / 4; ++ks) {
+      const uint32_t x = 4 * ks + g < a.D ? ((const uint32_t *)row)[4 * ks + g] : 0u;
+      fr.f[ks] = __uint_as_float((x & a.qand) ^ a.qxor);
+    }
   } else {
 #pragma unroll
-    for (int ks = 0; ks < DP / 32; ++ks)
-      fr.h[ks] = 32 * ks + 8 * g < D ? *(const s16x8 *)(row + 32 * ks + 8 * g) : s16x8{0, 0, 0, 0, 0, 0, 0, 0};
+    for (int ks = 0; ks < DP / 32; ++ks) {
+      u32x4 x = 32 * ks + 8 * g < a.D ? *(const u32x4 *)(row + 32 * ks + 8 * g) : u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = (x[e] & a.qand) ^ a.qxor;
+      fr.h[ks] = __builtin_bit_cast(s16x8, x);
+    }
   }
 }
 
-// Per-lane byte offsets of a wave's copy of a KC-row tile (swizzled chunks);
+// Per-lane byte offsets of a copy of a KC-row tile (swizzled chunks) by NW waves;
 // columns past the head dim read the row's last chunk.
-template <typename T, int DP> struct TilePlan {
-  using C = CacheCfg<T, DP>;
-  uint32_t off[C::LPT];
-  __device__ __forceinline__ void init(int64_t stride, int D, int lane) {
-    const int last = D * C::ES / 16 - 1;
+template <typename T, int DP, int KC, int NW> struct TilePlan {
+  static constexpr int ES = sizeof(T), CPR = DP * ES / 16, LPT = KC * CPR / (64 * NW);
+  static_assert(LPT * 64 * NW == KC * CPR, "a tile is whole loads of every wave");
+  uint32_t off[LPT];
+  __device__ __forceinline__ void init(int64_t stride, int D, int w, int lane) {
+    const int last = D * ES / 16 - 1;
 #pragma unroll
-    for (int n = 0; n < C::LPT; ++n) {
-      const int u = n * 64 + lane, row = u / C::CPR, c = (u % C::CPR) ^ swz(row, C::CPR);
-      off[n] = (uint32_t)(((int64_t)row * stride) * C::ES + (c < last ? c : last) * 16);
+    for (int n = 0; n < LPT; ++n) {
+      const int u = (n * NW + w) * 64 + lane, row = u / CPR, c = (u % CPR) ^ swz(row, CPR);
+      off[n] = (uint32_t)(((int64_t)row * stride) * ES + (c < last ? c : last) * 16);
     }
   }
   // rows [row0, ...) of a tensor of `rows` rows: rows past the end read its last one
-  __device__ __forceinline__ void issue(unsigned st, const char *base, uint32_t row0, uint32_t rows, int64_t step, int rowbytes) const {
+  __device__ __forceinline__ void issue(unsigned st, const char *base, uint32_t row0, uint32_t rows, int64_t step, int rowbytes, int w) const {
     const char *src = base + (int64_t)row0 * step;
-    const uint32_t lim = tail_limit<C::KC>(row0, rows, (uint32_t)step, (uint32_t)rowbytes);
+    const uint32_t lim = tail_limit<KC>(row0, rows, (uint32_t)step, (uint32_t)rowbytes);
 #pragma unroll
-    for (int n = 0; n < C::LPT; ++n) g2lds16_s(src, off[n] > lim ? lim : off[n], st + n * 1024);
+    for (int n = 0; n < LPT; ++n) g2lds16_s(src, off[n] > lim ? lim : off[n], st + (n * NW + w) * 1024);
   }
 };
+
+// A wave's online softmax over 16 rows (one to a lane column, 4 lanes to a row).
+// The running reference moves only when a score passes it by 2^TAU, so few
+// chunks rescale the accumulators.
+template <int DP> struct SoftmaxState {
+  static constexpr float TAU = 8.f;
+  float m = -INFINITY, l = 0.f;
+  f32x4 o[DP / 16];
+  __device__ __forceinline__ void init() {
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  // s: raw products (scaled by scale2 > 0 here), masked ones -inf; out: exponentials
+  template <int NM> __device__ __forceinline__ void step(const f32x4 (&s)[NM], float scale2, float (&x)[NM][4]) {
+    float mx = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < NM; ++k) mx = fmaxf(mx, fmaxf(fmaxf(s[k][0], s[k][1]), fmaxf(s[k][2], s[k][3])));
+    mx *= scale2;
+    if (__ballot(mx > m + TAU)) {
+      float mc = fmaxf(mx, shfl_xor_f(mx, 16));
+      mc = fmaxf(mc, shfl_xor_f(mc, 32));
+      if (mc > m + TAU) {
+        const float alpha = __builtin_amdgcn_exp2f(m - mc);
+        l *= alpha;
+#pragma unroll
+        for (int t = 0; t < DP / 16; ++t) o[t] *= alpha;
+        m = mc;
+      }
+    }
+    const float ref = m == -INFINITY ? 0.f : m;
+    float sum = 0.f;
+#pragma unroll
+    for (int k = 0; k < NM; ++k)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        x[k][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k][r], scale2, -ref));
+        sum += x[k][r];
+      }
+    l += sum;
+  }
+  __device__ __forceinline__ float total() const {  // the row's sum, on its four lanes
+    const float lt = l + shfl_xor_f(l, 16);
+    return lt + shfl_xor_f(lt, 32);
+  }
+};
+// keys at or past lim (counted from the chunk's first) drop out of the softmax
+template <int NM> __device__ __forceinline__ void mask_keys(f32x4 (&s)[NM], int lim, int g) {
+#pragma unroll
+  for (int m = 0; m < NM; ++m)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (16 * m + 4 * g + r >= lim) s[m][r] = -INFINITY;
+}
 
 // o[d .. d + 3] = acc * inv [* sigmoid(gate)] of a row
 template <typename T> __device__ __forceinline__ void store_row(const CacheArgs &a, const RowInfo &ri, f32x4 acc, float inv, int d) {
@@ -204,22 +271,18 @@ template <typename T, int DP> __global__ __launch_bounds__(64) void cache_part_k
   const int c0 = (int)(nc * split / np), c1 = (int)(nc * (split + 1) / np);
 
   RowFrag<T, DP> fr;
-  load_frag<T, DP>(fr, (const T *)a.q + ri.b * a.sq[0] + ri.hq * a.sq[1] + ri.t * a.sq[2], g, a.D);
-  TilePlan<T, DP> pk, pv;
-  pk.init(kstep / C::ES, a.D, lane);
-  pv.init(vstep / C::ES, a.D, lane);
+  load_frag<T, DP>(fr, (const T *)a.q + ri.b * a.sq[0] + ri.hq * a.sq[1] + ri.t * a.sq[2], g, a);
+  TilePlan<T, DP, KC, 1> pk, pv;
+  pk.init(kstep / C::ES, a.D, 0, lane);
+  pv.init(vstep / C::ES, a.D, 0, lane);
   auto issue = [&](int c) {
     const unsigned st = (unsigned)(uintptr_t)smem + (c % C::NST) * 2 * C::TILE;
-    pk.issue(st, kb, (uint32_t)c * KC, keys, kstep, a.D * C::ES);
-    pv.issue(st + C::TILE, vb, (uint32_t)c * KC, keys, vstep, a.D * C::ES);
+    pk.issue(st, kb, (uint32_t)c * KC, keys, kstep, a.D * C::ES, 0);
+    pv.issue(st + C::TILE, vb, (uint32_t)c * KC, keys, vstep, a.D * C::ES, 0);
   };
 
-  constexpr float TAU = 8.f;  // the running reference moves when a score passes it by 2^TAU
-  float m_run = -INFINITY, l_run = 0.f;
-  f32x4 oacc[DP / 16];
-#pragma unroll
-  for (int t = 0; t < DP / 16; ++t) oacc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-
+  SoftmaxState<DP> sm;
+  sm.init();
   for (int c = c0; c < c0 + C::NST - 1 && c < c1; ++c) issue(c);
   wait_vmcnt<0>();  // the query rows too: the compiler then waits for nothing in the loop
   for (int c = c0; c < c1; ++c) {
@@ -230,53 +293,253 @@ template <typename T, int DP> __global__ __launch_bounds__(64) void cache_part_k
     const char *Ks = smem + (c % C::NST) * 2 * C::TILE, *Vs = Ks + C::TILE;
     f32x4 s[NM];
     mm_rows_frag<T, DP, NM>(Ks, fr, s, g, p);
-#pragma unroll
-    for (int m = 0; m < NM; ++m) s[m] *= a.scale2;
-    if ((c + 1) * (int64_t)KC > low) {
-      const int lm = lim - c * KC - 4 * g;
-#pragma unroll
-      for (int m = 0; m < NM; ++m)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (16 * m + r >= lm) s[m][r] = -INFINITY;
-    }
+    if ((c + 1) * (int64_t)KC > low) mask_keys<NM>(s, lim - c * KC, g);
     if (score && ri.valid) {
 #pragma unroll
-      for (int m = 0; m < NM; ++m) *(f32x4 *)(score + (int64_t)c * KC + 16 * m + 4 * g) = s[m];
+      for (int m = 0; m < NM; ++m) *(f32x4 *)(score + (int64_t)c * KC + 16 * m + 4 * g) = s[m] * a.scale2;
     }
-    float mx = -INFINITY;
-#pragma unroll
-    for (int m = 0; m < NM; ++m) mx = fmaxf(mx, fmaxf(fmaxf(s[m][0], s[m][1]), fmaxf(s[m][2], s[m][3])));
-    if (__ballot(mx > m_run + TAU)) {
-      float mc = fmaxf(mx, shfl_xor_f(mx, 16));
-      mc = fmaxf(mc, shfl_xor_f(mc, 32));
-      if (mc > m_run + TAU) {
-        const float alpha = __builtin_amdgcn_exp2f(m_run - mc);
-        l_run *= alpha;
-#pragma unroll
-        for (int t = 0; t < DP / 16; ++t) oacc[t] *= alpha;
-        m_run = mc;
-      }
-    }
-    const float ref = m_run == -INFINITY ? 0.f : m_run;
     float x[NM][4];
-#pragma unroll
-    for (int m = 0; m < NM; ++m)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        x[m][r] = __builtin_amdgcn_exp2f(s[m][r] - ref);
-        l_run += x[m][r];
-      }
-    mm_tr_acc<T, DP, KC, 0, sizeof(T) == 2>(Vs, x, oacc, g, p);
+    sm.template step<NM>(s, a.scale2, x);
+    mm_tr_acc<T, DP, KC, 0, sizeof(T) == 2>(Vs, x, sm.o, g, p);
   }
 
-  float lt = l_run + shfl_xor_f(l_run, 16);
-  lt += shfl_xor_f(lt, 32);
-  if (g == 0) a.stat[slot + p] = float2{m_run, lt};
+  const float lt = sm.total();
+  if (g == 0) a.stat[slot + p] = float2{sm.m, lt};
   if (ri.valid && lt != 0.f) {  // (a NaN sum is kept)
     float *dst = a.part + (slot + p) * DP;
 #pragma unroll
-    for (int t = 0; t < DP / 16; ++t) *(f32x4 *)(dst + 16 * t + 4 * g) = oacc[t];
+    for (int t = 0; t < DP / 16; ++t) *(f32x4 *)(dst + 16 * t + 4 * g) = sm.o[t];
+  }
+}
+
+// ---- many rows: a workgroup per (tile of NW x 16 QT rows, share of the keys).
+// The K and V chunks are shared through a ring in LDS; each wave owns QT
+// 16-row fragments, and a fragment of K or V read from LDS feeds QT products.
+// P enters the value product rounded to the operand type (as in the block-sparse
+// forward; the row sums are of the unrounded values): the second product of a
+// split operand would cost half as much again where the matrix units are what
+// bounds the kernel.
+template <typename T, int DP, int QT, int NM>
+__device__ __forceinline__ void qk_tile(const char *tile, const RowFrag<T, DP> (&fr)[QT], f32x4 (&acc)[QT][NM], int g, int p) {
+  constexpr int CPR = DP * (int)sizeof(T) / 16;
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+    for (int m = 0; m < NM; ++m) acc[qt][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  if constexpr (sizeof(T) == 2) {
+    constexpr int KS = DP / 32, NK = NM * KS, KL = KS < 4 ? KS : 4, W = NK < 8 ? NK : 8;
+    unsigned kb[KL];
+#pragma unroll
+    for (int l = 0; l < KL; ++l) kb[l] = (unsigned)(uintptr_t)tile + tile_kbase(l, g, p, CPR);
+    s16x8 x[NK];
+    auto rd = [&](auto K) {
+      constexpr int k = decltype(K)::value, m = k / KS, ks = k % KS;
+      x[k] = lds_read_b128_at<(ks / 4) * 256 + m * 256 * CPR>(kb[ks % 4]);
+    };
+    static_for<W>(rd);
+    static_for<NK>([&](auto K) {
+      constexpr int k = decltype(K)::value;
+      constexpr int last = k + W - 1 < NK - 1 ? k + W - 1 : NK - 1;  // last read issued so far
+      lds_wait_le<last - k>();
+      lds_ready(x[k]);
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) acc[qt][k / KS] = Mfma16<T>::run(x[k], fr[qt].h[k % KS], acc[qt][k / KS]);
+      if constexpr (k + W < NK) rd(std::integral_constant<int, k + W>{});
+    });
+  } else {
+#pragma unroll
+    for (int m = 0; m < NM; ++m) {
+      const int row = 16 * m + p;
+#pragma unroll
+      for (int ks = 0; ks < DP / 4; ++ks) {
+        const float x = *(const float *)(tile + (row * CPR + (ks ^ swz(row, CPR))) * 16 + g * 4);
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) acc[qt][m] = mfma_f32_16x16x4(x, fr[qt].f[ks], acc[qt][m]);
+        if constexpr (DP >= 256) if (ks % 16 == 15) asm volatile("" ::: "memory");  // at most 16 loads ahead
+      }
+      if constexpr (DP >= 128) asm volatile("" ::: "memory");
+    }
+  }
+}
+template <typename T, int DP, int KC, int QT>
+__device__ __forceinline__ void pv_tile(const char *tile, const float (&x)[QT][KC / 16][4], SoftmaxState<DP> (&sm)[QT], int g, int p) {
+  constexpr int CPR = DP * (int)sizeof(T) / 16;
+  if constexpr (sizeof(T) == 2) {
+    constexpr int K2 = KC / 32, NTL = DP / 16, VL = NTL < 8 ? NTL : 8, RPT = 2 * K2, W = NTL < 4 ? NTL : 4;
+    s16x8 pk[QT][K2];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+      for (int k2 = 0; k2 < K2; ++k2) {
+        float y[8];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) { y[r] = x[qt][2 * k2][r]; y[4 + r] = x[qt][2 * k2 + 1][r]; }
+        pk[qt][k2] = pack8<T>(y);
+      }
+    s16x4 lo[NTL][K2], hi[NTL][K2];
+    unsigned vb[VL];
+#pragma unroll
+    for (int l = 0; l < VL; ++l) vb[l] = (unsigned)(uintptr_t)tile + tile_vbase(l, g, p, CPR);
+    auto rd = [&](auto TT) {
+      constexpr int t = decltype(TT)::value;
+      static_for<K2>([&](auto KK) {
+        constexpr int k2 = decltype(KK)::value, off = (t / 8) * 256 + k2 * 512 * CPR;
+        lo[t][k2] = lds_read_tr16_at<off>(vb[t % 8]);
+        hi[t][k2] = lds_read_tr16_at<off + 256 * CPR>(vb[t % 8]);
+      });
+    };
+    static_for<W>(rd);
+    static_for<NTL>([&](auto TT) {
+      constexpr int t = decltype(TT)::value;
+      constexpr int last = t + W - 1 < NTL - 1 ? t + W - 1 : NTL - 1, n = (last - t) * RPT;
+      lds_wait_le<(n < 15 ? n : 15)>();
+#pragma unroll
+      for (int k2 = 0; k2 < K2; ++k2) {
+        lds_ready(lo[t][k2]);
+        lds_ready(hi[t][k2]);
+        const s16x4 a = lo[t][k2], b = hi[t][k2];
+        const s16x8 av = s16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) sm[qt].o[t] = Mfma16<T>::run(av, pk[qt][k2], sm[qt].o[t]);
+      }
+      if constexpr (t + W < NTL) rd(std::integral_constant<int, t + W>{});
+    });
+  } else {
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) mm_tr_acc<T, DP, KC>(tile, x[qt], sm[qt].o, g, p);
+  }
+}
+
+template <typename T, int DP, int NW, int QT, int KC, int NST> struct TileCfg {
+  static constexpr int ES = sizeof(T), ROWS = NW * 16 * QT, TILE = KC * DP * ES, LDS = NST * 2 * TILE;
+  static_assert(LDS <= 160 * 1024 - 64, "LDS");
+};
+
+template <typename T, int DP, int NW, int QT, int KC, int NST>
+__global__ __launch_bounds__(NW * 64) void cache_tile_kernel(CacheArgs a, int64_t npre) {
+  using C = TileCfg<T, DP, NW, QT, KC, NST>;
+  constexpr int NM = KC / 16;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, p = lane & 15;
+  const bool pre = blockIdx.x < npre;
+  RowInfo ri[QT];
+  int64_t slot;  // the tile's first row among the parts
+  int split, np, keys;
+  const char *kb, *vb;
+  int64_t kstep, vstep;
+  if (pre) {
+    // (the tiles that share a share's keys run together on one XCD)
+    const uint32_t id = (uint32_t)xcd_remap(blockIdx.x, npre);
+    const int tile = id % a.rt_pre, hk = id / a.rt_pre / a.np_pre;
+    split = id / a.rt_pre % a.np_pre;
+    np = a.np_pre;
+    const int64_t rows = (int64_t)a.B * a.TG;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      const int64_t rho = (int64_t)tile * C::ROWS + (w * QT + qt) * 16 + p, x = rho < rows ? rho : 0;
+      ri[qt] = row_info(a, (int)(x / a.TG), hk, (int)(x % a.TG));
+      ri[qt].valid = ri[qt].valid && rho < rows;
+      ri[qt].lim = a.P;
+    }
+    keys = a.P;
+    slot = (((int64_t)hk * a.rt_pre + tile) * np + split) * C::ROWS;
+    kstep = a.skp[1] * C::ES;
+    vstep = a.svp[1] * C::ES;
+    kb = (const char *)a.kp + hk * a.skp[0] * C::ES;
+    vb = (const char *)a.vp + hk * a.svp[0] * C::ES;
+  } else {
+    // (the last tokens' tiles see the most keys: they start first)
+    const uint32_t id = blockIdx.x - (uint32_t)npre, per = (uint32_t)(a.Hkv * a.np_own * a.B), u = id % per;
+    const int tile = a.rt_own - 1 - (int)(id / per), hk = u / a.np_own % a.Hkv, b = u / a.np_own / a.Hkv;
+    split = u % a.np_own;
+    np = a.np_own;
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) ri[qt] = row_info(a, b, hk, tile * C::ROWS + (w * QT + qt) * 16 + p);
+    // the last real row of the tile sees the most keys
+    const int cnt = seq_count(a, b), t0 = tile * C::ROWS / a.G, t1 = min(min(tile * C::ROWS + C::ROWS, a.TG) - 1, cnt * a.G - 1) / a.G;
+    const int n = seq_len(a, b);
+    const int64_t most = (int64_t)n - cnt + t1 + 1;
+    keys = t0 >= cnt ? 0 : (int)(most < 0 ? 0 : most);
+    slot = own_slot(a) + ((((int64_t)b * a.Hkv + hk) * a.rt_own + tile) * np + split) * C::ROWS;
+    kstep = a.sk[2] * C::ES;
+    vstep = a.sv[2] * C::ES;
+    kb = (const char *)a.k + (b * a.sk[0] + hk * a.sk[1]) * C::ES;
+    vb = (const char *)a.v + (b * a.sv[0] + hk * a.sv[1]) * C::ES;
+  }
+  keys = __builtin_amdgcn_readfirstlane(keys);
+  int low = 0x7fffffff;  // below it every row of the wave sees every key
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) low = min(low, ri[qt].valid ? ri[qt].lim : 0x7fffffff);
+#pragma unroll
+  for (int x = 1; x < 16; x <<= 1) low = min(low, __shfl_xor(low, x, 64));
+  low = __builtin_amdgcn_readfirstlane(low);
+  low = min(low, keys);
+  const int64_t nc = ((int64_t)keys + KC - 1) / KC;
+  const int c0 = (int)(nc * split / np), c1 = (int)(nc * (split + 1) / np);
+
+  RowFrag<T, DP> fr[QT];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt)
+    load_frag<T, DP>(fr[qt], (const T *)a.q + ri[qt].b * a.sq[0] + ri[qt].hq * a.sq[1] + ri[qt].t * a.sq[2], g, a);
+  TilePlan<T, DP, KC, NW> pk, pv;
+  pk.init(kstep / C::ES, a.D, w, lane);
+  pv.init(vstep / C::ES, a.D, w, lane);
+  int ist = 0, cst = 0;  // ring places to fill and to read
+  auto issue = [&](int c) {
+    const unsigned st = (unsigned)(uintptr_t)smem + ist * 2 * C::TILE;
+    pk.issue(st, kb, (uint32_t)c * KC, keys, kstep, a.D * C::ES, w);
+    pv.issue(st + C::TILE, vb, (uint32_t)c * KC, keys, vstep, a.D * C::ES, w);
+    ist = ist + 1 == NST ? 0 : ist + 1;
+  };
+  SoftmaxState<DP> sm[QT];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) sm[qt].init();
+
+  for (int c = c0; c < c0 + NST - 1 && c < c1; ++c) issue(c);
+  wait_vmcnt<0>();  // the query rows too: the compiler then waits for nothing in the loop
+  for (int c = c0; c < c1; ++c) {
+    const int ahead = c1 - 1 - c;
+    wait_ring<2 * decltype(pk)::LPT>(ahead < NST - 2 ? ahead : NST - 2);
+    // every wave's part of chunk c has landed, and every wave has read chunk c - 1, whose place is filled next
+    lds_barrier();
+    if (c + NST - 1 < c1) issue(c + NST - 1);
+    const char *Ks = smem + cst * 2 * C::TILE, *Vs = Ks + C::TILE;
+    cst = cst + 1 == NST ? 0 : cst + 1;
+    f32x4 s[QT][NM];
+    qk_tile<T, DP, QT, NM>(Ks, fr, s, g, p);
+    if ((c + 1) * (int64_t)KC > low) {
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) mask_keys<NM>(s[qt], (ri[qt].valid ? ri[qt].lim : keys) - c * KC, g);
+    }
+    float x[QT][NM][4];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) sm[qt].template step<NM>(s[qt], a.scale2, x[qt]);
+    pv_tile<T, DP, KC, QT>(Vs, x, sm, g, p);
+  }
+
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) {
+    const int i = (w * QT + qt) * 16 + p;
+    const float lt = sm[qt].total();
+    if (!pre && a.direct) {
+      const int rho = (a.rt_own - 1 - (int)((blockIdx.x - (uint32_t)npre) / (uint32_t)(a.Hkv * a.np_own * a.B))) * C::ROWS + i;
+      if (rho >= a.TG) continue;
+      const float l = ri[qt].valid ? lt : 0.f, inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+      for (int t = 0; t < DP / 16; ++t) store_row<T>(a, ri[qt], ri[qt].valid ? sm[qt].o[t] : f32x4{0.f, 0.f, 0.f, 0.f}, inv, 16 * t + 4 * g);
+      if (g == 0) {
+        const float l2 = l == 0.f ? -INFINITY : sm[qt].m + __log2f(l);
+        if (a.lse) a.lse[((int64_t)ri[qt].b * a.Hq + ri[qt].hq) * a.T + ri[qt].t] = l2 * kLn2;
+        if (a.lse2) a.lse2[((int64_t)ri[qt].b * a.Hkv + ri[qt].hq / a.G) * a.TG + rho] = l2;
+      }
+      continue;
+    }
+    if (g == 0) a.stat[slot + i] = float2{sm[qt].m, lt};
+    if (ri[qt].valid && lt != 0.f) {  // (a NaN sum is kept)
+      float *dst = a.part + (slot + i) * DP;
+#pragma unroll
+      for (int t = 0; t < DP / 16; ++t) *(f32x4 *)(dst + 16 * t + 4 * g) = sm[qt].o[t];
+    }
   }
 }
 
@@ -409,55 +672,153 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void cache_combi
   }
 }
 
-// A wave per KC keys of a (sequence, KV head) over every row that sees them.
-template <typename T, int DP> __global__ __launch_bounds__(64) void cache_weight_kernel(CacheArgs a) {
-  using C = CacheCfg<T, DP>;
-  constexpr int KC = C::KC, NM = KC / 16;
-  extern __shared__ __attribute__((aligned(16))) char tile[];
-  const int lane = threadIdx.x, g = lane >> 4, p = lane & 15;
+// ---- weights of many rows: p = exp2(score - lse) summed over the rows that see a
+// key, scores formed again. A workgroup per 128 keys of a (sequence, KV head) and
+// share of its rows: the keys stay in registers (32 to a wave, B operands), the
+// query rows stream through a ring in LDS, 64 to a chunk, of which waves 0-3 take
+// the first half and waves 4-7 the second. A lane holds one column, a key, of the
+// product, so the sum over rows is a register each. Row rho is token rho / G;
+// key j is seen by the rows from G * (j - (len - count)) on.
+template <typename T, int DP> struct WeightCfg {
+  static constexpr int ES = sizeof(T), ROWS = 64, KEYS = 128, NT = 512, CPR = DP * ES / 16;
+  static constexpr int LPT = ROWS * CPR / NT;        // 16-byte loads per thread and chunk (0: fewer than the threads)
+  static constexpr int STAGE = ROWS * DP * ES + ROWS * 4;
+  static constexpr int NST = 2, LDS = NST * STAGE;
+  static constexpr int NL = LPT ? LPT : 1;
+};
+template <typename T, int DP> __global__ __launch_bounds__(512) void cache_weight_kernel(CacheArgs a) {
+  using C = WeightCfg<T, DP>;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  __shared__ float s_sum[4][32];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, p = lane & 15;
+  const int kg = w & 3, half = w >> 2;
   const int hk = blockIdx.y % a.Hkv, b = blockIdx.y / a.Hkv;
-  const int n = seq_len(a, b);
-  const int64_t key64 = (int64_t)blockIdx.x * KC;
-  if (key64 >= n) return;
-  const int key0 = (int)key64;
-  TilePlan<T, DP> pk;
-  pk.init(a.sk[2], a.D, lane);
-  pk.issue((unsigned)(uintptr_t)tile, (const char *)a.k + (b * a.sk[0] + hk * a.sk[1]) * C::ES, (uint32_t)key0, n,
-           a.sk[2] * C::ES, a.D * C::ES);
-  wait_vmcnt<0>();
-  lds_wait_all();  // (keeps the tile's reads behind the wait)
-  float acc[NM][4];
+  const int n = seq_len(a, b), cnt = seq_count(a, b), real = cnt * a.G;
+  const int64_t key064 = (int64_t)blockIdx.x * C::KEYS;
+  if (key064 >= n) return;
+  const int key0 = (int)key064;
+
+  // this wave's keys, two fragments (a key past the length: the last one's values, not stored)
+  RowFrag<T, DP> fr[2];
+  int first[2];  // the first row that sees this lane's key
+  const int64_t old = (int64_t)n - cnt;  // rows of the cache before the new tokens (negative: tokens before its start)
+  auto first_row = [&](int64_t key) {
+    const int64_t r = (key - old) * a.G;
+    return (int)(r < 0 ? 0 : r > real ? real : r);
+  };
 #pragma unroll
-  for (int m = 0; m < NM; ++m)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) acc[m][r] = 0.f;
-  for (int rt = 0; rt < a.rt_own; ++rt) {
-    const RowInfo ri = row_info(a, b, hk, rt * 16 + p);
-    if (!__ballot(ri.valid && ri.lim > key0)) continue;
-    const float l2 = ri.valid ? a.lse2[((int64_t)b * a.Hkv + hk) * a.TG + rt * 16 + p] : -INFINITY;
-    const int lm = l2 == -INFINITY ? 0 : ri.lim - key0 - 4 * g;  // (no row sees key 0 of a lane that has none)
-    RowFrag<T, DP> fr;
-    load_frag<T, DP>(fr, (const T *)a.q + b * a.sq[0] + ri.hq * a.sq[1] + ri.t * a.sq[2], g, a.D);
-    f32x4 s[NM];
-    mm_rows_frag<T, DP, NM>(tile, fr, s, g, p);
-#pragma unroll
-    for (int m = 0; m < NM; ++m)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (16 * m + r < lm) acc[m][r] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[m][r], a.scale2, -l2));
+  for (int f = 0; f < 2; ++f) {
+    const int key = key0 + kg * 32 + f * 16 + p, at = key < n ? key : n - 1;
+    // (the keys take the query's sign, and zeros past the head dim)
+    load_frag<T, DP>(fr[f], (const T *)a.k + b * a.sk[0] + hk * a.sk[1] + at * a.sk[2], g, a);
+    first[f] = first_row(key);
   }
+  const int r0 = first_row(key0) / C::ROWS * C::ROWS;
+  const int nc = r0 < real ? (real - r0 + C::ROWS - 1) / C::ROWS : 0;
+  const int c0 = (int)((int64_t)nc * blockIdx.z / gridDim.z), c1 = (int)((int64_t)nc * (blockIdx.z + 1) / gridDim.z);
+
+  // loads of this thread: row and chunk within the stage, and the row's place in q,
+  // stepped by 64 rows at a time
+  int rho[C::NL], gg[C::NL];
+  int64_t off[C::NL];
+  const int last = a.D * C::ES / 16 - 1;
+  const int dt = C::ROWS / a.G, dg = C::ROWS % a.G;
+  const int64_t sh = a.sq[1] * C::ES, st = a.sq[2] * C::ES;
 #pragma unroll
-  for (int m = 0; m < NM; ++m)
+  for (int x = 0; x < C::NL; ++x) {
+    const int u = x * C::NT + tid, row = u / C::CPR, c = (u % C::CPR) ^ swz(row, C::CPR);
+    rho[x] = r0 + c0 * C::ROWS + row;
+    gg[x] = rho[x] % a.G;
+    off[x] = (int64_t)(rho[x] / a.G) * st + gg[x] * sh + (c < last ? c : last) * 16;
+  }
+  const char *qb = (const char *)a.q + (b * a.sq[0] + (int64_t)hk * a.G * a.sq[1]) * C::ES;
+  const float *lse = a.lse2 + ((int64_t)b * a.Hkv + hk) * a.TG;
+  int ist = 0, cst = 0;
+  auto issue = [&](int c) {
+    char *stage = smem + ist * C::STAGE;
+    ist = ist + 1 == C::NST ? 0 : ist + 1;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-#pragma unroll
-      for (int x = 1; x < 16; x <<= 1) acc[m][r] += shfl_xor_f(acc[m][r], x);
-      const int key = key0 + 16 * m + 4 * g + r;
-      if (p == 0 && key < n) {
-        const float w0 = a.w ? a.w[b * a.sw[0] + hk * a.sw[1] + key] : 0.f;
-        a.wo[b * a.swo[0] + hk * a.swo[1] + key] = w0 + acc[m][r];
+    for (int x = 0; x < C::NL; ++x) {
+      // (rows past the last real one: the first row's values, left out of the sums)
+      if (C::LPT || tid < C::ROWS * C::CPR) g2lds16(qb + (rho[x] < real ? off[x] : 0), stage + (x * C::NT + w * 64) * 16);
+      rho[x] += C::ROWS;
+      gg[x] += dg;
+      off[x] += dt * st + dg * sh;
+      if (gg[x] >= a.G) {
+        gg[x] -= a.G;
+        off[x] += st - a.G * sh;
       }
     }
+    if (w == 0) {
+      const int r = r0 + c * C::ROWS + lane;
+      g2lds4(lse + (r < real ? r : 0), stage + C::ROWS * DP * C::ES);
+    }
+  };
+  float sum[2] = {0.f, 0.f};
+  const int most = first_row((int64_t)key0 + kg * 32 + 31);  // from here on every key of the wave is seen
+  for (int c = c0; c < c0 + C::NST - 1 && c < c1; ++c) issue(c);
+  wait_vmcnt<0>();
+  for (int c = c0; c < c1; ++c) {
+    // (the loads of a wave differ by the statistics', so all are waited for)
+    wait_vmcnt<0>();
+    lds_barrier();
+    if (c + C::NST - 1 < c1) issue(c + C::NST - 1);
+    const char *stage = smem + cst * C::STAGE, *tile = stage + half * 32 * DP * C::ES;
+    cst = cst + 1 == C::NST ? 0 : cst + 1;
+    const int row0 = r0 + c * C::ROWS + half * 32;
+    f32x4 l2[2], s[2][2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) l2[m] = *(const f32x4 *)(stage + C::ROWS * DP * C::ES + (half * 32 + 16 * m + 4 * g) * 4);
+    qk_tile<T, DP, 2, 2>(tile, fr, s, g, p);
+    if (row0 >= most && row0 + 32 <= real) {
+#pragma unroll
+      for (int f = 0; f < 2; ++f)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) sum[f] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[f][m][r], a.scale2, -l2[m][r]));
+    } else {
+#pragma unroll
+      for (int f = 0; f < 2; ++f)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const int row = row0 + 16 * m + 4 * g + r;
+            // (a row that sees nothing has no lse, and no key)
+            if (row >= first[f] && row < real) sum[f] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[f][m][r], a.scale2, -l2[m][r]));
+          }
+    }
+  }
+#pragma unroll
+  for (int f = 0; f < 2; ++f) {
+    sum[f] += shfl_xor_f(sum[f], 16);
+    sum[f] += shfl_xor_f(sum[f], 32);
+    if (half == 1 && g == 0) s_sum[kg][f * 16 + p] = sum[f];
+  }
+  __syncthreads();
+  if (half == 0 && g < 2) {
+    const int x = g * 16 + p, key = key0 + kg * 32 + x;
+    const float y = (g ? sum[1] : sum[0]) + s_sum[kg][x];
+    if (key < n) {
+      if (gridDim.z > 1) {
+        a.wpart[((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * a.S + key] = y;
+      } else {
+        const float w0 = a.w ? a.w[b * a.sw[0] + hk * a.sw[1] + key] : 0.f;
+        a.wo[b * a.swo[0] + hk * a.swo[1] + key] = w0 + y;
+      }
+    }
+  }
+}
+// the row shares' sums, in order
+__global__ __launch_bounds__(256) void cache_weight_sum_kernel(CacheArgs a, int shares) {
+  const int key = blockIdx.x * 256 + threadIdx.x;
+  const int hk = blockIdx.y % a.Hkv, b = blockIdx.y / a.Hkv;
+  if (key >= seq_len(a, b)) return;
+  float y = 0.f;
+  for (int z = 0; z < shares; ++z) y += a.wpart[((int64_t)z * gridDim.y + blockIdx.y) * a.S + key];
+  const float w0 = a.w ? a.w[b * a.sw[0] + hk * a.sw[1] + key] : 0.f;
+  a.wo[b * a.swo[0] + hk * a.swo[1] + key] = w0 + y;
 }
 
 static int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
@@ -465,63 +826,110 @@ static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 // Tiles and shares of a call, from its sizes alone (lengths are on the device:
 // the capacity stands for them).
+constexpr int64_t kCUs = 256;
+
+// Rows of a tile kernel's workgroup
+static int64_t tile_rows(int dtype, int64_t DP, int64_t rows) { return dtype == FBSA_F32 || rows <= 64 ? 64 : 128; }
+
 struct CachePlan {
   int64_t tr_own, tr_pre, rt_own, rt_pre, np_own, np_pre, rows, DP;
+  int64_t nz;  // shares of the rows in the weights of many rows
   bool few_own, few_pre, direct;
-  size_t stat, part, lse2, sc, total;
+  size_t stat, part, lse2, wpart, sc, total;
 };
 static CachePlan cache_plan(const fbsa_cache_desc *d) {
   CachePlan p;
   const int64_t G = d->Hq / d->Hkv, TG = d->T * G;
   p.DP = d->D <= 32 ? 32 : d->D <= 64 ? 64 : d->D <= 128 ? 128 : 256;
   const int64_t KC = d->dtype == FBSA_F32 && p.DP >= 128 ? 16 : 32;
-  constexpr int64_t kWaves = 1024;  // four waves to a CU
-  p.few_own = p.few_pre = true;
-  p.direct = false;
-  p.tr_own = p.tr_pre = 16;
+  const int64_t pre_rows = d->B * TG;
+  p.few_own = TG <= 16;
+  p.few_pre = pre_rows <= 16;
+  p.tr_own = p.few_own ? 16 : tile_rows(d->dtype, p.DP, TG);
+  p.tr_pre = p.few_pre ? 16 : tile_rows(d->dtype, p.DP, pre_rows);
   p.rt_own = cdiv(TG, p.tr_own);
-  p.rt_pre = d->P ? cdiv(d->B * TG, p.tr_pre) : 0;
-  auto shares = [&](int64_t tiles, int64_t keys) {
-    const int64_t want = cdiv(kWaves, tiles), most = cdiv(keys, 4 * KC);
+  p.rt_pre = d->P ? cdiv(pre_rows, p.tr_pre) : 0;
+  // a wave kernel's tile wants four waves to a CU, a tile kernel's one workgroup to a CU; a share is at least 4 chunks
+  auto shares = [&](bool few, int64_t tiles, int64_t keys) {
+    const int64_t want = few ? cdiv(4 * kCUs, tiles) : tiles >= kCUs ? 1 : kCUs / tiles, most = cdiv(keys, 4 * KC);
     const int64_t n = want < most ? want : most;
     return n < kMaxShares / 2 ? n : kMaxShares / 2;
   };
-  p.np_own = shares(d->B * d->Hkv * p.rt_own, d->S);
-  p.np_pre = d->P ? shares(d->Hkv * p.rt_pre, d->P) : 0;
+  p.np_own = shares(p.few_own, d->B * d->Hkv * p.rt_own, d->S);
+  p.np_pre = d->P ? shares(p.few_pre, d->Hkv * p.rt_pre, d->P) : 0;
+  p.direct = !p.few_own && !d->P && p.np_own == 1;
   p.rows = d->B * d->Hkv * p.rt_own * p.np_own * p.tr_own + d->Hkv * p.rt_pre * p.np_pre * p.tr_pre;
   p.stat = 0;
   p.part = up256((size_t)p.rows * 8);
   p.lse2 = p.part + up256((size_t)p.rows * p.DP * 4);
-  p.sc = p.lse2 + up256((size_t)(d->B * d->Hkv * TG) * 4);
-  p.total = p.sc + (d->flags & FBSA_CACHE_WEIGHT && p.rt_own == 1 ? up256((size_t)(d->B * d->Hkv * TG) * cdiv(d->S, 32) * 128) : 0);
+  // (a share is at least four chunks of 64 rows)
+  const int64_t wgs = d->B * d->Hkv * cdiv(d->S, 128), z = wgs >= kCUs ? 1 : kCUs / wgs, zmax = cdiv(TG, 256);
+  p.nz = z < zmax ? z : zmax;
+  const bool weight = d->flags & FBSA_CACHE_WEIGHT;
+  p.wpart = p.lse2 + up256((size_t)(d->B * d->Hkv * TG) * 4);
+  p.sc = p.wpart + (weight && !p.few_own && p.nz > 1 ? up256((size_t)p.nz * d->B * d->Hkv * d->S * 4) : 0);
+  p.total = p.sc + (weight && p.few_own ? up256((size_t)(d->B * d->Hkv * TG) * cdiv(d->S, 32) * 128) : 0);
   return p;
 }
 
-template <typename T, int DP> static int launch_cache(const CacheArgs &a, hipStream_t s) {
+template <typename T, int DP, int NW, int QT, int KC, int NST>
+static int launch_tiles(const CacheArgs &a, int64_t npre, int64_t nown, hipStream_t s) {
+  using C = TileCfg<T, DP, NW, QT, KC, NST>;
+  const int e = lds_optin((const void *)cache_tile_kernel<T, DP, NW, QT, KC, NST>, C::LDS, "hipFuncSetAttribute(cache_tile)");
+  if (e) return e;
+  hipLaunchKernelGGL((cache_tile_kernel<T, DP, NW, QT, KC, NST>), dim3((unsigned)(npre + nown)), dim3(NW * 64), C::LDS, s, a, npre);
+  return hip_check(hipGetLastError(), "cache_tile_kernel launch");
+}
+template <typename T, int DP> static int launch_tiles_of(const CacheArgs &a, int rows, int64_t npre, int64_t nown, hipStream_t s) {
+  if constexpr (sizeof(T) == 4) {
+    return launch_tiles<T, DP, 4, 1, DP >= 128 ? 16 : 32, 2>(a, npre, nown, s);
+  } else {
+    constexpr int KC = DP >= 256 ? 32 : 64;
+    if (rows == 64) return launch_tiles<T, DP, 4, 1, KC, 2>(a, npre, nown, s);
+    constexpr int NW = DP == 32 ? 4 : FBSA_CT_NW;
+    return launch_tiles<T, DP, NW, 8 / NW, KC, 2>(a, npre, nown, s);
+  }
+}
+
+template <typename T, int DP> static int launch_cache(const CacheArgs &a, int64_t nz, hipStream_t s) {
   using C = CacheCfg<T, DP>;
   const size_t lds = (size_t)C::NST * 2 * C::TILE;
   int e = lds_optin((const void *)cache_part_kernel<T, DP>, lds, "hipFuncSetAttribute(cache_part)");
   if (e) return e;
   const int64_t rows = (int64_t)a.B * a.Hkv * a.TG;
-  const int64_t parts = (int64_t)a.B * a.Hkv * a.rt_own * a.np_own + (int64_t)a.Hkv * a.rt_pre * a.np_pre;
-  hipLaunchKernelGGL((cache_part_kernel<T, DP>), dim3((unsigned)parts), dim3(64), lds, s, a);
-  if ((e = hip_check(hipGetLastError(), "cache_part_kernel launch"))) return e;
+  const int64_t nown = (int64_t)a.B * a.Hkv * a.rt_own * a.np_own, npre = (int64_t)a.Hkv * a.rt_pre * a.np_pre;
+  if (npre && !a.few_pre && (e = launch_tiles_of<T, DP>(a, a.tr_pre, npre, !a.few_own && a.tr_own == a.tr_pre ? nown : 0, s))) return e;
+  if (!a.few_own && !(npre && !a.few_pre && a.tr_own == a.tr_pre) && (e = launch_tiles_of<T, DP>(a, a.tr_own, 0, nown, s))) return e;
+  const int64_t parts = (a.few_own ? nown : 0) + (a.few_pre ? npre : 0);
+  if (parts) {
+    hipLaunchKernelGGL((cache_part_kernel<T, DP>), dim3((unsigned)parts), dim3(64), lds, s, a);
+    if ((e = hip_check(hipGetLastError(), "cache_part_kernel launch"))) return e;
+  }
   const int64_t wgs = a.sc ? (int64_t)a.B * a.Hkv * cdiv(a.S, kWeightKeys) : 0;
-  hipLaunchKernelGGL((cache_combine_kernel<T, DP>), dim3((unsigned)(rows + wgs)), dim3(256), 0, s, a);
-  if ((e = hip_check(hipGetLastError(), "cache_combine_kernel launch"))) return e;
+  if (!a.direct) {
+    hipLaunchKernelGGL((cache_combine_kernel<T, DP>), dim3((unsigned)(rows + wgs)), dim3(256), 0, s, a);
+    if ((e = hip_check(hipGetLastError(), "cache_combine_kernel launch"))) return e;
+  }
   if (a.wo && !a.sc) {
-    hipLaunchKernelGGL((cache_weight_kernel<T, DP>), dim3((unsigned)cdiv(a.S, C::KC), (unsigned)(a.B * a.Hkv)), dim3(64), C::TILE, s, a);
-    e = hip_check(hipGetLastError(), "cache_weight_kernel launch");
+    using W = WeightCfg<T, DP>;
+    if ((e = lds_optin((const void *)cache_weight_kernel<T, DP>, W::LDS, "hipFuncSetAttribute(cache_weight)"))) return e;
+    const unsigned seqs = (unsigned)(a.B * a.Hkv);
+    hipLaunchKernelGGL((cache_weight_kernel<T, DP>), dim3((unsigned)cdiv(a.S, W::KEYS), seqs, (unsigned)nz), dim3(W::NT), W::LDS, s, a);
+    if ((e = hip_check(hipGetLastError(), "cache_weight_kernel launch"))) return e;
+    if (nz > 1) {
+      hipLaunchKernelGGL(cache_weight_sum_kernel, dim3((unsigned)cdiv(a.S, 256), seqs), dim3(256), 0, s, a, (int)nz);
+      e = hip_check(hipGetLastError(), "cache_weight_sum_kernel launch");
+    }
   }
   return e;
 }
 
-template <typename T> static int dispatch_cache(const CacheArgs &a, int64_t DP, hipStream_t s) {
-  switch (DP) {
-    case 32: return launch_cache<T, 32>(a, s);
-    case 64: return launch_cache<T, 64>(a, s);
-    case 128: return launch_cache<T, 128>(a, s);
-    default: return launch_cache<T, 256>(a, s);
+template <typename T> static int dispatch_cache(const CacheArgs &a, const CachePlan &pl, hipStream_t s) {
+  switch (pl.DP) {
+    case 32: return launch_cache<T, 32>(a, pl.nz, s);
+    case 64: return launch_cache<T, 64>(a, pl.nz, s);
+    case 128: return launch_cache<T, 128>(a, pl.nz, s);
+    default: return launch_cache<T, 256>(a, pl.nz, s);
   }
 }
 
@@ -600,15 +1008,17 @@ int fbsa_cache_attn(const fbsa_cache_desc *d, const void *q, const void *k, cons
   a.tr_own = (int)pl.tr_own; a.tr_pre = (int)pl.tr_pre;
   a.rt_own = (int)pl.rt_own; a.rt_pre = (int)pl.rt_pre; a.np_own = (int)pl.np_own; a.np_pre = (int)pl.np_pre;
   a.few_own = pl.few_own; a.few_pre = pl.few_pre; a.direct = pl.direct;
-  a.scale2 = d->scale * kLog2e;
+  a.scale2 = d->scale == 0.f ? 1.f : fabsf(d->scale) * kLog2e;
+  a.qand = d->scale == 0.f ? 0u : 0xffffffffu;
+  a.qxor = d->scale < 0.f ? (d->dtype == FBSA_F32 ? 0x80000000u : 0x80008000u) : 0u;
   char *ws = (char *)workspace;
   a.stat = (float2 *)(ws + pl.stat); a.part = (float *)(ws + pl.part);
-  if (out_weight && pl.rt_own == 1) a.sc = (float *)(ws + pl.sc);
-  else if (out_weight) a.lse2 = (float *)(ws + pl.lse2);
+  if (out_weight && pl.few_own) a.sc = (float *)(ws + pl.sc);
+  else if (out_weight) { a.lse2 = (float *)(ws + pl.lse2); a.wpart = (float *)(ws + pl.wpart); }
   switch (d->dtype) {
-    case FBSA_BF16: return dispatch_cache<bf16>(a, pl.DP, (hipStream_t)stream);
-    case FBSA_F16: return dispatch_cache<f16>(a, pl.DP, (hipStream_t)stream);
-    default: return dispatch_cache<float>(a, pl.DP, (hipStream_t)stream);
+    case FBSA_BF16: return dispatch_cache<bf16>(a, pl, (hipStream_t)stream);
+    case FBSA_F16: return dispatch_cache<f16>(a, pl, (hipStream_t)stream);
+    default: return dispatch_cache<float>(a, pl, (hipStream_t)stream);
   }
 }
 

@@ -44,7 +44,7 @@ def attend(q, k, v, lens, count=None, kp=None, vp=None, scale=None, gate=None, w
     return o, lse, w, big
 
 
-def bounds(q, v, S, big):
+def bounds(q, v, S, big, rounded):
     """Absolute error bounds (o beyond its storage rounding as a multiple of |v|,
     lse, relative error of a probability).
 
@@ -56,18 +56,28 @@ def bounds(q, v, S, big):
     product is a pair of 16-bit numbers: for bf16 cut at 2^-7 and the rest
     rounded at 2^-9 of itself (2^-16 relative), for fp16 better than that, or
     2^-25 absolute where the rest is subnormal, at most S of them against a row
-    sum of at least 1; fp32 none."""
+    sum of at least 1; fp32 none. Where many rows share their keys (`rounded`)
+    it is rounded once to the operand type: each is off by at most half a step
+    of itself, so sum p v by at most half a step of sum p |v| (and, for fp16,
+    2^-25 for each subnormal one)."""
     D = q.shape[-1]
     score = (D + 4) * 2.0 ** -24 * big + 2.0 ** -22 * 4
     total = score + S * 2.0 ** -24
-    split = 0.0 if q.dtype == torch.float32 else 2.0 ** -16 + S * 2.0 ** -25
+    split = 0.0 if q.dtype == torch.float32 else (HALF[q.dtype] if rounded else 2.0 ** -16) + S * 2.0 ** -25
     return 2 * total + split, total + 2.0 ** -22, 2 * total
 
 
-def check_attend(got, ref, q, v, S, lens=None):
+def many_rows(q, Hkv, P=0):
+    """Whether the rows of a (sequence, KV head), or those that share a prefix,
+    are more than one 16-row tile."""
+    rows = q.shape[2] * (q.shape[1] // Hkv)
+    return rows > 16 or (P > 0 and q.shape[0] * rows > 16)
+
+
+def check_attend(got, ref, q, v, S, rounded):
     o, lse, w = got
     ro, rl, rw, big = ref
-    tol_o, tol_l, tol_p = bounds(q, v, S, big)
+    tol_o, tol_l, tol_p = bounds(q, v, S, big, rounded)
     o, lse = o.cpu().double(), lse.cpu().double()
     vmax = max(1.0, float(v.detach().abs().nan_to_num(0.0).max()))
     excess = ((o - ro).abs() - HALF[q.dtype] * ro.abs() - tol_o * vmax).max()

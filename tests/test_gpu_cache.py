@@ -61,7 +61,7 @@ def _run(dt, B, Hq, Hkv, T, S, D, lens, count=None, P=0, gate=False, weight=True
             assert (out_w[b, :, n:] == -7.0).all(), "rows behind the sequence were written"
             out_w[b, :, n:] = w[b, :, n:]
     both = torch.cat([v.flatten(), vp.flatten()]) if P else v
-    ref.check_attend((o, lse, out_w), ok, q, both, S + P)
+    ref.check_attend((o, lse, out_w), ok, q, both, S + P, ref.many_rows(q, Hkv, P))
 
 
 @pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
@@ -76,6 +76,13 @@ def test_lengths_around_a_tile(dt, D, Hq, Hkv, T):
 @pytest.mark.parametrize("D", [8, 24, 40, 80, 96, 136, 248])
 def test_head_dims_between(dt, D):
     _run(dt, 2, 6, 2, 3, 77, D, [77, 50], P=45, gate=True)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("D", [8, 40, 96, 200])
+def test_head_dims_between_with_many_rows(dt, D):
+    _run(dt, 2, 6, 2, 30, 177, D, [177, 50], P=45, gate=True)
+    _run(dt, 1, 5, 1, 61, 300, D, [299], count=[55])
 
 
 @pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
@@ -103,12 +110,25 @@ def test_layouts(layout, dt):
 @pytest.mark.parametrize("scale", [0.0, -0.3, 2.5])
 def test_scales(scale):
     _run("fp32", 2, 2, 1, 2, 90, 32, [90, 41], scale=scale)
+    _run("bf16", 2, 4, 1, 2, 90, 64, [90, 41], scale=scale, P=20)
+    _run("fp16", 2, 4, 2, 40, 290, 64, [290, 141], scale=scale)
 
 
 @pytest.mark.parametrize("T,S,lens", [(1, 5000, [5000, 4097]), (70, 1030, [1030, 700]), (257, 600, [600, 258])])
 @pytest.mark.parametrize("D", [64, 256])
 def test_many_rows_and_shares(T, S, lens, D):
     _run("bf16", 2, 8, 2, T, S, D, lens, count=[T, max(1, T - 3)])
+
+
+@pytest.mark.parametrize("Hq,Hkv,T,count", [(7, 1, 33, None), (64, 1, 9, [9, 2]), (65, 1, 5, [3, 5]), (96, 1, 3, None), (1, 1, 300, [300, 70])])
+def test_weights_of_groups_that_divide_nothing(Hq, Hkv, T, count):
+    _run("bf16", 2, Hq, Hkv, T, 400, 32, [400, 290], count=count)
+
+
+def test_weights_of_queries_before_the_cache():
+    # more new tokens than rows: the first ones stand before row 0 and see nothing
+    _run("bf16", 3, 8, 2, 50, 140, 64, [20, 140, 1], count=[50, 50, 30])
+    _run("bf16", 3, 8, 2, 50, 140, 64, [20, 140, 0], count=[50, 50, 30], P=70)
 
 
 def test_stacked_prefix_rows():
@@ -292,7 +312,8 @@ def test_decode_loop():
             for x in range(2):
                 dense[x][b, :, :lens[b]] = mine[x][b]
         want = ref.attend(q, *dense, lens, count, kp, vp, weight=w0)
-        ref.check_attend((o, lse, c.weight), want, q, torch.cat([dense[1].flatten(), vp.flatten()]), S + P)
+        ref.check_attend((o, lse, c.weight), want, q, torch.cat([dense[1].flatten(), vp.flatten()]), S + P,
+                         ref.many_rows(q, Hkv, P))
         keep = ref.evict(c.k, c.v, c.weight.cpu(), lens, budget, 8, 2)
         index = c.evict(budget, recent=8, sink=2)
         assert c.lens.tolist() == [min(n, budget) for n in lens]
