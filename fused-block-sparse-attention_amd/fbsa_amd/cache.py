@@ -20,17 +20,56 @@ whole prompts only and has no counterpart.
 import torch
 
 from . import _lib
-from .ops import _dtype_code, _kernel_ready, _ptr, _require_cuda, _stream
+from .ops import _dtype_code, _ptr
+
+# ---- layout plans -----------------------------------------------------------
+# What a call checks and describes follows from its tensors' shapes, strides,
+# types and device, so it is worked out once per layout: a decode loop, whose
+# layouts repeat, pays for a lookup. A plan holds the C descriptor and sizes, no
+# address and no value of a tensor; alignment and overlap are looked at each call.
+
+_plans = {}
+_PLANS_MAX = 1024
 
 
-def _check(what, *ts):
-    """On one GPU, and not part of a graph that would need their gradients."""
-    ts = [t for t in ts if t is not None]
-    _require_cuda(*ts)
-    if any(t.device != ts[0].device for t in ts):
-        raise ValueError(f"fbsa.{what}: tensors are on different GPUs")
-    if torch.is_grad_enabled() and any(t.requires_grad for t in ts):
+def _layout(ts):
+    return tuple(None if t is None else (t.shape, t.stride(), t.dtype, t.get_device()) for t in ts)
+
+
+def _plan(what, make, scalars, ts):
+    """The plan of tensors ts (None entries allowed) for the call ``what``."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
         raise ValueError(f"fbsa.{what}: no gradients are formed (call it under torch.no_grad())")
+    key = (what, scalars, _layout(ts))
+    p = _plans.get(key)
+    if p is None:
+        dev = next(t.get_device() for t in ts if t is not None)
+        if any(t is not None and not t.is_cuda for t in ts):
+            raise ValueError(f"fbsa.{what}: tensors must be on the GPU (no CPU path)")
+        if any(t is not None and t.get_device() != dev for t in ts):
+            raise ValueError(f"fbsa.{what}: tensors are on different GPUs")
+        p = make(what, scalars, *ts)
+        p.device = torch.device("cuda", dev)
+        p.index = dev
+        if len(_plans) >= _PLANS_MAX:
+            _plans.clear()
+        _plans[key] = p
+    return p
+
+
+class _Plan:
+    """One layout's descriptor and what the call needs besides."""
+
+
+def _launch(p, fn, what, *args):
+    """fn(descriptor, args..., stream) on the plan's device and its current stream."""
+    if torch.cuda.current_device() != p.index:
+        with torch.cuda.device(p.index):
+            st = fn(p.d, *args, torch._C._cuda_getCurrentRawStream(p.index))
+    else:
+        st = fn(p.d, *args, torch._C._cuda_getCurrentRawStream(p.index))
+    if st:
+        _lib.check(st, what)
 
 
 def _strides(t, n):
@@ -38,14 +77,16 @@ def _strides(t, n):
     return tuple(s if e > 1 else 0 for s, e in zip(t.stride()[:n], t.shape[:n]))
 
 
+def _strided(t, n):
+    return t.stride(-1) == 1 and all(s * t.element_size() % 16 == 0 for s in _strides(t, n))
+
+
 def _rows(what, name, t, shape, dtype, n=3):
     """A tensor of rows that the kernels address in place (caches are never copied)."""
     if tuple(t.shape) != tuple(shape) or t.dtype != dtype:
         raise ValueError(f"fbsa.{what}: {name} must be {tuple(shape)} {dtype}, got {tuple(t.shape)} {t.dtype}")
-    es = t.element_size()
-    if t.numel() and (t.stride(-1) != 1 or t.data_ptr() % 16 or any((s * es) % 16 for s in _strides(t, n))):
-        raise ValueError(f"fbsa.{what}: {name} must have contiguous rows and 16-byte aligned strides, got {t.stride()}")
-    return t
+    if t.numel() and not _strided(t, n):
+        raise ValueError(f"fbsa.{what}: {name} must have contiguous rows and strides of whole 16 bytes, got {t.stride()}")
 
 
 def _weights(what, name, t, shape):
@@ -53,39 +94,92 @@ def _weights(what, name, t, shape):
         raise ValueError(f"fbsa.{what}: {name} must be {tuple(shape)} float32, got {tuple(t.shape)} {t.dtype}")
     if t.shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"fbsa.{what}: {name} must be contiguous along its rows, got strides {t.stride()}")
-    return t
 
 
 def _ints(what, name, t, B):
-    if t.shape != (B,) or t.dtype not in (torch.int32, torch.int64):
+    if t is not None and (t.shape != (B,) or t.dtype not in (torch.int32, torch.int64)):
         raise ValueError(f"fbsa.{what}: {name} must be ({B},) int32 or int64, got {tuple(t.shape)} {t.dtype}")
-    return t.to(torch.int32).contiguous()
 
 
-def _span(t):
-    return t.data_ptr(), t.data_ptr() + (sum((e - 1) * s for e, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+def _int32(t):
+    return t if t is None or (t.dtype == torch.int32 and t.is_contiguous()) else t.to(torch.int32).contiguous()
 
 
-def _written(what, name, t, *others):
-    """A tensor that a kernel writes: no two of its entries in one place, and
-    apart from the tensors that the same call reads."""
+def _bytes(t):
+    """Bytes from a tensor's first entry to its last."""
+    return (sum((e - 1) * s for e, s in zip(t.shape, t.stride())) + 1) * t.element_size() if t.numel() else 0
+
+
+def _written(what, name, t):
+    """A tensor that a kernel writes has no two of its entries in one place."""
     end = 1
     for s, e in sorted((s, e) for s, e in zip(t.stride(), t.shape) if e > 1):
         if s < end:
             raise ValueError(f"fbsa.{what}: {name} is written but its entries overlap (strides {t.stride()})")
         end = s * (e - 1) + end
-    lo, hi = _span(t)
-    for x in others:
-        if x is not None and t.numel() and x.numel():
-            a, b = _span(x)
-            if a < hi and lo < b:
+
+
+def _apart(what, name, t, nt, *others):
+    """A tensor that a kernel writes (nt bytes long) shares no memory with the
+    ones that the same call reads, given as (tensor, bytes)."""
+    lo = t.data_ptr()
+    for x, nx in others:
+        if x is not None:
+            a = x.data_ptr()
+            if a < lo + nt and lo < a + nx:
                 raise ValueError(f"fbsa.{what}: {name} is written but overlaps a tensor that the call reads")
 
 
-def _apart(what, k, v):
+def _aligned(what, name, *ts):
+    for t in ts:
+        if t is not None and t.data_ptr() & 15:
+            raise ValueError(f"fbsa.{what}: {name} must be 16-byte aligned")
+
+
+def _ready(t, ok):
+    """t itself, or a copy whose rows the kernels can load 16 bytes at a time."""
+    return t if ok and not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _same_buffer(what, k, v):
     # (interleaved caches span the same addresses, so only the plain mistake is seen here)
-    if k.numel() and k.data_ptr() == v.data_ptr():
+    if k.data_ptr() == v.data_ptr() and k.numel():
         raise ValueError(f"fbsa.{what}: the key and value caches are the same buffer")
+
+
+# ---- the operators ----------------------------------------------------------
+
+
+def _plan_append(what, _, k, v, k_new, v_new, start, count, weight):
+    if k.dim() != 4 or k_new.dim() != 4:
+        raise ValueError("fbsa.append: caches and new rows must be 4-D (B, Hkv, rows, D)")
+    B, H, S, D = k.shape
+    T = k_new.shape[2]
+    p, d = _Plan(), _lib.AppendDesc()
+    d.dtype = _dtype_code(k)
+    _rows(what, "k", k, k.shape, k.dtype)
+    _rows(what, "v", v, k.shape, k.dtype)
+    for name, t in (("k_new", k_new), ("v_new", v_new)):
+        if tuple(t.shape) != (B, H, T, D) or t.dtype != k.dtype:
+            raise ValueError(f"fbsa.append: {name} must be {(B, H, T, D)} {k.dtype}, got {tuple(t.shape)} {t.dtype}")
+    _written(what, "k", k)
+    _written(what, "v", v)
+    if weight is not None:
+        _weights(what, "weight", weight, (B, H, S))
+        _written(what, "weight", weight)
+        d.sw[:] = _strides(weight, 2)
+    _ints(what, "start", start, B)
+    _ints(what, "count", count, B)
+    p.ok = (_strided(k_new, 3), _strided(v_new, 3))
+    p.bytes = tuple(_bytes(t) for t in (k, v, k_new, v_new))
+    p.empty = T == 0 or B == 0
+    d.B, d.H, d.T, d.S, d.D = B, H, T, S, D
+    d.sk[:], d.sv[:] = _strides(k, 3), _strides(v, 3)
+    packed = (H * T * D, T * D, D)
+    d.skn[:] = _strides(k_new, 3) if p.ok[0] else packed
+    d.svn[:] = _strides(v_new, 3) if p.ok[1] else packed
+    p.d, p.packed = d, packed
+    return p
 
 
 def append(k, v, k_new, v_new, start, *, count=None, weight=None):
@@ -93,99 +187,102 @@ def append(k, v, k_new, v_new, start, *, count=None, weight=None):
     rows start[b] + t, for t < count[b] where a padded batch gives counts, and
     zeroes ``weight`` (B, Hkv, S) fp32 there. Rows that would fall outside the
     cache are dropped; no other row changes. ``start`` is not advanced."""
-    _check("append", k, v, k_new, v_new, start, count, weight)
-    if k.dim() != 4 or k_new.dim() != 4:
-        raise ValueError("fbsa.append: caches and new rows must be 4-D (B, Hkv, rows, D)")
-    B, H, S, D = k.shape
-    T = k_new.shape[2]
-    d = _lib.AppendDesc()
-    d.dtype = _dtype_code(k)
-    _rows("append", "k", k, k.shape, k.dtype)
-    _rows("append", "v", v, k.shape, k.dtype)
-    for name, t in (("k_new", k_new), ("v_new", v_new)):
-        if tuple(t.shape) != (B, H, T, D) or t.dtype != k.dtype:
-            raise ValueError(f"fbsa.append: {name} must be {(B, H, T, D)} {k.dtype}, got {tuple(t.shape)} {t.dtype}")
-    _written("append", "k", k, k_new, v_new)
-    _written("append", "v", v, k_new, v_new)
-    _apart("append", k, v)
-    if weight is not None:
-        _weights("append", "weight", weight, (B, H, S))
-        _written("append", "weight", weight)
-    start = _ints("append", "start", start, B)
-    count = None if count is None else _ints("append", "count", count, B)
-    if T == 0 or B == 0:
+    p = _plan("append", _plan_append, (), (k, v, k_new, v_new, start, count, weight))
+    if p.empty:
         return
-    new = [_kernel_ready(t) for t in (k_new, v_new)]
-    d.B, d.H, d.T, d.S, d.D = B, H, T, S, D
-    d.sk[:], d.sv[:], d.skn[:], d.svn[:] = _strides(k, 3), _strides(v, 3), _strides(new[0], 3), _strides(new[1], 3)
-    d.sw[:] = (0, 0) if weight is None else _strides(weight, 2)
-    with torch.cuda.device(k.device):
-        _lib.check(_lib.load().fbsa_cache_append(d, _ptr(k), _ptr(v), _ptr(new[0]), _ptr(new[1]), _ptr(start), _ptr(count),
-                                                 _ptr(weight), _stream()), "fbsa_cache_append")
+    if (k_new.data_ptr() | v_new.data_ptr()) & 15 or not (p.ok[0] and p.ok[1]):
+        k_new, v_new = (t.clone(memory_format=torch.contiguous_format) for t in (k_new, v_new))
+        return append(k, v, k_new, v_new, start, count=count, weight=weight)
+    nk, nv, nkn, nvn = p.bytes
+    _aligned("append", "a cache", k, v)
+    _same_buffer("append", k, v)
+    _apart("append", "k", k, nk, (k_new, nkn), (v_new, nvn))
+    _apart("append", "v", v, nv, (k_new, nkn), (v_new, nvn))
+    start, count = _int32(start), _int32(count)
+    _launch(p, _lib.load().fbsa_cache_append, "fbsa_cache_append", k.data_ptr(), v.data_ptr(), k_new.data_ptr(),
+            v_new.data_ptr(), start.data_ptr(), _ptr(count), _ptr(weight))
 
 
-def _attend(what, q, kp, vp, k, v, lens, count, scale, out_gate, weight, out_weight, need_lse):
-    _check(what, q, kp, vp, k, v, lens, count, out_gate, weight, out_weight)
+def _plan_attend(what, scalars, q, kp, vp, k, v, lens, count, out_gate, weight, out_weight):
+    scale, = scalars
     if q.dim() != 4 or k.dim() != 4:
         raise ValueError(f"fbsa.{what}: q and the caches must be 4-D")
     B, Hq, T, D = q.shape
     Hkv, S = k.shape[1], k.shape[2]
     dt = q.dtype
-    code = _dtype_code(q)
+    p, d = _Plan(), _lib.CacheDesc()
+    d.dtype = _dtype_code(q)
     _rows(what, "k", k, (B, Hkv, S, D), dt)
     _rows(what, "v", v, (B, Hkv, S, D), dt)
-    P = 0
+    p.P = 0
     if kp is not None:
         if kp.dim() != 3:
             raise ValueError(f"fbsa.{what}: the prefix must be 3-D (Hkv, P, D)")
-        P = kp.shape[1]
-        _rows(what, "k_prefix", kp, (Hkv, P, D), dt, 2)
-        _rows(what, "v_prefix", vp, (Hkv, P, D), dt, 2)
-    if out_gate is not None and (out_gate.shape != q.shape or out_gate.dtype != dt):
-        raise ValueError(f"fbsa.{what}: out_gate must match q's shape and dtype")
-    if out_weight is None:
-        out_weight = weight
+        p.P = kp.shape[1]
+        _rows(what, "k_prefix", kp, (Hkv, p.P, D), dt, 2)
+        _rows(what, "v_prefix", vp, (Hkv, p.P, D), dt, 2)
+        if p.P:
+            d.skp[:], d.svp[:] = _strides(kp, 2), _strides(vp, 2)
+    if out_gate is not None:
+        if out_gate.shape != q.shape or out_gate.dtype != dt:
+            raise ValueError(f"fbsa.{what}: out_gate must match q's shape and dtype")
+        p.gate_ok = out_gate.stride(-1) == 1
+        d.sog[:] = _strides(out_gate, 3) if p.gate_ok else (Hq * T * D, T * D, D)
     if out_weight is not None:
         _weights(what, "out_weight", out_weight, (B, Hkv, S))
-        same = weight is not None and weight.data_ptr() == out_weight.data_ptr() and weight.stride() == out_weight.stride()
-        if weight is not None:
-            _weights(what, "weight", weight, (B, Hkv, S))
-        _written(what, "out_weight", out_weight, None if same else weight)
-    lens = (torch.full((B,), S, dtype=torch.int32, device=q.device) if lens is None else _ints(what, "lens", lens, B))
-    count = None if count is None else _ints(what, "count", count, B)
-    if q.numel() == 0:
-        if out_weight is not None and B:
-            raise ValueError(f"fbsa.{what}: no queries to take weights from")
-        o, lse = torch.empty_like(q), torch.empty(B, Hq, T, dtype=torch.float32, device=q.device)
-        return (o, lse) if need_lse else o
-    q = _kernel_ready(q)
-    og = out_gate
-    if og is not None and og.stride(-1) != 1:
-        og = og.contiguous()
-    o = torch.empty(B, Hq, T, D, dtype=dt, device=q.device)
-    lse = torch.empty(B, Hq, T, dtype=torch.float32, device=q.device) if need_lse else None
-    d = _lib.CacheDesc()
-    d.dtype = code
-    d.B, d.Hq, d.Hkv, d.T, d.S, d.P, d.D = B, Hq, Hkv, T, S, P, D
-    d.scale = float(D ** -0.5 if scale is None else scale)
-    d.sq[:], d.sk[:], d.sv[:], d.so[:] = _strides(q, 3), _strides(k, 3), _strides(v, 3), _strides(o, 3)
-    d.sog[:] = (0, 0, 0) if og is None else _strides(og, 3)
-    if P:
-        d.skp[:], d.svp[:] = _strides(kp, 2), _strides(vp, 2)
-    if weight is not None:
-        d.sw[:] = _strides(weight, 2)
-    if out_weight is not None:
+        _written(what, "out_weight", out_weight)
         d.flags = _lib.CACHE_WEIGHT
         d.swo[:] = _strides(out_weight, 2)
-    lib = _lib.load()
-    with torch.cuda.device(q.device):
-        nbytes = lib.fbsa_cache_attn_workspace_bytes(d)
-        if nbytes == 0:
-            _lib.check(_lib.EINVAL, f"fbsa_cache_attn ({what})")
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        _lib.check(lib.fbsa_cache_attn(d, _ptr(q), _ptr(k), _ptr(v), _ptr(lens), _ptr(count), _ptr(kp) if P else None,
-                                       _ptr(vp) if P else None, _ptr(og), _ptr(o), _ptr(lse), _ptr(weight), _ptr(out_weight),
-                                       _ptr(ws), nbytes, _stream()), f"fbsa_cache_attn ({what})")
+        p.same = weight is not None and weight.stride() == out_weight.stride()
+        p.bytes = (_bytes(out_weight), _bytes(weight) if weight is not None else 0)
+    if weight is not None:
+        _weights(what, "weight", weight, (B, Hkv, S))
+        d.sw[:] = _strides(weight, 2)
+    _ints(what, "lens", lens, B)
+    _ints(what, "count", count, B)
+    p.q_ok = _strided(q, 3)
+    p.empty = q.numel() == 0
+    if p.empty and out_weight is not None and B:
+        raise ValueError(f"fbsa.{what}: no queries to take weights from")
+    p.shape, p.S = (B, Hq, T, D), S
+    packed = (Hq * T * D, T * D, D)
+    d.B, d.Hq, d.Hkv, d.T, d.S, d.P, d.D = B, Hq, Hkv, T, S, p.P, D
+    d.scale = D ** -0.5 if scale is None else scale
+    d.sq[:] = _strides(q, 3) if p.q_ok else packed
+    d.sk[:], d.sv[:], d.so[:] = _strides(k, 3), _strides(v, 3), packed
+    p.d = d
+    p.nbytes = 0 if p.empty else _lib.load().fbsa_cache_attn_workspace_bytes(d)
+    if p.nbytes == 0 and not p.empty:
+        _lib.check(_lib.EINVAL, f"fbsa_cache_attn ({what})")
+    return p
+
+
+def _attend(what, q, kp, vp, k, v, lens, count, scale, out_gate, weight, out_weight, need_lse):
+    if out_weight is None:
+        out_weight = weight
+    scale = None if scale is None else float(scale)
+    p = _plan(what, _plan_attend, (scale,), (q, kp, vp, k, v, lens, count, out_gate, weight, out_weight))
+    o = torch.empty(p.shape, dtype=q.dtype, device=p.device)
+    lse = torch.empty(p.shape[:3], dtype=torch.float32, device=p.device) if need_lse else None
+    if p.empty:
+        return (o, lse) if need_lse else o
+    if q.data_ptr() & 15 or not p.q_ok:
+        q = q.clone(memory_format=torch.contiguous_format)
+        if p.q_ok:  # (the plan describes the tensor that was given)
+            return _attend(what, q, kp, vp, k, v, lens, count, scale, out_gate, weight, out_weight, need_lse)
+    if out_gate is not None and not p.gate_ok:
+        out_gate = out_gate.clone(memory_format=torch.contiguous_format)
+    _aligned(what, "a cache or prefix", k, v)
+    if p.P:
+        _aligned(what, "a cache or prefix", kp, vp)
+    if out_weight is not None and not (p.same and weight.data_ptr() == out_weight.data_ptr()):
+        _apart(what, "out_weight", out_weight, p.bytes[0], (weight, p.bytes[1]))
+    lens = torch.full(p.shape[:1], p.S, dtype=torch.int32, device=p.device) if lens is None else _int32(lens)
+    count = _int32(count)
+    ws = torch.empty(p.nbytes, dtype=torch.uint8, device=p.device)
+    _launch(p, _lib.load().fbsa_cache_attn, what, q.data_ptr(), k.data_ptr(), v.data_ptr(), lens.data_ptr(), _ptr(count),
+            kp.data_ptr() if p.P else None, vp.data_ptr() if p.P else None, _ptr(out_gate), o.data_ptr(), _ptr(lse),
+            _ptr(weight), _ptr(out_weight), ws.data_ptr(), p.nbytes)
     return (o, lse) if need_lse else o
 
 
@@ -229,6 +326,37 @@ def shared_prefix_attention(q, k_prefix, v_prefix, k, v, lens=None, *, count=Non
                    out_weight, need_lse)
 
 
+def _plan_evict(what, scalars, k, v, weight, lens, ko, vo, wo):
+    budget, recent, sink = scalars
+    if k.dim() != 4:
+        raise ValueError("fbsa.evict: caches must be 4-D (B, Hkv, S, D)")
+    B, H, S, D = k.shape
+    p, d = _Plan(), _lib.EvictDesc()
+    d.dtype = _dtype_code(k)
+    _rows(what, "k", k, k.shape, k.dtype)
+    _rows(what, "v", v, k.shape, k.dtype)
+    _weights(what, "weight", weight, (B, H, S))
+    _ints(what, "lens", lens, B)
+    inplace = ko is None
+    if inplace:
+        d.flags = _lib.EVICT_IN_PLACE
+        ko, vo, wo = k, v, weight
+    SO = ko.shape[2] if ko.dim() == 4 else 0
+    _rows(what, "k_out", ko, (B, H, SO, D), k.dtype)
+    _rows(what, "v_out", vo, (B, H, SO, D), k.dtype)
+    _weights(what, "weight_out", wo, (B, H, SO))
+    for name, t in (("k", ko), ("v", vo), ("weight", wo)):
+        _written(what, name, t)
+    d.B, d.H, d.S, d.SO, d.D, d.budget, d.recent, d.sink = B, H, S, SO, D, budget, recent, sink
+    d.sk[:], d.sv[:], d.sko[:], d.svo[:] = _strides(k, 3), _strides(v, 3), _strides(ko, 3), _strides(vo, 3)
+    d.sw[:], d.swo[:] = _strides(weight, 2), _strides(wo, 2)
+    p.d, p.inplace = d, inplace
+    p.B, p.shape = B, (B, H, max(0, min(budget, S)))
+    p.bytes = tuple(_bytes(t) for t in (k, v, weight, ko, vo, wo))
+    p.nbytes = _lib.load().fbsa_cache_evict_workspace_bytes(d)
+    return p
+
+
 def evict(k, v, weight, lens, budget, *, recent=0, sink=0, out=None):
     """Cuts every sequence of a cache to at most ``budget`` rows per head.
 
@@ -244,42 +372,25 @@ def evict(k, v, weight, lens, budget, *, recent=0, sink=0, out=None):
     each kept row had (-1 past the last); new_lens (B,) int32 = min(lens, budget).
     ``lens`` itself does not change.
     """
-    _check("evict", k, v, weight, lens, *(out or ()))
-    if k.dim() != 4:
-        raise ValueError("fbsa.evict: caches must be 4-D (B, Hkv, S, D)")
-    B, H, S, D = k.shape
-    d = _lib.EvictDesc()
-    d.dtype = _dtype_code(k)
-    _rows("evict", "k", k, k.shape, k.dtype)
-    _rows("evict", "v", v, k.shape, k.dtype)
-    _weights("evict", "weight", weight, (B, H, S))
-    lens = _ints("evict", "lens", lens, B)
-    budget, recent, sink = int(budget), int(recent), int(sink)
-    if out is None:
-        d.flags = _lib.EVICT_IN_PLACE
+    ko, vo, wo = out if out is not None else (None, None, None)
+    if out is not None and any(t is None for t in out):
+        raise ValueError("fbsa.evict: out must be (k_out, v_out, weight_out)")
+    p = _plan("evict", _plan_evict, (int(budget), int(recent), int(sink)), (k, v, weight, lens, ko, vo, wo))
+    if p.inplace:
         ko, vo, wo = k, v, weight
-        others = ()
     else:
-        ko, vo, wo = out
-        others = (k, v, weight)
-    SO = ko.shape[2] if ko.dim() == 4 else 0
-    _rows("evict", "k_out", ko, (B, H, SO, D), k.dtype)
-    _rows("evict", "v_out", vo, (B, H, SO, D), k.dtype)
-    _weights("evict", "weight_out", wo, (B, H, SO))
-    for name, t in (("k", ko), ("v", vo), ("weight", wo)):
-        _written("evict", name, t, *others)
-    _apart("evict", ko, vo)
-    index = torch.empty(B, H, max(0, min(budget, S)), dtype=torch.int32, device=k.device)
-    new_lens = torch.empty(B, dtype=torch.int32, device=k.device)
-    d.B, d.H, d.S, d.SO, d.D, d.budget, d.recent, d.sink = B, H, S, SO, D, budget, recent, sink
-    d.sk[:], d.sv[:], d.sko[:], d.svo[:] = _strides(k, 3), _strides(v, 3), _strides(ko, 3), _strides(vo, 3)
-    d.sw[:], d.swo[:] = _strides(weight, 2), _strides(wo, 2)
-    lib = _lib.load()
-    with torch.cuda.device(k.device):
-        nbytes = lib.fbsa_cache_evict_workspace_bytes(d)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=k.device) if nbytes else None
-        _lib.check(lib.fbsa_cache_evict(d, _ptr(k), _ptr(v), _ptr(weight), _ptr(lens), _ptr(ko), _ptr(vo), _ptr(wo), _ptr(index),
-                                        _ptr(new_lens), _ptr(ws), nbytes, _stream()), "fbsa_cache_evict")
+        nk, nv, nw, nko, nvo, nwo = p.bytes
+        read = ((k, nk), (v, nv), (weight, nw))
+        for name, t, n in (("k_out", ko, nko), ("v_out", vo, nvo), ("weight_out", wo, nwo)):
+            _apart("evict", name, t, n, *read)
+    _same_buffer("evict", ko, vo)
+    _aligned("evict", "a cache", k, v, ko, vo)
+    lens = _int32(lens)
+    index = torch.empty(p.shape, dtype=torch.int32, device=p.device)
+    new_lens = torch.empty(p.B, dtype=torch.int32, device=p.device)
+    ws = torch.empty(p.nbytes, dtype=torch.uint8, device=p.device) if p.nbytes else None
+    _launch(p, _lib.load().fbsa_cache_evict, "fbsa_cache_evict", k.data_ptr(), v.data_ptr(), weight.data_ptr(), lens.data_ptr(),
+            ko.data_ptr(), vo.data_ptr(), wo.data_ptr(), index.data_ptr(), new_lens.data_ptr(), _ptr(ws), p.nbytes)
     return index, new_lens
 
 

@@ -135,5 +135,13 @@ def test_written_tensors_must_not_overlap_themselves():
     with pytest.raises(ValueError, match="overlap"):
         cache._written("t", "x", x.as_strided((2, 8, 16), (64, 16, 1)))
     with pytest.raises(ValueError, match="reads"):
-        cache._written("t", "x", x[0], x[0, 4:])
-    cache._written("t", "x", x[0], x[1])
+        cache._apart("t", "x", x[0], cache._bytes(x[0]), (x[0, 4:], cache._bytes(x[0, 4:])))
+    cache._apart("t", "x", x[0], cache._bytes(x[0]), (x[1], cache._bytes(x[1])), (None, 0))
+
+
+def test_plans_follow_layouts_not_addresses():
+    def key(*ts):
+        return hash((cache._layout(ts)))
+    x = torch.zeros(2, 8, 16)
+    assert key(x, None) == key(torch.ones(2, 8, 16), None)
+    assert key(x) != key(x.half()) and key(x) != key(x.transpose(0, 1)) and key(x, x) != key(x, None)
