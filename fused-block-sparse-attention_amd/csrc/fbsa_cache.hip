@@ -25,10 +25,6 @@
 #include "fbsa_internal.h"
 #include "fbsa_tiles.h"
 
-#ifndef FBSA_CT_NW
-#define FBSA_CT_NW 8
-#endif
-
 namespace fbsa {
 
 struct CacheArgs {
@@ -422,6 +418,7 @@ __global__ __launch_bounds__(NW * 64) void cache_tile_kernel(CacheArgs a, int64_
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, p = lane & 15;
   const bool pre = blockIdx.x < npre;
+  const int tr = pre ? a.tr_pre : a.tr_own;  // rows of a tile: the waves past them only load
   RowInfo ri[QT];
   int64_t slot;  // the tile's first row among the parts
   int split, np, keys;
@@ -436,13 +433,13 @@ __global__ __launch_bounds__(NW * 64) void cache_tile_kernel(CacheArgs a, int64_
     const int64_t rows = (int64_t)a.B * a.TG;
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-      const int64_t rho = (int64_t)tile * C::ROWS + (w * QT + qt) * 16 + p, x = rho < rows ? rho : 0;
+      const int64_t rho = (int64_t)tile * tr + (w * QT + qt) * 16 + p, x = rho < rows ? rho : 0;
       ri[qt] = row_info(a, (int)(x / a.TG), hk, (int)(x % a.TG));
-      ri[qt].valid = ri[qt].valid && rho < rows;
+      ri[qt].valid = ri[qt].valid && rho < rows && (w * QT + qt) * 16 < tr;
       ri[qt].lim = a.P;
     }
     keys = a.P;
-    slot = (((int64_t)hk * a.rt_pre + tile) * np + split) * C::ROWS;
+    slot = (((int64_t)hk * a.rt_pre + tile) * np + split) * tr;
     kstep = a.skp[1] * C::ES;
     vstep = a.svp[1] * C::ES;
     kb = (const char *)a.kp + hk * a.skp[0] * C::ES;
@@ -454,13 +451,16 @@ __global__ __launch_bounds__(NW * 64) void cache_tile_kernel(CacheArgs a, int64_
     split = u % a.np_own;
     np = a.np_own;
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt) ri[qt] = row_info(a, b, hk, tile * C::ROWS + (w * QT + qt) * 16 + p);
+    for (int qt = 0; qt < QT; ++qt) {
+      ri[qt] = row_info(a, b, hk, tile * tr + (w * QT + qt) * 16 + p);
+      ri[qt].valid = ri[qt].valid && (w * QT + qt) * 16 < tr;
+    }
     // the last real row of the tile sees the most keys
-    const int cnt = seq_count(a, b), t0 = tile * C::ROWS / a.G, t1 = min(min(tile * C::ROWS + C::ROWS, a.TG) - 1, cnt * a.G - 1) / a.G;
+    const int cnt = seq_count(a, b), t0 = tile * tr / a.G, t1 = min(min(tile * tr + tr, a.TG) - 1, cnt * a.G - 1) / a.G;
     const int n = seq_len(a, b);
     const int64_t most = (int64_t)n - cnt + t1 + 1;
     keys = t0 >= cnt ? 0 : (int)(most < 0 ? 0 : most);
-    slot = own_slot(a) + ((((int64_t)b * a.Hkv + hk) * a.rt_own + tile) * np + split) * C::ROWS;
+    slot = own_slot(a) + ((((int64_t)b * a.Hkv + hk) * a.rt_own + tile) * np + split) * tr;
     kstep = a.sk[2] * C::ES;
     vstep = a.sv[2] * C::ES;
     kb = (const char *)a.k + (b * a.sk[0] + hk * a.sk[1]) * C::ES;
@@ -505,6 +505,7 @@ __global__ __launch_bounds__(NW * 64) void cache_tile_kernel(CacheArgs a, int64_
     if (c + NST - 1 < c1) issue(c + NST - 1);
     const char *Ks = smem + cst * 2 * C::TILE, *Vs = Ks + C::TILE;
     cst = cst + 1 == NST ? 0 : cst + 1;
+    if (w * QT * 16 >= tr) continue;
     f32x4 s[QT][NM];
     qk_tile<T, DP, QT, NM>(Ks, fr, s, g, p);
     if ((c + 1) * (int64_t)KC > low) {
@@ -520,9 +521,10 @@ __global__ __launch_bounds__(NW * 64) void cache_tile_kernel(CacheArgs a, int64_
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
     const int i = (w * QT + qt) * 16 + p;
+    if (i >= tr) continue;
     const float lt = sm[qt].total();
     if (!pre && a.direct) {
-      const int rho = (a.rt_own - 1 - (int)((blockIdx.x - (uint32_t)npre) / (uint32_t)(a.Hkv * a.np_own * a.B))) * C::ROWS + i;
+      const int rho = (a.rt_own - 1 - (int)((blockIdx.x - (uint32_t)npre) / (uint32_t)(a.Hkv * a.np_own * a.B))) * tr + i;
       if (rho >= a.TG) continue;
       const float l = ri[qt].valid ? lt : 0.f, inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
@@ -675,12 +677,17 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void cache_combi
 // ---- weights of many rows: p = exp2(score - lse) summed over the rows that see a
 // key, scores formed again. A workgroup per 128 keys of a (sequence, KV head) and
 // share of its rows: the keys stay in registers (32 to a wave, B operands), the
-// query rows stream through a ring in LDS, 64 to a chunk, of which waves 0-3 take
-// the first half and waves 4-7 the second. A lane holds one column, a key, of the
+// query rows stream through a ring in LDS, a chunk's first half to waves 0-3 and
+// its second to waves 4-7. A lane holds one column, a key, of the
 // product, so the sum over rows is a register each. Row rho is token rho / G;
 // key j is seen by the rows from G * (j - (len - count)) on.
 template <typename T, int DP> struct WeightCfg {
-  static constexpr int ES = sizeof(T), ROWS = 64, KEYS = 128, NT = 512, CPR = DP * ES / 16;
+  static constexpr int ES = sizeof(T), NT = 512, CPR = DP * ES / 16;
+  // 16-key fragments of a wave: a row fragment read from LDS feeds KF products
+  // (2048 tokens over 16301 rows, 16 heads over 2, d 256: KF 4 with 64 rows 286 us,
+  // KF 2 with 128 rows 323, with 64 364); fp32 has registers for two
+  static constexpr int KF = ES == 2 ? 4 : 2, KEYS = 4 * 16 * KF;
+  static constexpr int ROWS = DP * ES * KF <= 1024 ? 128 : 64, NM = ROWS / 32;  // NM 16-row tiles to a half
   static constexpr int LPT = ROWS * CPR / NT;        // 16-byte loads per thread and chunk (0: fewer than the threads)
   static constexpr int STAGE = ROWS * DP * ES + ROWS * 4;
   static constexpr int NST = 2, LDS = NST * STAGE;
@@ -689,7 +696,7 @@ template <typename T, int DP> struct WeightCfg {
 template <typename T, int DP> __global__ __launch_bounds__(512) void cache_weight_kernel(CacheArgs a) {
   using C = WeightCfg<T, DP>;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  __shared__ float s_sum[4][32];
+  __shared__ float s_sum[C::KEYS];
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, p = lane & 15;
   const int kg = w & 3, half = w >> 2;
   const int hk = blockIdx.y % a.Hkv, b = blockIdx.y / a.Hkv;
@@ -698,17 +705,17 @@ template <typename T, int DP> __global__ __launch_bounds__(512) void cache_weigh
   if (key064 >= n) return;
   const int key0 = (int)key064;
 
-  // this wave's keys, two fragments (a key past the length: the last one's values, not stored)
-  RowFrag<T, DP> fr[2];
-  int first[2];  // the first row that sees this lane's key
+  // this wave's keys (a key past the length: the last one's values, not stored)
+  RowFrag<T, DP> fr[C::KF];
+  int first[C::KF];  // the first row that sees this lane's key
   const int64_t old = (int64_t)n - cnt;  // rows of the cache before the new tokens (negative: tokens before its start)
   auto first_row = [&](int64_t key) {
     const int64_t r = (key - old) * a.G;
     return (int)(r < 0 ? 0 : r > real ? real : r);
   };
 #pragma unroll
-  for (int f = 0; f < 2; ++f) {
-    const int key = key0 + kg * 32 + f * 16 + p, at = key < n ? key : n - 1;
+  for (int f = 0; f < C::KF; ++f) {
+    const int key = key0 + (kg * C::KF + f) * 16 + p, at = key < n ? key : n - 1;
     // (the keys take the query's sign, and zeros past the head dim)
     load_frag<T, DP>(fr[f], (const T *)a.k + b * a.sk[0] + hk * a.sk[1] + at * a.sk[2], g, a);
     first[f] = first_row(key);
@@ -718,7 +725,7 @@ template <typename T, int DP> __global__ __launch_bounds__(512) void cache_weigh
   const int c0 = (int)((int64_t)nc * blockIdx.z / gridDim.z), c1 = (int)((int64_t)nc * (blockIdx.z + 1) / gridDim.z);
 
   // loads of this thread: row and chunk within the stage, and the row's place in q,
-  // stepped by 64 rows at a time
+  // stepped by a chunk at a time
   int rho[C::NL], gg[C::NL];
   int64_t off[C::NL];
   const int last = a.D * C::ES / 16 - 1;
@@ -749,13 +756,15 @@ template <typename T, int DP> __global__ __launch_bounds__(512) void cache_weigh
         off[x] += st - a.G * sh;
       }
     }
-    if (w == 0) {
-      const int r = r0 + c * C::ROWS + lane;
-      g2lds4(lse + (r < real ? r : 0), stage + C::ROWS * DP * C::ES);
+    if (w * 64 < C::ROWS) {
+      const int r = r0 + c * C::ROWS + w * 64 + lane;
+      g2lds4(lse + (r < real ? r : 0), stage + C::ROWS * DP * C::ES + w * 256);
     }
   };
-  float sum[2] = {0.f, 0.f};
-  const int most = first_row((int64_t)key0 + kg * 32 + 31);  // from here on every key of the wave is seen
+  float sum[C::KF];
+#pragma unroll
+  for (int f = 0; f < C::KF; ++f) sum[f] = 0.f;
+  const int most = first_row((int64_t)key0 + (kg + 1) * C::KF * 16 - 1);  // from here on every key of the wave is seen
   for (int c = c0; c < c0 + C::NST - 1 && c < c1; ++c) issue(c);
   wait_vmcnt<0>();
   for (int c = c0; c < c1; ++c) {
@@ -763,25 +772,25 @@ template <typename T, int DP> __global__ __launch_bounds__(512) void cache_weigh
     wait_vmcnt<0>();
     lds_barrier();
     if (c + C::NST - 1 < c1) issue(c + C::NST - 1);
-    const char *stage = smem + cst * C::STAGE, *tile = stage + half * 32 * DP * C::ES;
+    const char *stage = smem + cst * C::STAGE, *tile = stage + half * 16 * C::NM * DP * C::ES;
     cst = cst + 1 == C::NST ? 0 : cst + 1;
-    const int row0 = r0 + c * C::ROWS + half * 32;
-    f32x4 l2[2], s[2][2];
+    const int row0 = r0 + c * C::ROWS + half * 16 * C::NM;
+    f32x4 l2[C::NM], s[C::KF][C::NM];
 #pragma unroll
-    for (int m = 0; m < 2; ++m) l2[m] = *(const f32x4 *)(stage + C::ROWS * DP * C::ES + (half * 32 + 16 * m + 4 * g) * 4);
-    qk_tile<T, DP, 2, 2>(tile, fr, s, g, p);
-    if (row0 >= most && row0 + 32 <= real) {
+    for (int m = 0; m < C::NM; ++m) l2[m] = *(const f32x4 *)(stage + C::ROWS * DP * C::ES + (half * 16 * C::NM + 16 * m + 4 * g) * 4);
+    qk_tile<T, DP, C::KF, C::NM>(tile, fr, s, g, p);
+    if (row0 >= most && row0 + 16 * C::NM <= real) {
 #pragma unroll
-      for (int f = 0; f < 2; ++f)
+      for (int f = 0; f < C::KF; ++f)
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+        for (int m = 0; m < C::NM; ++m)
 #pragma unroll
           for (int r = 0; r < 4; ++r) sum[f] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[f][m][r], a.scale2, -l2[m][r]));
     } else {
 #pragma unroll
-      for (int f = 0; f < 2; ++f)
+      for (int f = 0; f < C::KF; ++f)
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+        for (int m = 0; m < C::NM; ++m)
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int row = row0 + 16 * m + 4 * g + r;
@@ -791,22 +800,23 @@ template <typename T, int DP> __global__ __launch_bounds__(512) void cache_weigh
     }
   }
 #pragma unroll
-  for (int f = 0; f < 2; ++f) {
+  for (int f = 0; f < C::KF; ++f) {
     sum[f] += shfl_xor_f(sum[f], 16);
     sum[f] += shfl_xor_f(sum[f], 32);
-    if (half == 1 && g == 0) s_sum[kg][f * 16 + p] = sum[f];
+    if (half == 1 && g == 0) s_sum[(kg * C::KF + f) * 16 + p] = sum[f];
   }
   __syncthreads();
-  if (half == 0 && g < 2) {
-    const int x = g * 16 + p, key = key0 + kg * 32 + x;
-    const float y = (g ? sum[1] : sum[0]) + s_sum[kg][x];
-    if (key < n) {
-      if (gridDim.z > 1) {
-        a.wpart[((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * a.S + key] = y;
-      } else {
-        const float w0 = a.w ? a.w[b * a.sw[0] + hk * a.sw[1] + key] : 0.f;
-        a.wo[b * a.swo[0] + hk * a.swo[1] + key] = w0 + y;
-      }
+  if (half == 1 || g) return;
+#pragma unroll
+  for (int f = 0; f < C::KF; ++f) {
+    const int i = (kg * C::KF + f) * 16 + p, key = key0 + i;
+    if (key >= n) continue;
+    const float y = sum[f] + s_sum[i];
+    if (gridDim.z > 1) {
+      a.wpart[((int64_t)blockIdx.z * gridDim.y + blockIdx.y) * a.S + key] = y;
+    } else {
+      const float w0 = a.w ? a.w[b * a.sw[0] + hk * a.sw[1] + key] : 0.f;
+      a.wo[b * a.swo[0] + hk * a.swo[1] + key] = w0 + y;
     }
   }
 }
@@ -828,8 +838,12 @@ static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 // the capacity stands for them).
 constexpr int64_t kCUs = 256;
 
-// Rows of a tile kernel's workgroup
-static int64_t tile_rows(int dtype, int64_t DP, int64_t rows) { return dtype == FBSA_F32 || rows <= 64 ? 64 : 128; }
+// Rows of a tile: as many tiles as workgroups of 64 or 128 rows would be, of even
+// sizes (160 rows are two tiles of 80, whose spare waves leave the CU to others)
+static int64_t tile_rows(int dtype, int64_t rows) {
+  const int64_t most = dtype == FBSA_F32 || rows <= 64 ? 64 : 128, n = cdiv(rows, most);
+  return cdiv(cdiv(rows, n), 16) * 16;
+}
 
 struct CachePlan {
   int64_t tr_own, tr_pre, rt_own, rt_pre, np_own, np_pre, rows, DP;
@@ -845,13 +859,15 @@ static CachePlan cache_plan(const fbsa_cache_desc *d) {
   const int64_t pre_rows = d->B * TG;
   p.few_own = TG <= 16;
   p.few_pre = pre_rows <= 16;
-  p.tr_own = p.few_own ? 16 : tile_rows(d->dtype, p.DP, TG);
-  p.tr_pre = p.few_pre ? 16 : tile_rows(d->dtype, p.DP, pre_rows);
+  p.tr_own = p.few_own ? 16 : tile_rows(d->dtype, TG);
+  p.tr_pre = p.few_pre ? 16 : tile_rows(d->dtype, pre_rows);
   p.rt_own = cdiv(TG, p.tr_own);
   p.rt_pre = d->P ? cdiv(pre_rows, p.tr_pre) : 0;
-  // a wave kernel's tile wants four waves to a CU, a tile kernel's one workgroup to a CU; a share is at least 4 chunks
+  // the wave kernel wants four waves to a CU, the tile kernel as many workgroups as
+  // a CU has room for (d 256: one); a share is at least 4 chunks
+  const int64_t room = kCUs * (p.DP <= 128 ? 2 : 1);
   auto shares = [&](bool few, int64_t tiles, int64_t keys) {
-    const int64_t want = few ? cdiv(4 * kCUs, tiles) : tiles >= kCUs ? 1 : kCUs / tiles, most = cdiv(keys, 4 * KC);
+    const int64_t want = few ? cdiv(4 * kCUs, tiles) : tiles >= room ? 1 : room / tiles, most = cdiv(keys, 4 * KC);
     const int64_t n = want < most ? want : most;
     return n < kMaxShares / 2 ? n : kMaxShares / 2;
   };
@@ -863,7 +879,7 @@ static CachePlan cache_plan(const fbsa_cache_desc *d) {
   p.part = up256((size_t)p.rows * 8);
   p.lse2 = p.part + up256((size_t)p.rows * p.DP * 4);
   // (a share is at least four chunks of 64 rows)
-  const int64_t wgs = d->B * d->Hkv * cdiv(d->S, 128), z = wgs >= kCUs ? 1 : kCUs / wgs, zmax = cdiv(TG, 256);
+  const int64_t wgs = d->B * d->Hkv * cdiv(d->S, d->dtype == FBSA_F32 ? 128 : 256), z = wgs >= kCUs ? 1 : kCUs / wgs, zmax = cdiv(TG, 256);
   p.nz = z < zmax ? z : zmax;
   const bool weight = d->flags & FBSA_CACHE_WEIGHT;
   p.wpart = p.lse2 + up256((size_t)(d->B * d->Hkv * TG) * 4);
@@ -884,10 +900,9 @@ template <typename T, int DP> static int launch_tiles_of(const CacheArgs &a, int
   if constexpr (sizeof(T) == 4) {
     return launch_tiles<T, DP, 4, 1, DP >= 128 ? 16 : 32, 2>(a, npre, nown, s);
   } else {
-    constexpr int KC = DP >= 256 ? 32 : 64;
-    if (rows == 64) return launch_tiles<T, DP, 4, 1, KC, 2>(a, npre, nown, s);
-    constexpr int NW = DP == 32 ? 4 : FBSA_CT_NW;
-    return launch_tiles<T, DP, NW, 8 / NW, KC, 2>(a, npre, nown, s);
+        if (rows <= 64) return launch_tiles<T, DP, 4, 1, 64, 2>(a, npre, nown, s);
+    constexpr int NW = DP == 32 ? 4 : 8;  // (a tile of 64 keys, d 32, is four waves' loads)
+    return launch_tiles<T, DP, NW, 8 / NW, 64, 2>(a, npre, nown, s);
   }
 }
 
