@@ -51,10 +51,11 @@ struct CacheArgs {
   float *sc;                 // [B][Hkv][TG][S rounded up to 32] log2-domain scores (few_own, with weights)
 };
 
-// keys per chunk: 32, 16 for fp32 at d >= 128 (registers)
+// keys per chunk of a wave's ring: 32; 16 where a row is 512 bytes or more, so that
+// more waves fit a CU's LDS
 template <typename T, int DP> struct CacheCfg {
   static constexpr int ES = sizeof(T);
-  static constexpr int KC = ES == 4 && DP >= 128 ? 16 : 32;
+  static constexpr int KC = DP * ES >= 512 ? 16 : 32;
   static constexpr int CPR = DP * ES / 16;
   static constexpr int TILE = KC * DP * ES;
   static constexpr int LPT = KC * CPR / 64;  // 16-byte loads per lane and tile
@@ -83,6 +84,23 @@ __device__ __forceinline__ RowInfo row_info(const CacheArgs &a, int b, int hk, i
   const int64_t m = (int64_t)n - c + r.t + 1;
   r.lim = m < 0 ? 0 : m > n ? n : (int)m;
   return r;
+}
+
+// Rows [r0, r1) of a (sequence, KV head): the keys that the last real one sees (0
+// if none is real), and those that the first sees.
+__device__ __forceinline__ void own_bounds(const CacheArgs &a, int b, int r0, int r1, int &keys, int &low) {
+  const int n = seq_len(a, b), c = seq_count(a, b), real = min(r1, c * a.G);
+  keys = low = 0;
+  if (r0 >= real) return;
+  const int64_t k1 = (int64_t)n - c + (real - 1) / a.G + 1, k0 = (int64_t)n - c + r0 / a.G + 1;
+  keys = __builtin_amdgcn_readfirstlane(k1 < 0 ? 0 : (int)k1);  // (at most n)
+  low = __builtin_amdgcn_readfirstlane(k0 < 0 ? 0 : (int)k0);
+}
+// chunks [c0, c1) of share `split` of np: nc / np each, one more for the first nc % np
+__device__ __forceinline__ void share_of(int nc, int split, int np, int &c0, int &c1) {
+  const int per = (int)((uint32_t)nc / (uint32_t)np), more = nc - per * np;
+  c0 = split * per + min(split, more);
+  c1 = c0 + per + (split < more ? 1 : 0);
 }
 
 template <typename T, int DP>
@@ -205,8 +223,9 @@ template <typename T> __device__ __forceinline__ void store_row(const CacheArgs 
 
 // first row of the own tiles' parts
 __device__ __forceinline__ int64_t own_slot(const CacheArgs &a) { return (int64_t)a.Hkv * a.rt_pre * a.np_pre * a.tr_pre; }
+__device__ __forceinline__ int64_t score_keys(const CacheArgs &a) { return ((int64_t)a.S + 31) / 32 * 32; }
 __device__ __forceinline__ int64_t score_row(const CacheArgs &a, int b, int hk, int rho) {
-  return (((int64_t)b * a.Hkv + hk) * a.TG + rho) * (((int64_t)a.S + 31) / 32 * 32);
+  return (((int64_t)b * a.Hkv + hk) * a.TG + rho) * score_keys(a);
 }
 
 template <typename T, int DP> __global__ __launch_bounds__(64) void cache_part_kernel(CacheArgs a) {
@@ -220,18 +239,17 @@ template <typename T, int DP> __global__ __launch_bounds__(64) void cache_part_k
   RowInfo ri;
   float *score = nullptr;  // this row's scores, where the weights are taken from them
   int64_t slot;  // the tile's first row among the parts
-  int split, np, keys;
+  int split, np, keys, low;  // keys that any row sees; below `low` every row sees every key
   const char *kb, *vb;
   int64_t kstep, vstep;
   if (pre) {
     const int tile = id % a.rt_pre, hk = id / a.rt_pre / a.np_pre;
     split = id / a.rt_pre % a.np_pre;
     np = a.np_pre;
-    const int64_t rho = (int64_t)tile * 16 + p, rows = (int64_t)a.B * a.TG;
-    const int64_t x = rho < rows ? rho : 0;
-    ri = row_info(a, (int)(x / a.TG), hk, (int)(x % a.TG));
+    const uint32_t rho = tile * 16 + p, rows = (uint32_t)a.B * a.TG, x = rho < rows ? rho : 0;  // (below 2^31)
+    ri = row_info(a, (int)(x / (uint32_t)a.TG), hk, (int)(x % (uint32_t)a.TG));
     ri.valid = ri.valid && rho < rows;
-    ri.lim = a.P;
+    ri.lim = keys = low = a.P;
     slot = (((int64_t)hk * a.rt_pre + tile) * np + split) * 16;
     kstep = a.skp[1] * C::ES;
     vstep = a.svp[1] * C::ES;
@@ -243,6 +261,7 @@ template <typename T, int DP> __global__ __launch_bounds__(64) void cache_part_k
     split = id / a.rt_own % a.np_own;
     np = a.np_own;
     ri = row_info(a, b, hk, tile * 16 + p);
+    own_bounds(a, b, tile * 16, min(tile * 16 + 16, a.TG), keys, low);
     if (a.sc) score = a.sc + score_row(a, b, hk, ri.valid ? p : 0);
     slot = own_slot(a) + (((int64_t)b * a.Hkv + hk) * a.rt_own + tile) * np * 16 + split * 16;
     kstep = a.sk[2] * C::ES;
@@ -250,21 +269,11 @@ template <typename T, int DP> __global__ __launch_bounds__(64) void cache_part_k
     kb = (const char *)a.k + (b * a.sk[0] + hk * a.sk[1]) * C::ES;
     vb = (const char *)a.v + (b * a.sv[0] + hk * a.sv[1]) * C::ES;
   }
-  // keys that any row sees; below `low` every row sees every key. A row that is
-  // none (past the end, or past the sequence's new tokens) sees what the tile
-  // sees, so that it asks for no masking, and is dropped by the combine.
-  int low = ri.valid ? ri.lim : 0x7fffffff;
-  keys = ri.valid ? ri.lim : 0;
-#pragma unroll
-  for (int x = 1; x < 16; x <<= 1) {
-    low = min(low, __shfl_xor(low, x, 64));
-    keys = max(keys, __shfl_xor(keys, x, 64));
-  }
-  keys = __builtin_amdgcn_readfirstlane(keys);
-  low = __builtin_amdgcn_readfirstlane(low);
+  // (a row that is none -- past the end, or past the sequence's new tokens -- sees
+  // what the tile sees, so that it asks for no masking; the combine drops it)
   const int lim = ri.valid ? ri.lim : keys;
-  const int64_t nc = ((int64_t)keys + KC - 1) / KC;
-  const int c0 = (int)(nc * split / np), c1 = (int)(nc * (split + 1) / np);
+  int c0, c1;
+  share_of((keys + KC - 1) / KC, split, np, c0, c1);
 
   RowFrag<T, DP> fr;
   load_frag<T, DP>(fr, (const T *)a.q + ri.b * a.sq[0] + ri.hq * a.sq[1] + ri.t * a.sq[2], g, a);
@@ -421,7 +430,7 @@ __global__ __launch_bounds__(NW * 64) void cache_tile_kernel(CacheArgs a, int64_
   const int tr = pre ? a.tr_pre : a.tr_own;  // rows of a tile: the waves past them only load
   RowInfo ri[QT];
   int64_t slot;  // the tile's first row among the parts
-  int split, np, keys;
+  int split, np, keys, low;  // keys that any row sees; below `low` every row of the wave sees every key
   const char *kb, *vb;
   int64_t kstep, vstep;
   if (pre) {
@@ -430,15 +439,15 @@ __global__ __launch_bounds__(NW * 64) void cache_tile_kernel(CacheArgs a, int64_
     const int tile = id % a.rt_pre, hk = id / a.rt_pre / a.np_pre;
     split = id / a.rt_pre % a.np_pre;
     np = a.np_pre;
-    const int64_t rows = (int64_t)a.B * a.TG;
+    const uint32_t rows = (uint32_t)a.B * a.TG;  // (below 2^31)
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) {
-      const int64_t rho = (int64_t)tile * tr + (w * QT + qt) * 16 + p, x = rho < rows ? rho : 0;
-      ri[qt] = row_info(a, (int)(x / a.TG), hk, (int)(x % a.TG));
+      const uint32_t rho = (uint32_t)tile * tr + (w * QT + qt) * 16 + p, x = rho < rows ? rho : 0;
+      ri[qt] = row_info(a, (int)(x / (uint32_t)a.TG), hk, (int)(x % (uint32_t)a.TG));
       ri[qt].valid = ri[qt].valid && rho < rows && (w * QT + qt) * 16 < tr;
       ri[qt].lim = a.P;
     }
-    keys = a.P;
+    keys = low = a.P;
     slot = (((int64_t)hk * a.rt_pre + tile) * np + split) * tr;
     kstep = a.skp[1] * C::ES;
     vstep = a.svp[1] * C::ES;
@@ -455,27 +464,21 @@ __global__ __launch_bounds__(NW * 64) void cache_tile_kernel(CacheArgs a, int64_
       ri[qt] = row_info(a, b, hk, tile * tr + (w * QT + qt) * 16 + p);
       ri[qt].valid = ri[qt].valid && (w * QT + qt) * 16 < tr;
     }
-    // the last real row of the tile sees the most keys
-    const int cnt = seq_count(a, b), t0 = tile * tr / a.G, t1 = min(min(tile * tr + tr, a.TG) - 1, cnt * a.G - 1) / a.G;
-    const int n = seq_len(a, b);
-    const int64_t most = (int64_t)n - cnt + t1 + 1;
-    keys = t0 >= cnt ? 0 : (int)(most < 0 ? 0 : most);
+    own_bounds(a, b, tile * tr, min(tile * tr + tr, a.TG), keys, low);
+    const int r0 = tile * tr + w * QT * 16;  // (the wave's first row: from it on, the later rows see more)
+    if (w > 0 && r0 < a.TG) {
+      int k;
+      own_bounds(a, b, r0, a.TG, k, low);
+      low = min(low, keys);
+    }
     slot = own_slot(a) + ((((int64_t)b * a.Hkv + hk) * a.rt_own + tile) * np + split) * tr;
     kstep = a.sk[2] * C::ES;
     vstep = a.sv[2] * C::ES;
     kb = (const char *)a.k + (b * a.sk[0] + hk * a.sk[1]) * C::ES;
     vb = (const char *)a.v + (b * a.sv[0] + hk * a.sv[1]) * C::ES;
   }
-  keys = __builtin_amdgcn_readfirstlane(keys);
-  int low = 0x7fffffff;  // below it every row of the wave sees every key
-#pragma unroll
-  for (int qt = 0; qt < QT; ++qt) low = min(low, ri[qt].valid ? ri[qt].lim : 0x7fffffff);
-#pragma unroll
-  for (int x = 1; x < 16; x <<= 1) low = min(low, __shfl_xor(low, x, 64));
-  low = __builtin_amdgcn_readfirstlane(low);
-  low = min(low, keys);
-  const int64_t nc = ((int64_t)keys + KC - 1) / KC;
-  const int c0 = (int)(nc * split / np), c1 = (int)(nc * (split + 1) / np);
+  int c0, c1;
+  share_of((keys + KC - 1) / KC, split, np, c0, c1);
 
   RowFrag<T, DP> fr[QT];
 #pragma unroll
@@ -555,10 +558,10 @@ struct RowParts {
 };
 __device__ __forceinline__ RowParts row_parts(const CacheArgs &a, int b, int hk, int rho) {
   RowParts r;
-  const int64_t rp = (int64_t)b * a.TG + rho;
+  const uint32_t rp = (uint32_t)b * a.TG + rho, tr = a.tr_pre;  // (B * TG is below 2^31)
   r.npre = a.np_pre;
   r.n = a.np_pre + a.np_own;
-  r.pre0 = a.np_pre ? ((int64_t)hk * a.rt_pre + rp / a.tr_pre) * a.np_pre * a.tr_pre + rp % a.tr_pre : 0;
+  r.pre0 = a.np_pre ? ((int64_t)hk * a.rt_pre + rp / tr) * a.np_pre * tr + rp % tr : 0;
   r.own0 = own_slot(a) + (((int64_t)b * a.Hkv + hk) * a.rt_own + rho / a.tr_own) * a.np_own * a.tr_own + rho % a.tr_own;
   return r;
 }
@@ -634,6 +637,13 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void cache_combi
   const RowInfo ri = row_info(a, b, hk, rho);
   const RowParts rp = row_parts(a, b, hk, rho);
   const int n = ri.valid ? rp.n : 0;
+  // the first parts are asked for before their statistics are known
+  constexpr int U = 4;
+  const int gi = tid / LG, e = tid % LG;
+  f32x4 ahead[U];
+#pragma unroll
+  for (int j = 0; j < U; ++j)
+    if (gi + j * NG < n) ahead[j] = *(const f32x4 *)(a.part + rp.at(a, gi + j * NG) * DP + 4 * e);
   float m = -INFINITY;
   for (int i = tid; i < n; i += 256) m = fmaxf(m, a.stat[rp.at(a, i)].x);
 #pragma unroll
@@ -654,9 +664,14 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void cache_combi
   if (lane == 0) s_red[4 + wave] = l;
   __syncthreads();
   l = (s_red[4] + s_red[5]) + (s_red[6] + s_red[7]);
-  const int gi = tid / LG, e = tid % LG;
   f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
-  for (int i = gi; i < n; i += NG) {
+#pragma unroll
+  for (int j = 0; j < U; ++j)
+    if (gi + j * NG < n) {
+      const float f = s_f[gi + j * NG];
+      if (f != -1.f) acc += f * ahead[j];
+    }
+  for (int i = gi + U * NG; i < n; i += NG) {
     const float f = s_f[i];
     if (f != -1.f) acc += f * *(const f32x4 *)(a.part + rp.at(a, i) * DP + 4 * e);
   }
@@ -855,7 +870,6 @@ static CachePlan cache_plan(const fbsa_cache_desc *d) {
   CachePlan p;
   const int64_t G = d->Hq / d->Hkv, TG = d->T * G;
   p.DP = d->D <= 32 ? 32 : d->D <= 64 ? 64 : d->D <= 128 ? 128 : 256;
-  const int64_t KC = d->dtype == FBSA_F32 && p.DP >= 128 ? 16 : 32;
   const int64_t pre_rows = d->B * TG;
   p.few_own = TG <= 16;
   p.few_pre = pre_rows <= 16;
@@ -863,11 +877,11 @@ static CachePlan cache_plan(const fbsa_cache_desc *d) {
   p.tr_pre = p.few_pre ? 16 : tile_rows(d->dtype, pre_rows);
   p.rt_own = cdiv(TG, p.tr_own);
   p.rt_pre = d->P ? cdiv(pre_rows, p.tr_pre) : 0;
-  // the wave kernel wants four waves to a CU, the tile kernel as many workgroups as
-  // a CU has room for (d 256: one); a share is at least 4 chunks
+  // the wave kernel wants four waves to a CU (d 256: eight), the tile kernel as many workgroups as
+  // a CU has room for (d 256: one); a share is at least 128 keys
   const int64_t room = kCUs * (p.DP <= 128 ? 2 : 1);
   auto shares = [&](bool few, int64_t tiles, int64_t keys) {
-    const int64_t want = few ? cdiv(4 * kCUs, tiles) : tiles >= room ? 1 : room / tiles, most = cdiv(keys, 4 * KC);
+    const int64_t want = few ? cdiv((p.DP == 256 ? 8 : 4) * kCUs, tiles) : tiles >= room ? 1 : room / tiles, most = cdiv(keys, 128);
     const int64_t n = want < most ? want : most;
     return n < kMaxShares / 2 ? n : kMaxShares / 2;
   };
@@ -913,8 +927,10 @@ template <typename T, int DP> static int launch_cache(const CacheArgs &a, int64_
   if (e) return e;
   const int64_t rows = (int64_t)a.B * a.Hkv * a.TG;
   const int64_t nown = (int64_t)a.B * a.Hkv * a.rt_own * a.np_own, npre = (int64_t)a.Hkv * a.rt_pre * a.np_pre;
-  if (npre && !a.few_pre && (e = launch_tiles_of<T, DP>(a, a.tr_pre, npre, !a.few_own && a.tr_own == a.tr_pre ? nown : 0, s))) return e;
-  if (!a.few_own && !(npre && !a.few_pre && a.tr_own == a.tr_pre) && (e = launch_tiles_of<T, DP>(a, a.tr_own, 0, nown, s))) return e;
+  // prefix and own tiles in one launch where one workgroup size serves both
+  const bool both = npre && !a.few_pre && !a.few_own && (a.tr_own <= 64) == (a.tr_pre <= 64);
+  if (npre && !a.few_pre && (e = launch_tiles_of<T, DP>(a, a.tr_pre, npre, both ? nown : 0, s))) return e;
+  if (!a.few_own && !both && (e = launch_tiles_of<T, DP>(a, a.tr_own, 0, nown, s))) return e;
   const int64_t parts = (a.few_own ? nown : 0) + (a.few_pre ? npre : 0);
   if (parts) {
     hipLaunchKernelGGL((cache_part_kernel<T, DP>), dim3((unsigned)parts), dim3(64), lds, s, a);
