@@ -566,6 +566,48 @@ __device__ __forceinline__ RowParts row_parts(const CacheArgs &a, int b, int hk,
   return r;
 }
 
+// A wave per row, where rows are many: DP / 4 lanes to a part, so 64 / (DP / 4)
+// parts at a time; their sums are joined across the lanes in order.
+template <typename T, int DP> __global__ __launch_bounds__(256) void cache_join_kernel(CacheArgs a) {
+  constexpr int LG = DP / 4, NG = 64 / LG;
+  const int lane = threadIdx.x & 63;
+  const uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 6), rows = (uint32_t)a.B * a.Hkv * a.TG;
+  if (row >= rows) return;
+  const int rho = (int)(row % a.TG), hk = (int)(row / a.TG % a.Hkv), b = (int)(row / a.TG / a.Hkv);
+  const RowInfo ri = row_info(a, b, hk, rho);
+  const RowParts rp = row_parts(a, b, hk, rho);
+  const int n = ri.valid ? rp.n : 0, gi = lane / LG, e = lane % LG;
+  float m = -INFINITY;
+  for (int i = lane; i < n; i += 64) m = fmaxf(m, a.stat[rp.at(a, i)].x);
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, shfl_xor_f(m, x));
+  const float ref = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+  for (int i = gi; i < n; i += NG) {
+    const int64_t at = rp.at(a, i);
+    const float2 st = a.stat[at];
+    if (st.y != 0.f) {  // (a part of no keys has no O)
+      const float f = __builtin_amdgcn_exp2f(st.x - ref);
+      l += f * st.y;
+      acc += f * *(const f32x4 *)(a.part + at * DP + 4 * e);
+    }
+  }
+#pragma unroll
+  for (int x = LG; x < 64; x <<= 1) {
+    l += shfl_xor_f(l, x);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) acc[r] += shfl_xor_f(acc[r], x);
+  }
+  if (gi == 0) store_row<T>(a, ri, acc, l == 0.f ? 0.f : 1.f / l, 4 * e);
+  if (lane == 0) {
+    const float l2 = l == 0.f ? -INFINITY : m + __log2f(l);
+    if (a.lse) a.lse[((int64_t)b * a.Hq + ri.hq) * a.T + ri.t] = l2 * kLn2;
+    if (a.lse2) a.lse2[row] = l2;
+  }
+}
+
 constexpr int kMaxShares = 512;    // np_own + np_pre
 constexpr int kWeightKeys = 1024;  // keys of a weight workgroup
 
@@ -671,9 +713,16 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void cache_combi
       const float f = s_f[gi + j * NG];
       if (f != -1.f) acc += f * ahead[j];
     }
-  for (int i = gi + U * NG; i < n; i += NG) {
-    const float f = s_f[i];
-    if (f != -1.f) acc += f * *(const f32x4 *)(a.part + rp.at(a, i) * DP + 4 * e);
+  // (loads of several parts in flight: one that was not written is loaded and left out)
+  for (int i = gi + U * NG; i < n; i += U * NG) {
+    f32x4 y[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) y[j] = *(const f32x4 *)(a.part + rp.at(a, i + j * NG < n ? i + j * NG : i) * DP + 4 * e);
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      const float f = i + j * NG < n ? s_f[i + j * NG] : -1.f;
+      if (f != -1.f) acc += f * y[j];
+    }
   }
   s_acc[tid] = acc;
   __syncthreads();
@@ -878,15 +927,20 @@ static CachePlan cache_plan(const fbsa_cache_desc *d) {
   p.rt_own = cdiv(TG, p.tr_own);
   p.rt_pre = d->P ? cdiv(pre_rows, p.tr_pre) : 0;
   // the wave kernel wants four waves to a CU (d 256: eight), the tile kernel as many workgroups as
-  // a CU has room for (d 256: one); a share is at least 128 keys
+  // a CU has room for (d 256: one). A share has at least so many keys that joining it
+  // costs less than it saves (swept over some 200 drawn shapes: 16-bit wave tiles 64
+  // keys up to 25% under 128, tile kernels 128 up to 30% under 64, fp32 32 up to 30%
+  // under 64)
   const int64_t room = kCUs * (p.DP <= 128 ? 2 : 1);
-  auto shares = [&](bool few, int64_t tiles, int64_t keys) {
-    const int64_t want = few ? cdiv((p.DP == 256 ? 8 : 4) * kCUs, tiles) : tiles >= room ? 1 : room / tiles, most = cdiv(keys, 128);
+  // (sequences of different lengths want them finer, so that the longest does not hold up the rest)
+  auto shares = [&](bool few, bool ragged, int64_t tiles, int64_t keys) {
+    const int64_t want = few ? cdiv((p.DP == 256 ? 8 : 4) * kCUs, tiles) : ragged ? cdiv(4 * room, tiles) : tiles >= room ? 1 : room / tiles;
+    const int64_t most = cdiv(keys, d->dtype == FBSA_F32 ? 32 : few ? 64 : 128);
     const int64_t n = want < most ? want : most;
     return n < kMaxShares / 2 ? n : kMaxShares / 2;
   };
-  p.np_own = shares(p.few_own, d->B * d->Hkv * p.rt_own, d->S);
-  p.np_pre = d->P ? shares(p.few_pre, d->Hkv * p.rt_pre, d->P) : 0;
+  p.np_own = shares(p.few_own, d->B > 1, d->B * d->Hkv * p.rt_own, d->S);
+  p.np_pre = d->P ? shares(p.few_pre, false, d->Hkv * p.rt_pre, d->P) : 0;
   p.direct = !p.few_own && !d->P && p.np_own == 1;
   p.rows = d->B * d->Hkv * p.rt_own * p.np_own * p.tr_own + d->Hkv * p.rt_pre * p.np_pre * p.tr_pre;
   p.stat = 0;
@@ -938,7 +992,11 @@ template <typename T, int DP> static int launch_cache(const CacheArgs &a, int64_
   }
   const int64_t wgs = a.sc ? (int64_t)a.B * a.Hkv * cdiv(a.S, kWeightKeys) : 0;
   if (!a.direct) {
-    hipLaunchKernelGGL((cache_combine_kernel<T, DP>), dim3((unsigned)(rows + wgs)), dim3(256), 0, s, a);
+    // many rows of few parts: a wave each (1152 rows of 26 parts, d 256: 71 us a call against 60)
+    if (!a.sc && (rows >= 16384 || (rows >= 1024 && (a.np_own + a.np_pre) * DP <= 2048)))
+      hipLaunchKernelGGL((cache_join_kernel<T, DP>), dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, s, a);
+    else
+      hipLaunchKernelGGL((cache_combine_kernel<T, DP>), dim3((unsigned)(rows + wgs)), dim3(256), 0, s, a);
     if ((e = hip_check(hipGetLastError(), "cache_combine_kernel launch"))) return e;
   }
   if (a.wo && !a.sc) {
