@@ -2,11 +2,13 @@
 // each sequence, and rows thrown away by the attention weight they gathered.
 //
 // Eviction keeps, of a (sequence, head) with n > budget rows, the first `sink`,
-// the last `recent` and the K = budget - sink - recent greatest weights between.
-// Weights become unsigned keys of the same order; the K-th greatest is found by
-// a radix select in three digits, and one ordered pass over the rows then writes
-// the kept rows' numbers and weights (ties to the lower row: of the rows that
-// equal the K-th greatest the first are kept). Another kernel moves the rows.
+// the last `recent` and of those between the greatest weights that fill the
+// budget. Weights become unsigned keys of the same order, and the rows that are
+// kept anyway the greatest key of all, so that the kept rows are those above the
+// budget-th greatest key and, of those that equal it, the first (ties go to the
+// lower row). That key is found by a radix select in three digits; one ordered
+// pass over the rows then writes the kept rows' numbers and weights. Another
+// kernel moves the rows.
 #include "fbsa_common.h"
 #include "fbsa_internal.h"
 
@@ -56,17 +58,19 @@ __device__ __forceinline__ int evict_len(const EvictArgs &a, int b) {
   return n < 0 ? 0 : n > a.S ? a.S : n;
 }
 
-// unsigned key of the same order; NaN as -inf, -0 as 0
-__device__ __forceinline__ uint32_t weight_key(float w) {
+// Row i's key: the weight's bits in unsigned order (NaN as -inf, -0 as 0), which
+// lie in [0x007fffff, 0xff800000]; the rows that are kept whatever they weigh have
+// the greatest key of all, places past the length the least.
+__device__ __forceinline__ uint32_t row_key(const EvictArgs &a, float w, int64_t i, int n) {
   if (!(w == w)) w = -INFINITY;
-  const uint32_t u = __float_as_uint(w + 0.f);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  const uint32_t u = __float_as_uint(w + 0.f), k = u & 0x80000000u ? ~u : u | 0x80000000u;
+  return i >= n ? 0u : i < a.sink || i >= n - a.recent ? 0xffffffffu : k;
 }
 
-// The K-th greatest key is found digit by digit: 11, 11 and 10 bits.
+// The budget-th greatest key is found digit by digit: 11, 11 and 10 bits.
 constexpr int kBins = 2048;
-__device__ __forceinline__ int digit_shift(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
-__device__ __forceinline__ int digit_bits(int pass) { return pass == 2 ? 10 : 11; }
+__device__ __forceinline__ constexpr int digit_shift(int pass) { return pass == 0 ? 21 : pass == 1 ? 10 : 0; }
+__device__ __forceinline__ constexpr int digit_bits(int pass) { return pass == 2 ? 10 : 11; }
 
 // The bin of the need-th greatest key, and how many of that bin are needed, from
 // a histogram in LDS; NT threads, each NB = kBins / NT bins in descending order.
@@ -101,8 +105,39 @@ template <int NT> __device__ __forceinline__ Pick pick_bin(const uint32_t *hist,
 
 constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64;
 
+// Counts (of rows above the key, and << 16 of rows that equal it) to the sums
+// before them, in row order; the first wave.
+template <int N> __device__ __forceinline__ int counts_before(int *cnt, int lane) {
+  constexpr int PL = (N + 63) / 64;
+  int c[PL], sum = 0;
+#pragma unroll
+  for (int j = 0; j < PL; ++j) {
+    const int u = lane * PL + j;
+    c[j] = u < N ? cnt[u] : 0;
+    sum += c[j];
+  }
+  int before = sum;
+#pragma unroll
+  for (int x = 1; x < 64; x <<= 1) {
+    const int y = __shfl_up(before, x, 64);
+    if (lane >= x) before += y;
+  }
+  const int all = __shfl(before, 63, 64);
+  before -= sum;
+#pragma unroll
+  for (int j = 0; j < PL; ++j) {
+    const int u = lane * PL + j;
+    if (u < N) cnt[u] = before;
+    before += c[j];
+  }
+  return all;
+}
+
 // A workgroup per (sequence, head) whose weights stay in registers, R a thread:
-// rows tid + 1024 r.
+// rows tid + 1024 r. One workgroup to a CU, so instructions per row are what it
+// costs: keys are formed once (16 rows of up to 16301 weights: 18.2 us with the keys
+// and bounds formed in every pass, 14.6 here; four copies of the first digit's
+// counters, against lanes that count in one place, changed nothing).
 template <int R> __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int h = blockIdx.x % a.H, b = blockIdx.x / a.H;
@@ -110,32 +145,31 @@ template <int R> __global__ __launch_bounds__(kSelThreads) void evict_select_ker
   const float *w = a.w + b * a.sw[0] + h * a.sw[1];
   float *wo = a.wo + b * a.swo[0] + h * a.swo[1];
   int32_t *index = a.index + (int64_t)blockIdx.x * a.ni;
-  const int kept = n < a.budget ? n : a.budget;
-  if (h == 0 && tid == 0) a.new_lens[b] = kept;
-  for (int i = kept + tid; i < a.ni; i += kSelThreads) index[i] = -1;
-
   __shared__ uint32_t hist[kBins];
   __shared__ uint32_t s_wave[kSelWaves];
   __shared__ Pick s_pick;
-  __shared__ int s_cnt[R][kSelWaves];  // rows kept for certain and rows that equal the K-th, packed
+  __shared__ int s_cnt[R][kSelWaves];
   float x[R];
+  uint32_t key[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) x[r] = tid + r * kSelThreads < n ? w[tid + r * kSelThreads] : 0.f;
-  const int lo = a.sink, hi = n - a.recent;  // rows that the weight decides about (n > budget)
-  const bool all = n <= a.budget;
-  uint32_t need = all ? 0 : (uint32_t)(a.budget - a.recent - a.sink), prefix = 0;
-  const bool mid = need > 0;
-  if (mid) {
+  const int kept = n < a.budget ? n : a.budget;
+  if (h == 0 && tid == 0) a.new_lens[b] = kept;
+  for (int i = kept + tid; i < a.ni; i += kSelThreads) index[i] = -1;
+#pragma unroll
+  for (int r = 0; r < R; ++r) key[r] = row_key(a, x[r], tid + r * kSelThreads, n);
+  uint32_t need = 0, prefix = 0;  // (a length within the budget: every row is above key 0)
+  if (n > a.budget) {
+    need = (uint32_t)a.budget;
+#pragma unroll
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = digit_shift(pass), bits = digit_bits(pass);
       for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
       __syncthreads();
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const int i = tid + r * kSelThreads;
-        const uint32_t key = weight_key(x[r]);
-        if (i >= lo && i < hi && (pass == 0 || key >> (shift + bits) == prefix)) atomicAdd(&hist[key >> shift & ((1u << bits) - 1)], 1u);
-      }
+      for (int r = 0; r < R; ++r)
+        if (pass == 0 ? r * kSelThreads < n : key[r] >> (shift + bits) == prefix)
+          atomicAdd(&hist[key[r] >> shift & ((1u << bits) - 1)], 1u);
       __syncthreads();
       const Pick pk = pick_bin<kSelThreads>(hist, need, s_wave, &s_pick);
       prefix = prefix << bits | pk.bin;
@@ -143,57 +177,23 @@ template <int R> __global__ __launch_bounds__(kSelThreads) void evict_select_ker
       __syncthreads();
     }
   }
-  // rows above the K-th greatest key are kept, and the first `need` that equal it
   const uint64_t below = (1ull << lane) - 1;
-  auto rank = [&](int r, bool &def, bool &eq) {  // (formed twice: held, they cost registers that R = 32 has not)
-    const int i = tid + r * kSelThreads;
-    const uint32_t key = weight_key(x[r]);
-    const bool free_ = i >= lo && i < hi && !all;
-    def = i < n && (!free_ || (mid && key > prefix));
-    eq = i < n && free_ && mid && key == prefix;
-  };
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    bool def, eq;
-    rank(r, def, eq);
-    const int d = __popcll(__ballot(def)), e = __popcll(__ballot(eq));
+    const int d = __popcll(__ballot(key[r] > prefix)), e = __popcll(__ballot(key[r] == prefix));
     if (lane == 0) s_cnt[r][wave] = d | e << 16;
   }
   wait_vmcnt<0>();  // (in place: this wave's weights are here before any wave writes one)
   __syncthreads();
-  if (wave == 0) {  // counts to the sums before them, in row order
-    constexpr int PL = (R * kSelWaves + 63) / 64;
-    int *cnt = &s_cnt[0][0], c[PL], sum = 0;
-#pragma unroll
-    for (int j = 0; j < PL; ++j) {
-      const int u = lane * PL + j;
-      c[j] = u < R * kSelWaves ? cnt[u] : 0;
-      sum += c[j];
-    }
-    int before = sum;
-#pragma unroll
-    for (int x = 1; x < 64; x <<= 1) {
-      const int y = __shfl_up(before, x, 64);
-      if (lane >= x) before += y;
-    }
-    before -= sum;
-#pragma unroll
-    for (int j = 0; j < PL; ++j) {
-      const int u = lane * PL + j;
-      if (u < R * kSelWaves) cnt[u] = before;
-      before += c[j];
-    }
-  }
+  if (wave == 0) counts_before<R * kSelWaves>(&s_cnt[0][0], lane);
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < R; ++r) {
     const uint32_t c = (uint32_t)s_cnt[r][wave];
-    bool def, eq;
-    rank(r, def, eq);
-    const int d0 = (int)(c & 0xffff) + __popcll(__ballot(def) & below);
-    const int e0 = (int)(c >> 16) + __popcll(__ballot(eq) & below);
-    if (def || (eq && e0 < (int)need)) {
-      const int at = d0 + (e0 < (int)need ? e0 : (int)need);
+    const bool def = key[r] > prefix, eq = key[r] == prefix;
+    const uint32_t d0 = (c & 0xffff) + __popcll(__ballot(def) & below), e0 = (c >> 16) + __popcll(__ballot(eq) & below);
+    if (def || (eq && e0 < need)) {
+      const uint32_t at = d0 + (e0 < need ? e0 : need);
       index[at] = tid + r * kSelThreads;
       wo[at] = x[r];
     }
@@ -202,7 +202,7 @@ template <int R> __global__ __launch_bounds__(kSelThreads) void evict_select_ker
 
 // Longer rows: chunks of kChunk weights, a workgroup each, in four steps over a
 // workspace. hist: the first digit's histogram of the row. cand: the chunk's keys
-// that share the K-th greatest's first digit, in order, and how many lie above.
+// that share the wanted key's first digit, in order, and how many lie above.
 // rank (a workgroup per row): the other two digits among those, and each chunk's
 // place in the output. place: kept rows' numbers and weights.
 constexpr int kChunkR = 8, kChunk = kSelThreads * kChunkR;
@@ -211,8 +211,8 @@ struct EvictWs {
   uint32_t *cand;   // [row][chunk][kChunk]
   float *copy;      // [row][chunk][kChunk]: the weights, where they are moved in place
   uint2 *count;     // [row][chunk]: keys above the first digit, keys of it
-  uint2 *start;     // [row][chunk]: kept for certain before the chunk, equal to the K-th before it
-  uint2 *pick;      // [row]: the K-th greatest key, and how many equal to it are kept
+  uint2 *start;     // [row][chunk]: keys above the wanted one before the chunk, equal to it before it
+  uint2 *pick;      // [row]: the first digit and how many of it are kept; then the same of the whole key
   int nch;
 };
 
@@ -221,150 +221,120 @@ __global__ __launch_bounds__(256) void evict_zero_kernel(uint32_t *x, int64_t n)
   if (i < n) x[i] = 0;
 }
 
-// what the steps need to know of a row: the range that the weight decides about
-// and how many of it are kept; `mid` false: nothing to rank
-struct EvictRow {
-  int b, h, n, lo, hi;
-  uint32_t need;
-  bool all, mid;
-};
-__device__ __forceinline__ EvictRow evict_row(const EvictArgs &a, int row) {
-  EvictRow r;
-  r.h = row % a.H;
-  r.b = row / a.H;
-  r.n = evict_len(a, r.b);
-  r.lo = a.sink;
-  r.hi = r.n - a.recent;
-  r.all = r.n <= a.budget;
-  r.need = r.all ? 0 : (uint32_t)(a.budget - a.recent - a.sink);
-  r.mid = r.need > 0;
-  return r;
+// a chunk's weights and keys
+__device__ __forceinline__ void chunk_keys(const EvictArgs &a, const float *w, int64_t base, int n, float (&x)[kChunkR], uint32_t (&key)[kChunkR]) {
+#pragma unroll
+  for (int r = 0; r < kChunkR; ++r) {
+    const int64_t i = base + threadIdx.x + r * kSelThreads;
+    x[r] = i < n ? w[i] : 0.f;
+  }
+#pragma unroll
+  for (int r = 0; r < kChunkR; ++r) key[r] = row_key(a, x[r], base + threadIdx.x + r * kSelThreads, n);
 }
 
 __global__ __launch_bounds__(kSelThreads) void evict_hist_kernel(EvictArgs a, EvictWs ws) {
-  const EvictRow er = evict_row(a, blockIdx.y);
+  const int h = blockIdx.y % a.H, b = blockIdx.y / a.H, n = evict_len(a, b), kept = n < a.budget ? n : a.budget;
   const int64_t base = (int64_t)blockIdx.x * kChunk;
-  const float *w = a.w + er.b * a.sw[0] + er.h * a.sw[1];
-  if (blockIdx.x == 0) {
-    const int kept = er.n < a.budget ? er.n : a.budget;
-    if (er.h == 0 && threadIdx.x == 0) a.new_lens[er.b] = kept;
-  }
-  const int kept = er.n < a.budget ? er.n : a.budget;
+  if (blockIdx.x == 0 && h == 0 && threadIdx.x == 0) a.new_lens[b] = kept;
   for (int r = 0; r < kChunkR; ++r) {
     const int64_t i = base + threadIdx.x + r * kSelThreads;
     if (i >= kept && i < a.ni) a.index[(int64_t)blockIdx.y * a.ni + i] = -1;
   }
-  if (base >= er.n) return;
+  if (base >= n) return;
   __shared__ uint32_t hist[kBins];
   for (int i = threadIdx.x; i < kBins; i += kSelThreads) hist[i] = 0;
   float x[kChunkR];
+  uint32_t key[kChunkR];
+  chunk_keys(a, a.w + b * a.sw[0] + h * a.sw[1], base, n, x, key);
+  if (ws.copy) {
+    float *to = ws.copy + (int64_t)blockIdx.y * ws.nch * kChunk + base;
 #pragma unroll
-  for (int r = 0; r < kChunkR; ++r) {
-    const int64_t i = base + threadIdx.x + r * kSelThreads;
-    x[r] = i < er.n ? w[i] : 0.f;
-    if (ws.copy && i < er.n) ws.copy[(int64_t)blockIdx.y * ws.nch * kChunk + i] = x[r];
+    for (int r = 0; r < kChunkR; ++r) to[threadIdx.x + r * kSelThreads] = x[r];
   }
-  if (!er.mid) return;
+  if (n <= a.budget) return;
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < kChunkR; ++r) {
-    const int64_t i = base + threadIdx.x + r * kSelThreads;
-    if (i >= er.lo && i < er.hi) atomicAdd(&hist[weight_key(x[r]) >> digit_shift(0)], 1u);
-  }
+  for (int r = 0; r < kChunkR; ++r) atomicAdd(&hist[key[r] >> digit_shift(0)], 1u);
   __syncthreads();
   for (int i = threadIdx.x; i < kBins; i += kSelThreads)
     if (hist[i]) atomicAdd(&ws.hist[(int64_t)blockIdx.y * kBins + i], hist[i]);  // (whole numbers: any order gives the same)
 }
 
 __global__ __launch_bounds__(kSelThreads) void evict_cand_kernel(EvictArgs a, EvictWs ws) {
-  const EvictRow er = evict_row(a, blockIdx.y);
+  const int h = blockIdx.y % a.H, b = blockIdx.y / a.H, n = evict_len(a, b);
   const int64_t base = (int64_t)blockIdx.x * kChunk;
-  if (!er.mid || base >= er.n) return;
+  if (n <= a.budget || base >= n) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   __shared__ uint32_t hist[kBins], s_wave[kSelWaves];
   __shared__ Pick s_pick;
   __shared__ int s_cnt[kChunkR][kSelWaves];
-  const float *w = a.w + er.b * a.sw[0] + er.h * a.sw[1];
   float x[kChunkR];
-#pragma unroll
-  for (int r = 0; r < kChunkR; ++r) {
-    const int64_t i = base + tid + r * kSelThreads;
-    x[r] = i < er.n ? w[i] : 0.f;
-  }
+  uint32_t key[kChunkR];
+  chunk_keys(a, a.w + b * a.sw[0] + h * a.sw[1], base, n, x, key);
   for (int i = tid; i < kBins; i += kSelThreads) hist[i] = ws.hist[(int64_t)blockIdx.y * kBins + i];
   __syncthreads();
-  const Pick pk = pick_bin<kSelThreads>(hist, er.need, s_wave, &s_pick);
-  bool in[kChunkR];
+  const Pick pk = pick_bin<kSelThreads>(hist, (uint32_t)a.budget, s_wave, &s_pick);
 #pragma unroll
   for (int r = 0; r < kChunkR; ++r) {
-    const int64_t i = base + tid + r * kSelThreads;
-    const uint32_t top = weight_key(x[r]) >> digit_shift(0);
-    const bool free_ = i >= er.lo && i < er.hi;
-    in[r] = free_ && top == pk.bin;
-    const int above = __popcll(__ballot(free_ && top > pk.bin)), c = __popcll(__ballot(in[r]));
+    const uint32_t top = key[r] >> digit_shift(0);
+    const int c = __popcll(__ballot(top == pk.bin)), above = __popcll(__ballot(top > pk.bin));
     if (lane == 0) s_cnt[r][wave] = c | above << 16;
   }
   __syncthreads();
+  if (wave == 0) {
+    const int all = counts_before<kChunkR * kSelWaves>(&s_cnt[0][0], lane);
+    if (lane == 0) ws.count[(int64_t)blockIdx.y * ws.nch + blockIdx.x] = uint2{(uint32_t)all >> 16, (uint32_t)all & 0xffff};
+    if (lane == 0 && blockIdx.x == 0) ws.pick[blockIdx.y] = uint2{pk.bin, pk.need};
+  }
+  __syncthreads();
   uint32_t *dst = ws.cand + ((int64_t)blockIdx.y * ws.nch + blockIdx.x) * kChunk;
-  int before = 0;
 #pragma unroll
   for (int r = 0; r < kChunkR; ++r) {
-    int at = 0;
-    for (int v = 0; v < kSelWaves; ++v) {
-      if (v == wave) at = before & 0xffff;
-      before += s_cnt[r][v];
-    }
-    at += __popcll(__ballot(in[r]) & ((1ull << lane) - 1));
-    if (in[r]) dst[at] = weight_key(x[r]);
+    const bool in = key[r] >> digit_shift(0) == pk.bin;
+    const int at = (s_cnt[r][wave] & 0xffff) + __popcll(__ballot(in) & ((1ull << lane) - 1));
+    if (in) dst[at] = key[r];
   }
-  if (tid == 0) ws.count[(int64_t)blockIdx.y * ws.nch + blockIdx.x] = uint2{(uint32_t)before >> 16, (uint32_t)before & 0xffff};
-  if (tid == 0 && blockIdx.x == 0) ws.pick[blockIdx.y] = uint2{pk.bin, pk.need};
 }
 
 __global__ __launch_bounds__(kSelThreads) void evict_rank_kernel(EvictArgs a, EvictWs ws) {
-  const EvictRow er = evict_row(a, blockIdx.x);
-  if (er.all) return;
+  const int n = evict_len(a, blockIdx.x / a.H);
+  if (n <= a.budget) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int nch = (int)(((int64_t)er.n + kChunk - 1) / kChunk);
+  const int nch = (int)(((int64_t)n + kChunk - 1) / kChunk);
   const uint2 *count = ws.count + (int64_t)blockIdx.x * ws.nch;
   uint2 *start = ws.start + (int64_t)blockIdx.x * ws.nch;
   const uint32_t *cand = ws.cand + (int64_t)blockIdx.x * ws.nch * kChunk;
   __shared__ uint32_t hist[kBins], s_wave[kSelWaves];
   __shared__ Pick s_pick;
-  uint32_t prefix = 0, need = 0;
-  if (er.mid) {
-    prefix = ws.pick[blockIdx.x].x;
-    need = ws.pick[blockIdx.x].y;
-    for (int pass = 1; pass < 3; ++pass) {
-      const int shift = digit_shift(pass), bits = digit_bits(pass);
-      for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
-      __syncthreads();
-      for (int c = wave; c < nch; c += kSelWaves) {  // a wave per chunk
-        const int m = (int)count[c].y;
-        for (int i = lane; i < m; i += 64) {
-          const uint32_t key = cand[(int64_t)c * kChunk + i];
-          if (key >> (shift + bits) == prefix) atomicAdd(&hist[key >> shift & ((1u << bits) - 1)], 1u);
-        }
+  uint32_t prefix = ws.pick[blockIdx.x].x, need = ws.pick[blockIdx.x].y;
+#pragma unroll
+  for (int pass = 1; pass < 3; ++pass) {
+    const int shift = digit_shift(pass), bits = digit_bits(pass);
+    for (int i = tid; i < kBins; i += kSelThreads) hist[i] = 0;
+    __syncthreads();
+    for (int c = wave; c < nch; c += kSelWaves) {  // a wave per chunk
+      const int m = (int)count[c].y;
+      for (int i = lane; i < m; i += 64) {
+        const uint32_t key = cand[(int64_t)c * kChunk + i];
+        if (key >> (shift + bits) == prefix) atomicAdd(&hist[key >> shift & ((1u << bits) - 1)], 1u);
       }
-      __syncthreads();
-      const Pick pk = pick_bin<kSelThreads>(hist, need, s_wave, &s_pick);
-      prefix = prefix << bits | pk.bin;
-      need = pk.need;
-      __syncthreads();
     }
+    __syncthreads();
+    const Pick pk = pick_bin<kSelThreads>(hist, need, s_wave, &s_pick);
+    prefix = prefix << bits | pk.bin;
+    need = pk.need;
+    __syncthreads();
   }
-  // each chunk's rows kept for certain and equal to the K-th, then their sums before it
+  // each chunk's keys above the wanted one and equal to it, then their sums before it
   for (int c = wave; c < nch; c += kSelWaves) {
     uint32_t d = 0, e = 0;
-    const int m = er.mid ? (int)count[c].y : 0;
+    const int m = (int)count[c].y;
     for (int i0 = 0; i0 < m; i0 += 64) {
-      const uint32_t key = i0 + lane < m ? cand[(int64_t)c * kChunk + i0 + lane] : 0;
-      d += __popcll(__ballot(i0 + lane < m && key > prefix));
-      e += __popcll(__ballot(i0 + lane < m && key == prefix));
+      const uint32_t key = i0 + lane < m ? cand[(int64_t)c * kChunk + i0 + lane] : 0;  // (no candidate's key is 0)
+      d += __popcll(__ballot(key > prefix));
+      e += __popcll(__ballot(key == prefix));
     }
-    const int64_t r0 = (int64_t)c * kChunk, r1 = r0 + kChunk < er.n ? r0 + kChunk : er.n;
-    const int64_t sink = r0 < er.lo ? (r1 < er.lo ? r1 : er.lo) - r0 : 0, tail = r1 > er.hi ? r1 - (r0 > er.hi ? r0 : er.hi) : 0;
-    if (lane == 0) start[c] = uint2{(er.mid ? count[c].x : 0) + d + (uint32_t)(sink + tail), e};
+    if (lane == 0) start[c] = uint2{count[c].x + d, e};
   }
   __syncthreads();
   if (wave == 0) {
@@ -387,65 +357,48 @@ __global__ __launch_bounds__(kSelThreads) void evict_rank_kernel(EvictArgs a, Ev
 }
 
 __global__ __launch_bounds__(kSelThreads) void evict_place_kernel(EvictArgs a, EvictWs ws) {
-  const EvictRow er = evict_row(a, blockIdx.y);
+  const int h = blockIdx.y % a.H, b = blockIdx.y / a.H, n = evict_len(a, b);
   const int64_t base = (int64_t)blockIdx.x * kChunk;
-  if (base >= er.n) return;
+  if (base >= n) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const float *w = ws.copy ? ws.copy + (int64_t)blockIdx.y * ws.nch * kChunk : a.w + er.b * a.sw[0] + er.h * a.sw[1];
-  float *wo = a.wo + er.b * a.swo[0] + er.h * a.swo[1];
+  // (in place: another chunk's rows may already lie where this one's weights were)
+  const float *w = ws.copy ? ws.copy + (int64_t)blockIdx.y * ws.nch * kChunk : a.w + b * a.sw[0] + h * a.sw[1];
+  float *wo = a.wo + b * a.swo[0] + h * a.swo[1];
   int32_t *index = a.index + (int64_t)blockIdx.y * a.ni;
-  if (er.all) {
-    for (int r = 0; r < kChunkR; ++r) {
-      const int64_t i = base + tid + r * kSelThreads;
-      if (i < er.n) {
-        index[i] = (int32_t)i;
-        wo[i] = w[i];
-      }
-    }
-    return;
-  }
-  __shared__ int s_cnt[kChunkR][kSelWaves];
-  const uint2 st = ws.start[(int64_t)blockIdx.y * ws.nch + blockIdx.x], pk = ws.pick[blockIdx.y];
   float x[kChunkR];
-  bool def[kChunkR], eq[kChunkR];
-#pragma unroll
-  for (int r = 0; r < kChunkR; ++r) {
-    const int64_t i = base + tid + r * kSelThreads;
-    x[r] = i < er.n ? w[i] : 0.f;
+  uint32_t key[kChunkR];
+  chunk_keys(a, w, base, n, x, key);
+  __shared__ int s_cnt[kChunkR][kSelWaves];
+  uint2 st = uint2{(uint32_t)base, 0}, pk = uint2{0, 0};  // (a length within the budget: every row is above key 0)
+  if (n > a.budget) {
+    st = ws.start[(int64_t)blockIdx.y * ws.nch + blockIdx.x];
+    pk = ws.pick[blockIdx.y];
   }
 #pragma unroll
   for (int r = 0; r < kChunkR; ++r) {
-    const int64_t i = base + tid + r * kSelThreads;
-    const uint32_t key = weight_key(x[r]);
-    const bool free_ = i >= er.lo && i < er.hi;
-    def[r] = i < er.n && (!free_ || (er.mid && key > pk.x));
-    eq[r] = free_ && er.mid && key == pk.x;
-    const int d = __popcll(__ballot(def[r])), e = __popcll(__ballot(eq[r]));
+    const int d = __popcll(__ballot(key[r] > pk.x)), e = __popcll(__ballot(key[r] == pk.x));
     if (lane == 0) s_cnt[r][wave] = d | e << 16;
   }
   __syncthreads();
+  if (wave == 0) counts_before<kChunkR * kSelWaves>(&s_cnt[0][0], lane);
+  __syncthreads();
   const uint64_t below = (1ull << lane) - 1;
-  int before = 0;
 #pragma unroll
   for (int r = 0; r < kChunkR; ++r) {
-    int at = 0;
-    for (int v = 0; v < kSelWaves; ++v) {
-      if (v == wave) at = before;
-      before += s_cnt[r][v];
-    }
-    const uint32_t d0 = st.x + ((uint32_t)at & 0xffff) + __popcll(__ballot(def[r]) & below);
-    const uint32_t e0 = st.y + ((uint32_t)at >> 16) + __popcll(__ballot(eq[r]) & below);
-    if (def[r] || (eq[r] && e0 < pk.y)) {
-      const uint32_t o = d0 + (e0 < pk.y ? e0 : pk.y);
-      index[o] = (int32_t)(base + tid + r * kSelThreads);
-      wo[o] = x[r];
+    const uint32_t c = (uint32_t)s_cnt[r][wave];
+    const bool def = key[r] > pk.x, eq = key[r] == pk.x;
+    const uint32_t d0 = st.x + (c & 0xffff) + __popcll(__ballot(def) & below), e0 = st.y + (c >> 16) + __popcll(__ballot(eq) & below);
+    if (def || (eq && e0 < pk.y)) {
+      const uint32_t at = d0 + (e0 < pk.y ? e0 : pk.y);
+      index[at] = (int32_t)(base + tid + r * kSelThreads);
+      wo[at] = x[r];
     }
   }
 }
 
 // Rows of up to this many weights: one workgroup, weights in registers. Longer
 // ones: the steps above, whose five launches cost more than they save below it.
-constexpr int64_t kOneGroup = 32768;
+constexpr int64_t kOneGroup = 16 * kSelThreads;
 
 struct EvictPlan {
   int64_t nch;
@@ -632,8 +585,7 @@ int fbsa_cache_evict(const fbsa_evict_desc *d, const void *k, const void *v, con
     const dim3 grid(rows), wg(kSelThreads);
     if (d->S <= 2 * kSelThreads) hipLaunchKernelGGL(evict_select_kernel<2>, grid, wg, 0, s, a);
     else if (d->S <= 8 * kSelThreads) hipLaunchKernelGGL(evict_select_kernel<8>, grid, wg, 0, s, a);
-    else if (d->S <= 16 * kSelThreads) hipLaunchKernelGGL(evict_select_kernel<16>, grid, wg, 0, s, a);
-    else hipLaunchKernelGGL(evict_select_kernel<32>, grid, wg, 0, s, a);
+    else hipLaunchKernelGGL(evict_select_kernel<16>, grid, wg, 0, s, a);
     if ((e = hip_check(hipGetLastError(), "evict_select_kernel launch"))) return e;
   } else {
     char *p = (char *)workspace;

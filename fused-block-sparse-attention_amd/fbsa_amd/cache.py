@@ -32,15 +32,22 @@ _plans = {}
 _PLANS_MAX = 1024
 
 
-def _layout(ts):
-    return tuple(None if t is None else (t.shape, t.stride(), t.dtype, t.get_device()) for t in ts)
+def _key(what, scalars, ts):
+    """What a plan depends on; refuses tensors that a recorded graph would need gradients of."""
+    key, grad = [what, scalars], torch.is_grad_enabled()
+    for t in ts:
+        if t is None:
+            key.append(None)
+        else:
+            if grad and t.requires_grad:
+                raise ValueError(f"fbsa.{what}: no gradients are formed (call it under torch.no_grad())")
+            key += (t.shape, t.stride(), t.dtype, t.get_device())
+    return tuple(key)
 
 
 def _plan(what, make, scalars, ts):
     """The plan of tensors ts (None entries allowed) for the call ``what``."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        raise ValueError(f"fbsa.{what}: no gradients are formed (call it under torch.no_grad())")
-    key = (what, scalars, _layout(ts))
+    key = _key(what, scalars, ts)
     p = _plans.get(key)
     if p is None:
         dev = next(t.get_device() for t in ts if t is not None)
@@ -119,32 +126,22 @@ def _written(what, name, t):
         end = s * (e - 1) + end
 
 
-def _apart(what, name, t, nt, *others):
-    """A tensor that a kernel writes (nt bytes long) shares no memory with the
-    ones that the same call reads, given as (tensor, bytes)."""
-    lo = t.data_ptr()
-    for x, nx in others:
-        if x is not None:
-            a = x.data_ptr()
-            if a < lo + nt and lo < a + nx:
-                raise ValueError(f"fbsa.{what}: {name} is written but overlaps a tensor that the call reads")
+def _apart(what, written, read):
+    """Tensors that a kernel writes share no memory with the ones that the same
+    call reads, both given as (address, bytes). (Interleaved key and value caches
+    span the same addresses: of two written tensors only the start is compared.)"""
+    for i, (lo, n) in enumerate(written):
+        for a, m in read:
+            if a < lo + n and lo < a + m:
+                raise ValueError(f"fbsa.{what}: a tensor that is written overlaps one that the call reads")
+        for a, m in written[:i]:
+            if a == lo and n and m:
+                raise ValueError(f"fbsa.{what}: two written tensors are the same buffer")
 
 
-def _aligned(what, name, *ts):
-    for t in ts:
-        if t is not None and t.data_ptr() & 15:
-            raise ValueError(f"fbsa.{what}: {name} must be 16-byte aligned")
-
-
-def _ready(t, ok):
-    """t itself, or a copy whose rows the kernels can load 16 bytes at a time."""
-    return t if ok and not t.data_ptr() & 15 else t.clone(memory_format=torch.contiguous_format)
-
-
-def _same_buffer(what, k, v):
-    # (interleaved caches span the same addresses, so only the plain mistake is seen here)
-    if k.data_ptr() == v.data_ptr() and k.numel():
-        raise ValueError(f"fbsa.{what}: the key and value caches are the same buffer")
+def _aligned(what, addresses):
+    if addresses & 15:
+        raise ValueError(f"fbsa.{what}: caches and prefixes must be 16-byte aligned")
 
 
 # ---- the operators ----------------------------------------------------------
@@ -194,13 +191,11 @@ def append(k, v, k_new, v_new, start, *, count=None, weight=None):
         k_new, v_new = (t.clone(memory_format=torch.contiguous_format) for t in (k_new, v_new))
         return append(k, v, k_new, v_new, start, count=count, weight=weight)
     nk, nv, nkn, nvn = p.bytes
-    _aligned("append", "a cache", k, v)
-    _same_buffer("append", k, v)
-    _apart("append", "k", k, nk, (k_new, nkn), (v_new, nvn))
-    _apart("append", "v", v, nv, (k_new, nkn), (v_new, nvn))
+    pk, pv, pkn, pvn = k.data_ptr(), v.data_ptr(), k_new.data_ptr(), v_new.data_ptr()
+    _aligned("append", pk | pv)
+    _apart("append", ((pk, nk), (pv, nv)), ((pkn, nkn), (pvn, nvn)))
     start, count = _int32(start), _int32(count)
-    _launch(p, _lib.load().fbsa_cache_append, "fbsa_cache_append", k.data_ptr(), v.data_ptr(), k_new.data_ptr(),
-            v_new.data_ptr(), start.data_ptr(), _ptr(count), _ptr(weight))
+    _launch(p, _lib.load().fbsa_cache_append, "fbsa_cache_append", pk, pv, pkn, pvn, start.data_ptr(), _ptr(count), _ptr(weight))
 
 
 def _plan_attend(what, scalars, q, kp, vp, k, v, lens, count, out_gate, weight, out_weight):
@@ -272,17 +267,17 @@ def _attend(what, q, kp, vp, k, v, lens, count, scale, out_gate, weight, out_wei
             return _attend(what, q, kp, vp, k, v, lens, count, scale, out_gate, weight, out_weight, need_lse)
     if out_gate is not None and not p.gate_ok:
         out_gate = out_gate.clone(memory_format=torch.contiguous_format)
-    _aligned(what, "a cache or prefix", k, v)
-    if p.P:
-        _aligned(what, "a cache or prefix", kp, vp)
-    if out_weight is not None and not (p.same and weight.data_ptr() == out_weight.data_ptr()):
-        _apart(what, "out_weight", out_weight, p.bytes[0], (weight, p.bytes[1]))
+    pk, pv = k.data_ptr(), v.data_ptr()
+    pkp, pvp = (kp.data_ptr(), vp.data_ptr()) if p.P else (None, None)
+    _aligned(what, pk | pv | pkp | pvp if p.P else pk | pv)
+    pw, pwo = _ptr(weight), _ptr(out_weight)
+    if pw is not None and not (p.same and pw == pwo):
+        _apart(what, ((pwo, p.bytes[0]),), ((pw, p.bytes[1]),))
     lens = torch.full(p.shape[:1], p.S, dtype=torch.int32, device=p.device) if lens is None else _int32(lens)
     count = _int32(count)
     ws = torch.empty(p.nbytes, dtype=torch.uint8, device=p.device)
-    _launch(p, _lib.load().fbsa_cache_attn, what, q.data_ptr(), k.data_ptr(), v.data_ptr(), lens.data_ptr(), _ptr(count),
-            kp.data_ptr() if p.P else None, vp.data_ptr() if p.P else None, _ptr(out_gate), o.data_ptr(), _ptr(lse),
-            _ptr(weight), _ptr(out_weight), ws.data_ptr(), p.nbytes)
+    _launch(p, _lib.load().fbsa_cache_attn, what, q.data_ptr(), pk, pv, lens.data_ptr(), _ptr(count), pkp, pvp,
+            _ptr(out_gate), o.data_ptr(), _ptr(lse), pw, pwo, ws.data_ptr(), p.nbytes)
     return (o, lse) if need_lse else o
 
 
@@ -376,21 +371,22 @@ def evict(k, v, weight, lens, budget, *, recent=0, sink=0, out=None):
     if out is not None and any(t is None for t in out):
         raise ValueError("fbsa.evict: out must be (k_out, v_out, weight_out)")
     p = _plan("evict", _plan_evict, (int(budget), int(recent), int(sink)), (k, v, weight, lens, ko, vo, wo))
+    pk, pv, pw = k.data_ptr(), v.data_ptr(), weight.data_ptr()
     if p.inplace:
-        ko, vo, wo = k, v, weight
+        pko, pvo, pwo = pk, pv, pw
     else:
+        pko, pvo, pwo = ko.data_ptr(), vo.data_ptr(), wo.data_ptr()
         nk, nv, nw, nko, nvo, nwo = p.bytes
-        read = ((k, nk), (v, nv), (weight, nw))
-        for name, t, n in (("k_out", ko, nko), ("v_out", vo, nvo), ("weight_out", wo, nwo)):
-            _apart("evict", name, t, n, *read)
-    _same_buffer("evict", ko, vo)
-    _aligned("evict", "a cache", k, v, ko, vo)
+        _apart("evict", ((pko, nko), (pvo, nvo), (pwo, nwo)), ((pk, nk), (pv, nv), (pw, nw)))
+    if pk == pv:
+        raise ValueError("fbsa.evict: the key and value caches are the same buffer")
+    _aligned("evict", pk | pv | pko | pvo)
     lens = _int32(lens)
     index = torch.empty(p.shape, dtype=torch.int32, device=p.device)
     new_lens = torch.empty(p.B, dtype=torch.int32, device=p.device)
     ws = torch.empty(p.nbytes, dtype=torch.uint8, device=p.device) if p.nbytes else None
-    _launch(p, _lib.load().fbsa_cache_evict, "fbsa_cache_evict", k.data_ptr(), v.data_ptr(), weight.data_ptr(), lens.data_ptr(),
-            ko.data_ptr(), vo.data_ptr(), wo.data_ptr(), index.data_ptr(), new_lens.data_ptr(), _ptr(ws), p.nbytes)
+    _launch(p, _lib.load().fbsa_cache_evict, "fbsa_cache_evict", pk, pv, pw, lens.data_ptr(), pko, pvo, pwo, index.data_ptr(),
+            new_lens.data_ptr(), _ptr(ws), p.nbytes)
     return index, new_lens
 
 

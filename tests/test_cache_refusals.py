@@ -135,13 +135,16 @@ def test_written_tensors_must_not_overlap_themselves():
     with pytest.raises(ValueError, match="overlap"):
         cache._written("t", "x", x.as_strided((2, 8, 16), (64, 16, 1)))
     with pytest.raises(ValueError, match="reads"):
-        cache._apart("t", "x", x[0], cache._bytes(x[0]), (x[0, 4:], cache._bytes(x[0, 4:])))
-    cache._apart("t", "x", x[0], cache._bytes(x[0]), (x[1], cache._bytes(x[1])), (None, 0))
+        cache._apart("t", ((64, 64),), ((0, 8), (120, 200)))
+    with pytest.raises(ValueError, match="same buffer"):
+        cache._apart("t", ((64, 64), (64, 32)), ())
+    cache._apart("t", ((64, 64), (128, 64)), ((0, 64), (192, 8)))
+    assert cache._bytes(x[0, 4:]) == 4 * 16 * 4 and cache._bytes(x[:, :, :1]) == (8 * 16 + 7 * 16 + 1) * 4
 
 
 def test_plans_follow_layouts_not_addresses():
     def key(*ts):
-        return hash((cache._layout(ts)))
+        return hash(cache._key("t", (1, None), ts))
     x = torch.zeros(2, 8, 16)
     assert key(x, None) == key(torch.ones(2, 8, 16), None)
     assert key(x) != key(x.half()) and key(x) != key(x.transpose(0, 1)) and key(x, x) != key(x, None)
