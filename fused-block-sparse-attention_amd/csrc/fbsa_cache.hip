@@ -21,6 +21,8 @@
 // Lengths are read on the device; nothing depends on launch order.
 #include <math.h>
 
+#include <algorithm>
+
 #include "fbsa_common.h"
 #include "fbsa_internal.h"
 #include "fbsa_tiles.h"
@@ -48,7 +50,7 @@ struct CacheArgs {
   float2 *stat;              // [tile, share][row] row maximum (log2 domain), row sum
   float *wpart;              // [row share][B][Hkv][S] weights, where the rows are shared out
   float *lse2;               // [B][Hkv][TG] log2-domain lse, -inf for rows that see nothing
-  float *sc;                 // [B][Hkv][TG][S rounded up to 32] log2-domain scores (few_own, with weights)
+  float *sc;                 // [B][Hkv][TG][S rounded up to 32] log2-domain scores (up to 16 rows, with weights)
 };
 
 // keys per chunk of a wave's ring: 32; 16 where a row is 512 bytes or more, so that
@@ -515,6 +517,14 @@ __global__ __launch_bounds__(NW * 64) void cache_tile_kernel(CacheArgs a, int64_
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) mask_keys<NM>(s[qt], (ri[qt].valid ? ri[qt].lim : keys) - c * KC, g);
     }
+    if (!pre && a.sc && ri[0].valid) {  // (one tile of up to 16 rows: the first fragment)
+      float *score = a.sc + score_row(a, ri[0].b, ri[0].hq / a.G, p);
+#pragma unroll
+      for (int m = 0; m < NM; ++m) {
+        const int64_t key = (int64_t)c * KC + 16 * m + 4 * g;
+        if (key < score_keys(a)) *(f32x4 *)(score + key) = s[0][m] * a.scale2;
+      }
+    }
     float x[QT][NM][4];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) sm[qt].template step<NM>(s[qt], a.scale2, x[qt]);
@@ -912,7 +922,7 @@ static int64_t tile_rows(int dtype, int64_t rows) {
 struct CachePlan {
   int64_t tr_own, tr_pre, rt_own, rt_pre, np_own, np_pre, rows, DP;
   int64_t nz;  // shares of the rows in the weights of many rows
-  bool few_own, few_pre, direct;
+  bool few_own, few_pre, direct, scores;  // scores: weights from stored scores (16 rows or fewer)
   size_t stat, part, lse2, wpart, sc, total;
 };
 static CachePlan cache_plan(const fbsa_cache_desc *d) {
@@ -920,9 +930,17 @@ static CachePlan cache_plan(const fbsa_cache_desc *d) {
   const int64_t G = d->Hq / d->Hkv, TG = d->T * G;
   p.DP = d->D <= 32 ? 32 : d->D <= 64 ? 64 : d->D <= 128 ? 128 : 256;
   const int64_t pre_rows = d->B * TG;
-  p.few_own = TG <= 16;
   p.few_pre = pre_rows <= 16;
-  p.tr_own = p.few_own ? 16 : tile_rows(d->dtype, TG);
+  // own tiles of few rows and keys beside a prefix that takes the tile kernel: they
+  // go into its launch, a tile of 16 rows each, instead of one of their own (64
+  // sequences, 16 heads over 2, d 256, up to 512 own rows: 38 us against 43; small
+  // batches 25 to 35% less; fp32, whose single wave is slow: 157 us against 107 at
+  // 1209 rows, so only short ones)
+  const int64_t seqs = d->B * d->Hkv, beside = std::min(cdiv(d->S, 256), std::max<int64_t>(1, 2 * kCUs / seqs));
+  const bool merge = TG <= 16 && d->P && !p.few_pre && seqs <= 2 * kCUs && cdiv(d->S, beside) <= (d->dtype == FBSA_F32 ? 128 : 1024);
+  p.scores = TG <= 16;
+  p.few_own = TG <= 16 && !merge;
+  p.tr_own = p.scores ? 16 : tile_rows(d->dtype, TG);
   p.tr_pre = p.few_pre ? 16 : tile_rows(d->dtype, pre_rows);
   p.rt_own = cdiv(TG, p.tr_own);
   p.rt_pre = d->P ? cdiv(pre_rows, p.tr_pre) : 0;
@@ -939,7 +957,7 @@ static CachePlan cache_plan(const fbsa_cache_desc *d) {
     const int64_t n = want < most ? want : most;
     return n < kMaxShares / 2 ? n : kMaxShares / 2;
   };
-  p.np_own = shares(p.few_own, d->B > 1, d->B * d->Hkv * p.rt_own, d->S);
+  p.np_own = merge ? beside : shares(p.few_own, d->B > 1, d->B * d->Hkv * p.rt_own, d->S);
   p.np_pre = d->P ? shares(p.few_pre, false, d->Hkv * p.rt_pre, d->P) : 0;
   p.direct = !p.few_own && !d->P && p.np_own == 1;
   p.rows = d->B * d->Hkv * p.rt_own * p.np_own * p.tr_own + d->Hkv * p.rt_pre * p.np_pre * p.tr_pre;
@@ -951,8 +969,8 @@ static CachePlan cache_plan(const fbsa_cache_desc *d) {
   p.nz = z < zmax ? z : zmax;
   const bool weight = d->flags & FBSA_CACHE_WEIGHT;
   p.wpart = p.lse2 + up256((size_t)(d->B * d->Hkv * TG) * 4);
-  p.sc = p.wpart + (weight && !p.few_own && p.nz > 1 ? up256((size_t)p.nz * d->B * d->Hkv * d->S * 4) : 0);
-  p.total = p.sc + (weight && p.few_own ? up256((size_t)(d->B * d->Hkv * TG) * cdiv(d->S, 32) * 128) : 0);
+  p.sc = p.wpart + (weight && !p.scores && p.nz > 1 ? up256((size_t)p.nz * d->B * d->Hkv * d->S * 4) : 0);
+  p.total = p.sc + (weight && p.scores ? up256((size_t)(d->B * d->Hkv * TG) * cdiv(d->S, 32) * 128) : 0);
   return p;
 }
 
@@ -981,9 +999,12 @@ template <typename T, int DP> static int launch_cache(const CacheArgs &a, int64_
   if (e) return e;
   const int64_t rows = (int64_t)a.B * a.Hkv * a.TG;
   const int64_t nown = (int64_t)a.B * a.Hkv * a.rt_own * a.np_own, npre = (int64_t)a.Hkv * a.rt_pre * a.np_pre;
-  // prefix and own tiles in one launch where one workgroup size serves both
-  const bool both = npre && !a.few_pre && !a.few_own && (a.tr_own <= 64) == (a.tr_pre <= 64);
-  if (npre && !a.few_pre && (e = launch_tiles_of<T, DP>(a, a.tr_pre, npre, both ? nown : 0, s))) return e;
+  // prefix and own tiles in one launch where one workgroup size serves both, or
+  // where the own ones are few enough to sit beside the others in larger ones (90
+  // rows a head over 138 shared keys and up to 728 own: 17 -> 12 us)
+  const bool both = npre && !a.few_pre && !a.few_own && (a.TG <= 16 || (a.tr_own <= 64) == (a.tr_pre <= 64) || nown <= 2 * kCUs);
+  const int tr = both && a.tr_own > a.tr_pre ? a.tr_own : a.tr_pre;
+  if (npre && !a.few_pre && (e = launch_tiles_of<T, DP>(a, tr, npre, both ? nown : 0, s))) return e;
   if (!a.few_own && !both && (e = launch_tiles_of<T, DP>(a, a.tr_own, 0, nown, s))) return e;
   const int64_t parts = (a.few_own ? nown : 0) + (a.few_pre ? npre : 0);
   if (parts) {
@@ -1102,7 +1123,7 @@ int fbsa_cache_attn(const fbsa_cache_desc *d, const void *q, const void *k, cons
   a.qxor = d->scale < 0.f ? (d->dtype == FBSA_F32 ? 0x80000000u : 0x80008000u) : 0u;
   char *ws = (char *)workspace;
   a.stat = (float2 *)(ws + pl.stat); a.part = (float *)(ws + pl.part);
-  if (out_weight && pl.few_own) a.sc = (float *)(ws + pl.sc);
+  if (out_weight && pl.scores) a.sc = (float *)(ws + pl.sc);
   else if (out_weight) { a.lse2 = (float *)(ws + pl.lse2); a.wpart = (float *)(ws + pl.wpart); }
   switch (d->dtype) {
     case FBSA_BF16: return dispatch_cache<bf16>(a, pl, (hipStream_t)stream);
