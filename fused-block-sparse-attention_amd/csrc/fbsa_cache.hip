@@ -201,14 +201,18 @@ template <int NM> __device__ __forceinline__ void mask_keys(f32x4 (&s)[NM], int 
       if (16 * m + 4 * g + r >= lim) s[m][r] = -INFINITY;
 }
 
-// o[d .. d + 3] = acc * inv [* sigmoid(gate)] of a row
+// o[d .. d + 3] = acc * inv [* sigmoid(gate)] of a row; inv 0: a row that sees
+// nothing, 0 whatever its gate holds
 template <typename T> __device__ __forceinline__ void store_row(const CacheArgs &a, const RowInfo &ri, f32x4 acc, float inv, int d) {
   if (d >= a.D) return;
   T *orow = (T *)a.o + ri.b * a.so[0] + ri.hq * a.so[1] + ri.t * a.so[2] + d;
   float y[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) y[r] = acc[r] * inv;
-  if (a.og) {
+  if (inv == 0.f) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) y[r] = 0.f;
+  } else if (a.og) {
     const T *og = (const T *)a.og + ri.b * a.sog[0] + ri.hq * a.sog[1] + ri.t * a.sog[2] + d;
 #pragma unroll
     for (int r = 0; r < 4; ++r) y[r] *= 1.f / (1.f + __expf(-to_f32<T>(og[r])));
@@ -936,7 +940,8 @@ static CachePlan cache_plan(const fbsa_cache_desc *d) {
   // sequences, 16 heads over 2, d 256, up to 512 own rows: 38 us against 43; small
   // batches 25 to 35% less; fp32, whose single wave is slow: 157 us against 107 at
   // 1209 rows, so only short ones)
-  const int64_t seqs = d->B * d->Hkv, beside = std::min(cdiv(d->S, 256), std::max<int64_t>(1, 2 * kCUs / seqs));
+  const int64_t seqs = d->B * d->Hkv;
+  const int64_t beside = std::min({cdiv(d->S, 256), std::max<int64_t>(1, 2 * kCUs / seqs), (int64_t)kMaxShares / 2});
   const bool merge = TG <= 16 && d->P && !p.few_pre && seqs <= 2 * kCUs && cdiv(d->S, beside) <= (d->dtype == FBSA_F32 ? 128 : 1024);
   p.scores = TG <= 16;
   p.few_own = TG <= 16 && !merge;
@@ -1072,8 +1077,8 @@ static int check_cache(const fbsa_cache_desc *d) {
   const int64_t rs[4] = {d->sk[2], d->sv[2], d->P ? d->skp[1] : 0, d->P ? d->svp[1] : 0};
   for (int64_t r : rs)
     if (r * es >= 1LL << 26) return fail(FBSA_EUNSUPPORTED, "%s: a row stride of %lld elements is 64 MiB or more", fn, (long long)r);
-  const CachePlan pl = cache_plan(d);
-  if (pl.rows > lim || d->B * d->Hkv * (d->T * (d->Hq / d->Hkv) + cdiv(d->S, kWeightKeys)) > lim) return fail(FBSA_EUNSUPPORTED, "%s: grid too large", fn);
+  // (a launch has fewer than 2^32 threads: 64 a row where a wave joins each)
+  if (cache_plan(d).rows > lim || d->B * d->Hq * d->T > 0x3ff0000LL) return fail(FBSA_EUNSUPPORTED, "%s: grid too large", fn);
   return FBSA_OK;
 }
 

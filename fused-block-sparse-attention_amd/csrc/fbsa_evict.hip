@@ -481,7 +481,7 @@ static int check_rows(const char *fn, int dtype, int64_t D, const int64_t (*cons
   return FBSA_OK;
 }
 
-constexpr int64_t kMaxRows = 0x7fff0000LL;
+constexpr int64_t kMaxRows = 0x7fff0000LL, kMaxThreads = 0xfffff000LL;  // (a launch has fewer than 2^32 threads)
 
 }  // namespace fbsa
 
@@ -503,7 +503,7 @@ int fbsa_cache_append(const fbsa_append_desc *d, void *k, void *v, const void *k
                 (long long)d->T, (long long)d->S);
   const int64_t es = d->dtype == FBSA_F32 ? 4 : 2, cpr = d->D * es / 16;
   if (d->B > kMaxRows || d->H > kMaxRows || d->T > kMaxRows || d->S > kMaxRows || d->B > kMaxRows / d->H ||
-      d->B * d->H > kMaxRows / d->T || (d->B * d->H * d->T * cpr + 255) / 256 > kMaxRows)
+      d->B * d->H > kMaxRows / d->T || d->B * d->H * d->T * cpr > kMaxThreads)
     return fail(FBSA_EUNSUPPORTED, "%s: sizes exceed the grid or 32-bit row indices", fn);
   if (!k || !v || !k_new || !v_new || !start) return fail(FBSA_EINVAL, "%s: null tensor pointer", fn);
   if (!aligned_to(k, 16) || !aligned_to(v, 16) || !aligned_to(k_new, 16) || !aligned_to(v_new, 16) || !aligned_to(start, 4) ||
@@ -537,7 +537,8 @@ static int check_evict(const fbsa_evict_desc *d) {
                 (long long)d->sink, (long long)d->budget);
   const int64_t ni = d->budget < d->S ? d->budget : d->S;
   if (d->SO < ni) return fail(FBSA_EINVAL, "%s: output capacity %lld is below %lld", fn, (long long)d->SO, (long long)ni);
-  if (d->S > kMaxRows || d->budget > kMaxRows || d->B > 65535 || d->H > 65535 || d->B * d->H > 65535)
+  const int64_t cpr = d->D * (d->dtype == FBSA_F32 ? 4 : 2) / 16;
+  if (d->S > kMaxRows || d->budget > kMaxRows || ni * cpr > kMaxThreads || d->B > 65535 || d->H > 65535 || d->B * d->H > 65535)
     return fail(FBSA_EUNSUPPORTED, "%s: sizes exceed the grid or 32-bit row indices", fn);
   return FBSA_OK;
 }

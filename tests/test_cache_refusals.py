@@ -36,7 +36,7 @@ def test_struct_layouts():
     ({"dtype": 5}, "dtype"), ({"flags": 2}, "flags"), ({"T": 0}, "positive"), ({"S": 0}, "positive"), ({"P": -1}, "positive"),
     ({"Hkv": 3}, "multiple"), ({"D": 60}, "head dim"), ({"D": 264}, "head dim"), ({"scale": float("nan")}, "scale"),
     ({"S": 1 << 31}, "32-bit"), ({"B": 40000}, "grid"), ({"sk": (8192, 4096, 63)}, "stride"), ({"sv": (8192, -64, 64)}, "stride"),
-    ({"sk": (0, 0, 1 << 26)}, "64 MiB"), ({"P": 8, "skp": (512, 60)}, "k_prefix"),
+    ({"sk": (0, 0, 1 << 26)}, "64 MiB"), ({"B": 64, "T": 1 << 19}, "grid"), ({"P": 8, "skp": (512, 60)}, "k_prefix"),
 ])
 def test_attention_descriptor(kw, needle):
     lib = _lib.load()
@@ -78,6 +78,7 @@ def _evict(**kw):
 @pytest.mark.parametrize("kw,needle", [
     ({"dtype": -1}, "dtype"), ({"flags": 2}, "flags"), ({"budget": 0}, "positive"), ({"recent": 61}, "budget"),
     ({"sink": -1}, "budget"), ({"SO": 63}, "capacity"), ({"D": 4}, "head dim"), ({"B": 70000}, "grid"),
+    ({"D": 256, "S": 1 << 28, "SO": 1 << 28, "budget": 1 << 28}, "grid"),
     ({"sko": (0, 0, 7)}, "stride"), ({"flags": 1}, "not the inputs"),
 ])
 def test_evict_descriptor(kw, needle):
@@ -100,7 +101,7 @@ def test_evict_pointers():
 
 
 @pytest.mark.parametrize("kw,needle", [({"T": 0}, "positive"), ({"D": 12}, "head dim"), ({"flags": 1}, "flags"),
-                                       ({"skn": (1, 1, 1)}, "stride"), ({"B": 1 << 20, "H": 1 << 20}, "grid")])
+                                       ({"skn": (1, 1, 1)}, "stride"), ({"B": 1 << 20, "H": 1 << 20}, "grid"), ({"B": 1 << 14, "H": 1 << 7, "T": 300}, "grid")])
 def test_append_descriptor(kw, needle):
     d = _lib.AppendDesc()
     d.dtype, d.B, d.H, d.T, d.S, d.D = _lib.BF16, 1, 2, 1, 16, 64

@@ -135,6 +135,27 @@ def test_stacked_prefix_rows():
     _run("bf16", 37, 8, 2, 2, 40, 128, [3 + b for b in range(37)], P=1000)
 
 
+@pytest.mark.parametrize("T,P", [(2, 0), (40, 0), (2, 50), (40, 300)])
+def test_padding_may_hold_anything(T, P):
+    """Queries and gates past a sequence's count, and rows past its length, are NaN."""
+    count, lens = [T, T // 2, 0], [T + 60, T // 2, 9]
+    q, k, v, kp, vp, g = _make("bf16", 3, 8, 2, T, T + 60, 64, lens, P=P)
+    og, w = _randn(g, 3, 8, T, 64, dtype=q.dtype), _randn(g, 3, 2, T + 60).abs()
+    bad = [x.clone() for x in (q, og)]
+    for b, c in enumerate(count):
+        for x in bad:
+            x[b, :, c:] = math.nan
+    a, b = torch.zeros_like(w), torch.zeros_like(w)
+
+    def call(q, og, out):
+        kw = dict(count=_ints(count), out_gate=og, weight=w, out_weight=out, need_lse=True)
+        return (cache.shared_prefix_attention(q, kp, vp, k, v, _ints(lens), **kw) if P else
+                cache.cache_attention(q, k, v, _ints(lens), **kw))
+    want, got = call(q, og, a), call(*bad, b)
+    assert torch.equal(want[0], got[0]) and torch.equal(want[1], got[1]) and torch.equal(a, b)
+    assert (got[0][2] == 0).all() and not torch.isnan(b).any()
+
+
 def test_weight_in_place_from_nothing_and_absent():
     q, k, v, _, _, g = _make("bf16", 2, 4, 2, 1, 100, 64, [100, 60])
     lens, w = _ints([100, 60]), _randn(g, 2, 2, 100).abs()
@@ -170,6 +191,19 @@ def test_far_rows_and_sequences():
     lens = _ints([140, 133])
     o = cache.cache_attention(q, k, v, lens, weight=w)
     assert torch.equal(o, cache.cache_attention(q, *near, lens))
+    # many rows, and far-apart queries, prefixes and outputs of an eviction
+    q = torch.empty(B * 2 * 40 * (1 << 23), dtype=torch.bfloat16, device=DEV).as_strided(
+        (B, 2, 40, D), (2 * 40 * (1 << 23), 40 * (1 << 23), 1 << 23, 1)).copy_(_randn(g, B, 2, 40, D))
+    a, b = torch.zeros_like(w), torch.zeros_like(w)
+    o = cache.shared_prefix_attention(q, k[1], v[1], k, v, lens, out_weight=a)
+    assert torch.equal(o, cache.shared_prefix_attention(q.contiguous(), near[0][1], near[1][1], *near, lens, out_weight=b))
+    assert torch.equal(a, b)
+    wide = (big.as_strided((B, 1, 70, D), (S * (1 << 24), 0, 1 << 24, 1), 8192), big.as_strided(
+        (B, 1, 70, D), (S * (1 << 24), 0, 1 << 24, 1), 12288), torch.zeros(B, 1, 70, device=DEV))
+    with pytest.raises(ValueError, match="overlaps"):
+        cache.evict(k, v, w, lens, 70, out=wide)  # (interleaved rows of one buffer: told apart by their span only)
+    thin = tuple(x.contiguous() for x in wide)
+    assert torch.equal(cache.evict(k, v, w, lens, 70, out=thin)[0], cache.evict(*near, w, lens, 70, out=thin)[0])
     new = [_randn(g, B, 1, 3, D, dtype=torch.bfloat16) for _ in range(2)]
     for caches in ((k, v), near):
         cache.append(*caches, *new, _ints([136, 130]))
