@@ -627,50 +627,65 @@ constexpr int kWeightKeys = 1024;  // keys of a weight workgroup
 
 // Workgroups [0, rows): a row each. Groups of DP / 4 threads take every NG-th
 // part, a float4 a thread, and are added in order at the end.
-// Workgroups past them (a.sc): kWeightKeys keys of a (sequence, KV head): each row's
+// Workgroups past them (WEIGHT): kWeightKeys keys of a (sequence, KV head): each row's
 // lse from its parts' statistics, then weight + sum over rows of exp2(score - lse).
-template <typename T, int DP> __global__ __launch_bounds__(256) void cache_combine_kernel(CacheArgs a) {
+template <typename T, int DP, bool WEIGHT> __global__ __launch_bounds__(256) void cache_combine_kernel(CacheArgs a) {
   constexpr int LG = DP / 4, NG = 256 / LG;
   __shared__ float s_f[kMaxShares];
   __shared__ f32x4 s_acc[256];
   __shared__ float s_red[8];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int64_t rows = (int64_t)a.B * a.Hkv * a.TG;
-  if (blockIdx.x >= rows) {
-    const int per = (a.S + kWeightKeys - 1) / kWeightKeys;
-    const int64_t u = blockIdx.x - rows;
+  const uint32_t rows = (uint32_t)a.B * a.Hkv * a.TG;
+  if (WEIGHT && blockIdx.x >= rows) {
+    const uint32_t per = (uint32_t)(a.S + kWeightKeys - 1) / kWeightKeys, u = blockIdx.x - rows;
     const int key0 = (int)(u % per) * kWeightKeys, hk = (int)(u / per % a.Hkv), b = (int)(u / per / a.Hkv);
     const int n = seq_len(a, b), c = seq_count(a, b);
     if (key0 >= n) return;
     __shared__ float s_lse[16];
     const int real = min(c * a.G, a.TG);  // rows of real queries
-    for (int rho = wave; rho < real; rho += 4) {
-      const RowParts rp = row_parts(a, b, hk, rho);
-      float m = -INFINITY, l = 0.f;
-      for (int i = lane; i < rp.n; i += 64) m = fmaxf(m, a.stat[rp.at(a, i)].x);
-#pragma unroll
-      for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, shfl_xor_f(m, x));
-      const float ref = m == -INFINITY ? 0.f : m;
-      for (int i = lane; i < rp.n; i += 64) {
-        const float2 st = a.stat[rp.at(a, i)];
-        if (st.y != 0.f) l += __builtin_amdgcn_exp2f(st.x - ref) * st.y;
-      }
-#pragma unroll
-      for (int x = 1; x < 64; x <<= 1) l += shfl_xor_f(l, x);
-      if (lane == 0) s_lse[rho] = l == 0.f ? -INFINITY : m + __log2f(l);
-    }
-    __syncthreads();
     const float *sc = a.sc + score_row(a, b, hk, 0);
     const int64_t step = score_row(a, 0, 0, 1);
-    // four keys a thread, four rows' scores in flight (rows of scores are whole multiples of 32)
+    // four keys a thread, four rows' scores in flight (rows of scores are whole
+    // multiples of 32); the first and the weights are asked for before the lse is known
     static_assert(kWeightKeys == 4 * 256, "four keys to a thread");
-    const int key = key0 + 4 * tid;
-    if (key >= n) return;
-    f32x4 w = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int r0 = 0; r0 < real; r0 += 4) {
-      f32x4 x[4];
+    const int key = key0 + 4 * tid, at = key < n ? key : key0;
+    f32x4 x[4], w = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto load = [&](int r0) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = *(const f32x4 *)(sc + (r0 + j < real ? r0 + j : r0) * step + key);
+      for (int j = 0; j < 4; ++j) x[j] = *(const f32x4 *)(sc + (r0 + j < real ? r0 + j : r0) * step + at);
+    };
+    if (real) load(0);
+    float w0[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w0[e] = a.w && key + e < n ? a.w[b * a.sw[0] + hk * a.sw[1] + key + e] : 0.f;
+    // 16 lanes a row: the parts' statistics joined as they come
+    {
+      const int rho = tid >> 4;
+      float m = -INFINITY, l = 0.f;
+      auto join = [&](float m2, float l2) {
+        if (l2 == 0.f) return;
+        const float mn = fmaxf(m, m2);
+        l = l * __builtin_amdgcn_exp2f(m - mn) + l2 * __builtin_amdgcn_exp2f(m2 - mn);
+        m = mn;
+      };
+      if (rho < real) {
+        const RowParts rp = row_parts(a, b, hk, rho);
+        for (int i = tid & 15; i < rp.n; i += 16) {
+          const float2 st = a.stat[rp.at(a, i)];
+          join(st.x, st.y);
+        }
+      }
+#pragma unroll
+      for (int y = 1; y < 16; y <<= 1) {
+        const float m2 = shfl_xor_f(m, y), l2 = shfl_xor_f(l, y);
+        join(m2, l2);
+      }
+      if ((tid & 15) == 0) s_lse[rho] = l == 0.f ? -INFINITY : m + __log2f(l);
+    }
+    __syncthreads();
+    if (key >= n) return;
+    for (int r0 = 0; r0 < real; r0 += 4) {
+      if (r0) load(r0);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const float l2 = r0 + j < real ? s_lse[r0 + j] : -INFINITY;
@@ -683,10 +698,7 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void cache_combi
     }
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      if (key + e < n) {
-        const float w0 = a.w ? a.w[b * a.sw[0] + hk * a.sw[1] + key + e] : 0.f;
-        a.wo[b * a.swo[0] + hk * a.swo[1] + key + e] = w0 + w[e];
-      }
+      if (key + e < n) a.wo[b * a.swo[0] + hk * a.swo[1] + key + e] = w0[e] + w[e];
     return;
   }
   const int rho = (int)(blockIdx.x % a.TG), hk = (int)(blockIdx.x / a.TG % a.Hkv), b = (int)(blockIdx.x / a.TG / a.Hkv);
@@ -700,8 +712,11 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void cache_combi
 #pragma unroll
   for (int j = 0; j < U; ++j)
     if (gi + j * NG < n) ahead[j] = *(const f32x4 *)(a.part + rp.at(a, gi + j * NG) * DP + 4 * e);
-  float m = -INFINITY;
-  for (int i = tid; i < n; i += 256) m = fmaxf(m, a.stat[rp.at(a, i)].x);
+  static_assert(kMaxShares <= 2 * 256, "two parts to a thread");
+  float2 st[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) st[j] = tid + 256 * j < n ? a.stat[rp.at(a, tid + 256 * j)] : float2{-INFINITY, 0.f};
+  float m = fmaxf(st[0].x, st[1].x);
 #pragma unroll
   for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, shfl_xor_f(m, x));
   if (lane == 0) s_red[wave] = m;
@@ -709,11 +724,11 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void cache_combi
   m = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
   const float ref = m == -INFINITY ? 0.f : m;
   float l = 0.f;
-  for (int i = tid; i < n; i += 256) {
-    const float2 st = a.stat[rp.at(a, i)];
-    const float f = st.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(st.x - ref);
-    if (st.y != 0.f) l += f * st.y;
-    s_f[i] = st.y == 0.f ? -1.f : f;  // (a part of no keys has no O)
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const float f = st[j].y == 0.f ? -1.f : __builtin_amdgcn_exp2f(st[j].x - ref);  // (-1: a part of no keys has no O)
+    if (st[j].y != 0.f) l += f * st[j].y;
+    if (tid + 256 * j < n) s_f[tid + 256 * j] = f;
   }
 #pragma unroll
   for (int x = 1; x < 64; x <<= 1) l += shfl_xor_f(l, x);
@@ -1021,8 +1036,10 @@ template <typename T, int DP> static int launch_cache(const CacheArgs &a, int64_
     // many rows of few parts: a wave each (1152 rows of 26 parts, d 256: 71 us a call against 60)
     if (!a.sc && (rows >= 16384 || (rows >= 1024 && (a.np_own + a.np_pre) * DP <= 2048)))
       hipLaunchKernelGGL((cache_join_kernel<T, DP>), dim3((unsigned)cdiv(rows, 4)), dim3(256), 0, s, a);
+    else if (a.sc)
+      hipLaunchKernelGGL((cache_combine_kernel<T, DP, true>), dim3((unsigned)(rows + wgs)), dim3(256), 0, s, a);
     else
-      hipLaunchKernelGGL((cache_combine_kernel<T, DP>), dim3((unsigned)(rows + wgs)), dim3(256), 0, s, a);
+      hipLaunchKernelGGL((cache_combine_kernel<T, DP, false>), dim3((unsigned)rows), dim3(256), 0, s, a);
     if ((e = hip_check(hipGetLastError(), "cache_combine_kernel launch"))) return e;
   }
   if (a.wo && !a.sc) {
