@@ -9,15 +9,13 @@
 // row's weight grows by its p_s summed over the group's heads and the tokens.
 //
 // The query rows that read one KV head (G heads x T tokens of a sequence; for
-// the prefix those of every sequence) are stacked, 16 rows to an MFMA tile,
-// ordered (token, head) so that a tile's rows see about the same keys.
-//   part     a wave per (16-row tile, share of the keys): K and V stream
-//            global -> LDS through a ring of the wave's own (no barrier), online
-//            softmax in the log2 domain; leaves unnormalised fp32 O, row
-//            maximum and row sum
-//   combine  a row's parts joined in a fixed order; O, lse
-//   tile     many rows: a workgroup per (64- or 128-row tile, share of the keys)
-//   weight   a workgroup per 128 keys over many rows, scores formed again
+// the prefix those of every sequence) are stacked, ordered (token, head) so that a
+// tile's rows see about the same keys.
+//   part     up to 16 rows: a wave per (tile, share of the keys), memory bound
+//   tile     more: a workgroup per (64- or 128-row tile, share of the keys)
+//   combine, join   a row's parts (unnormalised fp32 O, row maximum, row sum) added
+//            in a fixed order; O, lse; after `part` the weights too, from its scores
+//   weight   after `tile`: a workgroup per 128 or 256 keys, scores formed again
 // Lengths are read on the device; nothing depends on launch order.
 #include <math.h>
 
@@ -234,6 +232,16 @@ __device__ __forceinline__ int64_t score_row(const CacheArgs &a, int b, int hk, 
   return (((int64_t)b * a.Hkv + hk) * a.TG + rho) * score_keys(a);
 }
 
+// ---- few rows (16 or fewer): a wave per (tile, share of the keys). K and V stream
+// global -> LDS through a two-stage ring of the wave's own, so no wave waits for
+// another; P enters the value product as a pair of 16-bit numbers (the matrix
+// units are idle anyway: busy 5 to 7% of the time), online softmax in the log2
+// domain, and where weights are wanted the scores are stored (4 bytes a row and key
+// against 2 D to read the key again). Bound by memory: one token over 262144 rows, 8
+// heads, d 64, 94 us, 5.7 TB/s; 32 sequences of 1000 to 8192 rows, 16 heads over 2, d 256,
+// with weights, 61 to 63 us, 5.1 TB/s. A third and fourth stage changed nothing (d
+// 256, 16 keys), nor did equal numbers of chunks to every wave whatever caches they
+// lie in (85.8 -> 88.8 us a call: a wave that crosses caches starts its ring anew).
 template <typename T, int DP> __global__ __launch_bounds__(64) void cache_part_kernel(CacheArgs a) {
   using C = CacheCfg<T, DP>;
   constexpr int KC = C::KC, NM = KC / 16;
@@ -330,6 +338,13 @@ template <typename T, int DP> __global__ __launch_bounds__(64) void cache_part_k
 // forward; the row sums are of the unrounded values): the second product of a
 // split operand would cost half as much again where the matrix units are what
 // bounds the kernel.
+// Measured: 2048 tokens over 16301 rows, 16 heads over 2, d 256: 525 to 560 us, 0.92 to
+// 0.98 PFLOP/s (matrix units and LDS each busy 46% of the time: eight waves in step
+// at one barrier per 64 keys; 32 keys a chunk 610 us; four waves of 32 rows, one to a
+// SIMD, 789). 512 rows a head over 16301 keys, beside 64 own caches: 38 us, of which
+// about 17 are the chunks and the rest the start, 33 MB of parts and the own caches.
+// 160 rows a head over 65536 keys, d 64: 44 us, exponentials and their like at half
+// the vector issue.
 template <typename T, int DP, int QT, int NM>
 __device__ __forceinline__ void qk_tile(const char *tile, const RowFrag<T, DP> (&fr)[QT], f32x4 (&acc)[QT][NM], int g, int p) {
   constexpr int CPR = DP * (int)sizeof(T) / 16;
@@ -580,7 +595,8 @@ __device__ __forceinline__ RowParts row_parts(const CacheArgs &a, int b, int hk,
   return r;
 }
 
-// A wave per row, where rows are many: DP / 4 lanes to a part, so 64 / (DP / 4)
+// A wave per row, where rows are many (2432 rows of few parts took a workgroup each
+// most of their call: 49 -> 34 us): DP / 4 lanes to a part, so 64 / (DP / 4)
 // parts at a time; their sums are joined across the lanes in order.
 template <typename T, int DP> __global__ __launch_bounds__(256) void cache_join_kernel(CacheArgs a) {
   constexpr int LG = DP / 4, NG = 64 / LG;
@@ -625,6 +641,8 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void cache_join_
 constexpr int kMaxShares = 512;    // np_own + np_pre
 constexpr int kWeightKeys = 1024;  // keys of a weight workgroup
 
+// Bound by latency: a few microseconds for any few rows; 512 rows of 32 parts, d 256,
+// with 64 caches' weights 9.4 us.
 // Workgroups [0, rows): a row each. Groups of DP / 4 threads take every NG-th
 // part, a float4 a thread, and are added in order at the end.
 // Workgroups past them (WEIGHT): kWeightKeys keys of a (sequence, KV head): each row's
@@ -773,7 +791,9 @@ template <typename T, int DP, bool WEIGHT> __global__ __launch_bounds__(256) voi
 // query rows stream through a ring in LDS, a chunk's first half to waves 0-3 and
 // its second to waves 4-7. A lane holds one column, a key, of the
 // product, so the sum over rows is a register each. Row rho is token rho / G;
-// key j is seen by the rows from G * (j - (len - count)) on.
+// key j is seen by the rows from G * (j - (len - count)) on. 2048 tokens over 16301
+// rows, 16 heads over 2, d 256: 274 us, 0.94 PFLOP/s of these products (vector issue
+// 57%, matrix units 44% busy).
 template <typename T, int DP> struct WeightCfg {
   static constexpr int ES = sizeof(T), NT = 512, CPR = DP * ES / 16;
   // 16-key fragments of a wave: a row fragment read from LDS feeds KF products
