@@ -595,8 +595,8 @@ __device__ __forceinline__ RowParts row_parts(const CacheArgs &a, int b, int hk,
   return r;
 }
 
-// A wave per row, where rows are many (2432 rows of few parts took a workgroup each
-// most of their call: 49 -> 34 us): DP / 4 lanes to a part, so 64 / (DP / 4)
+// A wave per row, where rows are many (12480 rows of few parts, d 64: 49 us a call
+// with a workgroup each, 34 so): DP / 4 lanes to a part, so 64 / (DP / 4)
 // parts at a time; their sums are joined across the lanes in order.
 template <typename T, int DP> __global__ __launch_bounds__(256) void cache_join_kernel(CacheArgs a) {
   constexpr int LG = DP / 4, NG = 64 / LG;
