@@ -15,7 +15,7 @@
 //   tile     more: a workgroup per (64- or 128-row tile, share of the keys)
 //   combine, join   a row's parts (unnormalised fp32 O, row maximum, row sum) added
 //            in a fixed order; O, lse; after `part` the weights too, from its scores
-//   weight   after `tile`: a workgroup per 128 or 256 keys, scores formed again
+//   weight, weight_rows  after `tile`: scores formed again, the keys in registers
 // Lengths are read on the device; nothing depends on launch order.
 #include <math.h>
 
@@ -933,6 +933,90 @@ template <typename T, int DP> __global__ __launch_bounds__(512) void cache_weigh
     }
   }
 }
+// ---- weights of up to 128 rows: the rows stay in LDS, and each wave streams keys of
+// its own, KF fragments at a time straight into registers with the next ones on
+// their way, so after the rows are staged no wave waits for another. A row that sees
+// nothing, or is none, has an lse of +inf here: its probabilities are 0. Against the
+// kernel above, whose one or two chunks of such rows leave nothing to overlap: 56 rows a
+// head over up to 123654 keys, 48 caches, d 32, 216 -> 118 us; 108 rows, d 64, fp32,
+// 617 -> 377.
+template <typename T, int DP> struct WeightRowsCfg {
+  static constexpr int ES = sizeof(T), CPR = DP * ES / 16, MAXROWS = 128;
+  static constexpr int KF = ES == 2 ? (DP >= 256 ? 2 : 4) : (DP >= 128 ? 1 : 2), KEYS = 16 * KF;
+};
+template <typename T, int DP> __global__ __launch_bounds__(256) void cache_weight_rows_kernel(CacheArgs a) {
+  using C = WeightRowsCfg<T, DP>;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, p = lane & 15;
+  const int hk = blockIdx.y % a.Hkv, b = blockIdx.y / a.Hkv;
+  const int n = seq_len(a, b), cnt = seq_count(a, b), real = cnt * a.G, rp = (a.TG + 31) / 32 * 32;
+  int t0, t1;
+  share_of((n + C::KEYS - 1) / C::KEYS, blockIdx.x * 4 + w, gridDim.x * 4, t0, t1);
+  float *s_lse = (float *)(smem + rp * DP * C::ES);
+  for (int u = tid; u < rp * C::CPR; u += 256) {
+    const int row = u / C::CPR, c = u % C::CPR;
+    u32x4 x = u32x4{0, 0, 0, 0};
+    if (row < real && c * 16 < a.D * C::ES)
+      x = *(const u32x4 *)((const T *)a.q + b * a.sq[0] + (hk * a.G + row % a.G) * a.sq[1] + (row / a.G) * a.sq[2] + c * (16 / C::ES));
+    *(u32x4 *)(smem + (row * C::CPR + (c ^ swz(row, C::CPR))) * 16) = x;
+  }
+  for (int row = tid; row < rp; row += 256) {
+    const float l2 = row < real ? a.lse2[((int64_t)b * a.Hkv + hk) * a.TG + row] : INFINITY;
+    s_lse[row] = l2 == -INFINITY ? INFINITY : l2;
+  }
+  RowFrag<T, DP> next[C::KF];
+  const T *kb = (const T *)a.k + b * a.sk[0] + hk * a.sk[1];
+  // (the keys take the query's sign, and zeros past the head dim; a key past the
+  // length is the last one, not stored)
+  auto load = [&](int t) {
+#pragma unroll
+    for (int f = 0; f < C::KF; ++f) {
+      const int64_t key = (int64_t)t * C::KEYS + f * 16 + p;
+      load_frag<T, DP>(next[f], kb + (key < n ? key : n - 1) * a.sk[2], g, a);
+    }
+  };
+  if (t0 < t1) load(t0);
+  __syncthreads();
+  const int64_t old = (int64_t)n - cnt;  // rows of the cache before the new tokens
+  for (int t = t0; t < t1; ++t) {
+    RowFrag<T, DP> fr[C::KF];
+    float sum[C::KF], w0[C::KF];
+    int64_t first[C::KF];  // the first row that sees this lane's key
+#pragma unroll
+    for (int f = 0; f < C::KF; ++f) {
+      const int64_t key = (int64_t)t * C::KEYS + f * 16 + p;
+      fr[f] = next[f];
+      sum[f] = 0.f;
+      first[f] = (key - old) * a.G;
+      w0[f] = a.w && g == 0 && key < n ? a.w[b * a.sw[0] + hk * a.sw[1] + key] : 0.f;
+    }
+    if (t + 1 < t1) load(t + 1);
+    const bool all = (int64_t)(t + 1) * C::KEYS - 1 <= old;  // every row sees every key of the wave's
+    for (int r0 = 0; r0 < real; r0 += 32) {
+      f32x4 s[C::KF][2], l2[2];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) l2[m] = *(const f32x4 *)(s_lse + r0 + 16 * m + 4 * g);
+      qk_tile<T, DP, C::KF, 2>(smem + r0 * DP * C::ES, fr, s, g, p);
+#pragma unroll
+      for (int f = 0; f < C::KF; ++f)
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[f][m][r], a.scale2, -l2[m][r]));
+            if (all || r0 + 16 * m + 4 * g + r >= first[f]) sum[f] += x;
+          }
+    }
+#pragma unroll
+    for (int f = 0; f < C::KF; ++f) {
+      sum[f] += shfl_xor_f(sum[f], 16);
+      sum[f] += shfl_xor_f(sum[f], 32);
+      const int64_t key = (int64_t)t * C::KEYS + f * 16 + p;
+      if (g == 0 && key < n) a.wo[b * a.swo[0] + hk * a.swo[1] + key] = w0[f] + sum[f];
+    }
+  }
+}
+
 // the row shares' sums, in order
 __global__ __launch_bounds__(256) void cache_weight_sum_kernel(CacheArgs a, int shares) {
   const int key = blockIdx.x * 256 + threadIdx.x;
@@ -1062,7 +1146,15 @@ template <typename T, int DP> static int launch_cache(const CacheArgs &a, int64_
       hipLaunchKernelGGL((cache_combine_kernel<T, DP, false>), dim3((unsigned)rows), dim3(256), 0, s, a);
     if ((e = hip_check(hipGetLastError(), "cache_combine_kernel launch"))) return e;
   }
-  if (a.wo && !a.sc) {
+  if (a.wo && !a.sc && a.TG <= WeightRowsCfg<T, DP>::MAXROWS) {
+    using W = WeightRowsCfg<T, DP>;
+    const size_t rp = (size_t)cdiv(a.TG, 32) * 32, need = rp * DP * W::ES + rp * 4;
+    if ((e = lds_optin((const void *)cache_weight_rows_kernel<T, DP>, need, "hipFuncSetAttribute(cache_weight_rows)"))) return e;
+    // eight workgroups a CU (four: up to 7% more on long caches), no more than there are key tiles
+    const int64_t seqs = (int64_t)a.B * a.Hkv, wgs = std::min(std::max<int64_t>(1, cdiv(8 * kCUs, seqs)), cdiv(a.S, 4 * W::KEYS));
+    hipLaunchKernelGGL((cache_weight_rows_kernel<T, DP>), dim3((unsigned)wgs, (unsigned)seqs), dim3(256), need, s, a);
+    e = hip_check(hipGetLastError(), "cache_weight_rows_kernel launch");
+  } else if (a.wo && !a.sc) {
     using W = WeightCfg<T, DP>;
     if ((e = lds_optin((const void *)cache_weight_kernel<T, DP>, W::LDS, "hipFuncSetAttribute(cache_weight)"))) return e;
     const unsigned seqs = (unsigned)(a.B * a.Hkv);
