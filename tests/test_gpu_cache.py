@@ -2,6 +2,7 @@
 and one and those around a tile, padded batches, rows of NaN behind a sequence,
 strided and far-apart caches, every type, head dims that are no power of two."""
 import math
+import threading
 
 import pytest
 import torch
@@ -400,6 +401,47 @@ def test_captured_steps_follow_their_buffers():
             x.zero_()
         b = [*step(), out_w, *out, k, v]
         assert all(torch.equal(x, y) for x, y in zip(a, b)), f"replay {i}"
+
+
+def test_two_threads_on_their_own_streams(monkeypatch):
+    """Two host threads at once, each on a stream of its own, the plans turned over
+    all the while: every result as in sequence."""
+    monkeypatch.setattr(cache, "_PLANS_MAX", 3)
+    jobs = []
+    for i, (T, P, S) in enumerate([(1, 0, 700), (30, 0, 500), (1, 400, 90), (7, 90, 300), (1, 0, 40000), (200, 0, 260)]):
+        q, k, v, kp, vp, g = _make("bf16", 2, 8, 2, T, S, 64, [S, S // 2], seed=i, P=P)
+        jobs.append((q, k, v, kp, vp, _ints([S, S // 2]), _randn(g, 2, 2, S).abs()))
+
+    def run(job):
+        q, k, v, kp, vp, lens, w = job
+        out = torch.zeros_like(w)
+        o = (cache.cache_attention(q, k, v, lens, weight=w, out_weight=out) if kp is None else
+             cache.shared_prefix_attention(q, kp, vp, k, v, lens, weight=w, out_weight=out))
+        rows = (torch.zeros_like(k[:, :, :50]), torch.zeros_like(v[:, :, :50]), torch.zeros_like(w[:, :, :50]))
+        index, _ = cache.evict(k, v, out, lens, 50, recent=5, out=tuple(x.contiguous() for x in rows))
+        return o, out, index
+    want = [run(j) for j in jobs]
+    torch.cuda.synchronize()
+    got, errors = {}, []
+
+    def work(mine):
+        try:
+            s = torch.cuda.Stream()
+            with torch.cuda.stream(s):
+                for _ in range(10):
+                    for i in mine:
+                        got[i] = run(jobs[i])
+            s.synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(m,)) for m in ((0, 2, 4), (5, 3, 1))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for i, w in enumerate(want):
+        assert all(torch.equal(a, b) for a, b in zip(w, got[i])), f"job {i}"
 
 
 def test_refusals_on_the_gpu():
