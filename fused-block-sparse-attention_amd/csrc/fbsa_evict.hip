@@ -402,14 +402,34 @@ __global__ __launch_bounds__(kSelThreads) void evict_place_kernel(EvictArgs a, E
 // ones: the steps above, whose five launches cost more than they save below it.
 constexpr int64_t kOneGroup = 16 * kSelThreads;
 
+// In place, many rows of few heads pass through the workspace, up to kStage bytes
+// at a time: one more trip through memory, but at the whole card's rate, where the
+// move kernel has a workgroup per (head, k or v, 64 bytes of a row) and goes through
+// the rows kMove at a time. Calls, staged against moved: 16384 rows of 8 heads, d 64
+// (32 workgroups) 77 and 211 us; 2048 of 8, d 128 (64) 17 and 24; 32768 of 8, d 256
+// (128) 233 and 433; 4096 of 16, d 256 (256) 64 and 59; 4096 of 128, d 128 (1024) 224
+// and 168; 512 of 8, d 64 (32) 10.4 and 10.1; 768 of 4 (16) 9.1 and 11.7.
+constexpr int64_t kStage = 32 << 20, kStageWgs = 128;
+constexpr int kMoveU = 8, kMove = 64 * kMoveU;
+
 struct EvictPlan {
-  int64_t nch;
-  size_t hist, count, start, pick, cand, copy, total;
+  int64_t nch, part;  // part: rows of a head that pass through the workspace at a time (0: none do)
+  size_t hist, count, start, pick, cand, copy, stage, total;
 };
 static EvictPlan evict_plan(const fbsa_evict_desc *d) {
   EvictPlan p = {};
-  if (d->S <= kOneGroup) return p;
   const size_t rows = (size_t)(d->B * d->H);
+  const int64_t cpr = d->D * (d->dtype == FBSA_F32 ? 4 : 2) / 16, ni = d->budget < d->S ? d->budget : d->S;
+  size_t stage = 0;
+  if (d->flags & FBSA_EVICT_IN_PLACE && d->budget < d->S && ni > kMove && 2 * (int64_t)rows * ((cpr + 3) / 4) <= kStageWgs) {
+    const int64_t most = kStage / ((int64_t)rows * cpr * 32);
+    p.part = ni < most ? ni : most;
+    stage = (size_t)(p.part < ni ? 2 : 1) * rows * p.part * cpr * 32;
+  }
+  if (d->S <= kOneGroup) {
+    p.total = stage;
+    return p;
+  }
   p.nch = (d->S + kChunk - 1) / kChunk;
   p.hist = 0;
   p.count = p.hist + rows * kBins * 4;
@@ -417,7 +437,8 @@ static EvictPlan evict_plan(const fbsa_evict_desc *d) {
   p.pick = p.start + rows * p.nch * 8;
   p.cand = (p.pick + rows * 8 + 255) / 256 * 256;
   p.copy = p.cand + rows * p.nch * kChunk * 4;
-  p.total = p.copy + (d->flags & FBSA_EVICT_IN_PLACE ? rows * p.nch * kChunk * 4 : 0);
+  p.stage = p.copy + (d->flags & FBSA_EVICT_IN_PLACE ? rows * p.nch * kChunk * 4 : 0);
+  p.total = p.stage + stage;
   return p;
 }
 
@@ -441,7 +462,6 @@ __global__ __launch_bounds__(256) void evict_copy_kernel(EvictArgs a) {
 // 64 bytes of every row) walks the kept rows in order, kMove at a time. Row i
 // comes from index[i] >= i, so a step writes only rows that no later step
 // reads; within a step every read has ended before the first write.
-constexpr int kMoveU = 8, kMove = 64 * kMoveU;
 __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
   const int h = blockIdx.z % a.H, b = blockIdx.z / a.H;
   const int n = evict_len(a, b);
@@ -467,6 +487,36 @@ __global__ __launch_bounds__(256) void evict_move_kernel(EvictArgs a) {
       const int i = base + j * 64 + (threadIdx.x >> 2);
       if (go[j]) *(i32x4 *)(x + i * st[2]) = y[j];
     }
+  }
+}
+
+// The same through the workspace, `part` rows of every head a launch: launch t
+// takes part t in and part t - 1 out, which is written only after every row of it
+// and of the parts before has been read, and below every row that part t reads.
+__global__ __launch_bounds__(256) void evict_stage_kernel(EvictArgs a, char *stage, int part, int t, int nt) {
+  const bool out = blockIdx.z;
+  if (t - out < 0 || t - out >= nt) return;
+  t -= out;
+  const int h = blockIdx.y % a.H, b = blockIdx.y / a.H;
+  const uint32_t u = blockIdx.x * 256 + threadIdx.x;
+  const int c = (int)(u % (uint32_t)a.cpr), local = (int)(u / (uint32_t)a.cpr);
+  const int64_t i = (int64_t)t * part + local;
+  const int n = evict_len(a, b);
+  if (n <= a.budget || local >= part || i >= a.budget) return;
+  const int64_t s = a.index[(int64_t)blockIdx.y * a.ni + i];
+  if (s == i) return;
+  const int64_t size = (int64_t)part * a.cpr * 16;
+  char *at = stage + ((int64_t)(t & 1) * gridDim.y + blockIdx.y) * 2 * size + (int64_t)u * 16;
+  char *k = a.ko + b * a.sk[0] + h * a.sk[1] + (out ? i : s) * a.sk[2] + c * 16;
+  char *v = a.vo + b * a.sv[0] + h * a.sv[1] + (out ? i : s) * a.sv[2] + c * 16;
+  if (out) {
+    const i32x4 x = *(const i32x4 *)at, y = *(const i32x4 *)(at + size);
+    *(i32x4 *)k = x;
+    *(i32x4 *)v = y;
+  } else {
+    const i32x4 x = *(const i32x4 *)k, y = *(const i32x4 *)v;
+    *(i32x4 *)at = x;
+    *(i32x4 *)(at + size) = y;
   }
 }
 
@@ -603,6 +653,13 @@ int fbsa_cache_evict(const fbsa_evict_desc *d, const void *k, const void *v, con
     hipLaunchKernelGGL(evict_rank_kernel, dim3(rows), wg, 0, s, a, ws);
     hipLaunchKernelGGL(evict_place_kernel, grid, wg, 0, s, a, ws);
     if ((e = hip_check(hipGetLastError(), "evict kernels launch"))) return e;
+  }
+  if (pl.part) {
+    const int nt = (int)((ni + pl.part - 1) / pl.part);
+    for (int t = 0; t <= nt; ++t)
+      hipLaunchKernelGGL(evict_stage_kernel, dim3((unsigned)((pl.part * cpr + 255) / 256), rows, 2), dim3(256), 0, s, a,
+                         (char *)workspace + pl.stage, (int)pl.part, t, nt);
+    return hip_check(hipGetLastError(), "evict_stage_kernel launch");
   }
   if (inplace)
     hipLaunchKernelGGL(evict_move_kernel, dim3((unsigned)((cpr + 3) / 4), 2, rows), dim3(256), 0, s, a);

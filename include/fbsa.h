@@ -404,8 +404,8 @@ int fbsa_cache_attn(const fbsa_cache_desc *d, const void *q, const void *k, cons
  * are k, v and weight themselves (same pointers, strides and SO = S). lens and
  * new_lens may be the same array in neither case. The workspace (256-byte aligned)
  * may be NULL where fbsa_cache_evict_workspace_bytes returns 0, as it does for
- * capacities up to 16384 (and, with fbsa_last_error set, for a descriptor that
- * fbsa_cache_evict refuses). */
+ * capacities up to 16384 unless more than 512 rows are kept in place (and, with
+ * fbsa_last_error set, for a descriptor that fbsa_cache_evict refuses). */
 enum { FBSA_EVICT_IN_PLACE = 1 };
 
 typedef struct fbsa_evict_desc {

@@ -98,6 +98,12 @@ def test_evict_pointers():
     assert need > 0 and lib.fbsa_cache_evict(d, *p, DUMMY, need - 1, None) == _lib.EWORKSPACE
     assert lib.fbsa_cache_evict(d, *p, None, 0, None) == _lib.EWORKSPACE
     assert lib.fbsa_cache_evict(d, *p, DUMMY + 16, need, None) == _lib.EINVAL
+    # in place: room for the rows' way, a part of them at a time
+    size = lambda **kw: lib.fbsa_cache_evict_workspace_bytes(_evict(flags=1, **kw))
+    assert size(S=16384, SO=16384, budget=512) == 0 and 0 < size(S=16384, SO=16384, budget=16383) <= 64 << 20
+    d = _evict(flags=1, S=16384, SO=16384, budget=4096)
+    same = [p[0], p[1], p[2], p[3], p[0], p[1], p[2], p[7], p[8]]
+    assert lib.fbsa_cache_evict(d, *same, None, 0, None) == _lib.EWORKSPACE
 
 
 @pytest.mark.parametrize("kw,needle", [({"T": 0}, "positive"), ({"D": 12}, "head dim"), ({"flags": 1}, "flags"),

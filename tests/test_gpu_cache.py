@@ -317,6 +317,53 @@ def test_evict_at_each_register_count(inplace, S):
     _evict_case("fp16", 2, 1, S, 16, [S, S - 1], S // 3, 100, 4, "ties", inplace)
 
 
+def test_evict_in_place_in_parts():
+    # more kept rows than pass through the workspace at a time: 8192 of these heads
+    _evict_case("bf16", 2, 8, 30000, 64, [30000, 26000], 20001, 300, 4, "random", True)
+    _evict_case("bf16", 2, 8, 30000, 64, [20000, 29999], 20001, 300, 4, "equal", True)
+
+
+@pytest.mark.parametrize("budget", [512, 513, 1100])
+def test_evict_in_place_of_strided_caches(budget):
+    g, B, H, S, D = _gen(5), 2, 3, 1500, 40
+    kv = _randn(g, B, S, 2, H, D, dtype=torch.bfloat16)
+    k, v = kv[:, :, 0].transpose(1, 2), kv[:, :, 1].transpose(1, 2)
+    w, lens, before = _randn(g, B, H, S), [S, budget + 1], kv.clone()
+    keep = ref.evict(k, v, w.cpu(), lens, budget, 17, 3)
+    index, n = cache.evict(k, v, w, _ints(lens), budget, recent=17, sink=3)
+    want = before.clone()
+    for b in range(B):
+        for h in range(H):
+            rows = keep[b * H + h]
+            assert index[b, h].tolist() == rows and int(n[b]) == budget
+            want[b, :budget, :, h] = before[b, rows][:, :, h]
+    assert torch.equal(kv, want)
+
+
+def test_evict_in_place_replayed():
+    # a captured call, new rows before every replay, eager calls between them
+    g, B, H, S, D, budget = _gen(6), 1, 4, 3000, 64, 2000
+    k, v = (torch.zeros(B, H, S, D, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    w = torch.zeros(B, H, S, device=DEV)
+    lens = _ints([S])
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        cache.evict(k, v, w, lens, budget)
+    torch.cuda.current_stream().wait_stream(stream)
+    with torch.cuda.graph(graph):
+        index, n = cache.evict(k, v, w, lens, budget, recent=10)
+    for _ in range(4):
+        new = [_randn(g, *x.shape, dtype=x.dtype) for x in (k, v, w)]
+        eager = [x.clone() for x in new]
+        cache.evict(*eager, lens, budget, recent=10)
+        for x, y in zip((k, v, w), new):
+            x.copy_(y)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip((k, v, w), eager))
+
+
 def test_evict_lengths_past_the_capacity():
     _evict_case("bf16", 3, 1, 100, 32, [400, -3, 100], 60, 3, 2, "random", False)
 
