@@ -317,6 +317,28 @@ def test_evict_at_each_register_count(inplace, S):
     _evict_case("fp16", 2, 1, S, 16, [S, S - 1], S // 3, 100, 4, "ties", inplace)
 
 
+@pytest.mark.parametrize("kind", ["random", "ties", "equal"])
+def test_evict_of_very_long_sequences(kind):
+    # more chunks of a sequence than are ranked at a time (64 of 8192 rows)
+    _evict_case("bf16", 2, 1, 560000, 8, [560000, 524289], 30000, 600, 4, kind, False)
+
+
+def test_evict_again():
+    # rows that were kept before lie in the first places and outweigh the rest
+    g, B, H, S, D, budget = _gen(7), 1, 2, 40000, 16, 6000
+    k, v = (_randn(g, B, H, S, D, dtype=torch.bfloat16) for _ in range(2))
+    w = torch.rand(B, H, S, generator=g, device=DEV)
+    w[:, :, :budget] += 0.5
+    w[:, :, :2048] = 0.75
+    before = [x.clone() for x in (k, v, w)]
+    keep = ref.evict(k, v, w.cpu(), [S], budget, 100, 4)
+    index, _ = cache.evict(k, v, w, _ints([S]), budget, recent=100, sink=4)
+    for h in range(H):
+        assert index[0, h].tolist() == keep[h]
+        for x, y in zip((k, v, w), before):
+            assert torch.equal(x[0, h, :budget], y[0, h, keep[h]]) and torch.equal(x[0, h, budget:], y[0, h, budget:])
+
+
 def test_evict_in_place_in_parts():
     # more kept rows than pass through the workspace at a time: 8192 of these heads
     _evict_case("bf16", 2, 8, 30000, 64, [30000, 26000], 20001, 300, 4, "random", True)
