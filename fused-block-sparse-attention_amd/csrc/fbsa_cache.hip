@@ -936,7 +936,10 @@ template <typename T, int DP> __global__ __launch_bounds__(512) void cache_weigh
 // ---- weights of up to 128 rows: the rows stay in LDS, and each wave streams keys of
 // its own, KF fragments at a time straight into registers with the next ones on
 // their way, so after the rows are staged no wave waits for another. A row that sees
-// nothing, or is none, has an lse of +inf here: its probabilities are 0. Against the
+// nothing has an lse of +inf here, and a place past the last row holds that row with
+// an lse of +inf: their probabilities are 0 (zeros in such a place would make a NaN of a
+// key's infinities; the last row sees every key, so its own scores are NaN where the copy's are).
+// Against the
 // kernel above, whose one or two chunks of such rows leave nothing to overlap: 56 rows a
 // head over up to 123654 keys, 48 caches, d 32, 216 -> 118 us; 108 rows, d 64, fp32,
 // 617 -> 377.
@@ -956,8 +959,9 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void cache_weigh
   for (int u = tid; u < rp * C::CPR; u += 256) {
     const int row = u / C::CPR, c = u % C::CPR;
     u32x4 x = u32x4{0, 0, 0, 0};
-    if (row < real && c * 16 < a.D * C::ES)
-      x = *(const u32x4 *)((const T *)a.q + b * a.sq[0] + (hk * a.G + row % a.G) * a.sq[1] + (row / a.G) * a.sq[2] + c * (16 / C::ES));
+    const int at = row < real ? row : real - 1;
+    if (real && c * 16 < a.D * C::ES)
+      x = *(const u32x4 *)((const T *)a.q + b * a.sq[0] + (hk * a.G + at % a.G) * a.sq[1] + (at / a.G) * a.sq[2] + c * (16 / C::ES));
     *(u32x4 *)(smem + (row * C::CPR + (c ^ swz(row, C::CPR))) * 16) = x;
   }
   for (int row = tid; row < rp; row += 256) {

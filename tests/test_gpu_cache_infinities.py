@@ -1,0 +1,45 @@
+"""Infinite keys and values in a cache: a key scored -inf drops out, an infinite
+value reaches the queries that see it and no other, and no weight turns to NaN."""
+import math
+
+import pytest
+import torch
+
+import _cachetight as tight
+from fbsa_amd import cache
+from test_gpu_cache import DEV, _ints, _make, _randn
+
+pytestmark = pytest.mark.gpu
+
+
+def _call(q, k, v, kp, vp, lens, **kw):
+    if kp is None:
+        return cache.cache_attention(q, k, v, _ints(lens), need_lse=True, **kw)
+    return cache.shared_prefix_attention(q, kp, vp, k, v, _ints(lens), need_lse=True, **kw)
+
+
+def _check(q, k, v, kp, vp, lens, g, count=None, gate=None):
+    w = _randn(g, *k.shape[:3]).abs()
+    out = w.clone()
+    o, lse = _call(q, k, v, kp, vp, lens, count=_ints(count), weight=w, out_weight=out, out_gate=gate)
+    r = tight.attend(q, k, v, lens, count, kp, vp, None, gate, w)
+    rows = q.shape[2] * (q.shape[1] // k.shape[1])
+    P = 0 if kp is None else kp.shape[1]
+    rounded = rows > 16 or (P > 0 and q.shape[0] * rows > 16)
+    tight.check((o, lse, out), r, q, k.shape[2] + P, rounded, gate is not None)
+    return o, lse, out
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("D", [32, 64, 128, 256])
+@pytest.mark.parametrize("T", [5, 7, 20, 41, 60])
+def test_weights_beside_keys_scored_minus_infinity(dt, D, T):
+    # 15, 21, 60, 123 and 180 rows: no whole number of the kernels' row tiles
+    lens = [180, 61]
+    q, k, v, _, _, g = _make(dt, 2, 6, 2, T, 180, D, lens)
+    q[..., 3] = q[..., 3].abs() + 0.5
+    for s in (0, 17, 59, 60, 150, 179):
+        k[:, s % 2, s, 3] = -math.inf
+    for b, n in enumerate(lens):
+        k[b, :, n:] = math.nan
+    _check(q, k, v, None, None, lens, g)
