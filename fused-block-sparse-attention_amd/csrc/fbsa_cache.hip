@@ -47,7 +47,7 @@ struct CacheArgs {
   float *part;               // [tile, share][row] unnormalised O (DP floats): prefix tiles, then own
   float2 *stat;              // [tile, share][row] row maximum (log2 domain), row sum
   float *wpart;              // [row share][B][Hkv][S] weights, where the rows are shared out
-  float *lse2;               // [B][Hkv][TG] log2-domain lse, -inf for rows that see nothing
+  float *lse2;               // [B][Hkv][TG] log2-domain lse for the weights: +inf, probabilities of 0, for rows that see nothing
   float *sc;                 // [B][Hkv][TG][S rounded up to 32] log2-domain scores (up to 16 rows, with weights)
 };
 
@@ -564,7 +564,7 @@ __global__ __launch_bounds__(NW * 64) void cache_tile_kernel(CacheArgs a, int64_
       if (g == 0) {
         const float l2 = l == 0.f ? -INFINITY : sm[qt].m + __log2f(l);
         if (a.lse) a.lse[((int64_t)ri[qt].b * a.Hq + ri[qt].hq) * a.T + ri[qt].t] = l2 * kLn2;
-        if (a.lse2) a.lse2[((int64_t)ri[qt].b * a.Hkv + ri[qt].hq / a.G) * a.TG + rho] = l2;
+        if (a.lse2) a.lse2[((int64_t)ri[qt].b * a.Hkv + ri[qt].hq / a.G) * a.TG + rho] = l == 0.f ? INFINITY : l2;
       }
       continue;
     }
@@ -634,7 +634,7 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void cache_join_
   if (lane == 0) {
     const float l2 = l == 0.f ? -INFINITY : m + __log2f(l);
     if (a.lse) a.lse[((int64_t)b * a.Hq + ri.hq) * a.T + ri.t] = l2 * kLn2;
-    if (a.lse2) a.lse2[row] = l2;
+    if (a.lse2) a.lse2[row] = l == 0.f ? INFINITY : l2;
   }
 }
 
@@ -781,7 +781,7 @@ template <typename T, int DP, bool WEIGHT> __global__ __launch_bounds__(256) voi
   if (tid == 0) {
     const float l2 = l == 0.f ? -INFINITY : m + __log2f(l);
     if (a.lse) a.lse[((int64_t)b * a.Hq + ri.hq) * a.T + ri.t] = l2 * kLn2;
-    if (a.lse2) a.lse2[blockIdx.x] = l2;
+    if (a.lse2) a.lse2[blockIdx.x] = l == 0.f ? INFINITY : l2;
   }
 }
 
@@ -907,7 +907,6 @@ template <typename T, int DP> __global__ __launch_bounds__(512) void cache_weigh
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const int row = row0 + 16 * m + 4 * g + r;
-            // (a row that sees nothing has no lse, and no key)
             if (row >= first[f] && row < real) sum[f] += __builtin_amdgcn_exp2f(__builtin_fmaf(s[f][m][r], a.scale2, -l2[m][r]));
           }
     }
@@ -935,11 +934,10 @@ template <typename T, int DP> __global__ __launch_bounds__(512) void cache_weigh
 }
 // ---- weights of up to 128 rows: the rows stay in LDS, and each wave streams keys of
 // its own, KF fragments at a time straight into registers with the next ones on
-// their way, so after the rows are staged no wave waits for another. A row that sees
-// nothing has an lse of +inf here, and a place past the last row holds that row with
-// an lse of +inf: their probabilities are 0 (zeros in such a place would make a NaN of a
-// key's infinities; the last row sees every key, so its own scores are NaN where the copy's are).
-// Against the
+// their way, so after the rows are staged no wave waits for another. A place past the
+// last row holds that row with an lse of +inf: its probabilities are 0 (zeros there
+// would make a NaN of a key's infinities; the last row sees every key, so its own
+// scores are NaN where the copy's are). Against the
 // kernel above, whose one or two chunks of such rows leave nothing to overlap: 56 rows a
 // head over up to 123654 keys, 48 caches, d 32, 216 -> 118 us; 108 rows, d 64, fp32,
 // 617 -> 377.
@@ -964,10 +962,7 @@ template <typename T, int DP> __global__ __launch_bounds__(256) void cache_weigh
       x = *(const u32x4 *)((const T *)a.q + b * a.sq[0] + (hk * a.G + at % a.G) * a.sq[1] + (at / a.G) * a.sq[2] + c * (16 / C::ES));
     *(u32x4 *)(smem + (row * C::CPR + (c ^ swz(row, C::CPR))) * 16) = x;
   }
-  for (int row = tid; row < rp; row += 256) {
-    const float l2 = row < real ? a.lse2[((int64_t)b * a.Hkv + hk) * a.TG + row] : INFINITY;
-    s_lse[row] = l2 == -INFINITY ? INFINITY : l2;
-  }
+  for (int row = tid; row < rp; row += 256) s_lse[row] = row < real ? a.lse2[((int64_t)b * a.Hkv + hk) * a.TG + row] : INFINITY;
   RowFrag<T, DP> next[C::KF];
   const T *kb = (const T *)a.k + b * a.sk[0] + hk * a.sk[1];
   // (the keys take the query's sign, and zeros past the head dim; a key past the

@@ -300,7 +300,8 @@ def cache_attention(q, k, v, lens=None, *, count=None, scale=None, out_gate=None
     from zeros.
 
     Returns o (B, Hq, T, D), and with need_lse the fp32 natural-log normaliser
-    (B, Hq, T); padding queries, and queries that see no row, give 0 and -inf.
+    (B, Hq, T); padding queries, and queries that see no row or whose every score
+    is -inf, give 0 and -inf, and no weight.
     """
     return _attend("cache_attention", q, None, None, k, v, lens, count, scale, out_gate, weight, out_weight, need_lse)
 

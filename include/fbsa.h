@@ -365,7 +365,7 @@ int fbsa_cache_append(const fbsa_append_desc *d, void *k, void *v, const void *k
  *   o[b, h, t]   = softmax(scale q.k) v [* sigmoid(out_gate)], (B, Hq, T, D)
  *   lse[b, h, t] = the softmax's natural-log normaliser, (B, Hq, T) contiguous
  *                  fp32, nullable
- * a query that sees nothing, or t >= count[b]: o = 0, lse = -inf. With
+ * a query that sees nothing or scores every key -inf, or t >= count[b]: o = 0, lse = -inf. With
  * out_weight (fp32 (B, Hkv, S), rows contiguous) every own row s < lens[b]
  * has out_weight = weight (NULL: 0) + the probability that the sequence's
  * queries of the KV head's group gave it; weight may be out_weight. Softmax,

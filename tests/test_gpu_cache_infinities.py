@@ -43,3 +43,17 @@ def test_weights_beside_keys_scored_minus_infinity(dt, D, T):
     for b, n in enumerate(lens):
         k[b, :, n:] = math.nan
     _check(q, k, v, None, None, lens, g)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("T,P", [(1, 0), (4, 33), (40, 0), (150, 90)])
+def test_rows_whose_every_key_is_scored_minus_infinity(dt, T, P):
+    # as a row that sees nothing: 0, -inf, and no weight; the weights of the rest do not suffer
+    lens = [200, 150]
+    q, k, v, kp, vp, g = _make(dt, 2, 4, 2, T, 200, 64, lens, P=P)
+    q[..., 0] = q[..., 0].abs() + 0.5
+    k[0, 0, :200, 0] = -math.inf
+    if P:
+        kp[0, :, 0] = -math.inf
+    o, lse, out = _check(q, k, v, kp, vp, lens, g)
+    assert (lse[0, :2] == -math.inf).all() and (o[0, :2] == 0).all() and lse[0, 2:].isfinite().all()
