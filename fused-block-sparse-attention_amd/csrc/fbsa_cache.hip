@@ -189,6 +189,16 @@ template <int DP> struct SoftmaxState {
     const float lt = l + shfl_xor_f(l, 16);
     return lt + shfl_xor_f(lt, 32);
   }
+  // Whether O is finite (a NaN score makes all of it NaN). Products of two: half the
+  // instructions, and values of 2^63 may count as infinite, which costs time only.
+  __device__ __forceinline__ bool finite() const {
+    float z[2] = {0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) z[r] = __builtin_fmaf(o[t][2 * r], o[t][2 * r + 1], z[r]);
+    return fabsf(z[0] + z[1]) < INFINITY;
+  }
 };
 // keys at or past lim (counted from the chunk's first) drop out of the softmax
 template <int NM> __device__ __forceinline__ void mask_keys(f32x4 (&s)[NM], int lim, int g) {
@@ -197,6 +207,152 @@ template <int NM> __device__ __forceinline__ void mask_keys(f32x4 (&s)[NM], int 
 #pragma unroll
     for (int r = 0; r < 4; ++r)
       if (16 * m + 4 * g + r >= lim) s[m][r] = -INFINITY;
+}
+
+// ---- infinities. The matrix instructions add 0 * v for every key of a chunk that a
+// row does not see, and for the empty half of a split p: NaN where v is infinite or
+// NaN. Where a row's O is not finite its share of the keys is therefore gone through
+// once more: infinite values are zeros in the products, which are otherwise the same
+// instructions in the same order (so finite results are the same bits), and the rows
+// that see them get p * v added outside. Finite caches pay for the look at O: 0.1 to
+// 0.9 us a call (1.2% over 67 shapes).
+template <typename T> __device__ __forceinline__ void zero_infinities(s16x4 &x, bool &any) {
+  constexpr short EXP = __is_same(T, bf16) ? 0x7f80 : 0x7c00;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if ((x[e] & EXP) == EXP) {
+      x[e] = 0;
+      any = true;
+    }
+}
+// the scores of a chunk, as mm_rows_frag and qk_tile form them
+template <typename T, int DP, int QT, int NM>
+__device__ __forceinline__ void careful_scores(const char *tile, const RowFrag<T, DP> (&fr)[QT], f32x4 (&acc)[QT][NM], int g, int p) {
+  constexpr int CPR = DP * (int)sizeof(T) / 16, KS = sizeof(T) == 2 ? DP / 32 : DP / 4, KL = KS < 4 ? KS : 4;
+  const char *kb[KL];  // (few addresses and few loads ahead: registers count here, not time)
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int l = 0; l < KL; ++l) kb[l] = tile + tile_kbase(l, g, p, CPR);
+  }
+#pragma unroll
+  for (int m = 0; m < NM; ++m) {
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) acc[qt][m] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      if constexpr (sizeof(T) == 2) {
+        const s16x8 x = *(const s16x8 *)(kb[ks % KL] + (ks / 4) * 256 + m * 256 * CPR);
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) acc[qt][m] = Mfma16<T>::run(x, fr[qt].h[ks], acc[qt][m]);
+      } else {
+        const float x = *(const float *)(tile + ((16 * m + p) * CPR + (ks ^ swz(p, CPR))) * 16 + g * 4);
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt) acc[qt][m] = mfma_f32_16x16x4(x, fr[qt].f[ks], acc[qt][m]);
+      }
+      if (ks % 4 == 3) asm volatile("" ::: "memory");
+    }
+    asm volatile("" ::: "memory");
+  }
+}
+// sm.o += V^T p of a chunk; row p sees the chunk's keys below lim. SPLIT: p as a pair of 16-bit numbers
+template <typename T, int DP, int KC, int QT, bool SPLIT>
+__device__ __forceinline__ void careful_values(const char *tile, const float (&x)[QT][KC / 16][4], SoftmaxState<DP> (&sm)[QT],
+                                               const int (&lim)[QT], int g, int p) {
+  constexpr int CPR = DP * (int)sizeof(T) / 16, NM = KC / 16, K2 = NM / 2;
+  bool any = false;
+  if constexpr (sizeof(T) == 2) {
+    s16x8 pk[QT][K2 ? K2 : 1], pl[QT][K2 ? K2 : 1];
+    s16x4 qk[QT], ql[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+#pragma unroll
+      for (int k2 = 0; k2 < K2; ++k2) {
+        float y[8];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) { y[r] = x[qt][2 * k2][r]; y[4 + r] = x[qt][2 * k2 + 1][r]; }
+        if constexpr (SPLIT) pack8_split<T>(y, pk[qt][k2], pl[qt][k2]);
+        else pk[qt][k2] = pack8<T>(y);
+      }
+      if constexpr (K2 == 0) pack4_split<T>(x[qt][0], qk[qt], ql[qt]);
+    }
+    static_assert(K2 > 0 || SPLIT, "16 keys to a chunk: split");
+    constexpr int NTL = DP / 16, VL = NTL < 8 ? NTL : 8;
+    unsigned vb[VL];
+#pragma unroll
+    for (int l = 0; l < VL; ++l) vb[l] = (unsigned)(uintptr_t)tile + tile_vbase(l, g, p, CPR);
+    static_for<NTL>([&](auto TT) {
+      constexpr int t = decltype(TT)::value;
+      s16x4 v[NM];
+      static_for<NM>([&](auto MM) {
+        constexpr int m = decltype(MM)::value;
+        v[m] = lds_read_tr16_at<(t / 8) * 256 + m * 256 * CPR>(vb[t % 8]);
+      });
+      lds_wait_all();
+#pragma unroll
+      for (int m = 0; m < NM; ++m) {
+        lds_ready(v[m]);
+        zero_infinities<T>(v[m], any);
+      }
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        if constexpr (K2 == 0) {
+          sm[qt].o[t] = Mfma16<T>::run16(v[0], qk[qt], sm[qt].o[t]);
+          sm[qt].o[t] = Mfma16<T>::run16(v[0], ql[qt], sm[qt].o[t]);
+        } else {
+#pragma unroll
+          for (int half = 0; half < (SPLIT ? 2 : 1); ++half)
+#pragma unroll
+            for (int k2 = 0; k2 < K2; ++k2) {
+              const s16x4 a = v[2 * k2], b = v[2 * k2 + 1];
+              const s16x8 av = s16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+              sm[qt].o[t] = Mfma16<T>::run(av, half ? pl[qt][k2] : pk[qt][k2], sm[qt].o[t]);
+            }
+        }
+      }
+    });
+  } else {
+#pragma unroll
+    for (int t = 0; t < DP / 16; ++t) {
+#pragma unroll
+      for (int m = 0; m < NM; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = 16 * m + 4 * g + r;
+          float a = *(const float *)(tile + (row * CPR + ((4 * t + (p >> 2)) ^ swz(row, CPR))) * 16 + (p & 3) * 4);
+          if (!(fabsf(a) < INFINITY)) {
+            a = 0.f;
+            any = true;
+          }
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) sm[qt].o[t] = mfma_f32_16x16x4(a, x[qt][m][r], sm[qt].o[t]);
+          if (r == 3) asm volatile("" ::: "memory");
+        }
+    }
+  }
+  if (!__ballot(any)) return;
+#pragma unroll 1
+  for (int key = 0; key < KC; ++key) {
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) {
+      float y = 0.f;  // this key's p of row p lies with the row's lane of group key / 4 % 4
+#pragma unroll
+      for (int m = 0; m < NM; ++m)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) y = key >> 4 == m && (key & 3) == r ? x[qt][m][r] : y;
+      y = __shfl(y, (key >> 2 & 3) * 16 + p, 64);
+#pragma unroll
+      for (int t = 0; t < DP / 16; ++t) {
+        const int at = (16 * t + 4 * g) * (int)sizeof(T);
+        const T *v = (const T *)(tile + (key * CPR + ((at >> 4) ^ swz(key, CPR))) * 16 + (at & 15));
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float z = to_f32<T>(v[r]);
+          if (key < lim[qt] && !(fabsf(z) < INFINITY)) sm[qt].o[t][r] += y * z;
+        }
+        asm volatile("" ::: "memory");
+      }
+    }
+  }
 }
 
 // o[d .. d + 3] = acc * inv [* sigmoid(gate)] of a row; inv 0: a row that sees
@@ -322,6 +478,27 @@ template <typename T, int DP> __global__ __launch_bounds__(64) void cache_part_k
     mm_tr_acc<T, DP, KC, 0, sizeof(T) == 2>(Vs, x, sm.o, g, p);
   }
 
+  if (__builtin_expect(__ballot(ri.valid && !sm.finite()) != 0, 0)) {
+    RowFrag<T, DP> frs[1] = {fr};
+    SoftmaxState<DP> sms[1];
+    sms[0].init();
+    lds_wait_all();  // the last chunk's reads, whose stage may be written first
+    if (c0 < c1) issue(c0);
+    for (int c = c0; c < c1; ++c) {
+      wait_vmcnt<0>();
+      lds_wait_all();
+      if (c + 1 < c1) issue(c + 1);
+      const char *Ks = smem + (c % C::NST) * 2 * C::TILE, *Vs = Ks + C::TILE;
+      f32x4 s[1][NM];
+      careful_scores<T, DP, 1, NM>(Ks, frs, s, g, p);
+      mask_keys<NM>(s[0], lim - c * KC, g);
+      float x[1][NM][4];
+      sms[0].template step<NM>(s[0], a.scale2, x[0]);
+      careful_values<T, DP, KC, 1, true>(Vs, x, sms, {lim - c * KC}, g, p);
+    }
+    sm = sms[0];
+  }
+
   const float lt = sm.total();
   if (g == 0) a.stat[slot + p] = float2{sm.m, lt};
   if (ri.valid && lt != 0.f) {  // (a NaN sum is kept)
@@ -437,12 +614,14 @@ __device__ __forceinline__ void pv_tile(const char *tile, const float (&x)[QT][K
 }
 
 template <typename T, int DP, int NW, int QT, int KC, int NST> struct TileCfg {
-  static constexpr int ES = sizeof(T), ROWS = NW * 16 * QT, TILE = KC * DP * ES, LDS = NST * 2 * TILE;
-  static_assert(LDS <= 160 * 1024 - 64, "LDS");
+  static constexpr int ES = sizeof(T), TILE = KC * DP * ES, RING = NST * 2 * TILE, LDS = RING + NW * 4;
+  static_assert(LDS <= 160 * 1024, "LDS");
 };
 
+// (d 32: registers for three waves to a SIMD, as the loop needs, also where the second look would take more: 19.2 us against 21.3,
+// 448 rows a head over 22876 keys)
 template <typename T, int DP, int NW, int QT, int KC, int NST>
-__global__ __launch_bounds__(NW * 64) void cache_tile_kernel(CacheArgs a, int64_t npre) {
+__global__ __launch_bounds__(NW * 64, DP == 32 ? 3 : 1) void cache_tile_kernel(CacheArgs a, int64_t npre) {
   using C = TileCfg<T, DP, NW, QT, KC, NST>;
   constexpr int NM = KC / 16;
   extern __shared__ __attribute__((aligned(16))) char smem[];
@@ -548,6 +727,43 @@ __global__ __launch_bounds__(NW * 64) void cache_tile_kernel(CacheArgs a, int64_
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) sm[qt].template step<NM>(s[qt], a.scale2, x[qt]);
     pv_tile<T, DP, KC, QT>(Vs, x, sm, g, p);
+  }
+
+  bool bad = false;
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) bad = bad || (ri[qt].valid && !sm[qt].finite());
+  // (the chunks are every wave's: all go through them again if one has to)
+  uint32_t *vote = (uint32_t *)(smem + C::RING);
+  bad = __ballot(bad) != 0;
+  if (lane == 0) vote[w] = bad;
+  lds_barrier();
+  if (__builtin_expect(__ballot(vote[lane % NW] != 0) != 0, 0)) {
+    SoftmaxState<DP> sm2[QT];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) sm2[qt].init();
+    ist = cst = 0;
+    if (c0 < c1) issue(c0);
+    for (int c = c0; c < c1; ++c) {
+      wait_vmcnt<0>();
+      lds_barrier();
+      if (c + 1 < c1) issue(c + 1);
+      const char *Ks = smem + cst * 2 * C::TILE, *Vs = Ks + C::TILE;
+      cst = cst + 1 == NST ? 0 : cst + 1;
+      if (w * QT * 16 >= tr) continue;
+      f32x4 s[QT][NM];
+      careful_scores<T, DP, QT, NM>(Ks, fr, s, g, p);
+      float x[QT][NM][4];
+      int lim[QT];
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt) {
+        lim[qt] = (ri[qt].valid ? ri[qt].lim : keys) - c * KC;
+        mask_keys<NM>(s[qt], lim[qt], g);
+        sm2[qt].template step<NM>(s[qt], a.scale2, x[qt]);
+      }
+      careful_values<T, DP, KC, QT, false>(Vs, x, sm2, lim, g, p);
+    }
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) sm[qt] = sm2[qt];
   }
 
 #pragma unroll

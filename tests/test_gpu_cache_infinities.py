@@ -57,3 +57,49 @@ def test_rows_whose_every_key_is_scored_minus_infinity(dt, T, P):
         kp[0, :, 0] = -math.inf
     o, lse, out = _check(q, k, v, kp, vp, lens, g)
     assert (lse[0, :2] == -math.inf).all() and (o[0, :2] == 0).all() and lse[0, 2:].isfinite().all()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("D", [32, 64, 72, 128, 256])
+@pytest.mark.parametrize("Hq,T,P", [(2, 1, 0), (4, 4, 0), (4, 3, 60), (6, 50, 0), (4, 80, 60)])
+def test_infinite_values(dt, D, Hq, T, P):
+    lens, count = [150, 81, 1], [T, max(1, T - 2), 1]
+    q, k, v, kp, vp, g = _make(dt, 3, Hq, 2, T, 150, D, lens, P=P)
+    place = [(0, 0, 149, 1, math.inf), (0, 1, 148, D - 1, -math.inf), (0, 0, 100, 0, math.inf), (0, 0, 70, 0, -math.inf),
+             (1, 0, 80, 5, math.nan), (1, 1, 0, 7, math.inf), (2, 0, 0, 2, -math.inf)]
+    plain = v.clone()
+    for b, h, s, d, x in place:
+        v[b, h, s, d], plain[b, h, s, d] = x, 0.0
+    if P:
+        vp[1, 31, 4], first = -math.inf, vp.clone()
+        first[1, 31, 4] = 0.0
+    gate = _randn(g, *q.shape, dtype=q.dtype)
+    o, lse, out = _check(q, k, v, kp, vp, lens, g, count, gate)
+    # every other output as if the infinities were zeros, bit for bit
+    o0, lse0 = _call(q, k, plain, kp, first if P else None, lens, count=_ints(count), out_gate=gate)
+    assert torch.equal(lse, lse0)
+    fin = o.isfinite()
+    assert torch.equal(o[fin], o0[fin])
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+def test_one_row_of_infinite_values(dt):
+    # p = 1 exactly
+    q, k, v, _, _, g = _make(dt, 1, 2, 1, 1, 40, 64, [1])
+    v[0, 0, 0, ::3], v[0, 0, 0, 1::3] = math.inf, -math.inf
+    o = cache.cache_attention(q, k, v, _ints([1]))
+    assert torch.equal(o, v[:, :, :1].expand(1, 2, 1, 64))
+
+
+@pytest.mark.parametrize("Hq,T,Hkv,S", [(8, 1, 8, 9000), (16, 300, 2, 700)])
+def test_infinite_values_in_one_of_many_shares(Hq, T, Hkv, S):
+    # the other shares, tiles and sequences keep their bits
+    q, k, v, _, _, g = _make("bf16", 2, Hq, Hkv, T, S, 128, [S, S - 77])
+    want = cache.cache_attention(q, k, v, _ints([S, S - 77]))
+    v[1, 0, S - 200, 9] = math.inf
+    got = cache.cache_attention(q, k, v, _ints([S, S - 77]))
+    t = torch.arange(T, device=DEV)
+    sees = (S - 77 - T + t >= S - 200).view(1, T).expand(Hq // Hkv, T)
+    assert torch.equal(got[1, :Hq // Hkv, :, 9] == math.inf, sees)
+    got[1, :Hq // Hkv, :, 9] = torch.where(sees, want[1, :Hq // Hkv, :, 9], got[1, :Hq // Hkv, :, 9])
+    assert torch.equal(got, want)
