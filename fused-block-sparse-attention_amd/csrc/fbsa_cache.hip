@@ -211,7 +211,7 @@ template <int NM> __device__ __forceinline__ void mask_keys(f32x4 (&s)[NM], int 
 
 // ---- infinities. The matrix instructions add 0 * v for every key of a chunk that a
 // row does not see, and for the empty half of a split p: NaN where v is infinite or
-// NaN. Where a row's O is not finite its share of the keys is therefore gone through
+// NaN; a key's infinities past the head dim's columns do the same to its scores. Where a row's O is not finite its share of the keys is therefore gone through
 // once more: infinite values are zeros in the products, which are otherwise the same
 // instructions in the same order (so finite results are the same bits), and the rows
 // that see them get p * v added outside. Finite caches pay for the look at O: 0.1 to
@@ -225,9 +225,11 @@ template <typename T> __device__ __forceinline__ void zero_infinities(s16x4 &x, 
       any = true;
     }
 }
-// the scores of a chunk, as mm_rows_frag and qk_tile form them
+// the scores of a chunk, as mm_rows_frag and qk_tile form them, without the columns past
+// the head dim: copies of the row's last chunk there, whose infinities the query's zeros
+// would turn to NaN
 template <typename T, int DP, int QT, int NM>
-__device__ __forceinline__ void careful_scores(const char *tile, const RowFrag<T, DP> (&fr)[QT], f32x4 (&acc)[QT][NM], int g, int p) {
+__device__ __forceinline__ void careful_scores(const char *tile, const RowFrag<T, DP> (&fr)[QT], f32x4 (&acc)[QT][NM], int D, int g, int p) {
   constexpr int CPR = DP * (int)sizeof(T) / 16, KS = sizeof(T) == 2 ? DP / 32 : DP / 4, KL = KS < 4 ? KS : 4;
   const char *kb[KL];  // (few addresses and few loads ahead: registers count here, not time)
   if constexpr (sizeof(T) == 2) {
@@ -241,11 +243,12 @@ __device__ __forceinline__ void careful_scores(const char *tile, const RowFrag<T
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       if constexpr (sizeof(T) == 2) {
-        const s16x8 x = *(const s16x8 *)(kb[ks % KL] + (ks / 4) * 256 + m * 256 * CPR);
+        s16x8 x = *(const s16x8 *)(kb[ks % KL] + (ks / 4) * 256 + m * 256 * CPR);
+        if (32 * ks + 8 * g >= D) x = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) acc[qt][m] = Mfma16<T>::run(x, fr[qt].h[ks], acc[qt][m]);
       } else {
-        const float x = *(const float *)(tile + ((16 * m + p) * CPR + (ks ^ swz(p, CPR))) * 16 + g * 4);
+        const float y = *(const float *)(tile + ((16 * m + p) * CPR + (ks ^ swz(p, CPR))) * 16 + g * 4), x = 4 * ks + g < D ? y : 0.f;
 #pragma unroll
         for (int qt = 0; qt < QT; ++qt) acc[qt][m] = mfma_f32_16x16x4(x, fr[qt].f[ks], acc[qt][m]);
       }
@@ -456,6 +459,13 @@ template <typename T, int DP> __global__ __launch_bounds__(64) void cache_part_k
     pv.issue(st + C::TILE, vb, (uint32_t)c * KC, keys, vstep, a.D * C::ES, 0);
   };
 
+  auto store_scores = [&](int c, const f32x4 (&s)[NM]) {
+    if (score && ri.valid) {
+#pragma unroll
+      for (int m = 0; m < NM; ++m) *(f32x4 *)(score + (int64_t)c * KC + 16 * m + 4 * g) = s[m] * a.scale2;
+    }
+  };
+
   SoftmaxState<DP> sm;
   sm.init();
   for (int c = c0; c < c0 + C::NST - 1 && c < c1; ++c) issue(c);
@@ -469,10 +479,7 @@ template <typename T, int DP> __global__ __launch_bounds__(64) void cache_part_k
     f32x4 s[NM];
     mm_rows_frag<T, DP, NM>(Ks, fr, s, g, p);
     if ((c + 1) * (int64_t)KC > low) mask_keys<NM>(s, lim - c * KC, g);
-    if (score && ri.valid) {
-#pragma unroll
-      for (int m = 0; m < NM; ++m) *(f32x4 *)(score + (int64_t)c * KC + 16 * m + 4 * g) = s[m] * a.scale2;
-    }
+    store_scores(c, s);
     float x[NM][4];
     sm.template step<NM>(s, a.scale2, x);
     mm_tr_acc<T, DP, KC, 0, sizeof(T) == 2>(Vs, x, sm.o, g, p);
@@ -490,8 +497,9 @@ template <typename T, int DP> __global__ __launch_bounds__(64) void cache_part_k
       if (c + 1 < c1) issue(c + 1);
       const char *Ks = smem + (c % C::NST) * 2 * C::TILE, *Vs = Ks + C::TILE;
       f32x4 s[1][NM];
-      careful_scores<T, DP, 1, NM>(Ks, frs, s, g, p);
+      careful_scores<T, DP, 1, NM>(Ks, frs, s, a.D, g, p);
       mask_keys<NM>(s[0], lim - c * KC, g);
+      store_scores(c, s[0]);
       float x[1][NM][4];
       sms[0].template step<NM>(s[0], a.scale2, x[0]);
       careful_values<T, DP, KC, 1, true>(Vs, x, sms, {lim - c * KC}, g, p);
@@ -694,6 +702,16 @@ __global__ __launch_bounds__(NW * 64, DP == 32 ? 3 : 1) void cache_tile_kernel(C
     pv.issue(st + C::TILE, vb, (uint32_t)c * KC, keys, vstep, a.D * C::ES, w);
     ist = ist + 1 == NST ? 0 : ist + 1;
   };
+  auto store_scores = [&](int c, const f32x4 (&s)[NM]) {
+    if (!pre && a.sc && ri[0].valid) {  // (one tile of up to 16 rows: the first fragment)
+      float *score = a.sc + score_row(a, ri[0].b, ri[0].hq / a.G, p);
+#pragma unroll
+      for (int m = 0; m < NM; ++m) {
+        const int64_t key = (int64_t)c * KC + 16 * m + 4 * g;
+        if (key < score_keys(a)) *(f32x4 *)(score + key) = s[m] * a.scale2;
+      }
+    }
+  };
   SoftmaxState<DP> sm[QT];
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) sm[qt].init();
@@ -715,14 +733,7 @@ __global__ __launch_bounds__(NW * 64, DP == 32 ? 3 : 1) void cache_tile_kernel(C
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) mask_keys<NM>(s[qt], (ri[qt].valid ? ri[qt].lim : keys) - c * KC, g);
     }
-    if (!pre && a.sc && ri[0].valid) {  // (one tile of up to 16 rows: the first fragment)
-      float *score = a.sc + score_row(a, ri[0].b, ri[0].hq / a.G, p);
-#pragma unroll
-      for (int m = 0; m < NM; ++m) {
-        const int64_t key = (int64_t)c * KC + 16 * m + 4 * g;
-        if (key < score_keys(a)) *(f32x4 *)(score + key) = s[0][m] * a.scale2;
-      }
-    }
+    store_scores(c, s[0]);
     float x[QT][NM][4];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) sm[qt].template step<NM>(s[qt], a.scale2, x[qt]);
@@ -751,13 +762,14 @@ __global__ __launch_bounds__(NW * 64, DP == 32 ? 3 : 1) void cache_tile_kernel(C
       cst = cst + 1 == NST ? 0 : cst + 1;
       if (w * QT * 16 >= tr) continue;
       f32x4 s[QT][NM];
-      careful_scores<T, DP, QT, NM>(Ks, fr, s, g, p);
+      careful_scores<T, DP, QT, NM>(Ks, fr, s, a.D, g, p);
       float x[QT][NM][4];
       int lim[QT];
 #pragma unroll
       for (int qt = 0; qt < QT; ++qt) {
         lim[qt] = (ri[qt].valid ? ri[qt].lim : keys) - c * KC;
         mask_keys<NM>(s[qt], lim[qt], g);
+        if (qt == 0) store_scores(c, s[0]);
         sm2[qt].template step<NM>(s[qt], a.scale2, x[qt]);
       }
       careful_values<T, DP, KC, QT, false>(Vs, x, sm2, lim, g, p);

@@ -46,6 +46,23 @@ def test_weights_beside_keys_scored_minus_infinity(dt, D, T):
 
 
 @pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("D", [8, 24, 40, 80, 136, 248])
+@pytest.mark.parametrize("T,P", [(1, 0), (3, 45), (40, 0), (30, 70)])
+def test_keys_scored_minus_infinity_at_head_dims_between(dt, D, T, P):
+    # the last 16 bytes of a row hold the infinity
+    lens = [170, 57]
+    q, k, v, kp, vp, g = _make(dt, 2, 6, 2, T, 170, D, lens, P=P)
+    q[..., D - 1] = q[..., D - 1].abs() + 0.5
+    for s in (0, 31, 50, 169):
+        k[:, s % 2, s, D - 1] = -math.inf
+    for b, n in enumerate(lens):
+        k[b, :, n:] = math.nan
+    if P:
+        kp[0, P // 2, D - 1] = -math.inf
+    _check(q, k, v, kp, vp, lens, g, gate=_randn(g, *q.shape, dtype=q.dtype))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("T,P", [(1, 0), (4, 33), (40, 0), (150, 90)])
 def test_rows_whose_every_key_is_scored_minus_infinity(dt, T, P):
     # as a row that sees nothing: 0, -inf, and no weight; the weights of the rest do not suffer
