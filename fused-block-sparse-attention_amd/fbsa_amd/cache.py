@@ -109,7 +109,12 @@ def _ints(what, name, t, B):
 
 
 def _int32(t):
-    return t if t is None or (t.dtype == torch.int32 and t.is_contiguous()) else t.to(torch.int32).contiguous()
+    """The kernels' integers: 32 bits, contiguous; a 64-bit one beyond them is as far out as 32 bits say."""
+    if t is None or (t.dtype == torch.int32 and t.is_contiguous()):
+        return t
+    if t.dtype != torch.int32:
+        t = t.clamp(-(1 << 31), (1 << 31) - 1).to(torch.int32)
+    return t.contiguous()
 
 
 def _bytes(t):

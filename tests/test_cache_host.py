@@ -1,0 +1,29 @@
+"""The cache operators' host side: what is refused before a launch, workspaces,
+64-bit lengths, forward-mode gradients."""
+import ctypes
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fw
+
+from fbsa_amd import _lib, cache
+
+
+def _desc(**kw):
+    d = _lib.CacheDesc()
+    d.dtype, d.B, d.Hq, d.Hkv, d.T, d.S, d.P, d.D, d.scale = _lib.BF16, 1, 1, 1, 1, 128, 0, 64, 0.125
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+def _bytes(**kw):
+    return _lib.load().fbsa_cache_attn_workspace_bytes(ctypes.byref(_desc(**kw)))
+
+
+def test_lengths_beyond_32_bits_are_clamped_not_wrapped():
+    x = torch.tensor([1 << 32, (1 << 32) + 5, -(1 << 40), 7, -3, (1 << 31) - 1], dtype=torch.int64)
+    assert cache._int32(x).tolist() == [(1 << 31) - 1, (1 << 31) - 1, -(1 << 31), 7, -3, (1 << 31) - 1]
+    assert cache._int32(x).dtype == torch.int32 and cache._int32(None) is None
+    y = torch.tensor([1, 2, 3, 4], dtype=torch.int32)
+    assert cache._int32(y) is y and cache._int32(y[::2]).tolist() == [1, 3] and cache._int32(y[::2]).is_contiguous()
