@@ -14,10 +14,12 @@ call synchronises and a captured graph follows their values.
 * ``KVCache``                  the four over one set of buffers
 
 They are for inference: no gradients are formed, and inputs that require grad
-are refused while gradients are being recorded. The reference attends over
-whole prompts only and has no counterpart.
+are refused while gradients are being recorded, those with a forward-mode
+tangent always. The reference attends over whole prompts only and has no
+counterpart.
 """
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .ops import _dtype_code, _ptr
@@ -33,14 +35,14 @@ _PLANS_MAX = 1024
 
 
 def _key(what, scalars, ts):
-    """What a plan depends on; refuses tensors that a recorded graph would need gradients of."""
-    key, grad = [what, scalars], torch.is_grad_enabled()
+    """What a plan depends on; refuses tensors that a recorded graph, or a tangent, would need gradients of."""
+    key, grad, dual = [what, scalars], torch.is_grad_enabled(), forward_ad._current_level >= 0
     for t in ts:
         if t is None:
             key.append(None)
         else:
-            if grad and t.requires_grad:
-                raise ValueError(f"fbsa.{what}: no gradients are formed (call it under torch.no_grad())")
+            if (grad and t.requires_grad) or (dual and forward_ad.unpack_dual(t).tangent is not None):
+                raise ValueError(f"fbsa.{what}: no gradients are formed (call it under torch.no_grad(), without forward-mode tangents)")
             key += (t.shape, t.stride(), t.dtype, t.get_device())
     return tuple(key)
 

@@ -27,3 +27,13 @@ def test_lengths_beyond_32_bits_are_clamped_not_wrapped():
     assert cache._int32(x).dtype == torch.int32 and cache._int32(None) is None
     y = torch.tensor([1, 2, 3, 4], dtype=torch.int32)
     assert cache._int32(y) is y and cache._int32(y[::2]).tolist() == [1, 3] and cache._int32(y[::2]).is_contiguous()
+
+
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_gradients_are_refused(grad):
+    x = torch.zeros(1, 2, 8, 64)
+    with fw.dual_level(), torch.set_grad_enabled(grad):
+        cache._key("t", (), (x, None))
+        dual = fw.make_dual(x, torch.ones_like(x))
+        with pytest.raises(ValueError, match="gradients"):
+            cache._key("t", (), (x, dual))
