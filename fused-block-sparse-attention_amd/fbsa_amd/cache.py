@@ -20,6 +20,7 @@ counterpart.
 """
 import torch
 from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from .ops import _dtype_code, _ptr
@@ -203,6 +204,8 @@ def append(k, v, k_new, v_new, start, *, count=None, weight=None):
     _apart("append", ((pk, nk), (pv, nv)), ((pkn, nkn), (pvn, nvn)))
     start, count = _int32(start), _int32(count)
     _launch(p, _lib.load().fbsa_cache_append, "fbsa_cache_append", pk, pv, pkn, pvn, start.data_ptr(), _ptr(count), _ptr(weight))
+    # (what a kernel writes through an address counts as modified in place, as torch's own operations do)
+    increment_version((k, v) if weight is None else (k, v, weight))
 
 
 def _plan_attend(what, scalars, q, kp, vp, k, v, lens, count, out_gate, weight, out_weight):
@@ -285,6 +288,8 @@ def _attend(what, q, kp, vp, k, v, lens, count, scale, out_gate, weight, out_wei
     ws = torch.empty(p.nbytes, dtype=torch.uint8, device=p.device)
     _launch(p, _lib.load().fbsa_cache_attn, what, q.data_ptr(), pk, pv, lens.data_ptr(), _ptr(count), pkp, pvp,
             _ptr(out_gate), o.data_ptr(), _ptr(lse), pw, pwo, ws.data_ptr(), p.nbytes)
+    if out_weight is not None:
+        increment_version(out_weight)
     return (o, lse) if need_lse else o
 
 
@@ -395,6 +400,7 @@ def evict(k, v, weight, lens, budget, *, recent=0, sink=0, out=None):
     ws = torch.empty(p.nbytes, dtype=torch.uint8, device=p.device) if p.nbytes else None
     _launch(p, _lib.load().fbsa_cache_evict, "fbsa_cache_evict", pk, pv, pw, lens.data_ptr(), pko, pvo, pwo, index.data_ptr(),
             new_lens.data_ptr(), _ptr(ws), p.nbytes)
+    increment_version((k, v, weight) if p.inplace else (ko, vo, wo))
     return index, new_lens
 
 

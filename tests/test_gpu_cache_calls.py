@@ -32,3 +32,42 @@ def _saved(t):
 def _raises(loss):
     with pytest.raises(RuntimeError, match="inplace operation"):
         loss.backward()
+
+
+def test_what_a_call_writes_counts_as_modified():
+    q, k, v, _, _, g = _make("bf16", 1, 4, 2, 1, 40, 64, [40])
+    w, lens = _randn(g, 1, 2, 40).abs(), _ints([40])
+    losses = [_saved(x) for x in (k, v, w)]
+    cache.append(k, v, q[:, :2], q[:, :2], _ints([3]), weight=w)
+    for x in losses:
+        _raises(x)
+    a, b, out = _saved(k), _saved(w), torch.zeros_like(w)
+    c = _saved(out)
+    cache.cache_attention(q, k, v, lens, weight=w, out_weight=out)
+    a.backward()
+    b.backward()
+    _raises(c)
+    c = _saved(w)
+    cache.cache_attention(q, k, v, lens, weight=w)
+    _raises(c)
+    dst = [torch.zeros(1, 2, 8, 64, dtype=k.dtype, device=DEV) for _ in range(2)] + [torch.zeros(1, 2, 8, device=DEV)]
+    losses, kept = [_saved(x) for x in dst], [_saved(x) for x in (k, v, w)]
+    cache.evict(k, v, w, lens, 8, out=dst)
+    for x in losses:
+        _raises(x)
+    for x in kept:
+        x.backward()
+    losses = [_saved(x) for x in (k, v, w)]
+    cache.evict(k, v, w, lens, 8)
+    for x in losses:
+        _raises(x)
+
+
+def test_caches_made_in_inference_mode():
+    with torch.inference_mode():
+        c = cache.KVCache(2, 2, 64, 64, weight=True)
+        x = _randn(_gen(0), 2, 2, 3, 64, dtype=torch.bfloat16)
+        c.append(x, x)
+        c.attend(x)
+        c.evict(2)
+    assert c.lens.tolist() == [2, 2]
