@@ -247,8 +247,6 @@ def _plan_attend(what, scalars, q, kp, vp, k, v, lens, count, out_gate, weight, 
     _ints(what, "count", count, B)
     p.q_ok = _strided(q, 3)
     p.empty = q.numel() == 0
-    if p.empty and out_weight is not None and B:
-        raise ValueError(f"fbsa.{what}: no queries to take weights from")
     p.shape, p.S = (B, Hq, T, D), S
     packed = (Hq * T * D, T * D, D)
     d.B, d.Hq, d.Hkv, d.T, d.S, d.P, d.D = B, Hq, Hkv, T, S, p.P, D
@@ -270,6 +268,8 @@ def _attend(what, q, kp, vp, k, v, lens, count, scale, out_gate, weight, out_wei
     o = torch.empty(p.shape, dtype=q.dtype, device=p.device)
     lse = torch.empty(p.shape[:3], dtype=torch.float32, device=p.device) if need_lse else None
     if p.empty:
+        if out_weight is not None and out_weight is not weight and out_weight.numel():
+            raise ValueError(f"fbsa.{what}: no queries to take weights from")
         return (o, lse) if need_lse else o
     if q.data_ptr() & 15 or not p.q_ok:
         q = q.clone(memory_format=torch.contiguous_format)
@@ -309,7 +309,8 @@ def cache_attention(q, k, v, lens=None, *, count=None, scale=None, out_gate=None
     out_weight (default: weight itself) receives weight plus the probability
     that these queries, summed over the group's heads, gave each row below
     lens; rows at or past lens are left as they were. out_weight alone starts
-    from zeros.
+    from zeros. No new tokens (T = 0) leave weight itself as it is; another
+    out_weight is refused then.
 
     Returns o (B, Hq, T, D), and with need_lse the fp32 natural-log normaliser
     (B, Hq, T); padding queries, and queries that see no row or whose every score

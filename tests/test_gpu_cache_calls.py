@@ -71,3 +71,21 @@ def test_caches_made_in_inference_mode():
         c.attend(x)
         c.evict(2)
     assert c.lens.tolist() == [2, 2]
+
+
+def test_no_new_tokens():
+    g = _gen(0)
+    for weight in (False, True):
+        c = cache.KVCache(2, 2, 64, 64, weight=weight)
+        c.append(*(_randn(g, 2, 2, 5, 64, dtype=torch.bfloat16) for _ in range(2)))
+        none = torch.zeros(2, 4, 0, 64, dtype=torch.bfloat16, device=DEV)
+        if weight:
+            c.weight.copy_(_randn(g, 2, 2, 64))
+            before = c.weight.clone()
+        c.append(none[:, :2], none[:, :2])
+        o, lse = c.attend(none, need_lse=True)
+        assert o.shape == (2, 4, 0, 64) and lse.shape == (2, 4, 0) and c.lens.tolist() == [5, 5]
+        if weight:
+            assert torch.equal(c.weight, before)
+            with pytest.raises(ValueError, match="no queries"):   # nothing would fill another tensor
+                cache.cache_attention(none, c.k, c.v, c.lens, weight=c.weight, out_weight=torch.zeros_like(c.weight))
