@@ -1028,6 +1028,7 @@ template <typename T, int DP> struct WeightCfg {
   // (2048 tokens over 16301 rows, 16 heads over 2, d 256: KF 4 with 64 rows 286 us,
   // KF 2 with 128 rows 323, with 64 364); fp32 has registers for two
   static constexpr int KF = ES == 2 ? 4 : 2, KEYS = 4 * 16 * KF;
+  static_assert(KEYS == (ES == 2 ? 256 : 128), "the launch's limit in check_cache");
   static constexpr int ROWS = DP * ES * KF <= 1024 ? 128 : 64, NM = ROWS / 32;  // NM 16-row tiles to a half
   static constexpr int LPT = ROWS * CPR / NT;        // 16-byte loads per thread and chunk (0: fewer than the threads)
   static constexpr int STAGE = ROWS * DP * ES + ROWS * 4;
@@ -1170,7 +1171,7 @@ template <typename T, int DP> __global__ __launch_bounds__(512) void cache_weigh
 // head over up to 123654 keys, 48 caches, d 32, 216 -> 118 us; 108 rows, d 64, fp32,
 // 617 -> 377.
 template <typename T, int DP> struct WeightRowsCfg {
-  static constexpr int ES = sizeof(T), CPR = DP * ES / 16, MAXROWS = 128;
+  static constexpr int ES = sizeof(T), CPR = DP * ES / 16, MAXROWS = 128;  // (check_cache knows it)
   static constexpr int KF = ES == 2 ? (DP >= 256 ? 2 : 4) : (DP >= 128 ? 1 : 2), KEYS = 16 * KF;
 };
 template <typename T, int DP> __global__ __launch_bounds__(256) void cache_weight_rows_kernel(CacheArgs a) {
@@ -1433,8 +1434,16 @@ static int check_cache(const fbsa_cache_desc *d) {
   const int64_t rs[4] = {d->sk[2], d->sv[2], d->P ? d->skp[1] : 0, d->P ? d->svp[1] : 0};
   for (int64_t r : rs)
     if (r * es >= 1LL << 26) return fail(FBSA_EUNSUPPORTED, "%s: a row stride of %lld elements is 64 MiB or more", fn, (long long)r);
-  // (a launch has fewer than 2^32 threads: 64 a row where a wave joins each)
-  if (cache_plan(d).rows > lim || d->B * d->Hq * d->T > 0x3ff0000LL) return fail(FBSA_EUNSUPPORTED, "%s: grid too large", fn);
+  // A launch has fewer than 2^32 threads along an axis: 64 a row where a wave joins
+  // each; with weights 256 per 1024 keys beside a short step's rows, or 512 per 128 keys
+  // (fp32; 16 bits: 256 keys) for more than 128 rows
+  const CachePlan pl = cache_plan(d);
+  const int64_t TG = d->T * (d->Hq / d->Hkv), most = 0xfffff000LL;
+  const int64_t short_step = (d->B * d->Hq * d->T + d->B * d->Hkv * cdiv(d->S, kWeightKeys)) * 256;
+  const int64_t long_step = cdiv(d->S, d->dtype == FBSA_F32 ? 128 : 256) * 512;
+  if (pl.rows > lim || d->B * d->Hq * d->T > 0x3ff0000LL ||
+      ((d->flags & FBSA_CACHE_WEIGHT) && (pl.scores ? short_step > most : TG > 128 && long_step > most)))
+    return fail(FBSA_EUNSUPPORTED, "%s: grid too large", fn);
   return FBSA_OK;
 }
 

@@ -37,3 +37,13 @@ def test_forward_mode_gradients_are_refused(grad):
         dual = fw.make_dual(x, torch.ones_like(x))
         with pytest.raises(ValueError, match="gradients"):
             cache._key("t", (), (x, dual))
+
+
+@pytest.mark.parametrize("kw", [
+    dict(dtype=_lib.F32, S=(1 << 30) + (1 << 20), D=8, T=129, flags=_lib.CACHE_WEIGHT),   # 128 keys of 512 threads each
+    dict(B=65535, S=1 << 28, D=8, flags=_lib.CACHE_WEIGHT),                               # 1024 keys of 256 threads each
+])
+def test_launches_of_more_than_32_bits_of_threads_are_refused(kw):
+    assert _bytes(**kw) == 0 and b"grid" in _lib.load().fbsa_last_error()
+    assert _bytes(**{**kw, "S": 1 << 16}) > 0
+    assert _bytes(**{**kw, "flags": 0}) > 0
