@@ -1313,16 +1313,19 @@ static CachePlan cache_plan(const fbsa_cache_desc *d) {
   p.np_pre = d->P ? shares(p.few_pre, false, d->Hkv * p.rt_pre, d->P) : 0;
   p.direct = !p.few_own && !d->P && p.np_own == 1;
   p.rows = d->B * d->Hkv * p.rt_own * p.np_own * p.tr_own + d->Hkv * p.rt_pre * p.np_pre * p.tr_pre;
+  // (tiles that write their results have no parts; 32 x 1024 tokens, 32 heads over 8, d 256: 1 GiB of them)
+  const size_t parts = p.direct ? 0 : (size_t)p.rows;
   p.stat = 0;
-  p.part = up256((size_t)p.rows * 8);
-  p.lse2 = p.part + up256((size_t)p.rows * p.DP * 4);
+  p.part = up256(parts * 8);
+  p.lse2 = p.part + up256(parts * p.DP * 4);
   // (a share is at least four chunks of 64 rows)
   const int64_t wgs = d->B * d->Hkv * cdiv(d->S, d->dtype == FBSA_F32 ? 128 : 256), z = wgs >= kCUs ? 1 : kCUs / wgs, zmax = cdiv(TG, 256);
   p.nz = z < zmax ? z : zmax;
   const bool weight = d->flags & FBSA_CACHE_WEIGHT;
-  p.wpart = p.lse2 + up256((size_t)(d->B * d->Hkv * TG) * 4);
+  p.wpart = p.lse2 + (weight && !p.scores ? up256((size_t)(d->B * d->Hkv * TG) * 4) : 0);
   p.sc = p.wpart + (weight && !p.scores && p.nz > 1 ? up256((size_t)p.nz * d->B * d->Hkv * d->S * 4) : 0);
   p.total = p.sc + (weight && p.scores ? up256((size_t)(d->B * d->Hkv * TG) * cdiv(d->S, 32) * 128) : 0);
+  if (p.total == 0) p.total = 256;  // (0 says that a descriptor is refused)
   return p;
 }
 

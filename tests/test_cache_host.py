@@ -47,3 +47,12 @@ def test_launches_of_more_than_32_bits_of_threads_are_refused(kw):
     assert _bytes(**kw) == 0 and b"grid" in _lib.load().fbsa_last_error()
     assert _bytes(**{**kw, "S": 1 << 16}) > 0
     assert _bytes(**{**kw, "flags": 0}) > 0
+
+
+@pytest.mark.parametrize("kw", [dict(B=32, Hq=32, Hkv=8, T=1024, S=8192, D=256), dict(B=16, Hq=64, Hkv=8, T=2048, S=4096, D=128)])
+def test_tiles_that_write_their_results_need_no_parts(kw):
+    assert 0 < _bytes(**kw) <= 256
+    # with weights: the rows' normalisers
+    rows = kw["B"] * kw["Hq"] * kw["T"]
+    assert 4 * rows <= _bytes(**kw, flags=_lib.CACHE_WEIGHT) <= 4 * rows + 4096
+    assert _bytes(**kw, P=64) > 4 * rows * kw["D"]
