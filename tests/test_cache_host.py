@@ -6,6 +6,7 @@ import pytest
 import torch
 import torch.autograd.forward_ad as fw
 
+import _cachetight as tight
 from fbsa_amd import _lib, cache
 
 
@@ -56,3 +57,18 @@ def test_tiles_that_write_their_results_need_no_parts(kw):
     rows = kw["B"] * kw["Hq"] * kw["T"]
     assert 4 * rows <= _bytes(**kw, flags=_lib.CACHE_WEIGHT) <= 4 * rows + 4096
     assert _bytes(**kw, P=64) > 4 * rows * kw["D"]
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rounded", [False, True])
+def test_the_bounds_pass_a_rounded_result_and_see_a_missing_key(dt, rounded):
+    g = torch.Generator().manual_seed(0)
+    q, k, v = (torch.randn(1, 2, n, 64, generator=g).to(dt) for n in (40, 1000, 1000))
+    lens = [1000]
+    r = tight.attend(q, k, v, lens, weight=torch.zeros(1, 2, 1000))
+    tight.check((r["o"].to(dt), r["lse"].float(), r["w"].float()), r, q, 1000, rounded)
+    less = v.clone()
+    less[0, 1, 500] = 0   # one of a thousand values left out, of one head
+    o = tight.attend(q, k, less, lens)["o"].to(dt)
+    with pytest.raises(AssertionError, match="bound"):
+        tight.check((o, r["lse"].float(), None), r, q, 1000, rounded)
