@@ -214,8 +214,8 @@ template <int NM> __device__ __forceinline__ void mask_keys(f32x4 (&s)[NM], int 
 // NaN; a key's infinities past the head dim's columns do the same to its scores. Where a row's O is not finite its share of the keys is therefore gone through
 // once more: infinite values are zeros in the products, which are otherwise the same
 // instructions in the same order (so finite results are the same bits), and the rows
-// that see them get p * v added outside. Finite caches pay for the look at O: 0.1 to
-// 0.9 us a call (1.2% over 67 shapes).
+// that see them get p * v added outside. Finite caches pay for the look at O: up to
+// 2 us a call (three of 87 shapes over 4%, their mean as before).
 template <typename T> __device__ __forceinline__ void zero_infinities(s16x4 &x, bool &any) {
   constexpr short EXP = __is_same(T, bf16) ? 0x7f80 : 0x7c00;
 #pragma unroll
@@ -487,6 +487,9 @@ template <typename T, int DP> __global__ __launch_bounds__(64) void cache_part_k
 
   if (__builtin_expect(__ballot(ri.valid && !sm.finite()) != 0, 0)) {
     RowFrag<T, DP> frs[1] = {fr};
+    // (addresses of its own: shared with the loop above they would cost that its registers: fp32, d 256, 34372 keys 227 us, 190 so)
+    int gg = g, pp = p;
+    asm volatile("" : "+v"(gg), "+v"(pp));
     SoftmaxState<DP> sms[1];
     sms[0].init();
     lds_wait_all();  // the last chunk's reads, whose stage may be written first
@@ -497,12 +500,12 @@ template <typename T, int DP> __global__ __launch_bounds__(64) void cache_part_k
       if (c + 1 < c1) issue(c + 1);
       const char *Ks = smem + (c % C::NST) * 2 * C::TILE, *Vs = Ks + C::TILE;
       f32x4 s[1][NM];
-      careful_scores<T, DP, 1, NM>(Ks, frs, s, a.D, g, p);
+      careful_scores<T, DP, 1, NM>(Ks, frs, s, a.D, gg, pp);
       mask_keys<NM>(s[0], lim - c * KC, g);
       store_scores(c, s[0]);
       float x[1][NM][4];
       sms[0].template step<NM>(s[0], a.scale2, x[0]);
-      careful_values<T, DP, KC, 1, true>(Vs, x, sms, {lim - c * KC}, g, p);
+      careful_values<T, DP, KC, 1, true>(Vs, x, sms, {lim - c * KC}, gg, pp);
     }
     sm = sms[0];
   }
@@ -752,6 +755,8 @@ __global__ __launch_bounds__(NW * 64, DP == 32 ? 3 : 1) void cache_tile_kernel(C
     SoftmaxState<DP> sm2[QT];
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) sm2[qt].init();
+    int gg = g, pp = p;
+    asm volatile("" : "+v"(gg), "+v"(pp));  // (as above)
     ist = cst = 0;
     if (c0 < c1) issue(c0);
     for (int c = c0; c < c1; ++c) {
@@ -762,7 +767,7 @@ __global__ __launch_bounds__(NW * 64, DP == 32 ? 3 : 1) void cache_tile_kernel(C
       cst = cst + 1 == NST ? 0 : cst + 1;
       if (w * QT * 16 >= tr) continue;
       f32x4 s[QT][NM];
-      careful_scores<T, DP, QT, NM>(Ks, fr, s, a.D, g, p);
+      careful_scores<T, DP, QT, NM>(Ks, fr, s, a.D, gg, pp);
       float x[QT][NM][4];
       int lim[QT];
 #pragma unroll
@@ -772,7 +777,7 @@ __global__ __launch_bounds__(NW * 64, DP == 32 ? 3 : 1) void cache_tile_kernel(C
         if (qt == 0) store_scores(c, s[0]);
         sm2[qt].template step<NM>(s[qt], a.scale2, x[qt]);
       }
-      careful_values<T, DP, KC, QT, false>(Vs, x, sm2, lim, g, p);
+      careful_values<T, DP, KC, QT, false>(Vs, x, sm2, lim, gg, pp);
     }
 #pragma unroll
     for (int qt = 0; qt < QT; ++qt) sm[qt] = sm2[qt];
