@@ -56,10 +56,7 @@ struct CacheArgs {
 template <typename T, int DP> struct CacheCfg {
   static constexpr int ES = sizeof(T);
   static constexpr int KC = DP * ES >= 512 ? 16 : 32;
-  static constexpr int CPR = DP * ES / 16;
   static constexpr int TILE = KC * DP * ES;
-  static constexpr int LPT = KC * CPR / 64;  // 16-byte loads per lane and tile
-  static constexpr int NST = 2;
 };
 
 // Row rho of a (sequence, KV head): token rho / G, head rho % G. The keys it
@@ -140,6 +137,7 @@ template <typename T, int DP, int KC, int NW> struct TilePlan {
   // rows [row0, ...) of a tensor of `rows` rows: rows past the end read its last one
   __device__ __forceinline__ void issue(unsigned st, const char *base, uint32_t row0, uint32_t rows, int64_t step, int rowbytes, int w) const {
     const char *src = base + (int64_t)row0 * step;
+    static_assert(KC <= 64, "the strides' limit in check_cache");
     const uint32_t lim = tail_limit<KC>(row0, rows, (uint32_t)step, (uint32_t)rowbytes);
 #pragma unroll
     for (int n = 0; n < LPT; ++n) g2lds16_s(src, off[n] > lim ? lim : off[n], st + (n * NW + w) * 1024);
@@ -214,8 +212,8 @@ template <int NM> __device__ __forceinline__ void mask_keys(f32x4 (&s)[NM], int 
 // NaN; a key's infinities past the head dim's columns do the same to its scores. Where a row's O is not finite its share of the keys is therefore gone through
 // once more: infinite values are zeros in the products, which are otherwise the same
 // instructions in the same order (so finite results are the same bits), and the rows
-// that see them get p * v added outside. Finite caches pay for the look at O: up to
-// 2 us a call (three of 87 shapes over 4%, their mean as before).
+// that see them get p * v added outside. Finite caches pay for the look at O: over
+// 154 shapes up to 8% of a call (4 us of 47), 0.5% in the mean.
 template <typename T> __device__ __forceinline__ void zero_infinities(s16x4 &x, bool &any) {
   constexpr short EXP = __is_same(T, bf16) ? 0x7f80 : 0x7c00;
 #pragma unroll
@@ -454,7 +452,7 @@ template <typename T, int DP> __global__ __launch_bounds__(64) void cache_part_k
   pk.init(kstep / C::ES, a.D, 0, lane);
   pv.init(vstep / C::ES, a.D, 0, lane);
   auto issue = [&](int c) {
-    const unsigned st = (unsigned)(uintptr_t)smem + (c % C::NST) * 2 * C::TILE;
+    const unsigned st = (unsigned)(uintptr_t)smem + (c & 1) * 2 * C::TILE;
     pk.issue(st, kb, (uint32_t)c * KC, keys, kstep, a.D * C::ES, 0);
     pv.issue(st + C::TILE, vb, (uint32_t)c * KC, keys, vstep, a.D * C::ES, 0);
   };
@@ -468,14 +466,13 @@ template <typename T, int DP> __global__ __launch_bounds__(64) void cache_part_k
 
   SoftmaxState<DP> sm;
   sm.init();
-  for (int c = c0; c < c0 + C::NST - 1 && c < c1; ++c) issue(c);
+  if (c0 < c1) issue(c0);
   wait_vmcnt<0>();  // the query rows too: the compiler then waits for nothing in the loop
   for (int c = c0; c < c1; ++c) {
-    const int ahead = c1 - 1 - c;
-    wait_ring<2 * C::LPT>(ahead < C::NST - 2 ? ahead : C::NST - 2);
+    wait_vmcnt<0>();
     lds_wait_all();  // the previous chunk's reads, whose stage is written next
-    if (c + C::NST - 1 < c1) issue(c + C::NST - 1);
-    const char *Ks = smem + (c % C::NST) * 2 * C::TILE, *Vs = Ks + C::TILE;
+    if (c + 1 < c1) issue(c + 1);
+    const char *Ks = smem + (c & 1) * 2 * C::TILE, *Vs = Ks + C::TILE;
     f32x4 s[NM];
     mm_rows_frag<T, DP, NM>(Ks, fr, s, g, p);
     if ((c + 1) * (int64_t)KC > low) mask_keys<NM>(s, lim - c * KC, g);
@@ -498,7 +495,7 @@ template <typename T, int DP> __global__ __launch_bounds__(64) void cache_part_k
       wait_vmcnt<0>();
       lds_wait_all();
       if (c + 1 < c1) issue(c + 1);
-      const char *Ks = smem + (c % C::NST) * 2 * C::TILE, *Vs = Ks + C::TILE;
+      const char *Ks = smem + (c & 1) * 2 * C::TILE, *Vs = Ks + C::TILE;
       f32x4 s[1][NM];
       careful_scores<T, DP, 1, NM>(Ks, frs, s, a.D, gg, pp);
       mask_keys<NM>(s[0], lim - c * KC, g);
@@ -624,16 +621,16 @@ __device__ __forceinline__ void pv_tile(const char *tile, const float (&x)[QT][K
   }
 }
 
-template <typename T, int DP, int NW, int QT, int KC, int NST> struct TileCfg {
-  static constexpr int ES = sizeof(T), TILE = KC * DP * ES, RING = NST * 2 * TILE, LDS = RING + NW * 4;
+template <typename T, int DP, int NW, int QT, int KC> struct TileCfg {
+  static constexpr int ES = sizeof(T), TILE = KC * DP * ES, RING = 2 * 2 * TILE, LDS = RING + NW * 4;
   static_assert(LDS <= 160 * 1024, "LDS");
 };
 
 // (d 32: registers for three waves to a SIMD, as the loop needs, also where the second look would take more: 19.2 us against 21.3,
 // 448 rows a head over 22876 keys)
-template <typename T, int DP, int NW, int QT, int KC, int NST>
+template <typename T, int DP, int NW, int QT, int KC>
 __global__ __launch_bounds__(NW * 64, DP == 32 ? 3 : 1) void cache_tile_kernel(CacheArgs a, int64_t npre) {
-  using C = TileCfg<T, DP, NW, QT, KC, NST>;
+  using C = TileCfg<T, DP, NW, QT, KC>;
   constexpr int NM = KC / 16;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, p = lane & 15;
@@ -703,7 +700,7 @@ __global__ __launch_bounds__(NW * 64, DP == 32 ? 3 : 1) void cache_tile_kernel(C
     const unsigned st = (unsigned)(uintptr_t)smem + ist * 2 * C::TILE;
     pk.issue(st, kb, (uint32_t)c * KC, keys, kstep, a.D * C::ES, w);
     pv.issue(st + C::TILE, vb, (uint32_t)c * KC, keys, vstep, a.D * C::ES, w);
-    ist = ist + 1 == NST ? 0 : ist + 1;
+    ist ^= 1;
   };
   auto store_scores = [&](int c, const f32x4 (&s)[NM]) {
     if (!pre && a.sc && ri[0].valid) {  // (one tile of up to 16 rows: the first fragment)
@@ -719,16 +716,15 @@ __global__ __launch_bounds__(NW * 64, DP == 32 ? 3 : 1) void cache_tile_kernel(C
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) sm[qt].init();
 
-  for (int c = c0; c < c0 + NST - 1 && c < c1; ++c) issue(c);
+  if (c0 < c1) issue(c0);
   wait_vmcnt<0>();  // the query rows too: the compiler then waits for nothing in the loop
   for (int c = c0; c < c1; ++c) {
-    const int ahead = c1 - 1 - c;
-    wait_ring<2 * decltype(pk)::LPT>(ahead < NST - 2 ? ahead : NST - 2);
+    wait_vmcnt<0>();
     // every wave's part of chunk c has landed, and every wave has read chunk c - 1, whose place is filled next
     lds_barrier();
-    if (c + NST - 1 < c1) issue(c + NST - 1);
+    if (c + 1 < c1) issue(c + 1);
     const char *Ks = smem + cst * 2 * C::TILE, *Vs = Ks + C::TILE;
-    cst = cst + 1 == NST ? 0 : cst + 1;
+    cst ^= 1;
     if (w * QT * 16 >= tr) continue;
     f32x4 s[QT][NM];
     qk_tile<T, DP, QT, NM>(Ks, fr, s, g, p);
@@ -764,7 +760,7 @@ __global__ __launch_bounds__(NW * 64, DP == 32 ? 3 : 1) void cache_tile_kernel(C
       lds_barrier();
       if (c + 1 < c1) issue(c + 1);
       const char *Ks = smem + cst * 2 * C::TILE, *Vs = Ks + C::TILE;
-      cst = cst + 1 == NST ? 0 : cst + 1;
+      cst ^= 1;
       if (w * QT * 16 >= tr) continue;
       f32x4 s[QT][NM];
       careful_scores<T, DP, QT, NM>(Ks, fr, s, a.D, gg, pp);
@@ -1019,10 +1015,10 @@ template <typename T, int DP, bool WEIGHT> __global__ __launch_bounds__(256) voi
 }
 
 // ---- weights of many rows: p = exp2(score - lse) summed over the rows that see a
-// key, scores formed again. A workgroup per 128 keys of a (sequence, KV head) and
-// share of its rows: the keys stay in registers (32 to a wave, B operands), the
-// query rows stream through a ring in LDS, a chunk's first half to waves 0-3 and
-// its second to waves 4-7. A lane holds one column, a key, of the
+// key, scores formed again. A workgroup per 256 keys (fp32: 128) of a (sequence, KV
+// head) and share of its rows: the keys stay in registers (64 to a wave, fp32 32, B
+// operands), the query rows stream through a ring in LDS, a chunk's first half to
+// waves 0-3 and its second to waves 4-7. A lane holds one column, a key, of the
 // product, so the sum over rows is a register each. Row rho is token rho / G;
 // key j is seen by the rows from G * (j - (len - count)) on. 2048 tokens over 16301
 // rows, 16 heads over 2, d 256: 274 us, 0.94 PFLOP/s of these products (vector issue
@@ -1035,10 +1031,9 @@ template <typename T, int DP> struct WeightCfg {
   static constexpr int KF = ES == 2 ? 4 : 2, KEYS = 4 * 16 * KF;
   static_assert(KEYS == (ES == 2 ? 256 : 128), "the launch's limit in check_cache");
   static constexpr int ROWS = DP * ES * KF <= 1024 ? 128 : 64, NM = ROWS / 32;  // NM 16-row tiles to a half
-  static constexpr int LPT = ROWS * CPR / NT;        // 16-byte loads per thread and chunk (0: fewer than the threads)
-  static constexpr int STAGE = ROWS * DP * ES + ROWS * 4;
-  static constexpr int NST = 2, LDS = NST * STAGE;
-  static constexpr int NL = LPT ? LPT : 1;
+  static constexpr int LPT = ROWS * CPR / NT;        // 16-byte loads per thread and chunk
+  static_assert(LPT * NT == ROWS * CPR, "a chunk is whole loads of every thread");
+  static constexpr int STAGE = ROWS * DP * ES + ROWS * 4, LDS = 2 * STAGE;
 };
 template <typename T, int DP> __global__ __launch_bounds__(512) void cache_weight_kernel(CacheArgs a) {
   using C = WeightCfg<T, DP>;
@@ -1073,13 +1068,13 @@ template <typename T, int DP> __global__ __launch_bounds__(512) void cache_weigh
 
   // loads of this thread: row and chunk within the stage, and the row's place in q,
   // stepped by a chunk at a time
-  int rho[C::NL], gg[C::NL];
-  int64_t off[C::NL];
+  int rho[C::LPT], gg[C::LPT];
+  int64_t off[C::LPT];
   const int last = a.D * C::ES / 16 - 1;
   const int dt = C::ROWS / a.G, dg = C::ROWS % a.G;
   const int64_t sh = a.sq[1] * C::ES, st = a.sq[2] * C::ES;
 #pragma unroll
-  for (int x = 0; x < C::NL; ++x) {
+  for (int x = 0; x < C::LPT; ++x) {
     const int u = x * C::NT + tid, row = u / C::CPR, c = (u % C::CPR) ^ swz(row, C::CPR);
     rho[x] = r0 + c0 * C::ROWS + row;
     gg[x] = rho[x] % a.G;
@@ -1090,11 +1085,11 @@ template <typename T, int DP> __global__ __launch_bounds__(512) void cache_weigh
   int ist = 0, cst = 0;
   auto issue = [&](int c) {
     char *stage = smem + ist * C::STAGE;
-    ist = ist + 1 == C::NST ? 0 : ist + 1;
+    ist ^= 1;
 #pragma unroll
-    for (int x = 0; x < C::NL; ++x) {
+    for (int x = 0; x < C::LPT; ++x) {
       // (rows past the last real one: the first row's values, left out of the sums)
-      if (C::LPT || tid < C::ROWS * C::CPR) g2lds16(qb + (rho[x] < real ? off[x] : 0), stage + (x * C::NT + w * 64) * 16);
+      g2lds16(qb + (rho[x] < real ? off[x] : 0), stage + (x * C::NT + w * 64) * 16);
       rho[x] += C::ROWS;
       gg[x] += dg;
       off[x] += dt * st + dg * sh;
@@ -1112,15 +1107,14 @@ template <typename T, int DP> __global__ __launch_bounds__(512) void cache_weigh
 #pragma unroll
   for (int f = 0; f < C::KF; ++f) sum[f] = 0.f;
   const int most = first_row((int64_t)key0 + (kg + 1) * C::KF * 16 - 1);  // from here on every key of the wave is seen
-  for (int c = c0; c < c0 + C::NST - 1 && c < c1; ++c) issue(c);
-  wait_vmcnt<0>();
+  if (c0 < c1) issue(c0);
+  wait_vmcnt<0>();  // the keys too: the compiler then waits for nothing in the loop
   for (int c = c0; c < c1; ++c) {
-    // (the loads of a wave differ by the statistics', so all are waited for)
     wait_vmcnt<0>();
     lds_barrier();
-    if (c + C::NST - 1 < c1) issue(c + C::NST - 1);
+    if (c + 1 < c1) issue(c + 1);
     const char *stage = smem + cst * C::STAGE, *tile = stage + half * 16 * C::NM * DP * C::ES;
-    cst = cst + 1 == C::NST ? 0 : cst + 1;
+    cst ^= 1;
     const int row0 = r0 + c * C::ROWS + half * 16 * C::NM;
     f32x4 l2[C::NM], s[C::KF][C::NM];
 #pragma unroll
@@ -1334,27 +1328,27 @@ static CachePlan cache_plan(const fbsa_cache_desc *d) {
   return p;
 }
 
-template <typename T, int DP, int NW, int QT, int KC, int NST>
+template <typename T, int DP, int NW, int QT, int KC>
 static int launch_tiles(const CacheArgs &a, int64_t npre, int64_t nown, hipStream_t s) {
-  using C = TileCfg<T, DP, NW, QT, KC, NST>;
-  const int e = lds_optin((const void *)cache_tile_kernel<T, DP, NW, QT, KC, NST>, C::LDS, "hipFuncSetAttribute(cache_tile)");
+  using C = TileCfg<T, DP, NW, QT, KC>;
+  const int e = lds_optin((const void *)cache_tile_kernel<T, DP, NW, QT, KC>, C::LDS, "hipFuncSetAttribute(cache_tile)");
   if (e) return e;
-  hipLaunchKernelGGL((cache_tile_kernel<T, DP, NW, QT, KC, NST>), dim3((unsigned)(npre + nown)), dim3(NW * 64), C::LDS, s, a, npre);
+  hipLaunchKernelGGL((cache_tile_kernel<T, DP, NW, QT, KC>), dim3((unsigned)(npre + nown)), dim3(NW * 64), C::LDS, s, a, npre);
   return hip_check(hipGetLastError(), "cache_tile_kernel launch");
 }
 template <typename T, int DP> static int launch_tiles_of(const CacheArgs &a, int rows, int64_t npre, int64_t nown, hipStream_t s) {
   if constexpr (sizeof(T) == 4) {
-    return launch_tiles<T, DP, 4, 1, DP >= 128 ? 16 : 32, 2>(a, npre, nown, s);
+    return launch_tiles<T, DP, 4, 1, DP >= 128 ? 16 : 32>(a, npre, nown, s);
   } else {
-        if (rows <= 64) return launch_tiles<T, DP, 4, 1, 64, 2>(a, npre, nown, s);
+    if (rows <= 64) return launch_tiles<T, DP, 4, 1, 64>(a, npre, nown, s);
     constexpr int NW = DP == 32 ? 4 : 8;  // (a tile of 64 keys, d 32, is four waves' loads)
-    return launch_tiles<T, DP, NW, 8 / NW, 64, 2>(a, npre, nown, s);
+    return launch_tiles<T, DP, NW, 8 / NW, 64>(a, npre, nown, s);
   }
 }
 
 template <typename T, int DP> static int launch_cache(const CacheArgs &a, int64_t nz, hipStream_t s) {
   using C = CacheCfg<T, DP>;
-  const size_t lds = (size_t)C::NST * 2 * C::TILE;
+  const size_t lds = (size_t)2 * 2 * C::TILE;
   int e = lds_optin((const void *)cache_part_kernel<T, DP>, lds, "hipFuncSetAttribute(cache_part)");
   if (e) return e;
   const int64_t rows = (int64_t)a.B * a.Hkv * a.TG;
@@ -1438,7 +1432,8 @@ static int check_cache(const fbsa_cache_desc *d) {
     for (int x = 0; x < t.n; ++x)
       if (t.s[x] < 0 || (t.s[x] * es) % 16)
         return fail(FBSA_EINVAL, "%s: %s stride[%d]=%lld must be a non-negative multiple of 16 bytes", fn, t.name, x, (long long)t.s[x]);
-  // the copies address the rows of a chunk (at most 32) with 32-bit offsets from its first
+  // the copies address the rows of a chunk (at most 64) with unsigned 32-bit offsets from
+  // its first: 63 strides of less than 64 MiB and a row fall short of 4 GiB by almost 64 MiB
   const int64_t rs[4] = {d->sk[2], d->sv[2], d->P ? d->skp[1] : 0, d->P ? d->svp[1] : 0};
   for (int64_t r : rs)
     if (r * es >= 1LL << 26) return fail(FBSA_EUNSUPPORTED, "%s: a row stride of %lld elements is 64 MiB or more", fn, (long long)r);
