@@ -1420,7 +1420,7 @@ static int check_cache(const fbsa_cache_desc *d) {
   if (d->Hq % d->Hkv) return fail(FBSA_EINVAL, "%s: Hq=%lld not a multiple of Hkv=%lld", fn, (long long)d->Hq, (long long)d->Hkv);
   if (d->D < 8 || d->D > 256 || d->D % 8)
     return fail(FBSA_EUNSUPPORTED, "%s: head dim %lld is not a multiple of 8 up to 256", fn, (long long)d->D);
-  if (!isfinite(d->scale)) return fail(FBSA_EINVAL, "%s: scale is not finite", fn);
+  if (!isfinite(d->scale * kLog2e)) return fail(FBSA_EINVAL, "%s: scale times log2(e) is not finite", fn);
   const int64_t lim = 0x7fff0000LL;
   if (d->S > lim || d->P > lim || d->B > lim || d->Hq > 65535 || d->T > lim || d->T * (d->Hq / d->Hkv) > lim ||
       d->B > lim / d->Hq || d->B * d->Hq > lim / d->T || d->B * d->Hkv > 65535)

@@ -50,6 +50,13 @@ def test_launches_of_more_than_32_bits_of_threads_are_refused(kw):
     assert _bytes(**{**kw, "flags": 0}) > 0
 
 
+@pytest.mark.parametrize("scale", [3e38, -3e38, float("inf"), float("nan")])
+def test_scales_that_overflow_the_exponent_are_refused(scale):
+    # x = scale q.k goes through exp2, its scale times log2(e): 2.36e38 is the largest that stays finite
+    assert _bytes(scale=scale) == 0 and b"scale" in _lib.load().fbsa_last_error()
+    assert _bytes(scale=2.3e38) > 0 and _bytes(scale=-2.3e38) > 0 and _bytes(scale=0.0) > 0
+
+
 @pytest.mark.parametrize("kw", [dict(B=32, Hq=32, Hkv=8, T=1024, S=8192, D=256), dict(B=16, Hq=64, Hkv=8, T=2048, S=4096, D=128)])
 def test_tiles_that_write_their_results_need_no_parts(kw):
     assert 0 < _bytes(**kw) <= 256
