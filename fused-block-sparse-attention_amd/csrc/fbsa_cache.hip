@@ -519,14 +519,15 @@ template <typename T, int DP> __global__ __launch_bounds__(64) void cache_part_k
 // ---- many rows: a workgroup per (tile of NW x 16 QT rows, share of the keys).
 // The K and V chunks are shared through a ring in LDS; each wave owns QT
 // 16-row fragments, and a fragment of K or V read from LDS feeds QT products.
-// P enters the value product rounded to the operand type (as in the block-sparse
-// forward; the row sums are of the unrounded values): the second product of a
-// split operand would cost half as much again where the matrix units are what
-// bounds the kernel.
+// P enters the value product rounded to the operand type, as in the block-sparse
+// forward; the row sums are of the unrounded values. The bf16 results are then off by
+// 0.0023 in relative L2, where their own rounding is 0.0017; P as a pair, as for up to
+// 16 rows, would leave 0.0017 and take 12 to 25% more time (2048 tokens over 16301 rows
+// 762 -> 914 us a call, 64 sequences behind 16301 shared rows 47 -> 53).
 // Measured: 2048 tokens over 16301 rows, 16 heads over 2, d 256: 525 to 560 us, 0.92 to
-// 0.98 PFLOP/s (matrix units and LDS each busy 46% of the time: eight waves in step
+// 0.98 PFLOP/s (matrix units and LDS each busy 47% of the time: eight waves in step
 // at one barrier per 64 keys; 32 keys a chunk 610 us; four waves of 32 rows, one to a
-// SIMD, 789). 512 rows a head over 16301 keys, beside 64 own caches: 38 us, of which
+// SIMD, 789). 512 rows a head over 16301 keys, beside 64 own caches: 40 us, of which
 // about 17 are the chunks and the rest the start, 33 MB of parts and the own caches.
 // 160 rows a head over 65536 keys, d 64: 44 us, exponentials and their like at half
 // the vector issue.
