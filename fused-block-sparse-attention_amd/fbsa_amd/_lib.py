@@ -104,6 +104,26 @@ class EvictDesc(ctypes.Structure):
     ]
 
 
+class Rows4Desc(ctypes.Structure):
+    """Mirror of ``fbsa_rows4_desc``."""
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("flags", ctypes.c_int32),
+        ("B", ctypes.c_int64), ("H", ctypes.c_int64), ("T", ctypes.c_int64), ("S", ctypes.c_int64), ("D", ctypes.c_int64),
+        ("sk4", _i64x3), ("sv4", _i64x3), ("ss", _i64x2), ("sk", _i64x3), ("sv", _i64x3),
+    ]
+
+
+class Attn4Desc(ctypes.Structure):
+    """Mirror of ``fbsa_attn4_desc``."""
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("flags", ctypes.c_int32),
+        ("B", ctypes.c_int64), ("Hq", ctypes.c_int64), ("Hkv", ctypes.c_int64), ("T", ctypes.c_int64),
+        ("S", ctypes.c_int64), ("D", ctypes.c_int64),
+        ("scale", ctypes.c_float), ("reserved", ctypes.c_int32),
+        ("sq", _i64x3), ("sk4", _i64x3), ("sv4", _i64x3), ("ss", _i64x2), ("so", _i64x3), ("sog", _i64x3),
+    ]
+
+
 _vp = ctypes.c_void_p
 # name -> (restype, argtypes); every symbol declared in include/fbsa.h
 SIGNATURES = {
@@ -138,6 +158,10 @@ SIGNATURES = {
     "fbsa_cache_attn": (ctypes.c_int, [ctypes.POINTER(CacheDesc)] + [_vp] * 13 + [ctypes.c_size_t, _vp]),
     "fbsa_cache_evict_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(EvictDesc)]),
     "fbsa_cache_evict": (ctypes.c_int, [ctypes.POINTER(EvictDesc)] + [_vp] * 10 + [ctypes.c_size_t, _vp]),
+    "fbsa_cache4_append": (ctypes.c_int, [ctypes.POINTER(Rows4Desc)] + [_vp] * 8),
+    "fbsa_cache4_read": (ctypes.c_int, [ctypes.POINTER(Rows4Desc)] + [_vp] * 8),
+    "fbsa_cache4_attn_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(Attn4Desc)]),
+    "fbsa_cache4_attn": (ctypes.c_int, [ctypes.POINTER(Attn4Desc)] + [_vp] * 10 + [ctypes.c_size_t, _vp]),
 }
 
 _lib = None

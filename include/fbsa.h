@@ -420,6 +420,54 @@ int fbsa_cache_evict(const fbsa_evict_desc *d, const void *k, const void *v, con
                      const int32_t *lens, void *k_out, void *v_out, float *w_out, int32_t *index,
                      int32_t *new_lens, void *workspace, size_t workspace_bytes, void *stream);
 
+/* ---- caches in 4 bits ---------------------------------------------------
+ * Rows as above, each value held as step * code. Codes are 4-bit floats (sign, 2
+ * exponent bits, 1 of mantissa: 0, 0.5, 1, 1.5, 2, 3, 4, 6), two to a byte, element
+ * 2i in the low half: k4, v4 (B, H, S, D / 2) bytes, strides {b, h, row} in bytes,
+ * multiples of 16. step (B, H, S, 2, ng), ng = ceil(D / 64): of each 64 elements of
+ * the key row (the last 32 where D is an odd multiple of 32), then of the value row;
+ * fp16 for F16 rows, bf16 for the others; strides {b, h} in elements, even, each
+ * (b, h)'s S rows contiguous, 4-byte aligned. D is a multiple of 32 up to 256.
+ * step is the group's largest magnitude / 6 rounded to 6 significant bits (ties to
+ * even; its last bit at least 2^-125, F16: 2^-23; at most 42 * 2^120, F16: 10752), a
+ * code x / step rounded to the nearest, ties to the even code, 6 at most. Every
+ * value is then a bf16 number (F16: an fp16 number). A (sequence, head)'s row with a
+ * NaN or an infinity among its key or value elements has NaN for all of its steps.
+ * lens, start, first and count as above. No counterpart in the reference. */
+typedef struct fbsa_rows4_desc {
+  int32_t dtype, flags;                     /* flags: 0 */
+  int64_t B, H, T, S, D;
+  int64_t sk4[3], sv4[3];                   /* codes: {b, h, row}, bytes */
+  int64_t ss[2];                            /* steps: {b, h} */
+  int64_t sk[3], sv[3];                     /* k, v of the call: {b, h, row}, elements */
+} fbsa_rows4_desc;
+
+/* New rows k_new, v_new (B, H, T, D) of type dtype into rows start[b] + t of the cache
+ * for t < count[b] (NULL: T). Rows outside [0, S) are dropped. */
+int fbsa_cache4_append(const fbsa_rows4_desc *d, void *k4, void *v4, void *step, const void *k_new, const void *v_new,
+                       const int32_t *start, const int32_t *count, void *stream);
+
+/* k, v (B, H, T, D) of type dtype = rows first[b] + t (NULL: 0) of the cache for t <
+ * count[b] (NULL: T), exactly; zeros for the other t and for rows outside [0, S). */
+int fbsa_cache4_read(const fbsa_rows4_desc *d, const void *k4, const void *v4, const void *step, const int32_t *first,
+                     const int32_t *count, void *k, void *v, void *stream);
+
+/* fbsa_cache_attn over a cache in 4 bits (no prefix, no weights): the softmax and
+ * products of the values above, in 32 bits; with more than 16 rows (tokens x heads of a
+ * group) 16-bit types round each probability once. */
+typedef struct fbsa_attn4_desc {
+  int32_t dtype, flags;                     /* flags: 0 */
+  int64_t B, Hq, Hkv, T, S, D;
+  float scale;
+  int32_t reserved;
+  int64_t sq[3], sk4[3], sv4[3], ss[2], so[3], sog[3];
+} fbsa_attn4_desc;
+
+size_t fbsa_cache4_attn_workspace_bytes(const fbsa_attn4_desc *d);
+int fbsa_cache4_attn(const fbsa_attn4_desc *d, const void *q, const void *k4, const void *v4, const void *step,
+                     const int32_t *lens, const int32_t *count, const void *out_gate, void *o, float *lse,
+                     void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
