@@ -90,11 +90,16 @@ struct Rows4Args {
   int32_t B, H, T, S, D, ng;
 };
 
-// Eight lanes' group: the largest magnitude of its elements
-__device__ __forceinline__ float group_max(float x) {
-  x = fmaxf(x, shfl_xor_f(x, 1));
-  x = fmaxf(x, shfl_xor_f(x, 2));
-  return fmaxf(x, shfl_xor_f(x, 4));
+// Eight lanes' group (four at LPR 4): the largest magnitude of its elements
+template <int LPR> __device__ __forceinline__ float group_max(float x) {
+  auto with = [&](auto CTRL) {
+    const int y = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(CTRL)::value, 0xf, 0xf, false);
+    x = fmaxf(x, __builtin_bit_cast(float, y));
+  };
+  with(std::integral_constant<int, 0xb1>{});                           // lane ^ 1
+  with(std::integral_constant<int, 0x4e>{});                           // lane ^ 2
+  if constexpr (LPR >= 8) with(std::integral_constant<int, 0x141>{});  // 7 - lane of eight
+  return x;
 }
 // largest magnitude / 6 to 6 significant bits, ties to even. The division is correctly
 // rounded and a quotient next to a tie never rounds onto one: x = 6 t (1 + d) with x and
@@ -109,95 +114,130 @@ template <typename T> __device__ __forceinline__ float step_of(float most) {
   if (want < LEAST) s = __builtin_rintf(want * (1.f / UNIT)) * UNIT;
   return fminf(s, HALF ? 10752.f : 42.f * 0x1p120f);
 }
-
-// New rows: 8 elements a lane, LPR lanes a key or value row and both side by side, so the
-// row's NaN or infinity is known to all of them. The quotient x / step goes to the
-// converter, which rounds to the nearest code, ties to the even one, and saturates. As
-// above a quotient is never rounded onto a tie that it is not.
-// Bound by memory, long prompts; a step's rows by latency.
-template <typename T, int LPR> __global__ __launch_bounds__(256) void cache4_append_kernel(Rows4Args a) {
-  constexpr int RPB = 256 / (2 * LPR);
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int which = (tid / LPR) & 1, e = tid % LPR;  // key or value; elements 8 e ...
-  const uint32_t row = blockIdx.x * RPB + tid / (2 * LPR), rows = (uint32_t)a.B * a.H * a.T;
-  const bool in = row < rows && 8 * e < a.D;
-  const uint32_t x = row < rows ? row : 0;
-  const int t = (int)(x % (uint32_t)a.T), h = (int)(x / (uint32_t)a.T % (uint32_t)a.H), b = (int)(x / (uint32_t)a.T / (uint32_t)a.H);
-  const int count = a.count ? a.count[b] : a.T;
-  const int64_t at = (int64_t)a.first[b] + t;
-  const bool live = in && t < count && at >= 0 && at < a.S;
-  float y[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = 0.f;
-  if (live) {
-    const int64_t *st = which ? a.sv : a.sk;
-    const T *src = (const T *)(which ? a.v : a.k) + b * st[0] + h * st[1] + t * st[2] + 8 * e;
-    if constexpr (sizeof(T) == 4) {
-      const f32x4 p = ((const f32x4 *)src)[0], q = ((const f32x4 *)src)[1];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) { y[i] = p[i]; y[4 + i] = q[i]; }
-    } else {
-      const s16x8 p = *(const s16x8 *)src;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = to_f32<T>(__builtin_bit_cast(T, (short)p[i]));
-    }
-  }
-  float most = 0.f;
-  bool odd = false;  // (a maximum passes NaN over)
+// The codes of 8 elements: x / step goes to the converter, which rounds to the nearest
+// code, ties to the even one, and saturates; what matters is that a quotient on a border
+// is formed as the border and one beside it is not. With step = m 2^e, 1 <= m <= 63/32:
+// z = x 2^-e exactly, t = z / m to a unit in the last place, and t + (z - t m) / m is
+// within 0.5 + 2^-20 units of the quotient (the residual is exact). A quotient beside a
+// border c (c m has 9 bits, z 24) is at least 1 / m >= 0.507 units from it, one on it is exact.
+__device__ __forceinline__ uint32_t codes_of(const float (&y)[8], float step) {
+  if (!(step > 0.f)) return 0;  // (zeros, and rows held as NaN)
+  const uint32_t bits = __float_as_uint(step);
+  const float m = __uint_as_float((bits & 0x007fffffu) | 0x3f800000u), pw = __uint_as_float((254u << 23) - (bits & 0x7f800000u)), r = 1.f / m;
+  float q[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    most = fmaxf(most, fabsf(y[i]));
-    odd = odd || !(fabsf(y[i]) < INFINITY);
+    const float z = y[i] * pw, t = z * r;
+    q[i] = __builtin_fmaf(__builtin_fmaf(-t, m, z), r, t);
   }
-  const uint64_t vote = __ballot(odd);
-  constexpr uint64_t ROW = LPR == 32 ? ~0ull : (1ull << (2 * LPR % 64)) - 1;
-  const bool bad = (vote >> (lane / (2 * LPR) * (2 * LPR)) & ROW) != 0;
-  most = LPR >= 8 ? group_max(most) : fmaxf(fmaxf(most, shfl_xor_f(most, 1)), shfl_xor_f(fmaxf(most, shfl_xor_f(most, 1)), 2));
-  if (!live) return;
-  const float step = bad ? __uint_as_float(0x7fc00000u) : step_of<T>(most);
   uint32_t w = 0;
-  if (!bad && step > 0.f) {
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[0] / step, y[1] / step, 1.f, 0);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[2] / step, y[3] / step, 1.f, 1);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[4] / step, y[5] / step, 1.f, 2);
-    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, y[6] / step, y[7] / step, 1.f, 3);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[0], q[1], 1.f, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[2], q[3], 1.f, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[4], q[5], 1.f, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[6], q[7], 1.f, 3);
+}
+
+// Rows of a block: 8 elements a lane, LPR lanes to a key or value row and the two side by
+// side, RPB rows at a time, U times. LPR = 4, 8, 16, 32 for D up to 32, 64, 128, 256.
+template <typename T, int LPR> struct Rows4 {
+  static constexpr int RPB = 256 / (2 * LPR), U = 4;
+};
+template <typename T> __device__ __forceinline__ void load8(const T *src, float (&y)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    const f32x4 p = ((const f32x4 *)src)[0], q = ((const f32x4 *)src)[1];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { y[i] = p[i]; y[4 + i] = q[i]; }
+  } else {
+    const s16x8 p = *(const s16x8 *)src;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = to_f32<T>(__builtin_bit_cast(T, (short)p[i]));
   }
-  const int64_t *s4 = which ? a.sv4 : a.sk4;
-  char *dst = (char *)(which ? a.v4 : a.k4) + b * s4[0] + h * s4[1] + at * s4[2] + 4 * e;
-  *(uint32_t *)dst = w;
-  if (e % 8 == 0) {
-    uint16_t *sd = a.step + b * a.ss[0] + h * a.ss[1] + (at * 2 + which) * a.ng + e / 8;
-    if constexpr (__is_same(T, f16)) *sd = __builtin_bit_cast(uint16_t, (f16)step);
-    else *sd = (uint16_t)(__float_as_uint(step) >> 16);
+}
+
+// New rows: key and value of a row side by side, so that all its lanes know of a NaN or
+// an infinity in either. Bound by memory, long prompts; a step's rows by latency.
+template <typename T, int LPR> __global__ __launch_bounds__(256) void cache4_append_kernel(Rows4Args a) {
+  using C = Rows4<T, LPR>;
+  const int tid = threadIdx.x, lane = tid & 63, which = (tid / LPR) & 1, e = tid % LPR;  // key or value; elements 8 e ...
+  const int h = (int)(blockIdx.y % (uint32_t)a.H), b = (int)(blockIdx.y / (uint32_t)a.H);
+  const int t0 = blockIdx.x * (C::RPB * C::U) + tid / (2 * LPR), first = a.first[b], count = min(a.count ? a.count[b] : a.T, a.T);
+  const int64_t *st = which ? a.sv : a.sk, *s4 = which ? a.sv4 : a.sk4;
+  const T *src = (const T *)(which ? a.v : a.k) + b * st[0] + h * st[1] + 8 * e;
+  const int64_t tstep = st[2];
+  float y[C::U][8];
+  bool live[C::U];
+#pragma unroll
+  for (int i = 0; i < C::U; ++i) {
+    const int t = t0 + i * C::RPB;
+    const int64_t at = (int64_t)first + t;
+    live[i] = 8 * e < a.D && t < count && at >= 0 && at < a.S;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[i][j] = 0.f;
+    if (live[i]) load8<T>(src + t * tstep, y[i]);
+  }
+  char *dst = (char *)(which ? a.v4 : a.k4) + b * s4[0] + h * s4[1] + 4 * e;
+  const int64_t rstep = s4[2];
+  uint16_t *sd = a.step + b * a.ss[0] + h * a.ss[1] + which * a.ng + e / 8;
+#pragma unroll
+  for (int i = 0; i < C::U; ++i) {
+    float most = 0.f, sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      most = fmaxf(most, fabsf(y[i][j]));  // (passes NaN over)
+      sum = __builtin_fmaf(y[i][j], 0.f, sum);  // 0, or NaN
+    }
+    const uint64_t vote = __ballot(sum != 0.f);
+    constexpr uint64_t ROW = LPR == 32 ? ~0ull : (1ull << (2 * LPR % 64)) - 1;
+    const bool bad = (vote >> (lane / (2 * LPR) * (2 * LPR)) & ROW) != 0;
+    most = group_max<LPR>(most);
+    if (!live[i]) continue;
+    const float step = bad ? __uint_as_float(0x7fc00000u) : step_of<T>(most);
+    const int64_t at = (int64_t)first + t0 + i * C::RPB;
+    *(uint32_t *)(dst + at * rstep) = codes_of(y[i], step);
+    if (e % 8 == 0) {
+      if constexpr (__is_same(T, f16)) sd[at * 2 * a.ng] = __builtin_bit_cast(uint16_t, (f16)step);
+      else sd[at * 2 * a.ng] = (uint16_t)(__float_as_uint(step) >> 16);
+    }
   }
 }
 
 // Rows first[b] + t of each sequence as numbers of type T; rows outside the cache, and
 // those from count[b] on, are zeros. 8 values a lane, written whole lines at a time.
 template <typename T, int LPR> __global__ __launch_bounds__(256) void cache4_read_kernel(Rows4Args a) {
-  constexpr int RPB = 256 / (2 * LPR);
+  using C = Rows4<T, LPR>;
   const int tid = threadIdx.x, which = (tid / LPR) & 1, e = tid % LPR;
-  const uint32_t row = blockIdx.x * RPB + tid / (2 * LPR), rows = (uint32_t)a.B * a.H * a.T;
-  if (row >= rows || 8 * e >= a.D) return;
-  const int t = (int)(row % (uint32_t)a.T), h = (int)(row / (uint32_t)a.T % (uint32_t)a.H), b = (int)(row / (uint32_t)a.T / (uint32_t)a.H);
-  const int count = a.count ? a.count[b] : a.T;
-  const int64_t at = (int64_t)(a.first ? a.first[b] : 0) + t;
-  uint32_t w = 0;
-  float step = 0.f;
-  if (t < count && at >= 0 && at < a.S) {
-    const int64_t *s4 = which ? a.sv4 : a.sk4;
-    w = *(const uint32_t *)((const char *)(which ? a.v4 : a.k4) + b * s4[0] + h * s4[1] + at * s4[2] + 4 * e);
-    step = step_f32<T>(a.step[b * a.ss[0] + h * a.ss[1] + (at * 2 + which) * a.ng + e / 8]);
+  const int h = (int)(blockIdx.y % (uint32_t)a.H), b = (int)(blockIdx.y / (uint32_t)a.H);
+  if (8 * e >= a.D) return;
+  const int t0 = blockIdx.x * (C::RPB * C::U) + tid / (2 * LPR), first = a.first ? a.first[b] : 0, count = a.count ? a.count[b] : a.T;
+  const int64_t *st = which ? a.sv : a.sk, *s4 = which ? a.sv4 : a.sk4;
+  const char *src = (const char *)(which ? a.v4 : a.k4) + b * s4[0] + h * s4[1] + 4 * e;
+  const int64_t rstep = s4[2], tstep = st[2];
+  const uint16_t *sd = a.step + b * a.ss[0] + h * a.ss[1] + which * a.ng + e / 8;
+  uint32_t w[C::U], s[C::U];
+#pragma unroll
+  for (int i = 0; i < C::U; ++i) {
+    const int t = t0 + i * C::RPB;
+    const int64_t at = (int64_t)first + t;
+    w[i] = s[i] = 0;
+    if (t < count && at >= 0 && at < a.S) {
+      w[i] = *(const uint32_t *)(src + at * rstep);
+      s[i] = sd[at * 2 * a.ng];
+    }
   }
-  const int64_t *st = which ? a.sv : a.sk;
-  T *dst = (T *)(which ? a.v : a.k) + b * st[0] + h * st[1] + t * st[2] + 8 * e;
-  if constexpr (sizeof(T) == 4) {
-    float x[8];
-    values8_f32(w, step, x);
-    ((f32x4 *)dst)[0] = f32x4{x[0], x[1], x[2], x[3]};
-    ((f32x4 *)dst)[1] = f32x4{x[4], x[5], x[6], x[7]};
-  } else {
-    *(s16x8 *)dst = values8<T>(w, step);
+  T *dst = (T *)(which ? a.v : a.k) + b * st[0] + h * st[1] + 8 * e;
+#pragma unroll
+  for (int i = 0; i < C::U; ++i) {
+    const int t = t0 + i * C::RPB;
+    if (t >= a.T) continue;
+    const float step = step_f32<T>(s[i]);
+    if constexpr (sizeof(T) == 4) {
+      float x[8];
+      values8_f32(w[i], step, x);
+      ((f32x4 *)(dst + t * tstep))[0] = f32x4{x[0], x[1], x[2], x[3]};
+      ((f32x4 *)(dst + t * tstep))[1] = f32x4{x[4], x[5], x[6], x[7]};
+    } else {
+      *(s16x8 *)(dst + t * tstep) = values8<T>(w[i], step);
+    }
   }
 }
 
@@ -207,7 +247,64 @@ struct Cache4Args {
   const uint16_t *step;
   int64_t ss[2];
   int32_t ng;            // steps of a key or value row
+  int32_t want;          // few rows: shares that the call's chunks are cut into, all (sequence, KV head)s together
+  int2 *used;            // few rows: a sequence's first share and its number of them
 };
+
+template <int CTRL> __device__ __forceinline__ float dpp_f(float x, float old = 0.f) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, old), __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ int wave_sum(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0xb1, 0xf, 0xf, false);   // lane ^ 1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x4e, 0xf, 0xf, false);   // lane ^ 2
+  x += __builtin_amdgcn_update_dpp(0, x, 0x141, 0xf, 0xf, false);  // 7 - lane of eight
+  x += __builtin_amdgcn_update_dpp(0, x, 0x140, 0xf, 0xf, false);  // 15 - lane of sixteen
+  x += __shfl_xor(x, 16, 64);
+  return x + __shfl_xor(x, 32, 64);
+}
+// sums of lanes 0 .. lane
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // one lane to the right, of sixteen
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // the last of sixteen to the next sixteen
+  return x + __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+}
+// Share i of the sequences' chunks, which are cut into pieces of about the same number
+// (want of them over all KV heads, and one more for each sequence at most): sequence,
+// piece and number of pieces of it. The lengths are on the device, so every wave counts
+// (pieces by the capacity leave the longest sequence's to end last: 16 sequences of 1000
+// to 16301 rows). False: there is none.
+__device__ __forceinline__ int chunks4(const CacheArgs &a, int b) {
+  return b < a.B && seq_count(a, b) > 0 ? (int)(((uint32_t)seq_len(a, b) + 63u) / 64u) : 0;
+}
+__device__ __forceinline__ bool share4(const Cache4Args &c4, int i, int lane, int &b, int &split, int &np, int &before) {
+  const CacheArgs &a = c4.a;
+  if (a.B == 1) {
+    b = 0; split = i; np = a.np_own; before = 0;
+    return i < np;
+  }
+  int total = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) total += wave_sum(chunks4(a, b0 + lane));  // (B H of 65535 at most: below 2^31 up to 2^37 rows; plan4)
+  const int most = c4.want / a.Hkv, each = max(1, (total + most - 1) / most);
+  before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int mine = b0 + lane < a.B ? max(1, (chunks4(a, b0 + lane) + each - 1) / each) : 0;
+    const int upto = wave_scan(mine);
+    const uint64_t past = __ballot(before + upto > i);
+    if (past) {
+      const int l = __builtin_ctzll(past);
+      b = b0 + l;
+      np = __builtin_amdgcn_readlane(mine, l);
+      before += __builtin_amdgcn_readlane(upto, l) - np;
+      split = i - before;
+      return true;
+    }
+    before += __builtin_amdgcn_readlane(upto, 63);
+  }
+  return false;
+}
 
 // Queries and probabilities enter the products as sums of 16-bit numbers: a 32-bit number
 // is three bf16 exactly (8 bits each).
@@ -237,32 +334,35 @@ template <int N> __device__ __forceinline__ void split8(const float *x, s16x8 *o
   }
   out[N - 1] = pack8<bf16>(r);
 }
-// elements d .. d + 7 of a query row (zeros past the head dim), the scale's sign applied
-template <typename T> __device__ __forceinline__ void load_q8(const CacheArgs &a, const T *row, int d, s16x8 *out) {
+// elements d .. d + 7 of a query row (zeros past the head dim, or where `in` says), the scale's sign applied
+template <typename T> __device__ __forceinline__ void load_q8(const CacheArgs &a, const T *row, int d, bool in, s16x8 *out) {
+  u32x4 w[sizeof(T) / 2];
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+    w[i] = u32x4{0, 0, 0, 0};
+    if (in && d < a.D) w[i] = ((const u32x4 *)(row + d))[i];
+    if (a.qand != 0xffffffffu || a.qxor) {  // (a scale below or of zero)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[i][e] = (w[i][e] & a.qand) ^ a.qxor;
+    }
+  }
   if constexpr (sizeof(T) == 4) {
     float x[8];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const u32x4 w = d < a.D ? ((const u32x4 *)(row + d))[i] : u32x4{0, 0, 0, 0};
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[4 * i + e] = __uint_as_float((w[e] & a.qand) ^ a.qxor);
-    }
+    for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(w[e / 4][e % 4]);
     split8<3>(x, out);
   } else {
-    u32x4 w = d < a.D ? *(const u32x4 *)(row + d) : u32x4{0, 0, 0, 0};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = (w[e] & a.qand) ^ a.qxor;
-    out[0] = __builtin_bit_cast(s16x8, w);
+    out[0] = __builtin_bit_cast(s16x8, w[0]);
   }
 }
 
-// A chunk of 64 rows in LDS: codes of keys, codes of values, steps. A row of codes is CPR
-// units of 16 bytes, unit c at c ^ swk(row) (values: swv), which keeps the reads below
-// off each other's banks as far as 16-byte units can: none for keys, two lanes to a bank for values.
+// A chunk of 64 rows in LDS: keys' codes, values' codes, and steps twice. A row of codes
+// is CPR units of 16 bytes, unit c at c ^ swk(row) (values: swv), which keeps the reads
+// below off each other's banks as far as 16-byte units can: no two lanes on a bank for
+// keys, two for values.
 template <int DP> struct Part4 {
   static constexpr int KC = 64, RB = DP / 2, CPR = RB / 16, NG = DP <= kGroup4 ? 1 : DP / kGroup4;
-  static constexpr int TILE = KC * RB, STEPS = KC * 4 * NG, STAGE = 2 * TILE + STEPS, LOADS = 2 * CPR + NG;
-  static constexpr int NS = DP <= 64 ? 4 : DP == 128 ? 3 : 2;  // stages of the ring
+  static constexpr int TILE = KC * RB, STEPS = KC * 4 * NG, LDS = 2 * TILE + 2 * STEPS;
   __device__ static __forceinline__ int swk(int row) {
     return CPR == 1 ? 0 : CPR == 4 ? (row >> 2) & 3 : CPR == 8 ? (row >> 1) & 7 : (row >> 3) & 1;
   }
@@ -271,102 +371,131 @@ template <int DP> struct Part4 {
   }
 };
 
-// Steps of four keys from `at` on (a multiple of 4): number e of 2 NG of key r
+// Steps of four rows from `at` on (a multiple of 4): of group j of row r's key, or value
 template <typename T, int NG> struct Steps4 {
   u32x4 w[NG];
   __device__ __forceinline__ void load(const char *steps, int at) {
 #pragma unroll
     for (int i = 0; i < NG; ++i) w[i] = ((const u32x4 *)(steps + at * 4 * NG))[i];
   }
-  __device__ __forceinline__ float get(int r, int e) const { return step_half<T>(w[(r * NG + e / 2) / 4][(r * NG + e / 2) % 4], e); }
+  __device__ __forceinline__ float key(int r, int j) const { return step_half<T>(w[(r * NG + j / 2) / 4][(r * NG + j / 2) % 4], j); }
+  __device__ __forceinline__ float value(int r, int j) const { return step_half<T>(w[(r * NG + (NG + j) / 2) / 4][(r * NG + (NG + j) / 2) % 4], NG + j); }
 };
 
-// Up to 16 rows: a wave per (tile, share of the keys). Codes go to LDS through a ring of
-// the wave's own and are made 16-bit numbers on their way into the matrix units (one
-// instruction for two), the steps applied in 32 bits: to the scores of a group's product,
-// and to the probabilities before the value product, one set of them for each group.
-// Keys past what a row sees have p = 0, codes are finite whatever they are, and a step
-// that is NaN counts as 0 there, so nothing that is not seen comes through.
-//   scores: S^T = K Q^T, 16 keys x 16 rows a product; lane (g, p) has keys 16 m + 4 g + r of row p
+// Few rows (16 QT): a wave per (sequence, KV head, share of the keys). Codes go to LDS
+// (keys of the next chunk while this one's values are used, and the other way round) and
+// are made 16-bit numbers on their way into the matrix units, one instruction for two;
+// the steps are applied in 32 bits: to the scores of a group's product, and to the
+// probabilities before the value product, one set of them for each group. Keys past what
+// a row sees have p = 0, codes are finite whatever they are, and a value's
+// step is 0 where it is NaN, so nothing that is not seen comes through.
+//   scores: S^T = K Q^T, 16 keys x 16 columns a product; lane (g, p) has four keys of column p
 //   values: O^T = V^T P, 16 columns x 16 rows over 32 keys; a transposing read gives lane
 //   (g, i) one column's 16 keys 16 a + 4 g + b, a, b < 4: the order that P has anyway.
-// QUAD (up to 4 rows): the columns of Q are 4 rows x 4 quarters of the chunk, zero outside
-// the quarter's own lanes, so a product of 16 x 16 has the scores of 64 keys and no lane
-// holds one twice: a quarter of the exponentials and splits. Each (row, quarter) has a
-// softmax of its own, joined at the end.
-template <typename T, int DP, bool QUAD> __global__ __launch_bounds__(64) void cache4_part_kernel(Cache4Args c4) {
+// SUB > 1: up to 16 / SUB rows. The columns of Q are those rows SUB times, once for each
+// SUB-th of the chunk and zero outside the lanes that hold its keys, so a product has the
+// scores of 16 SUB keys and no lane holds one twice: a SUB-th of the exponentials and
+// splits. For the value product the first part's columns take the others' probabilities.
+// QT > 1: that many 16-row tiles, for which the codes are made numbers once; 16-bit P is
+// then rounded once (bf16), as in the kernel of many rows.
+template <typename T, int DP, int SUB, int QT> constexpr int part4_waves() {  // to a SIMD: one where 256 registers are too few
+  constexpr int regs = QT * (DP / 4 + DP / 8 * SUB * Pieces<T>::Q + 32 / SUB) + 64 + DP / 4;
+  return regs < 256 || (DP == 256 && SUB == 2) ? 2 : 1;
+}
+template <typename T, int DP, int SUB, int QT>
+__global__ __launch_bounds__(64, (part4_waves<T, DP, SUB, QT>())) void cache4_part_kernel(Cache4Args c4) {
   using C = Part4<DP>;
   using K = typename Pieces<T>::K;
-  constexpr int KC = C::KC, NM = QUAD ? 1 : KC / 16, NG = C::NG, NQ = Pieces<T>::Q, NP = Pieces<T>::P, NT = DP / 16;
-  constexpr int NF = QUAD ? DP / 8 : DP / 32, PITCH = DP == 192 ? 256 : DP;
+  static_assert(SUB == 1 || QT == 1, "parts of the chunk are for one tile");
+  constexpr int KC = C::KC, NM = 4 / SUB, ROWS = 16 / SUB, LPS = 4 / SUB;  // LPS: lane groups that hold a part's keys
+  constexpr int NG = C::NG, NQ = Pieces<T>::Q, NP = QT > 1 && __is_same(T, bf16) ? 1 : Pieces<T>::P, NT = DP / 16;
+  constexpr int NF = DP / 32 * SUB, FG = DP == 32 ? NF : 2 * SUB;  // products of a score; of a group
+  constexpr int PITCH = DP == 192 ? 256 : DP;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const CacheArgs &a = c4.a;
-  const int lane = threadIdx.x, g = lane >> 4, p = lane & 15, quarter = p >> 2;
-  const uint32_t id = blockIdx.x;
-  const int tile = id % a.rt_own, hk = id / a.rt_own / a.np_own % a.Hkv, b = id / a.rt_own / a.np_own / a.Hkv;
-  const int split = id / a.rt_own % a.np_own, rho = tile * a.tr_own + (QUAD ? p & 3 : p);
-  const RowInfo ri = row_info(a, b, hk, rho);
-  int keys, low;
-  own_bounds(a, b, tile * a.tr_own, min(tile * a.tr_own + a.tr_own, a.TG), keys, low);
-  const int64_t slot = (((int64_t)b * a.Hkv + hk) * a.rt_own + tile) * a.np_own * a.tr_own + split * a.tr_own;
-  const int lim = ri.valid ? ri.lim : keys;
-  int c0, c1;
-  share_of((keys + KC - 1) / KC, split, a.np_own, c0, c1);
-
-  s16x8 fr[NF][NQ];
-  const T *qrow = (const T *)a.q + ri.b * a.sq[0] + ri.hq * a.sq[1] + ri.t * a.sq[2];
+  const int lane = threadIdx.x, g = lane >> 4, p = lane & 15, sub = p / ROWS;
+  const int hk = blockIdx.x;
+  int b, split, np, before;
+  if (!share4(c4, blockIdx.y, lane, b, split, np, before)) return;
+  if (split == 0 && hk == 0 && lane == 0 && !a.direct) c4.used[b] = int2{before, np};
+  const int n = seq_len(a, b), count = seq_count(a, b), keys = count > 0 ? n : 0;
+  int low = n - count + 1;  // below it every row sees every key
+  low = low < 0 ? 0 : low;
+  // rows: token, head, keys seen (a row that is none sees what the last one sees, so it asks for no masking)
+  const T *qrow[QT];
+  int tok[QT], head[QT], lim[QT];
+  bool valid[QT];
+  const float inv_g = 1.f / (float)a.G;
 #pragma unroll
-  for (int f = 0; f < NF; ++f) {
-    load_q8<T>(a, qrow, QUAD ? 8 * f : DP == 32 ? 8 * g : 64 * (f / 2) + 16 * g + 8 * (f % 2), fr[f]);
-    if (QUAD && g != quarter) {
-#pragma unroll
-      for (int n = 0; n < NQ; ++n) fr[f][n] = s16x8{0, 0, 0, 0, 0, 0, 0, 0};
-    }
+  for (int qt = 0; qt < QT; ++qt) {
+    const int rho = qt * 16 + p % ROWS, x = rho < a.TG ? rho : 0;
+    tok[qt] = (int)(((float)x + 0.5f) * inv_g);  // (x / G: both below 2^7, exact)
+    head[qt] = hk * a.G + x - tok[qt] * a.G;
+    valid[qt] = rho < a.TG && tok[qt] < count;
+    lim[qt] = valid[qt] ? clampi(n - count + tok[qt] + 1, 0, n) : keys;
+    qrow[qt] = (const T *)a.q + b * a.sq[0] + head[qt] * a.sq[1] + tok[qt] * a.sq[2];
   }
+  int c0, c1;
+  share_of((int)(((uint32_t)keys + KC - 1) / KC), split, np, c0, c1);
 
   const int64_t kstep = a.sk[2], vstep = a.sv[2];
   const char *kb = (const char *)a.k + b * a.sk[0] + hk * a.sk[1], *vb = (const char *)a.v + b * a.sv[0] + hk * a.sv[1];
   const char *sb = (const char *)(c4.step + b * c4.ss[0] + hk * c4.ss[1]);
   uint32_t koff[C::CPR], voff[C::CPR];
 #pragma unroll
-  for (int n = 0; n < C::CPR; ++n) {
-    const int u = n * 64 + lane, row = u / C::CPR, c = u % C::CPR, last = a.D / 32 - 1;
+  for (int i = 0; i < C::CPR; ++i) {
+    const int u = i * 64 + lane, row = u / C::CPR, c = u % C::CPR, last = a.D / 32 - 1;
     const int ck = c ^ C::swk(row), cv = c ^ C::swv(row);  // (columns past the head dim: the row's last unit)
-    koff[n] = (uint32_t)(row * kstep + (ck < last ? ck : last) * 16);
-    voff[n] = (uint32_t)(row * vstep + (cv < last ? cv : last) * 16);
+    koff[i] = (uint32_t)row * (uint32_t)kstep + (ck < last ? ck : last) * 16;  // (64 strides of less than 2^26: check_held)
+    voff[i] = (uint32_t)row * (uint32_t)vstep + (cv < last ? cv : last) * 16;
   }
-  auto issue = [&](int c, int stage) {
-    const unsigned st = (unsigned)(uintptr_t)smem + stage * C::STAGE;
-    const uint32_t row0 = (uint32_t)c * KC;
-    const uint32_t klim = tail_limit<KC>(row0, keys, (uint32_t)kstep, (uint32_t)a.D / 2), vlim = tail_limit<KC>(row0, keys, (uint32_t)vstep, (uint32_t)a.D / 2);
+  auto issue_codes = [&](const char *src, int64_t step, const uint32_t (&off)[C::CPR], int left, char *dst) {
+    if (left >= KC) {
 #pragma unroll
-    for (int n = 0; n < C::CPR; ++n) g2lds16_s(kb + row0 * kstep, koff[n] > klim ? klim : koff[n], st + n * 1024);
+      for (int i = 0; i < C::CPR; ++i) g2lds16_s(src, off[i], dst + i * 1024);
+    } else {  // (rows past the end: the end of the last one)
+      const uint32_t lim0 = (uint32_t)(left - 1) * (uint32_t)step + (uint32_t)a.D / 2 - 16;
 #pragma unroll
-    for (int n = 0; n < C::CPR; ++n) g2lds16_s(vb + row0 * vstep, voff[n] > vlim ? vlim : voff[n], st + C::TILE + n * 1024);
-    const uint32_t words = min((uint32_t)KC, keys - row0) * NG;  // (rows past the end: the last step)
-#pragma unroll
-    for (int n = 0; n < NG; ++n) {
-      const uint32_t u = n * 64 + lane;
-      g2lds4(sb + ((int64_t)row0 * NG + (u < words ? u : words - 1)) * 4, smem + stage * C::STAGE + 2 * C::TILE + n * 256);
+      for (int i = 0; i < C::CPR; ++i) g2lds16_s(src, off[i] > lim0 ? lim0 : off[i], dst + i * 1024);
     }
   };
-  // this lane's keys: 16 m + 4 g + r (QUAD: 16 quarter + 4 g + r)
-  const int key0 = QUAD ? 16 * quarter + 4 * g : 4 * g;
-  const int vrow = 16 * (p >> 2) + 4 * g + (p & 3), vswz = C::swv(vrow), krow = QUAD ? lane : p, kswz = C::swk(krow);
+  auto issue_keys = [&](int c) {  // and steps
+    const int left = keys - c * KC;  // (c is a chunk of the sequence: at least 1)
+    issue_codes(kb + (int64_t)c * KC * kstep, kstep, koff, left, smem);
+    const uint32_t words = (uint32_t)min(KC, left) * NG;  // (rows past the end: the last step)
+    char *sd = smem + 2 * C::TILE + (c & 1) * C::STEPS;
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      const uint32_t u = i * 64 + lane;
+      g2lds4_s(sb + (int64_t)c * KC * NG * 4, (u < words ? u : words - 1) * 4, sd + i * 256);
+    }
+  };
+  auto issue_values = [&](int c) { issue_codes(vb + (int64_t)c * KC * vstep, vstep, voff, keys - c * KC, smem + C::TILE); };
+  if (c0 < c1) {
+    issue_keys(c0);
+    issue_values(c0);
+  }
 
-  SoftmaxState<DP> sm;
-  sm.init();
-  for (int n = 0; n < C::NS - 1; ++n)
-    if (c0 + n < c1) issue(c0 + n, n);
-  int stage = 0;
+  s16x8 fr[QT][NF][NQ];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+      // product f of the group's FG: elements 8 f .. of this lane's, a LPS-th of the group
+      load_q8<T>(a, qrow[qt], (DP == 32 ? 0 : 64 * (f / FG)) + (g % LPS) * 8 * FG + 8 * (f % FG), SUB == 1 || g / LPS == sub, fr[qt][f]);
+    }
+  // this lane's scores: keys 16 (sub NM + m) + 4 g + r; the row that it reads of 16-row tile m
+  const int key0 = 16 * sub * NM + 4 * g, krow = 16 * (g / LPS) * NM + p, kswz = C::swk(p);
+  const int vrow = 16 * (p >> 2) + 4 * g + (p & 3), vswz = C::swv(vrow);
+
+  SoftmaxState<DP> sm[QT];
+#pragma unroll
+  for (int qt = 0; qt < QT; ++qt) sm[qt].init();
   for (int c = c0; c < c1; ++c) {
-    wait_ring<C::LOADS>(min(C::NS - 2, c1 - 1 - c));
-    lds_wait_all();  // the previous chunk's reads, whose stage is written next
-    if (c + C::NS - 1 < c1) issue(c + C::NS - 1, stage == 0 ? C::NS - 1 : stage - 1);
-    const char *Ks = smem + stage * C::STAGE, *Vs = Ks + C::TILE, *Ss = Vs + C::TILE;
-    stage = stage == C::NS - 1 ? 0 : stage + 1;
-
-    f32x4 s[NM];
+    wait_vmcnt<C::CPR>();  // keys and steps are here, the values may be under way
+    lds_wait_all();
+    const char *Ks = smem, *Vs = smem + C::TILE, *Ss = Vs + C::TILE + (c & 1) * C::STEPS;
+    f32x4 s[QT][NM];
 #pragma unroll
     for (int m = 0; m < NM; ++m) {
       Steps4<T, NG> st;
@@ -374,79 +503,115 @@ template <typename T, int DP, bool QUAD> __global__ __launch_bounds__(64) void c
       const char *row = Ks + (krow + 16 * m) * C::RB;
 #pragma unroll
       for (int j = 0; j < NG; ++j) {
-        f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
-        auto mul = [&](uint32_t w, const s16x8 *q) {
-          const s16x8 x = codes8<K>(w);
+        f32x4 acc[QT];
 #pragma unroll
-          for (int n = NQ - 1; n >= 0; --n) acc = Mfma16<K>::run(x, q[n], acc);
-        };
-        if constexpr (QUAD) {
+        for (int qt = 0; qt < QT; ++qt) acc[qt] = f32x4{0.f, 0.f, 0.f, 0.f};
+        uint32_t w[FG];  // this lane's codes of the group: 4 FG bytes
+        if constexpr (FG >= 4) {
 #pragma unroll
-          for (int u = 2 * j; u < (DP == 32 ? 1 : 2 * j + 2); ++u) {
-            const u32x4 w = *(const u32x4 *)(row + ((u ^ kswz) << 4));
+          for (int u = 0; u < FG / 4; ++u) {
+            const int unit = DP == 32 ? 0 : 2 * j + (g % LPS) * (FG / 4) + u;
+            const u32x4 x = *(const u32x4 *)(row + ((unit ^ kswz) << 4));
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mul(w[i], fr[4 * u + i]);
+            for (int i = 0; i < 4; ++i) w[4 * u + i] = x[i];
           }
-        } else if constexpr (DP == 32) {
-          mul(*(const uint32_t *)(row + 4 * g), fr[0]);
+        } else if constexpr (FG == 2) {
+          // (16 elements of four lane groups, or of two at d 32)
+          const int unit = DP == 32 ? 0 : 2 * j + (g >> 1);
+          const u32x2 x = *(const u32x2 *)(row + ((unit ^ kswz) << 4) + (g & 1) * 8);
+          w[0] = x[0];
+          w[1] = x[1];
         } else {
-          const u32x2 w = *(const u32x2 *)(row + (((2 * j + (g >> 1)) ^ kswz) << 4) + (g & 1) * 8);
-          mul(w[0], fr[2 * j]);
-          mul(w[1], fr[2 * j + 1]);
+          w[0] = *(const uint32_t *)(row + 4 * g);
         }
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s[m][r] = j ? __builtin_fmaf(acc[r], st.get(r, j), s[m][r]) : acc[r] * st.get(r, 0);
-      }
-    }
-    if ((c + 1) * (int64_t)KC > low) {
+        for (int i = 0; i < FG; ++i) {
+          const s16x8 x = codes8<K>(w[i]);
 #pragma unroll
-      for (int m = 0; m < NM; ++m)
+          for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (key0 + 16 * m + r >= lim - c * KC) s[m][r] = -INFINITY;
-    }
-    float x[NM][4];
-    sm.template step<NM>(s, a.scale2, x);
-
-#pragma unroll
-    for (int j = 0; j < NG; ++j) {
-      s16x8 pk[2][NP];  // keys of the transposing read's first and second word
-      if constexpr (QUAD) {
-        Steps4<T, NG> st;
-        st.load(Ss, key0);
-        float y[8];
+            for (int y = NQ - 1; y >= 0; --y) acc[qt] = Mfma16<K>::run(x, fr[qt][j * FG + i][y], acc[qt]);
+        }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          y[r] = x[0][r] * fmaxf(st.get(r, NG + j), 0.f);
-          y[4 + r] = 0.f;
+          const float y = st.key(r, j);
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) s[qt][m][r] = j ? __builtin_fmaf(acc[qt][r], y, s[qt][m][r]) : acc[qt][r] * y;
+        }
+      }
+    }
+    lds_wait_all();  // the keys' reads, whose place is filled next
+    const bool more = c + 1 < c1;
+    if (more) issue_keys(c + 1);
+    if ((c + 1) * (int64_t)KC > low) {
+#pragma unroll
+      for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+        for (int m = 0; m < NM; ++m)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (key0 + 16 * m + r >= lim[qt] - c * KC) s[qt][m][r] = -INFINITY;
+      // (a value's step that is NaN, as its key's is: 0 for the rows that do not see it)
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        uint16_t *v = (uint16_t *)(smem + 2 * C::TILE + (c & 1) * C::STEPS) + lane * 2 * NG + NG + j;
+        if ((*v & 0x7fff) > (__is_same(T, f16) ? 0x7c00 : 0x7f80)) *v = 0;
+      }
+    }
+    float x[QT][NM][4];
+#pragma unroll
+    for (int qt = 0; qt < QT; ++qt) sm[qt].template step<NM, ROWS>(s[qt], a.scale2, x[qt]);
+
+    if (more) wait_vmcnt<C::CPR + NG>();
+    else wait_vmcnt<0>();
+    lds_wait_all();
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      s16x8 pk[QT][2][NP];  // keys of the transposing read's first and second word
+      float y[QT][NM][4];
+#pragma unroll
+      for (int m = 0; m < NM; ++m) {
+        Steps4<T, NG> st;
+        st.load(Ss, key0 + 16 * m);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float z = st.value(r, j);
+#pragma unroll
+          for (int qt = 0; qt < QT; ++qt) y[qt][m][r] = x[qt][m][r] * z;
+        }
+      }
+      if constexpr (SUB == 1) {
+#pragma unroll
+        for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) split8<NP>(&y[qt][2 * h][0], pk[qt][h]);
+      } else {
+        // the columns of the first part take the others' (theirs hold what no one reads)
+        float z[8];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          z[r] = y[0][0][r];
+          z[4 + r] = SUB == 2 ? y[0][NM - 1][r] : 0.f;
         }
         s16x8 one[NP];
-        split8<NP>(y, one);
+        split8<NP>(z, one);
 #pragma unroll
-        for (int n = 0; n < NP; ++n) {
-          const u32x4 w = __builtin_bit_cast(u32x4, one[n]);
+        for (int i = 0; i < NP; ++i) {
+          const u32x4 w = __builtin_bit_cast(u32x4, one[i]);
+          u32x4 v[2];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            u32x4 z;
-            z[0] = quarter == 2 * h ? w[0] : 0u;
-            z[1] = quarter == 2 * h ? w[1] : 0u;
-            z[2] = quarter == 2 * h + 1 ? w[0] : 0u;
-            z[3] = quarter == 2 * h + 1 ? w[1] : 0u;
-            pk[h][n] = __builtin_bit_cast(s16x8, z);
+          for (int e = 0; e < 4; ++e) {
+            auto from = [&](auto N, uint32_t x) { return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x120 + decltype(N)::value, 0xf, 0xf, false); };  // lane p + 16 - N
+            if constexpr (SUB == 2) {
+              v[0][e] = w[e];
+              v[1][e] = from(std::integral_constant<int, 8>{}, w[e]);
+            } else {
+              v[0][e] = e < 2 ? w[e] : from(std::integral_constant<int, 12>{}, w[e % 2]);
+              v[1][e] = e < 2 ? from(std::integral_constant<int, 8>{}, w[e % 2]) : from(std::integral_constant<int, 4>{}, w[e % 2]);
+            }
           }
-        }
-      } else {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float y[8];
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            Steps4<T, NG> st;
-            st.load(Ss, key0 + 16 * (2 * h + i));
-#pragma unroll
-            for (int r = 0; r < 4; ++r) y[4 * i + r] = x[2 * h + i][r] * fmaxf(st.get(r, NG + j), 0.f);
-          }
-          split8<NP>(y, pk[h]);
+          pk[0][0][i] = __builtin_bit_cast(s16x8, v[0]);
+          pk[0][1][i] = __builtin_bit_cast(s16x8, v[1]);
         }
       }
       constexpr int TG4 = NT < 4 ? NT : 4;  // 16-column tiles of a group
@@ -461,47 +626,45 @@ template <typename T, int DP, bool QUAD> __global__ __launch_bounds__(64) void c
       for (int t = 0; t < TG4; ++t) {
         const s16x8 v0 = codes8<bf16>((uint32_t)w[t][0]), v1 = codes8<bf16>((uint32_t)w[t][1]);
 #pragma unroll
-        for (int n = NP - 1; n >= 0; --n) {
-          sm.o[4 * j + t] = Mfma16<bf16>::run(v0, pk[0][n], sm.o[4 * j + t]);
-          sm.o[4 * j + t] = Mfma16<bf16>::run(v1, pk[1][n], sm.o[4 * j + t]);
-        }
+        for (int qt = 0; qt < QT; ++qt)
+#pragma unroll
+          for (int i = NP - 1; i >= 0; --i) {
+            sm[qt].o[4 * j + t] = Mfma16<bf16>::run(v0, pk[qt][0][i], sm[qt].o[4 * j + t]);
+            sm[qt].o[4 * j + t] = Mfma16<bf16>::run(v1, pk[qt][1][i], sm[qt].o[4 * j + t]);
+          }
       }
     }
+    lds_wait_all();  // the values' reads
+    if (more) issue_values(c + 1);
   }
 
-  float lt = sm.total(), m = sm.m;
-  if constexpr (QUAD) {
-    // the four quarters of a row, lanes p & 3 of each
-    float mq = fmaxf(m, shfl_xor_f(m, 4));
-    mq = fmaxf(mq, shfl_xor_f(mq, 8));
-    const float f = m == -INFINITY ? (lt == 0.f ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - mq);  // (NaN sums are kept)
-    m = mq;
-    lt *= f;
-    lt += shfl_xor_f(lt, 4);
-    lt += shfl_xor_f(lt, 8);
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
+  for (int qt = 0; qt < QT; ++qt) {
+    float lt = sm[qt].total();
+    const float m = sm[qt].m;
+    if constexpr (SUB > 1) {
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float y = sm.o[t][r] * f;
-        y += shfl_xor_f(y, 4);
-        sm.o[t][r] = y + shfl_xor_f(y, 8);
-      }
-    if (p >= 4) return;
-  }
-  if (a.direct) {
-    if (rho >= a.TG) return;
-    const float l = ri.valid ? lt : 0.f, inv = l == 0.f ? 0.f : 1.f / l;
+      for (int x = ROWS; x < 16; x <<= 1) lt += shfl_xor_f(lt, x);
+      if (p >= ROWS) return;
+    }
+    const int rho = qt * 16 + p;
+    if (rho >= a.TG) continue;
+    if (a.direct) {
+      RowInfo ri;
+      ri.b = b; ri.t = tok[qt]; ri.hq = head[qt];
+      const float l = valid[qt] ? lt : 0.f, inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) store_row<T>(a, ri, sm.o[t], inv, 16 * t + 4 * g);
-    if (g == 0 && a.lse) a.lse[((int64_t)ri.b * a.Hq + ri.hq) * a.T + ri.t] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
-    return;
-  }
-  if (g == 0) a.stat[slot + p] = float2{m, lt};
-  if (ri.valid && lt != 0.f) {  // (a NaN sum is kept)
-    float *dst = a.part + (slot + p) * PITCH;
+      for (int t = 0; t < NT; ++t) store_row<T>(a, ri, sm[qt].o[t], inv, 16 * t + 4 * g);
+      if (g == 0 && a.lse) a.lse[((int64_t)b * a.Hq + head[qt]) * a.T + tok[qt]] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
+      continue;
+    }
+    const int64_t at = ((int64_t)hk * gridDim.y + blockIdx.y) * a.TG + rho;
+    if (g == 0) a.stat[at] = float2{m, lt};
+    if (valid[qt] && lt != 0.f) {  // (a NaN sum is kept)
+      float *dst = a.part + at * PITCH;
 #pragma unroll
-    for (int t = 0; t < NT; ++t) *(f32x4 *)(dst + 16 * t + 4 * g) = sm.o[t];
+      for (int t = 0; t < NT; ++t) *(f32x4 *)(dst + 16 * t + 4 * g) = sm[qt].o[t];
+    }
   }
 }
 
@@ -529,13 +692,13 @@ __device__ __forceinline__ void qk_pieces(const char *tile, const RowFrag<K, DP>
 template <typename T, int DP, int NW> struct Tile4 {
   using K = typename Pieces<T>::K;
   static constexpr int KC = 64, NT = NW * 64, CPR = DP / 8, TILE = KC * DP * 2, STAGE = 2 * TILE, LDS = 2 * STAGE;
-  static constexpr int BYTES = KC * DP / NT, LB = BYTES < 16 ? BYTES : 16, NL = BYTES / LB;  // codes of a thread: NL loads of LB bytes
+  static constexpr int BYTES = KC * DP / NT, LB = BYTES / 2 < 16 ? BYTES / 2 : 16, NL = BYTES / LB;  // codes of a thread: NL loads of LB bytes, half of keys
   static constexpr int UPR = DP / 2 / LB;                                                    // loads of a row
   static_assert(LDS <= 160 * 1024, "LDS");
 };
 
 template <typename T, int DP, int NW, int QT>
-__global__ __launch_bounds__(NW * 64) void cache4_tile_kernel(Cache4Args c4) {
+__global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 256 ? 1 : 2) void cache4_tile_kernel(Cache4Args c4) {
   using C = Tile4<T, DP, NW>;
   using K = typename C::K;
   constexpr int KC = C::KC, NM = KC / 16, N = Pieces<T>::Q;
@@ -544,8 +707,8 @@ __global__ __launch_bounds__(NW * 64) void cache4_tile_kernel(Cache4Args c4) {
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, p = lane & 15;
   const int tr = a.tr_own;
   // (the last tokens' tiles see the most keys: they start first)
-  const uint32_t per = (uint32_t)(a.Hkv * a.np_own * a.B), u0 = blockIdx.x % per;
-  const int tile = a.rt_own - 1 - (int)(blockIdx.x / per), hk = u0 / a.np_own % a.Hkv, b = u0 / a.np_own / a.Hkv, split = u0 % a.np_own;
+  const uint32_t per = (uint32_t)(a.Hkv * a.B), u0 = blockIdx.x % per, u1 = blockIdx.x / per;
+  const int hk = u0 % a.Hkv, b = u0 / a.Hkv, tile = a.rt_own - 1 - (int)(u1 % a.rt_own), split = (int)(u1 / a.rt_own);
   RowInfo ri[QT];
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
@@ -562,7 +725,7 @@ __global__ __launch_bounds__(NW * 64) void cache4_tile_kernel(Cache4Args c4) {
   }
   const int64_t slot = ((((int64_t)b * a.Hkv + hk) * a.rt_own + tile) * a.np_own + split) * tr;
   int c0, c1;
-  share_of((keys + KC - 1) / KC, split, a.np_own, c0, c1);
+  share_of((int)(((uint32_t)keys + KC - 1) / KC), split, a.np_own, c0, c1);
 
   RowFrag<K, DP> fr[N][QT];
 #pragma unroll
@@ -570,59 +733,67 @@ __global__ __launch_bounds__(NW * 64) void cache4_tile_kernel(Cache4Args c4) {
 #pragma unroll
     for (int ks = 0; ks < DP / 32; ++ks) {
       s16x8 x[N];
-      load_q8<T>(a, (const T *)a.q + ri[qt].b * a.sq[0] + ri[qt].hq * a.sq[1] + ri[qt].t * a.sq[2], 32 * ks + 8 * g, x);
+      load_q8<T>(a, (const T *)a.q + ri[qt].b * a.sq[0] + ri[qt].hq * a.sq[1] + ri[qt].t * a.sq[2], 32 * ks + 8 * g, true, x);
 #pragma unroll
       for (int n = 0; n < N; ++n) fr[n][qt].h[ks] = x[n];
     }
 
-  // this thread's loads: row, tensor (keys, then values; the same across a wave), place in the row
-  int row[C::NL], place[C::NL];
-  uint32_t off[C::NL], cw[C::NL][C::LB / 4];
-  float st[C::NL];
-  bool val[C::NL];
+  // this thread's loads: half of keys, half of values, at the same rows and places
+  constexpr int NH = C::NL / 2;
+  int row[NH], place[NH], sj[NH];
+  uint32_t koff[NH], voff[NH], cw[C::NL][C::LB / 4], sw[C::NL];
+  bool in[NH];
 #pragma unroll
-  for (int n = 0; n < C::NL; ++n) {
-    const int u = n * C::NT + tid, last = a.D / 2 / C::LB - 1, c = u % C::UPR;
-    val[n] = u / (KC * C::UPR);
-    row[n] = u / C::UPR % KC;
+  for (int n = 0; n < NH; ++n) {
+    const int u = n * C::NT + tid, last = a.D / 2 / C::LB - 1, c = u % C::UPR, at = (c < last ? c : last) * C::LB;
+    row[n] = u / C::UPR;
     place[n] = c;
-    off[n] = (uint32_t)(row[n] * (val[n] ? a.sv[2] : a.sk[2]) + (c < last ? c : last) * C::LB);
+    sj[n] = at * 2 / kGroup4;
+    koff[n] = (uint32_t)(row[n] * a.sk[2] + at);
+    voff[n] = (uint32_t)(row[n] * a.sv[2] + at);
   }
   const char *kb = (const char *)a.k + b * a.sk[0] + hk * a.sk[1], *vb = (const char *)a.v + b * a.sv[0] + hk * a.sv[1];
   const uint16_t *sb = c4.step + b * c4.ss[0] + hk * c4.ss[1];
+  const int64_t kchunk = a.sk[2] * KC, vchunk = a.sv[2] * KC;
+  const int ng = c4.ng;
+  auto fetch = [&](const char *src, uint32_t (&y)[C::LB / 4]) {
+    if constexpr (C::LB == 16) {
+      const u32x4 x = *(const u32x4 *)src;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = x[i];
+    } else if constexpr (C::LB == 8) {
+      const u32x2 x = *(const u32x2 *)src;
+      y[0] = x[0];
+      y[1] = x[1];
+    } else {
+      y[0] = *(const uint32_t *)src;
+    }
+  };
   auto load = [&](int c) {
-    const uint32_t row0 = (uint32_t)c * KC;
+    const int left = keys - c * KC;  // rows from the chunk's first on (below 2^31)
+    const char *kc = kb + c * kchunk, *vc = vb + c * vchunk;
+    const uint16_t *sc = sb + (int64_t)c * KC * 2 * ng;
 #pragma unroll
-    for (int n = 0; n < C::NL; ++n) {
-      const int64_t step = val[n] ? a.sv[2] : a.sk[2];
-      const uint32_t lim = tail_limit<KC>(row0, keys, (uint32_t)step, (uint32_t)a.D / 2) == 0xffffffffu ? 0xffffffffu
-                                                                                                       : (uint32_t)((keys - 1 - row0) * step + a.D / 2 - C::LB);
-      const char *src = (val[n] ? vb : kb) + row0 * step + (off[n] > lim ? lim : off[n]);
-      if constexpr (C::LB == 16) {
-        const u32x4 y = *(const u32x4 *)src;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) cw[n][i] = y[i];
-      } else if constexpr (C::LB == 8) {
-        const u32x2 y = *(const u32x2 *)src;
-        cw[n][0] = y[0];
-        cw[n][1] = y[1];
-      } else {
-        cw[n][0] = *(const uint32_t *)src;
-      }
-      const bool in = row0 + row[n] < (uint32_t)keys;
-      const int j = min(place[n] * C::LB * 2 / kGroup4, c4.ng - 1);
-      const uint16_t bits = sb[((int64_t)(in ? row0 + row[n] : keys - 1) * 2 + (val[n] ? 1 : 0)) * c4.ng + j];
-      const float y = step_f32<T>(bits);
-      st[n] = !in ? 0.f : val[n] ? fmaxf(y, 0.f) : y;  // (rows past the end are zeros; a value's NaN is its key's too)
+    for (int n = 0; n < NH; ++n) {
+      in[n] = row[n] < left;
+      // (rows past the end: the first one's codes, and steps of zero)
+      fetch(kc + (in[n] ? koff[n] : 0u), cw[n]);
+      fetch(vc + (in[n] ? voff[n] : 0u), cw[NH + n]);
+      const uint32_t at = in[n] ? (uint32_t)(row[n] * 2 * ng + sj[n]) : 0u;
+      sw[n] = sc[at];
+      sw[NH + n] = sc[at + ng];
     }
   };
   auto store = [&](int stage) {
 #pragma unroll
     for (int n = 0; n < C::NL; ++n) {
-      char *tl = smem + stage * C::STAGE + (val[n] ? C::TILE : 0) + row[n] * DP * 2;
+      const float y = step_f32<T>(sw[n]);
+      // (a value's NaN is its key's too)
+      const float st = !in[n % NH] ? 0.f : n < NH ? y : fmaxf(y, 0.f);
+      char *tl = smem + stage * C::STAGE + (n < NH ? 0 : C::TILE) + row[n % NH] * DP * 2;
 #pragma unroll
       for (int i = 0; i < C::LB / 4; ++i)
-        *(s16x8 *)(tl + ((place[n] * (C::LB / 4) + i) ^ swz(row[n], C::CPR)) * 16) = values8<K>(cw[n][i], st[n]);
+        *(s16x8 *)(tl + ((place[n % NH] * (C::LB / 4) + i) ^ swz(row[n % NH], C::CPR)) * 16) = values8<K>(cw[n][i], st);
     }
   };
 
@@ -694,38 +865,159 @@ __global__ __launch_bounds__(NW * 64) void cache4_tile_kernel(Cache4Args c4) {
   }
 }
 
+// A row's parts added up: 8 threads to a part's 32 columns (a block has CW columns of a
+// row), so NG parts at a time, each thread with a running maximum of its own parts; then
+// across the threads in a fixed order.
+template <typename T, int TEAM, int CW> __global__ __launch_bounds__(256) void cache4_join_kernel(Cache4Args c4, int pitch, int shares) {
+  constexpr int LG = CW / 4, NG = TEAM / LG, U = 4;
+  __shared__ f32x4 s_acc[256];
+  __shared__ float2 s_ml[256];
+  const CacheArgs &a = c4.a;
+  const int tid = threadIdx.x, in = tid % TEAM, gi = in / LG, e = in % LG;
+  const uint32_t row = blockIdx.x * (256 / TEAM) + tid / TEAM, rows = (uint32_t)a.B * a.Hkv * a.TG;
+  if (TEAM < 256 && row >= rows) return;
+  const uint32_t seq = row / (uint32_t)a.TG;
+  const int rho = (int)(row - seq * (uint32_t)a.TG), b = (int)(seq / (uint32_t)a.Hkv), hk = (int)(seq - (uint32_t)b * a.Hkv);
+  const RowInfo ri = row_info(a, b, hk, rho);
+  const int col = blockIdx.y * CW + 4 * e;
+  // part i of the row: first + i * tr_own
+  int64_t first;
+  int n = a.np_own;
+  if (c4.want) {
+    const int2 u = a.B > 1 ? c4.used[b] : int2{0, n};
+    first = ((int64_t)hk * shares + u.x) * a.TG + rho;
+    n = u.y;
+  } else {
+    const int tile = rho / a.tr_own;
+    first = ((int64_t)seq * a.rt_own + tile) * n * a.tr_own + (rho - tile * a.tr_own);
+  }
+  if (!ri.valid) n = 0;
+  float m = -INFINITY, l = 0.f;
+  f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+  for (int i = gi; i < n; i += U * NG) {
+    float2 st[U];
+    f32x4 y[U];
+#pragma unroll
+    for (int j = 0; j < U; ++j) {  // (one that there is not: the first again, left out)
+      const int64_t at = first + (int64_t)(i + j * NG < n ? i + j * NG : i) * a.tr_own;
+      st[j] = a.stat[at];
+      y[j] = *(const f32x4 *)(a.part + at * pitch + col);
+    }
+#pragma unroll
+    for (int j = 0; j < U; ++j) {
+      if (i + j * NG >= n || st[j].y == 0.f) continue;  // (a part of no keys has no O)
+      const float mn = fmaxf(m, st[j].x), ref = mn == -INFINITY ? 0.f : mn;
+      const float f0 = __builtin_amdgcn_exp2f(m - ref), f1 = st[j].x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st[j].x - ref);
+      l = l * f0 + st[j].y * f1;
+      acc = acc * f0 + y[j] * f1;
+      m = mn;
+    }
+  }
+  // threads e of the groups: neighbours first
+  auto add = [&](float m2, float l2, f32x4 a2) {
+    const float mn = fmaxf(m, m2), ref = mn == -INFINITY ? 0.f : mn;
+    const float f0 = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - ref), f1 = m2 == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m2 - ref);
+    l = l * f0 + l2 * f1;
+    acc = acc * f0 + a2 * f1;
+    m = mn;
+  };
+#pragma unroll
+  for (int x = LG; x < 64; x <<= 1) {
+    f32x4 a2;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) a2[r] = shfl_xor_f(acc[r], x);
+    add(shfl_xor_f(m, x), shfl_xor_f(l, x), a2);
+  }
+  if constexpr (TEAM == 256) {
+    if ((tid & 63) < LG) {
+      s_acc[tid] = acc;
+      s_ml[tid] = float2{m, l};
+    }
+    __syncthreads();
+    if (tid >= LG) return;
+#pragma unroll
+    for (int w = 1; w < 4; ++w) add(s_ml[w * 64 + tid].x, s_ml[w * 64 + tid].y, s_acc[w * 64 + tid]);
+  } else if (gi) {
+    return;
+  }
+  store_row<T>(a, ri, acc, l == 0.f ? 0.f : 1.f / l, col);
+  if (col == 0 && a.lse) a.lse[((int64_t)b * a.Hq + ri.hq) * a.T + ri.t] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
+}
+
 // ---- host ---------------------------------------------------------------------
 struct Plan4 {
-  int64_t DP, pitch, tr, rt, np, rows;
-  bool few, quad;
-  size_t part, total;
+  int64_t DP, pitch, tr, rt, np, want, rows;
+  int sub, qt;  // 0: the tile kernel
+  bool direct;  // each row's one share is its whole answer
+  size_t used, part, total;
 };
+// (queries take D SUB / 2 registers, 32-bit ones three times as many; O D / 4 for each 16 rows)
+constexpr int most_sub4(bool f32, int64_t dp) { return f32 ? (dp <= 64 ? 4 : dp == 128 ? 2 : 1) : dp <= 128 ? 4 : 2; }
+constexpr int most_tiles4(bool f32, int64_t dp) { return dp <= (f32 ? 64 : 128) ? 2 : 1; }
 static Plan4 plan4(const fbsa_attn4_desc *d) {
   Plan4 p;
   const int64_t TG = d->T * (d->Hq / d->Hkv), seqs = d->B * d->Hkv;
-  p.few = TG <= 16;
-  p.DP = d->D <= 32 ? 32 : d->D <= 64 ? 64 : d->D <= 128 ? 128 : p.few && d->D <= 192 ? 192 : 256;
+  const bool f32 = d->dtype == FBSA_F32;
+  p.DP = d->D <= 32 ? 32 : d->D <= 64 ? 64 : d->D <= 128 ? 128 : d->D <= 192 ? 192 : 256;
+  // Two 16-row tiles to a wave against the tile kernel, 16 sequences of 2000 to 16384
+  // rows, 24 rows a head: d 64 21.0 us against 23.2, d 128 27.6 against 33.5, fp32 d 64
+  // 25.5 against 36.5; three tiles lose (48 rows, d 128: 42.0 against 36.1)
+  const bool few = TG <= 16 * most_tiles4(f32, p.DP);
+  if (!few && p.DP == 192) p.DP = 256;
   p.pitch = p.DP == 192 ? 256 : p.DP;
-  p.quad = TG <= 4 && (p.DP <= 64 || (p.DP == 128 && d->dtype != FBSA_F32));
-  p.tr = p.quad ? 4 : p.few ? 16 : tile_rows(d->dtype, TG);
+  p.sub = !few ? 0 : (int)std::min<int64_t>(most_sub4(f32, p.DP), TG <= 4 ? 4 : TG <= 8 ? 2 : 1);
+  p.qt = few ? (int)cdiv(TG, 16) : 0;
+  p.tr = few ? TG : tile_rows(d->dtype, TG);
   p.rt = cdiv(TG, p.tr);
-  const int64_t tiles = seqs * p.rt, room = kCUs * (p.DP <= 128 ? 2 : 1);
-  const int64_t want = p.few ? cdiv((p.DP >= 192 ? 4 : 8) * kCUs, tiles) : d->B > 1 ? cdiv(4 * room, tiles) : tiles >= room ? 1 : room / tiles;
-  p.np = std::max<int64_t>(1, std::min({want, cdiv(d->S, p.few ? 64 : 128), (int64_t)kMaxShares / 2}));
-  p.rows = tiles * p.np * p.tr;
-  const size_t parts = p.np == 1 ? 0 : (size_t)p.rows;
-  p.part = up256(parts * 8);
+  const int64_t tiles = seqs * p.rt;
+  if (few) {
+    // Shares of the chunks: as many as run at a time with two waves to a SIMD, or one
+    // where a wave has more to do or rows are long (32 sequences, 16 heads over 2, d 256:
+    // 28.9 us against 30.3; one of 131072 rows 27.8 against 31.4; d 64, 262144 rows: 40.0
+    // against 29.9). Sequences round theirs up.
+    const int64_t each = std::max<int64_t>(1, kCUs * (p.qt > 1 || p.DP >= 192 ? 4 : 8) / d->Hkv), nc = cdiv(d->S, 64);
+    p.want = each * d->Hkv;
+    p.np = d->B == 1 ? std::min(each, nc) : std::min(each + d->B, nc * d->B);
+    p.rows = d->Hkv * p.np * TG;
+  } else {
+    // As many as a CU's LDS holds (48 rows, d 128, 16 sequences: two to a CU 36.1 us, four
+    // 41.0; d 64: 29.6 and 27.8), of 128 keys at least
+    const int64_t room = kCUs * (p.DP <= 64 ? 4 : p.DP == 128 ? 2 : 1);
+    p.want = 0;
+    p.np = std::max<int64_t>(1, std::min({room / tiles, cdiv(d->S, 128), (int64_t)256}));
+    p.rows = tiles * p.np * p.tr;
+  }
+  p.direct = p.np == (few ? d->B : 1);
+  const size_t parts = p.direct ? 0 : (size_t)p.rows;
+  p.used = up256(parts * 8);
+  p.part = p.used + (p.direct || !few ? 0 : up256((size_t)d->B * 8));
   p.total = p.part + up256(parts * p.pitch * 4);
   if (p.total == 0) p.total = 256;  // (0 says that a descriptor is refused)
   return p;
 }
 
-template <typename T, int DP, bool QUAD> static int launch_part4(const Cache4Args &c, int64_t wgs, hipStream_t s) {
-  constexpr size_t lds = (size_t)Part4<DP>::NS * Part4<DP>::STAGE;
-  const int e = lds_optin((const void *)cache4_part_kernel<T, DP, QUAD>, lds, "hipFuncSetAttribute(cache4_part)");
+template <typename T, int DP, int SUB, int QT> static int launch_part4(const Cache4Args &c, const Plan4 &pl, hipStream_t s) {
+  constexpr size_t lds = Part4<DP>::LDS;
+  const int e = lds_optin((const void *)cache4_part_kernel<T, DP, SUB, QT>, lds, "hipFuncSetAttribute(cache4_part)");
   if (e) return e;
-  hipLaunchKernelGGL((cache4_part_kernel<T, DP, QUAD>), dim3((unsigned)wgs), dim3(64), lds, s, c);
+  hipLaunchKernelGGL((cache4_part_kernel<T, DP, SUB, QT>), dim3((unsigned)c.a.Hkv, (unsigned)pl.np), dim3(64), lds, s, c);
   return hip_check(hipGetLastError(), "cache4_part_kernel launch");
+}
+template <typename T> static int launch_join4(const Cache4Args &c, const Plan4 &pl, hipStream_t s) {
+  const int64_t rows = (int64_t)c.a.B * c.a.Hkv * c.a.TG;
+  const int pitch = (int)pl.pitch, np = (int)pl.np;
+  // many rows: a wave each (of up to 128 columns); few: a workgroup for 128 or 32 columns
+  if (rows >= 2048) {
+    const unsigned wgs = (unsigned)cdiv(rows, 4);
+    if (pitch == 32) hipLaunchKernelGGL((cache4_join_kernel<T, 64, 32>), dim3(wgs), dim3(256), 0, s, c, pitch, np);
+    else if (pitch == 64) hipLaunchKernelGGL((cache4_join_kernel<T, 64, 64>), dim3(wgs), dim3(256), 0, s, c, pitch, np);
+    else hipLaunchKernelGGL((cache4_join_kernel<T, 64, 128>), dim3(wgs, (unsigned)(pitch / 128)), dim3(256), 0, s, c, pitch, np);
+  } else if (pitch >= 128 && rows * pitch >= 32 * 4 * kCUs) {
+    hipLaunchKernelGGL((cache4_join_kernel<T, 256, 128>), dim3((unsigned)rows, (unsigned)(pitch / 128)), dim3(256), 0, s, c, pitch, np);
+  } else {
+    hipLaunchKernelGGL((cache4_join_kernel<T, 256, 32>), dim3((unsigned)rows, (unsigned)cdiv(c.a.D, 32)), dim3(256), 0, s, c, pitch, np);
+  }
+  return hip_check(hipGetLastError(), "cache4_join_kernel launch");
 }
 template <typename T, int DP, int NW, int QT> static int launch_tile4(const Cache4Args &c, int64_t wgs, hipStream_t s) {
   using C = Tile4<T, DP, NW>;
@@ -736,10 +1028,17 @@ template <typename T, int DP, int NW, int QT> static int launch_tile4(const Cach
 }
 template <typename T, int DP> static int launch_attn4(const Cache4Args &c, const Plan4 &pl, hipStream_t s) {
   const int64_t wgs = (int64_t)c.a.B * c.a.Hkv * pl.rt * pl.np;
-  if constexpr (DP <= 64 || (DP == 128 && sizeof(T) == 2)) {
-    if (pl.quad) return launch_part4<T, DP, true>(c, wgs, s);
+  constexpr int MOST = most_sub4(sizeof(T) == 4, DP);
+  if constexpr (MOST >= 4) {
+    if (pl.sub == 4) return launch_part4<T, DP, 4, 1>(c, pl, s);
   }
-  if (pl.few) return launch_part4<T, DP, false>(c, wgs, s);
+  if constexpr (MOST >= 2) {
+    if (pl.sub == 2) return launch_part4<T, DP, 2, 1>(c, pl, s);
+  }
+  if constexpr (most_tiles4(sizeof(T) == 4, DP) == 2) {
+    if (pl.qt == 2) return launch_part4<T, DP, 1, 2>(c, pl, s);
+  }
+  if (pl.qt == 1) return launch_part4<T, DP, 1, 1>(c, pl, s);
   if constexpr (DP != 192) {
     if (pl.tr <= 64) return launch_tile4<T, DP, 4, 1>(c, wgs, s);
     if constexpr (sizeof(T) == 2) {
@@ -757,6 +1056,11 @@ template <typename T> static int dispatch_attn4(const Cache4Args &c, const Plan4
     case 192: return launch_attn4<T, 192>(c, pl, s);
     default: return launch_attn4<T, 256>(c, pl, s);
   }
+}
+
+template <typename T> static int run_attn4(const Cache4Args &c, const Plan4 &pl, hipStream_t s) {
+  const int e = dispatch_attn4<T>(c, pl, s);
+  return e || c.a.direct ? e : launch_join4<T>(c, pl, s);
 }
 
 static bool aligned_to(const void *p, int64_t n) { return (uintptr_t)p % (uintptr_t)n == 0; }
@@ -788,7 +1092,7 @@ static int check_rows4(const char *fn, const fbsa_rows4_desc *d) {
   for (int x = 0; x < 3; ++x)
     if (d->sk[x] < 0 || d->sv[x] < 0 || d->sk[x] * es % 16 || d->sv[x] * es % 16)
       return fail(FBSA_EINVAL, "%s: strides of the rows must be non-negative multiples of 16 bytes", fn);
-  // (2 lanes' groups of up to 32 to a row, fewer than 2^32 threads)
+  // (a launch has fewer than 2^32 threads along an axis: at least 16 rows to 256 here)
   if (d->B * d->H * d->T > 0x3ff0000LL) return fail(FBSA_EUNSUPPORTED, "%s: grid too large", fn);
   return FBSA_OK;
 }
@@ -815,7 +1119,7 @@ static int check_attn4(const fbsa_attn4_desc *d) {
       return fail(FBSA_EINVAL, "%s: strides of q and o must be non-negative multiples of 16 bytes", fn);
   // (fewer than 2^32 threads: up to 512 a tile and share, 64 or 256 a row that is joined)
   const Plan4 pl = plan4(d);
-  if (pl.rows > lim || d->B * d->Hq * d->T > 0x3ff0000LL || d->B * d->Hkv * pl.rt * pl.np > 0x7f0000LL)
+  if (pl.rows > lim || d->B * d->Hq * d->T > 0x3ff0000LL || (pl.qt ? pl.np > 65535 : d->B * d->Hkv * pl.rt * pl.np > 0x7f0000LL))
     return fail(FBSA_EUNSUPPORTED, "%s: grid too large", fn);
   return FBSA_OK;
 }
@@ -826,9 +1130,9 @@ static void fill_rows4(Rows4Args &a, const fbsa_rows4_desc *d) {
   a.B = (int)d->B; a.H = (int)d->H; a.T = (int)d->T; a.S = (int)d->S; a.D = (int)d->D; a.ng = (int)cdiv(d->D, kGroup4);
 }
 template <typename T, int LPR> static int launch_rows4(const Rows4Args &a, bool read, hipStream_t s) {
-  const unsigned wgs = (unsigned)cdiv((int64_t)a.B * a.H * a.T, 256 / (2 * LPR));
-  if (read) hipLaunchKernelGGL((cache4_read_kernel<T, LPR>), dim3(wgs), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((cache4_append_kernel<T, LPR>), dim3(wgs), dim3(256), 0, s, a);
+  const dim3 wgs((unsigned)cdiv(a.T, Rows4<T, LPR>::RPB * Rows4<T, LPR>::U), (unsigned)(a.B * a.H));
+  if (read) hipLaunchKernelGGL((cache4_read_kernel<T, LPR>), wgs, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((cache4_append_kernel<T, LPR>), wgs, dim3(256), 0, s, a);
   return hip_check(hipGetLastError(), read ? "cache4_read_kernel launch" : "cache4_append_kernel launch");
 }
 template <typename T> static int rows4_of(const Rows4Args &a, bool read, hipStream_t s) {
@@ -902,14 +1206,19 @@ int fbsa_cache4_attn(const fbsa_attn4_desc *d, const void *q, const void *k4, co
   a.B = (int)d->B; a.Hq = (int)d->Hq; a.Hkv = (int)d->Hkv; a.T = (int)d->T; a.S = (int)d->S; a.D = (int)d->D;
   a.G = (int)(d->Hq / d->Hkv); a.TG = a.T * a.G;
   a.tr_own = (int)pl.tr; a.tr_pre = 16; a.rt_own = (int)pl.rt; a.np_own = (int)pl.np;
-  a.direct = pl.np == 1;
+  a.direct = pl.direct;
+  c.want = (int)pl.want;
+  c.used = (int2 *)((char *)workspace + pl.used);
   a.scale2 = d->scale == 0.f ? 1.f : fabsf(d->scale) * kLog2e;
   a.qand = d->scale == 0.f ? 0u : 0xffffffffu;
   a.qxor = d->scale < 0.f ? (d->dtype == FBSA_F32 ? 0x80000000u : 0x80008000u) : 0u;
   a.stat = (float2 *)workspace; a.part = (float *)((char *)workspace + pl.part);
   hipStream_t s = (hipStream_t)stream;
-  e = d->dtype == FBSA_BF16 ? dispatch_attn4<bf16>(c, pl, s) : d->dtype == FBSA_F16 ? dispatch_attn4<f16>(c, pl, s) : dispatch_attn4<float>(c, pl, s);
-  return e || a.direct ? e : launch_cache_join(a, d->dtype, pl.pitch, s);
+  switch (d->dtype) {
+    case FBSA_BF16: return run_attn4<bf16>(c, pl, s);
+    case FBSA_F16: return run_attn4<f16>(c, pl, s);
+    default: return run_attn4<float>(c, pl, s);
+  }
 }
 
 }  // extern "C"
