@@ -247,8 +247,9 @@ struct Cache4Args {
   const uint16_t *step;
   int64_t ss[2];
   int32_t ng;            // steps of a key or value row
-  int32_t want;          // few rows: shares that the call's chunks are cut into, all (sequence, KV head)s together
-  int2 *used;            // few rows: a sequence's first share and its number of them
+  int32_t want;          // one tile a (sequence, KV head): shares that the call's chunks are cut into; 0: several tiles
+  int32_t least;         // chunks of a share
+  int2 *used;            // a sequence's first share and its number of them (want, several sequences)
 };
 
 template <int CTRL> __device__ __forceinline__ float dpp_f(float x, float old = 0.f) {
@@ -287,7 +288,7 @@ __device__ __forceinline__ bool share4(const Cache4Args &c4, int i, int lane, in
   }
   int total = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) total += wave_sum(chunks4(a, b0 + lane));  // (B H of 65535 at most: below 2^31 up to 2^37 rows; plan4)
-  const int most = c4.want / a.Hkv, each = max(1, (total + most - 1) / most);
+  const int most = c4.want / a.Hkv, each = max(c4.least, (total + most - 1) / most);
   before = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const int mine = b0 + lane < a.B ? max(1, (chunks4(a, b0 + lane) + each - 1) / each) : 0;
@@ -396,14 +397,17 @@ template <typename T, int NG> struct Steps4 {
 // SUB-th of the chunk and zero outside the lanes that hold its keys, so a product has the
 // scores of 16 SUB keys and no lane holds one twice: a SUB-th of the exponentials and
 // splits. For the value product the first part's columns take the others' probabilities.
+// W > 1: a workgroup's waves share a sequence's chunks and join their parts in LDS, where
+// that spares short caches the second launch.
 // QT > 1: that many 16-row tiles, for which the codes are made numbers once; 16-bit P is
 // then rounded once (bf16), as in the kernel of many rows.
-template <typename T, int DP, int SUB, int QT> constexpr int part4_waves() {  // to a SIMD: one where 256 registers are too few
-  constexpr int regs = QT * (DP / 4 + DP / 8 * SUB * Pieces<T>::Q + 32 / SUB) + 64 + DP / 4;
-  return regs < 256 || (DP == 256 && SUB == 2) ? 2 : 1;
+// waves to a SIMD: one where 256 registers are too few
+constexpr int part4_waves(bool f32, int dp, int sub, int qt) {
+  const int regs = qt * (dp / 4 + dp / 8 * sub * (f32 ? 3 : 1) + 32 / sub) + 64 + dp / 4;
+  return regs < 256 || (dp == 256 && sub == 2) ? 2 : 1;
 }
-template <typename T, int DP, int SUB, int QT>
-__global__ __launch_bounds__(64, (part4_waves<T, DP, SUB, QT>())) void cache4_part_kernel(Cache4Args c4) {
+template <typename T, int DP, int SUB, int QT, int W>
+__global__ __launch_bounds__(64 * W, part4_waves(sizeof(T) == 4, DP, SUB, QT)) void cache4_part_kernel(Cache4Args c4) {
   using C = Part4<DP>;
   using K = typename Pieces<T>::K;
   static_assert(SUB == 1 || QT == 1, "parts of the chunk are for one tile");
@@ -411,13 +415,19 @@ __global__ __launch_bounds__(64, (part4_waves<T, DP, SUB, QT>())) void cache4_pa
   constexpr int NG = C::NG, NQ = Pieces<T>::Q, NP = QT > 1 && __is_same(T, bf16) ? 1 : Pieces<T>::P, NT = DP / 16;
   constexpr int NF = DP / 32 * SUB, FG = DP == 32 ? NF : 2 * SUB;  // products of a score; of a group
   constexpr int PITCH = DP == 192 ? 256 : DP;
-  extern __shared__ __attribute__((aligned(16))) char smem[];
+  extern __shared__ __attribute__((aligned(16))) char smem_all[];
   const CacheArgs &a = c4.a;
-  const int lane = threadIdx.x, g = lane >> 4, p = lane & 15, sub = p / ROWS;
+  const int wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  char *smem = smem_all + wave * C::LDS;
+  const int lane = threadIdx.x & 63, g = lane >> 4, p = lane & 15, sub = p / ROWS;
   const int hk = blockIdx.x;
   int b, split, np, before;
-  if (!share4(c4, blockIdx.y, lane, b, split, np, before)) return;
-  if (split == 0 && hk == 0 && lane == 0 && !a.direct) c4.used[b] = int2{before, np};
+  if constexpr (W > 1) {
+    b = blockIdx.y; split = wave; np = W; before = 0;
+  } else {
+    if (!share4(c4, blockIdx.y, lane, b, split, np, before)) return;
+    if (split == 0 && hk == 0 && lane == 0 && !a.direct) c4.used[b] = int2{before, np};
+  }
   const int n = seq_len(a, b), count = seq_count(a, b), keys = count > 0 ? n : 0;
   int low = n - count + 1;  // below it every row sees every key
   low = low < 0 ? 0 : low;
@@ -638,6 +648,48 @@ __global__ __launch_bounds__(64, (part4_waves<T, DP, SUB, QT>())) void cache4_pa
     if (more) issue_values(c + 1);
   }
 
+  if constexpr (W > 1) {
+    // the waves' parts through LDS, each in its own ring's place (O's rows are as long
+    // as the two tiles), added up in order by threads of four columns each
+    static_assert(QT == 1, "one tile's O in a wave's ring");
+    constexpr int RING = C::LDS, STAT = 2 * C::TILE;
+    float lt = sm[0].total();
+#pragma unroll
+    for (int x = ROWS; x < 16; x <<= 1) lt += shfl_xor_f(lt, x);
+    if (p < ROWS) {
+      if (g == 0) ((float2 *)(smem + STAT))[p] = float2{sm[0].m, lt};
+#pragma unroll
+      for (int t = 0; t < NT; ++t) *(f32x4 *)(smem + (p * DP + 16 * t + 4 * g) * 4) = sm[0].o[t];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.TG * (DP / 4); i += 64 * W) {
+      const int row = i / (DP / 4), d = i % (DP / 4) * 4;
+      float m = -INFINITY, l = 0.f;
+      float2 st[W];
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        st[w] = ((const float2 *)(smem_all + w * RING + STAT))[row];
+        m = fmaxf(m, st[w].x);
+      }
+      const float ref = m == -INFINITY ? 0.f : m;
+      f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        if (st[w].y == 0.f) continue;  // (a NaN sum is kept)
+        const float f = st[w].x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(st[w].x - ref);
+        l += f * st[w].y;
+        acc += f * *(const f32x4 *)(smem_all + w * RING + (row * DP + d) * 4);
+      }
+      RowInfo ri;
+      ri.b = b;
+      ri.t = (int)(((float)row + 0.5f) * inv_g);
+      ri.hq = hk * a.G + row - ri.t * a.G;
+      if (ri.t >= count) l = 0.f;
+      store_row<T>(a, ri, acc, l == 0.f ? 0.f : 1.f / l, d);
+      if (d == 0 && a.lse) a.lse[((int64_t)b * a.Hq + ri.hq) * a.T + ri.t] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
+    }
+    return;
+  }
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
     float lt = sm[qt].total();
@@ -707,8 +759,23 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 256 ? 1 : 2) void 
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, p = lane & 15;
   const int tr = a.tr_own;
   // (the last tokens' tiles see the most keys: they start first)
-  const uint32_t per = (uint32_t)(a.Hkv * a.B), u0 = blockIdx.x % per, u1 = blockIdx.x / per;
-  const int hk = u0 % a.Hkv, b = u0 / a.Hkv, tile = a.rt_own - 1 - (int)(u1 % a.rt_own), split = (int)(u1 / a.rt_own);
+  int b, hk, tile = 0, split, np = a.np_own;
+  int64_t slot;
+  if (c4.want) {
+    const int i = (int)(blockIdx.x / (uint32_t)a.Hkv);
+    int before;
+    hk = (int)(blockIdx.x - (uint32_t)i * a.Hkv);
+    if (!share4(c4, i, lane, b, split, np, before)) return;
+    if (split == 0 && hk == 0 && tid == 0 && !a.direct) c4.used[b] = int2{before, np};
+    slot = ((int64_t)hk * a.np_own + i) * tr;
+  } else {
+    const uint32_t per = (uint32_t)(a.Hkv * a.B), u0 = blockIdx.x % per, u1 = blockIdx.x / per;
+    hk = u0 % a.Hkv;
+    b = u0 / a.Hkv;
+    tile = a.rt_own - 1 - (int)(u1 % a.rt_own);
+    split = (int)(u1 / a.rt_own);
+    slot = ((((int64_t)b * a.Hkv + hk) * a.rt_own + tile) * np + split) * tr;
+  }
   RowInfo ri[QT];
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
@@ -723,9 +790,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 256 ? 1 : 2) void 
     own_bounds(a, b, r0, a.TG, k, low);
     low = min(low, keys);
   }
-  const int64_t slot = ((((int64_t)b * a.Hkv + hk) * a.rt_own + tile) * a.np_own + split) * tr;
   int c0, c1;
-  share_of((int)(((uint32_t)keys + KC - 1) / KC), split, a.np_own, c0, c1);
+  share_of((int)(((uint32_t)keys + KC - 1) / KC), split, np, c0, c1);
 
   RowFrag<K, DP> fr[N][QT];
 #pragma unroll
@@ -791,9 +857,24 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 256 ? 1 : 2) void 
       // (a value's NaN is its key's too)
       const float st = !in[n % NH] ? 0.f : n < NH ? y : fmaxf(y, 0.f);
       char *tl = smem + stage * C::STAGE + (n < NH ? 0 : C::TILE) + row[n % NH] * DP * 2;
+      // a load's words are 16-byte units side by side, and lanes next to each other would
+      // write to a few banks: each starts at another word
+      constexpr int NWD = C::LB / 4;
+      const int first = NWD == 4 ? (C::UPR == 8 ? place[n % NH] + (place[n % NH] >> 2) : place[n % NH]) & 3 : place[n % NH] & (NWD - 1);
+      uint32_t x[NWD];
 #pragma unroll
-      for (int i = 0; i < C::LB / 4; ++i)
-        *(s16x8 *)(tl + ((place[n % NH] * (C::LB / 4) + i) ^ swz(row[n % NH], C::CPR)) * 16) = values8<K>(cw[n][i], st);
+      for (int i = 0; i < NWD; ++i) x[i] = first & 1 ? cw[n][(i + 1) % NWD] : cw[n][i];
+      if constexpr (NWD == 4) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t y0 = x[i], y1 = x[i + 2];
+          x[i] = first & 2 ? y1 : y0;
+          x[i + 2] = first & 2 ? y0 : y1;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NWD; ++i)
+        *(s16x8 *)(tl + ((place[n % NH] * NWD + ((i + first) & (NWD - 1))) ^ swz(row[n % NH], C::CPR)) * 16) = values8<K>(x[i], st);
     }
   };
 
@@ -885,7 +966,7 @@ template <typename T, int TEAM, int CW> __global__ __launch_bounds__(256) void c
   int n = a.np_own;
   if (c4.want) {
     const int2 u = a.B > 1 ? c4.used[b] : int2{0, n};
-    first = ((int64_t)hk * shares + u.x) * a.TG + rho;
+    first = ((int64_t)hk * shares + u.x) * a.tr_own + rho;
     n = u.y;
   } else {
     const int tile = rho / a.tr_own;
@@ -949,10 +1030,12 @@ struct Plan4 {
   int64_t DP, pitch, tr, rt, np, want, rows;
   int sub, qt;  // 0: the tile kernel
   bool direct;  // each row's one share is its whole answer
+  bool joined;  // the waves of a workgroup share a sequence's chunks
   size_t used, part, total;
 };
 // (queries take D SUB / 2 registers, 32-bit ones three times as many; O D / 4 for each 16 rows)
 constexpr int most_sub4(bool f32, int64_t dp) { return f32 ? (dp <= 64 ? 4 : dp == 128 ? 2 : 1) : dp <= 128 ? 4 : 2; }
+constexpr int kJoined4 = 8;  // waves of a workgroup that joins its own parts
 constexpr int most_tiles4(bool f32, int64_t dp) { return dp <= (f32 ? 64 : 128) ? 2 : 1; }
 static Plan4 plan4(const fbsa_attn4_desc *d) {
   Plan4 p;
@@ -970,6 +1053,7 @@ static Plan4 plan4(const fbsa_attn4_desc *d) {
   p.tr = few ? TG : tile_rows(d->dtype, TG);
   p.rt = cdiv(TG, p.tr);
   const int64_t tiles = seqs * p.rt;
+  p.joined = false;
   if (few) {
     // Shares of the chunks: as many as run at a time with two waves to a SIMD, or one
     // where a wave has more to do or rows are long (32 sequences, 16 heads over 2, d 256:
@@ -979,29 +1063,50 @@ static Plan4 plan4(const fbsa_attn4_desc *d) {
     p.want = each * d->Hkv;
     p.np = d->B == 1 ? std::min(each, nc) : std::min(each + d->B, nc * d->B);
     p.rows = d->Hkv * p.np * TG;
+    // (kernels of one wave to a SIMD have no such form)
+    // One launch against two, where the waves have few chunks each, or the card many
+    // workgroups (8 heads, d 64, 1024 rows 6.8 us against 7.7, 4096 10.8 against 8.0; 32
+    // sequences of those 15.5 against 18.5, of 8192 rows 24.1 against 25.9; 32 x 2 heads, d
+    // 256, 256 rows 9.9 against 12.6, 2048 22.3 against 19.3)
+    const int64_t chunks = std::max<int64_t>(1, 256 / p.DP) * std::min<int64_t>(4, std::max<int64_t>(1, seqs / 64));
+    p.joined = TG <= 16 && part4_waves(f32, (int)p.DP, p.sub, 1) == 2 && nc > 1 && nc <= kJoined4 * chunks;
   } else {
     // As many as a CU's LDS holds (48 rows, d 128, 16 sequences: two to a CU 36.1 us, four
     // 41.0; d 64: 29.6 and 27.8), of 128 keys at least
     const int64_t room = kCUs * (p.DP <= 64 ? 4 : p.DP == 128 ? 2 : 1);
-    p.want = 0;
-    p.np = std::max<int64_t>(1, std::min({room / tiles, cdiv(d->S, 128), (int64_t)256}));
-    p.rows = tiles * p.np * p.tr;
+    if (p.rt == 1) {
+      const int64_t each = std::max<int64_t>(1, room / d->Hkv), nc = cdiv(d->S, 128);
+      p.want = each * d->Hkv;
+      p.np = d->B == 1 ? std::min(each, nc) : std::min(each + d->B, nc * d->B);
+      p.rows = d->Hkv * p.np * p.tr;
+    } else {
+      p.want = 0;
+      p.np = std::max<int64_t>(1, std::min({room / tiles, cdiv(d->S, 128), (int64_t)256}));
+      p.rows = tiles * p.np * p.tr;
+    }
   }
-  p.direct = p.np == (few ? d->B : 1);
+  p.direct = p.joined || p.np == (p.want ? d->B : 1);
   const size_t parts = p.direct ? 0 : (size_t)p.rows;
   p.used = up256(parts * 8);
-  p.part = p.used + (p.direct || !few ? 0 : up256((size_t)d->B * 8));
+  p.part = p.used + (p.direct || !p.want ? 0 : up256((size_t)d->B * 8));
   p.total = p.part + up256(parts * p.pitch * 4);
   if (p.total == 0) p.total = 256;  // (0 says that a descriptor is refused)
   return p;
 }
 
-template <typename T, int DP, int SUB, int QT> static int launch_part4(const Cache4Args &c, const Plan4 &pl, hipStream_t s) {
-  constexpr size_t lds = Part4<DP>::LDS;
-  const int e = lds_optin((const void *)cache4_part_kernel<T, DP, SUB, QT>, lds, "hipFuncSetAttribute(cache4_part)");
+template <typename T, int DP, int SUB, int QT, int W> static int launch_part4(const Cache4Args &c, const Plan4 &pl, hipStream_t s) {
+  constexpr size_t lds = (size_t)W * Part4<DP>::LDS;
+  static_assert(lds <= 160 * 1024, "LDS");
+  const int e = lds_optin((const void *)cache4_part_kernel<T, DP, SUB, QT, W>, lds, "hipFuncSetAttribute(cache4_part)");
   if (e) return e;
-  hipLaunchKernelGGL((cache4_part_kernel<T, DP, SUB, QT>), dim3((unsigned)c.a.Hkv, (unsigned)pl.np), dim3(64), lds, s, c);
+  hipLaunchKernelGGL((cache4_part_kernel<T, DP, SUB, QT, W>), dim3((unsigned)c.a.Hkv, (unsigned)(W > 1 ? c.a.B : pl.np)), dim3(64 * W), lds, s, c);
   return hip_check(hipGetLastError(), "cache4_part_kernel launch");
+}
+template <typename T, int DP, int SUB> static int launch_few4(const Cache4Args &c, const Plan4 &pl, hipStream_t s) {
+  if constexpr (part4_waves(sizeof(T) == 4, DP, SUB, 1) == 2) {
+    if (pl.joined) return launch_part4<T, DP, SUB, 1, kJoined4>(c, pl, s);
+  }
+  return launch_part4<T, DP, SUB, 1, 1>(c, pl, s);
 }
 template <typename T> static int launch_join4(const Cache4Args &c, const Plan4 &pl, hipStream_t s) {
   const int64_t rows = (int64_t)c.a.B * c.a.Hkv * c.a.TG;
@@ -1027,18 +1132,18 @@ template <typename T, int DP, int NW, int QT> static int launch_tile4(const Cach
   return hip_check(hipGetLastError(), "cache4_tile_kernel launch");
 }
 template <typename T, int DP> static int launch_attn4(const Cache4Args &c, const Plan4 &pl, hipStream_t s) {
-  const int64_t wgs = (int64_t)c.a.B * c.a.Hkv * pl.rt * pl.np;
+  const int64_t wgs = (pl.want ? 1 : (int64_t)c.a.B * pl.rt) * c.a.Hkv * pl.np;
   constexpr int MOST = most_sub4(sizeof(T) == 4, DP);
   if constexpr (MOST >= 4) {
-    if (pl.sub == 4) return launch_part4<T, DP, 4, 1>(c, pl, s);
+    if (pl.sub == 4) return launch_few4<T, DP, 4>(c, pl, s);
   }
   if constexpr (MOST >= 2) {
-    if (pl.sub == 2) return launch_part4<T, DP, 2, 1>(c, pl, s);
+    if (pl.sub == 2) return launch_few4<T, DP, 2>(c, pl, s);
   }
   if constexpr (most_tiles4(sizeof(T) == 4, DP) == 2) {
-    if (pl.qt == 2) return launch_part4<T, DP, 1, 2>(c, pl, s);
+    if (pl.qt == 2) return launch_part4<T, DP, 1, 2, 1>(c, pl, s);
   }
-  if (pl.qt == 1) return launch_part4<T, DP, 1, 1>(c, pl, s);
+  if (pl.qt == 1) return launch_few4<T, DP, 1>(c, pl, s);
   if constexpr (DP != 192) {
     if (pl.tr <= 64) return launch_tile4<T, DP, 4, 1>(c, wgs, s);
     if constexpr (sizeof(T) == 2) {
@@ -1119,7 +1224,7 @@ static int check_attn4(const fbsa_attn4_desc *d) {
       return fail(FBSA_EINVAL, "%s: strides of q and o must be non-negative multiples of 16 bytes", fn);
   // (fewer than 2^32 threads: up to 512 a tile and share, 64 or 256 a row that is joined)
   const Plan4 pl = plan4(d);
-  if (pl.rows > lim || d->B * d->Hq * d->T > 0x3ff0000LL || (pl.qt ? pl.np > 65535 : d->B * d->Hkv * pl.rt * pl.np > 0x7f0000LL))
+  if (pl.rows > lim || d->B * d->Hq * d->T > 0x3ff0000LL || (pl.qt ? pl.np > 65535 : (pl.want ? 1 : d->B * pl.rt) * d->Hkv * pl.np > 0x7f0000LL))
     return fail(FBSA_EUNSUPPORTED, "%s: grid too large", fn);
   return FBSA_OK;
 }
@@ -1208,6 +1313,7 @@ int fbsa_cache4_attn(const fbsa_attn4_desc *d, const void *q, const void *k4, co
   a.tr_own = (int)pl.tr; a.tr_pre = 16; a.rt_own = (int)pl.rt; a.np_own = (int)pl.np;
   a.direct = pl.direct;
   c.want = (int)pl.want;
+  c.least = pl.qt ? 1 : 2;
   c.used = (int2 *)((char *)workspace + pl.used);
   a.scale2 = d->scale == 0.f ? 1.f : fabsf(d->scale) * kLog2e;
   a.qand = d->scale == 0.f ? 0u : 0xffffffffu;
