@@ -90,15 +90,15 @@ struct Rows4Args {
   int32_t B, H, T, S, D, ng;
 };
 
-// Eight lanes' group (four at LPR 4): the largest magnitude of its elements
-template <int LPR> __device__ __forceinline__ float group_max(float x) {
+// The largest magnitude of a group's N lanes (4 or 8)
+template <int N> __device__ __forceinline__ float group_max(float x) {
   auto with = [&](auto CTRL) {
     const int y = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(CTRL)::value, 0xf, 0xf, false);
     x = fmaxf(x, __builtin_bit_cast(float, y));
   };
-  with(std::integral_constant<int, 0xb1>{});                           // lane ^ 1
-  with(std::integral_constant<int, 0x4e>{});                           // lane ^ 2
-  if constexpr (LPR >= 8) with(std::integral_constant<int, 0x141>{});  // 7 - lane of eight
+  with(std::integral_constant<int, 0xb1>{});                         // lane ^ 1
+  with(std::integral_constant<int, 0x4e>{});                         // lane ^ 2
+  if constexpr (N >= 8) with(std::integral_constant<int, 0x141>{});  // 7 - lane of eight
   return x;
 }
 // largest magnitude / 6 to 6 significant bits, ties to even. The division is correctly
@@ -137,27 +137,18 @@ __device__ __forceinline__ uint32_t codes_of(const float (&y)[8], float step) {
   return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, q[6], q[7], 1.f, 3);
 }
 
-// Rows of a block: 8 elements a lane, LPR lanes to a key or value row and the two side by
-// side, RPB rows at a time, U times. LPR = 4, 8, 16, 32 for D up to 32, 64, 128, 256.
-template <typename T, int LPR> struct Rows4 {
-  static constexpr int RPB = 256 / (2 * LPR), U = 4;
+// Rows of a block: EL elements a lane, LPR lanes to a key or value row and the two side by
+// side, RPB rows at a time, U times.
+template <int EL_, int LPR> struct Rows4 {
+  static constexpr int EL = EL_, RPB = 256 / (2 * LPR), U = 4;
 };
-template <typename T> __device__ __forceinline__ void load8(const T *src, float (&y)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const f32x4 p = ((const f32x4 *)src)[0], q = ((const f32x4 *)src)[1];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { y[i] = p[i]; y[4 + i] = q[i]; }
-  } else {
-    const s16x8 p = *(const s16x8 *)src;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = to_f32<T>(__builtin_bit_cast(T, (short)p[i]));
-  }
-}
 
 // New rows: key and value of a row side by side, so that all its lanes know of a NaN or
-// an infinity in either. Bound by memory, long prompts; a step's rows by latency.
+// an infinity in either. Bound by memory, long prompts: 65531 fp32 rows of 8 heads, d 96,
+// 94 us, 4.9 TB/s (four elements a lane, whole lines a load, 112: codes leave two bytes at
+// a time); a step's rows by latency, 3 us.
 template <typename T, int LPR> __global__ __launch_bounds__(256) void cache4_append_kernel(Rows4Args a) {
-  using C = Rows4<T, LPR>;
+  using C = Rows4<8, LPR>;
   const int tid = threadIdx.x, lane = tid & 63, which = (tid / LPR) & 1, e = tid % LPR;  // key or value; elements 8 e ...
   const int h = (int)(blockIdx.y % (uint32_t)a.H), b = (int)(blockIdx.y / (uint32_t)a.H);
   const int t0 = blockIdx.x * (C::RPB * C::U) + tid / (2 * LPR), first = a.first[b], count = min(a.count ? a.count[b] : a.T, a.T);
@@ -173,7 +164,17 @@ template <typename T, int LPR> __global__ __launch_bounds__(256) void cache4_app
     live[i] = 8 * e < a.D && t < count && at >= 0 && at < a.S;
 #pragma unroll
     for (int j = 0; j < 8; ++j) y[i][j] = 0.f;
-    if (live[i]) load8<T>(src + t * tstep, y[i]);
+    if (live[i]) {
+      if constexpr (sizeof(T) == 4) {
+        const f32x4 p = ((const f32x4 *)(src + t * tstep))[0], q = ((const f32x4 *)(src + t * tstep))[1];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { y[i][j] = p[j]; y[i][4 + j] = q[j]; }
+      } else {
+        const s16x8 p = *(const s16x8 *)(src + t * tstep);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[i][j] = to_f32<T>(__builtin_bit_cast(T, (short)p[j]));
+      }
+    }
   }
   char *dst = (char *)(which ? a.v4 : a.k4) + b * s4[0] + h * s4[1] + 4 * e;
   const int64_t rstep = s4[2];
@@ -183,13 +184,13 @@ template <typename T, int LPR> __global__ __launch_bounds__(256) void cache4_app
     float most = 0.f, sum = 0.f;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      most = fmaxf(most, fabsf(y[i][j]));  // (passes NaN over)
+      most = fmaxf(most, fabsf(y[i][j]));       // (passes NaN over)
       sum = __builtin_fmaf(y[i][j], 0.f, sum);  // 0, or NaN
     }
     const uint64_t vote = __ballot(sum != 0.f);
     constexpr uint64_t ROW = LPR == 32 ? ~0ull : (1ull << (2 * LPR % 64)) - 1;
     const bool bad = (vote >> (lane / (2 * LPR) * (2 * LPR)) & ROW) != 0;
-    most = group_max<LPR>(most);
+    most = group_max<(LPR < 8 ? LPR : 8)>(most);
     if (!live[i]) continue;
     const float step = bad ? __uint_as_float(0x7fc00000u) : step_of<T>(most);
     const int64_t at = (int64_t)first + t0 + i * C::RPB;
@@ -202,41 +203,42 @@ template <typename T, int LPR> __global__ __launch_bounds__(256) void cache4_app
 }
 
 // Rows first[b] + t of each sequence as numbers of type T; rows outside the cache, and
-// those from count[b] on, are zeros. 8 values a lane, written whole lines at a time.
+// those from count[b] on, are zeros. 16 bytes of values a lane, so that a store is whole
+// lines, past the caches (nothing here reads them again): 262144 bf16 rows of 8 heads, d
+// 64, 119 us, 5.7 TB/s, 126 with ordinary stores.
 template <typename T, int LPR> __global__ __launch_bounds__(256) void cache4_read_kernel(Rows4Args a) {
-  using C = Rows4<T, LPR>;
+  using C = Rows4<16 / sizeof(T), LPR>;
+  constexpr int EL = C::EL, RPB = C::RPB, U = C::U;
   const int tid = threadIdx.x, which = (tid / LPR) & 1, e = tid % LPR;
   const int h = (int)(blockIdx.y % (uint32_t)a.H), b = (int)(blockIdx.y / (uint32_t)a.H);
-  if (8 * e >= a.D) return;
-  const int t0 = blockIdx.x * (C::RPB * C::U) + tid / (2 * LPR), first = a.first ? a.first[b] : 0, count = a.count ? a.count[b] : a.T;
+  if (EL * e >= a.D) return;
+  const int t0 = blockIdx.x * (RPB * U) + tid / (2 * LPR), first = a.first ? a.first[b] : 0, count = a.count ? a.count[b] : a.T;
   const int64_t *st = which ? a.sv : a.sk, *s4 = which ? a.sv4 : a.sk4;
-  const char *src = (const char *)(which ? a.v4 : a.k4) + b * s4[0] + h * s4[1] + 4 * e;
+  const char *src = (const char *)(which ? a.v4 : a.k4) + b * s4[0] + h * s4[1] + EL / 2 * e;
   const int64_t rstep = s4[2], tstep = st[2];
-  const uint16_t *sd = a.step + b * a.ss[0] + h * a.ss[1] + which * a.ng + e / 8;
-  uint32_t w[C::U], s[C::U];
+  const uint16_t *sd = a.step + b * a.ss[0] + h * a.ss[1] + which * a.ng + e / (kGroup4 / EL);
+  uint32_t w[U], s[U];
 #pragma unroll
-  for (int i = 0; i < C::U; ++i) {
-    const int t = t0 + i * C::RPB;
+  for (int i = 0; i < U; ++i) {
+    const int t = t0 + i * RPB;
     const int64_t at = (int64_t)first + t;
     w[i] = s[i] = 0;
     if (t < count && at >= 0 && at < a.S) {
-      w[i] = *(const uint32_t *)(src + at * rstep);
+      w[i] = EL == 8 ? *(const uint32_t *)(src + at * rstep) : *(const uint16_t *)(src + at * rstep);
       s[i] = sd[at * 2 * a.ng];
     }
   }
-  T *dst = (T *)(which ? a.v : a.k) + b * st[0] + h * st[1] + 8 * e;
+  T *dst = (T *)(which ? a.v : a.k) + b * st[0] + h * st[1] + EL * e;
 #pragma unroll
-  for (int i = 0; i < C::U; ++i) {
-    const int t = t0 + i * C::RPB;
+  for (int i = 0; i < U; ++i) {
+    const int t = t0 + i * RPB;
     if (t >= a.T) continue;
     const float step = step_f32<T>(s[i]);
     if constexpr (sizeof(T) == 4) {
-      float x[8];
-      values8_f32(w[i], step, x);
-      ((f32x4 *)(dst + t * tstep))[0] = f32x4{x[0], x[1], x[2], x[3]};
-      ((f32x4 *)(dst + t * tstep))[1] = f32x4{x[4], x[5], x[6], x[7]};
+      const f32x2 x = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], 1.f, 0), y = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w[i], 1.f, 1);
+      __builtin_nontemporal_store(f32x4{x[0] * step, x[1] * step, y[0] * step, y[1] * step}, (f32x4 *)(dst + t * tstep));
     } else {
-      *(s16x8 *)(dst + t * tstep) = values8<T>(w[i], step);
+      __builtin_nontemporal_store(values8<T>(w[i], step), (s16x8 *)(dst + t * tstep));
     }
   }
 }
@@ -726,19 +728,57 @@ __global__ __launch_bounds__(64 * W, part4_waves(sizeof(T) == 4, DP, SUB, QT)) v
 // queries and of probabilities: six products of the matrix units' fastest type cost less
 // than two of the slow 32-bit one.
 template <typename K, int DP, int QT, int NM, int N>
-__device__ __forceinline__ void qk_pieces(const char *tile, const RowFrag<K, DP> (&fr)[N][QT], f32x4 (&acc)[QT][NM], int g, int p) {
-  qk_tile<K, DP, QT, NM>(tile, fr[0], acc, g, p);
-  if constexpr (N > 1) {
+__device__ __forceinline__ void qk_pieces(const char *tile, const RowFrag<K, DP> (&fr)[N * QT], f32x4 (&s)[QT][NM], int g, int p) {
+  if constexpr (N == 1) {
+    qk_tile<K, DP, QT, NM>(tile, fr, s, g, p);
+  } else {  // (a fragment of K read once, the smallest pieces' products added first)
+    f32x4 acc[N * QT][NM];
+    qk_tile<K, DP, N * QT, NM>(tile, fr, acc, g, p);
 #pragma unroll
-    for (int n = 1; n < N; ++n) {
-      f32x4 more[QT][NM];
-      qk_tile<K, DP, QT, NM>(tile, fr[n], more, g, p);
+    for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
-      for (int qt = 0; qt < QT; ++qt)
+      for (int m = 0; m < NM; ++m) {
+        s[qt][m] = acc[(N - 1) * QT + qt][m];
 #pragma unroll
-        for (int m = 0; m < NM; ++m) acc[qt][m] += more[qt][m];
-    }
+        for (int n = N - 2; n >= 0; --n) s[qt][m] += acc[n * QT + qt][m];
+      }
   }
+}
+// O += V^T P with P as N bf16 pieces, a fragment of V read once
+template <int DP, int KC, int N>
+__device__ __forceinline__ void pv_pieces(const char *tile, const float (&x)[KC / 16][4], SoftmaxState<DP> &sm, int g, int p) {
+  constexpr int CPR = DP / 8, K2 = KC / 32, NTL = DP / 16, VL = NTL < 8 ? NTL : 8, RPT = 2 * K2, W = NTL < 4 ? NTL : 4;
+  s16x8 pk[K2][N];
+#pragma unroll
+  for (int k2 = 0; k2 < K2; ++k2) split8<N>(&x[2 * k2][0], pk[k2]);
+  s16x4 lo[NTL][K2], hi[NTL][K2];
+  unsigned vb[VL];
+#pragma unroll
+  for (int l = 0; l < VL; ++l) vb[l] = (unsigned)(uintptr_t)tile + tile_vbase(l, g, p, CPR);
+  auto rd = [&](auto TT) {
+    constexpr int t = decltype(TT)::value;
+    static_for<K2>([&](auto KK) {
+      constexpr int k2 = decltype(KK)::value, off = (t / 8) * 256 + k2 * 512 * CPR;
+      lo[t][k2] = lds_read_tr16_at<off>(vb[t % 8]);
+      hi[t][k2] = lds_read_tr16_at<off + 256 * CPR>(vb[t % 8]);
+    });
+  };
+  static_for<W>(rd);
+  static_for<NTL>([&](auto TT) {
+    constexpr int t = decltype(TT)::value;
+    constexpr int last = t + W - 1 < NTL - 1 ? t + W - 1 : NTL - 1, n = (last - t) * RPT;
+    lds_wait_le<(n < 15 ? n : 15)>();
+#pragma unroll
+    for (int k2 = 0; k2 < K2; ++k2) {
+      lds_ready(lo[t][k2]);
+      lds_ready(hi[t][k2]);
+      const s16x4 a = lo[t][k2], b = hi[t][k2];
+      const s16x8 av = s16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+#pragma unroll
+      for (int i = N - 1; i >= 0; --i) sm.o[t] = Mfma16<bf16>::run(av, pk[k2][i], sm.o[t]);
+    }
+    if constexpr (t + W < NTL) rd(std::integral_constant<int, t + W>{});
+  });
 }
 
 template <typename T, int DP, int NW> struct Tile4 {
@@ -793,7 +833,8 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 256 ? 1 : 2) void 
   int c0, c1;
   share_of((int)(((uint32_t)keys + KC - 1) / KC), split, np, c0, c1);
 
-  RowFrag<K, DP> fr[N][QT];
+  static_assert(N == 1 || QT == 1, "pieces of one fragment");
+  RowFrag<K, DP> fr[N * QT];
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
@@ -801,7 +842,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 256 ? 1 : 2) void 
       s16x8 x[N];
       load_q8<T>(a, (const T *)a.q + ri[qt].b * a.sq[0] + ri[qt].hq * a.sq[1] + ri[qt].t * a.sq[2], 32 * ks + 8 * g, true, x);
 #pragma unroll
-      for (int n = 0; n < N; ++n) fr[n][qt].h[ks] = x[n];
+      for (int n = 0; n < N; ++n) fr[n * QT + qt].h[ks] = x[n];
     }
 
   // this thread's loads: half of keys, half of values, at the same rows and places
@@ -906,21 +947,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 256 ? 1 : 2) void 
     if constexpr (N == 1) {
       pv_tile<K, DP, KC, QT>(Vs, x, sm, g, p);
     } else {
-      // (pieces cut off one after the other; what a product takes rounded is exact)
-#pragma unroll
-      for (int n = 0; n < N; ++n) {
-        float y[QT][NM][4];
-#pragma unroll
-        for (int qt = 0; qt < QT; ++qt)
-#pragma unroll
-          for (int m = 0; m < NM; ++m)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              y[qt][m][r] = n + 1 < N ? __uint_as_float(__float_as_uint(x[qt][m][r]) & 0xffff0000u) : x[qt][m][r];
-              x[qt][m][r] -= y[qt][m][r];
-            }
-        pv_tile<K, DP, KC, QT>(Vs, y, sm, g, p);
-      }
+      pv_pieces<DP, KC, N>(Vs, x[0], sm[0], g, p);
     }
   }
 
@@ -1071,9 +1098,9 @@ static Plan4 plan4(const fbsa_attn4_desc *d) {
     const int64_t chunks = std::max<int64_t>(1, 256 / p.DP) * std::min<int64_t>(4, std::max<int64_t>(1, seqs / 64));
     p.joined = TG <= 16 && part4_waves(f32, (int)p.DP, p.sub, 1) == 2 && nc > 1 && nc <= kJoined4 * chunks;
   } else {
-    // As many as a CU's LDS holds (48 rows, d 128, 16 sequences: two to a CU 36.1 us, four
+    // As many as a CU holds (48 rows, d 128, 16 sequences: two to a CU 36.1 us, four
     // 41.0; d 64: 29.6 and 27.8), of 128 keys at least
-    const int64_t room = kCUs * (p.DP <= 64 ? 4 : p.DP == 128 ? 2 : 1);
+    const int64_t room = kCUs * (p.DP <= 64 ? (f32 ? 3 : 4) : p.DP == 128 ? 2 : 1);
     if (p.rt == 1) {
       const int64_t each = std::max<int64_t>(1, room / d->Hkv), nc = cdiv(d->S, 128);
       p.want = each * d->Hkv;
@@ -1197,7 +1224,7 @@ static int check_rows4(const char *fn, const fbsa_rows4_desc *d) {
   for (int x = 0; x < 3; ++x)
     if (d->sk[x] < 0 || d->sv[x] < 0 || d->sk[x] * es % 16 || d->sv[x] * es % 16)
       return fail(FBSA_EINVAL, "%s: strides of the rows must be non-negative multiples of 16 bytes", fn);
-  // (a launch has fewer than 2^32 threads along an axis: at least 16 rows to 256 here)
+  // (a launch has fewer than 2^32 threads along an axis: at least 8 rows to 256 here)
   if (d->B * d->H * d->T > 0x3ff0000LL) return fail(FBSA_EUNSUPPORTED, "%s: grid too large", fn);
   return FBSA_OK;
 }
@@ -1234,9 +1261,13 @@ static void fill_rows4(Rows4Args &a, const fbsa_rows4_desc *d) {
   a.ss[0] = d->ss[0]; a.ss[1] = d->ss[1];
   a.B = (int)d->B; a.H = (int)d->H; a.T = (int)d->T; a.S = (int)d->S; a.D = (int)d->D; a.ng = (int)cdiv(d->D, kGroup4);
 }
+// LPR: 8 elements a lane, to read as many as are 16 bytes
 template <typename T, int LPR> static int launch_rows4(const Rows4Args &a, bool read, hipStream_t s) {
-  const dim3 wgs((unsigned)cdiv(a.T, Rows4<T, LPR>::RPB * Rows4<T, LPR>::U), (unsigned)(a.B * a.H));
-  if (read) hipLaunchKernelGGL((cache4_read_kernel<T, LPR>), wgs, dim3(256), 0, s, a);
+  using A = Rows4<8, LPR>;
+  constexpr int LPR_READ = LPR * (int)sizeof(T) / 2;
+  using R = Rows4<16 / sizeof(T), LPR_READ>;
+  const dim3 wgs((unsigned)cdiv(a.T, read ? R::RPB * R::U : A::RPB * A::U), (unsigned)(a.B * a.H));
+  if (read) hipLaunchKernelGGL((cache4_read_kernel<T, LPR_READ>), wgs, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((cache4_append_kernel<T, LPR>), wgs, dim3(256), 0, s, a);
   return hip_check(hipGetLastError(), read ? "cache4_read_kernel launch" : "cache4_append_kernel launch");
 }
