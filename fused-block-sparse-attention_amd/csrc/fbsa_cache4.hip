@@ -254,8 +254,14 @@ struct Cache4Args {
   int2 *used;            // a sequence's first share and its number of them (want, several sequences)
 };
 
-template <int CTRL> __device__ __forceinline__ float dpp_f(float x, float old = 0.f) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, old), __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false));
+// An address that is the same on every lane, in scalar registers from here on: without the
+// empty statements the compiler keeps what it forms with 64-bit products in vector registers
+// and reads it back for each load (one token over 32 sequences, d 256: 28 us so, 45 without).
+__device__ __forceinline__ const char *uniform(const char *x) {
+  uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)((uintptr_t)x >> 32));
+  asm("" : "+s"(lo));
+  asm("" : "+s"(hi));
+  return (const char *)(uintptr_t)((uint64_t)hi << 32 | lo);
 }
 __device__ __forceinline__ int wave_sum(int x) {
   x += __builtin_amdgcn_update_dpp(0, x, 0xb1, 0xf, 0xf, false);   // lane ^ 1
@@ -288,8 +294,14 @@ __device__ __forceinline__ bool share4(const Cache4Args &c4, int i, int lane, in
     b = 0; split = i; np = a.np_own; before = 0;
     return i < np;
   }
-  int total = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) total += wave_sum(chunks4(a, b0 + lane));  // (B H of 65535 at most: below 2^31 up to 2^37 rows; plan4)
+  if (a.direct) {
+    b = i; split = 0; np = 1; before = i;
+    return i < a.B;
+  }
+  int total = 0;  // (below 2^31: check_attn4)
+#pragma unroll 4
+  for (int b0 = lane; b0 < a.B; b0 += 64) total += chunks4(a, b0);
+  total = wave_sum(total);
   const int most = c4.want / a.Hkv, each = max(c4.least, (total + most - 1) / most);
   before = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
@@ -366,6 +378,9 @@ template <typename T> __device__ __forceinline__ void load_q8(const CacheArgs &a
 template <int DP> struct Part4 {
   static constexpr int KC = 64, RB = DP / 2, CPR = RB / 16, NG = DP <= kGroup4 ? 1 : DP / kGroup4;
   static constexpr int TILE = KC * RB, STEPS = KC * 4 * NG, LDS = 2 * TILE + 2 * STEPS;
+  // Load i of a tile has rows RL i .. (six units to a row: no whole number of them), and
+  // of the units' places only so many are different: number i % KV of keys, i / VD of values
+  static constexpr int RL = 64 % CPR ? 0 : 64 / CPR, KV = CPR == 8 ? 2 : CPR == 6 ? 6 : 1, VD = CPR == 8 ? 2 : CPR <= 2 ? CPR : 1, VV = CPR / VD;
   __device__ static __forceinline__ int swk(int row) {
     return CPR == 1 ? 0 : CPR == 4 ? (row >> 2) & 3 : CPR == 8 ? (row >> 1) & 7 : (row >> 3) & 1;
   }
@@ -422,15 +437,16 @@ __global__ __launch_bounds__(64 * W, part4_waves(sizeof(T) == 4, DP, SUB, QT)) v
   const int wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   char *smem = smem_all + wave * C::LDS;
   const int lane = threadIdx.x & 63, g = lane >> 4, p = lane & 15, sub = p / ROWS;
-  const int hk = blockIdx.x;
+  const int hk = blockIdx.y;
   int b, split, np, before;
   if constexpr (W > 1) {
-    b = blockIdx.y; split = wave; np = W; before = 0;
+    b = blockIdx.x; split = wave; np = W;
   } else {
-    if (!share4(c4, blockIdx.y, lane, b, split, np, before)) return;
+    if (!share4(c4, blockIdx.x, lane, b, split, np, before)) return;
     if (split == 0 && hk == 0 && lane == 0 && !a.direct) c4.used[b] = int2{before, np};
   }
-  const int n = seq_len(a, b), count = seq_count(a, b), keys = count > 0 ? n : 0;
+  const int n = __builtin_amdgcn_readfirstlane(seq_len(a, b)), count = __builtin_amdgcn_readfirstlane(seq_count(a, b));
+  const int keys = count > 0 ? n : 0;
   int low = n - count + 1;  // below it every row sees every key
   low = low < 0 ? 0 : low;
   // rows: token, head, keys seen (a row that is none sees what the last one sees, so it asks for no masking)
@@ -451,38 +467,57 @@ __global__ __launch_bounds__(64 * W, part4_waves(sizeof(T) == 4, DP, SUB, QT)) v
   share_of((int)(((uint32_t)keys + KC - 1) / KC), split, np, c0, c1);
 
   const int64_t kstep = a.sk[2], vstep = a.sv[2];
-  const char *kb = (const char *)a.k + b * a.sk[0] + hk * a.sk[1], *vb = (const char *)a.v + b * a.sv[0] + hk * a.sv[1];
-  const char *sb = (const char *)(c4.step + b * c4.ss[0] + hk * c4.ss[1]);
-  uint32_t koff[C::CPR], voff[C::CPR];
+  // the next chunk to load
+  const char *knext = uniform((const char *)a.k + b * a.sk[0] + hk * a.sk[1] + (int64_t)c0 * KC * kstep);
+  const char *vnext = uniform((const char *)a.v + b * a.sv[0] + hk * a.sv[1] + (int64_t)c0 * KC * vstep);
+  const char *snext = uniform((const char *)(c4.step + b * c4.ss[0] + hk * c4.ss[1]) + (int64_t)c0 * C::STEPS);
+  uint32_t koff[C::KV], voff[C::VV];
+  {
+    const int last = a.D / 32 - 1;  // (columns past the head dim: the row's last unit; 64 strides of less than 2^26: check_held)
+    auto off = [&](int i, int row, int c, int64_t step) {
+      return (uint32_t)(C::RL ? row - C::RL * i : row) * (uint32_t)step + (c < last ? c : last) * 16;
+    };
 #pragma unroll
-  for (int i = 0; i < C::CPR; ++i) {
-    const int u = i * 64 + lane, row = u / C::CPR, c = u % C::CPR, last = a.D / 32 - 1;
-    const int ck = c ^ C::swk(row), cv = c ^ C::swv(row);  // (columns past the head dim: the row's last unit)
-    koff[i] = (uint32_t)row * (uint32_t)kstep + (ck < last ? ck : last) * 16;  // (64 strides of less than 2^26: check_held)
-    voff[i] = (uint32_t)row * (uint32_t)vstep + (cv < last ? cv : last) * 16;
+    for (int i = 0; i < C::KV; ++i) {
+      const int u = i * 64 + lane, row = u / C::CPR;
+      koff[i] = off(i, row, u % C::CPR ^ C::swk(row), kstep);
+    }
+#pragma unroll
+    for (int i = 0; i < C::VV; ++i) {
+      const int u = i * C::VD * 64 + lane, row = u / C::CPR;
+      voff[i] = off(i * C::VD, row, u % C::CPR ^ C::swv(row), vstep);
+    }
   }
-  auto issue_codes = [&](const char *src, int64_t step, const uint32_t (&off)[C::CPR], int left, char *dst) {
+  auto issue_codes = [&](const char *src, int64_t step, auto offset, int left, char *dst) {
     if (left >= KC) {
 #pragma unroll
-      for (int i = 0; i < C::CPR; ++i) g2lds16_s(src, off[i], dst + i * 1024);
+      for (int i = 0; i < C::CPR; ++i) g2lds16_s(src + i * C::RL * step, offset(i), dst + i * 1024);
     } else {  // (rows past the end: the end of the last one)
       const uint32_t lim0 = (uint32_t)(left - 1) * (uint32_t)step + (uint32_t)a.D / 2 - 16;
 #pragma unroll
-      for (int i = 0; i < C::CPR; ++i) g2lds16_s(src, off[i] > lim0 ? lim0 : off[i], dst + i * 1024);
+      for (int i = 0; i < C::CPR; ++i) {
+        const uint32_t o = offset(i) + (uint32_t)(i * C::RL) * (uint32_t)step;
+        g2lds16_s(src, o > lim0 ? lim0 : o, dst + i * 1024);
+      }
     }
   };
   auto issue_keys = [&](int c) {  // and steps
     const int left = keys - c * KC;  // (c is a chunk of the sequence: at least 1)
-    issue_codes(kb + (int64_t)c * KC * kstep, kstep, koff, left, smem);
+    issue_codes(knext, kstep, [&](int i) { return koff[i % C::KV]; }, left, smem);
     const uint32_t words = (uint32_t)min(KC, left) * NG;  // (rows past the end: the last step)
     char *sd = smem + 2 * C::TILE + (c & 1) * C::STEPS;
 #pragma unroll
     for (int i = 0; i < NG; ++i) {
       const uint32_t u = i * 64 + lane;
-      g2lds4_s(sb + (int64_t)c * KC * NG * 4, (u < words ? u : words - 1) * 4, sd + i * 256);
+      g2lds4_s(snext, (u < words ? u : words - 1) * 4, sd + i * 256);
     }
+    knext += KC * kstep;
+    snext += C::STEPS;
   };
-  auto issue_values = [&](int c) { issue_codes(vb + (int64_t)c * KC * vstep, vstep, voff, keys - c * KC, smem + C::TILE); };
+  auto issue_values = [&](int c) {
+    issue_codes(vnext, vstep, [&](int i) { return voff[i / C::VD]; }, keys - c * KC, smem + C::TILE);
+    vnext += KC * vstep;
+  };
   if (c0 < c1) {
     issue_keys(c0);
     issue_values(c0);
@@ -712,7 +747,7 @@ __global__ __launch_bounds__(64 * W, part4_waves(sizeof(T) == 4, DP, SUB, QT)) v
       if (g == 0 && a.lse) a.lse[((int64_t)b * a.Hq + head[qt]) * a.T + tok[qt]] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
       continue;
     }
-    const int64_t at = ((int64_t)hk * gridDim.y + blockIdx.y) * a.TG + rho;
+    const int64_t at = ((int64_t)hk * gridDim.x + blockIdx.x) * a.TG + rho;
     if (g == 0) a.stat[at] = float2{m, lt};
     if (valid[qt] && lt != 0.f) {  // (a NaN sum is kept)
       float *dst = a.part + at * PITCH;
@@ -783,7 +818,8 @@ __device__ __forceinline__ void pv_pieces(const char *tile, const float (&x)[KC 
 
 template <typename T, int DP, int NW> struct Tile4 {
   using K = typename Pieces<T>::K;
-  static constexpr int KC = 64, NT = NW * 64, CPR = DP / 8, TILE = KC * DP * 2, STAGE = 2 * TILE, LDS = 2 * STAGE;
+  static constexpr int KC = 64, NT = NW * 64, CPR = DP / 8, TILE = KC * DP * 2, STAGE = 2 * TILE;
+  static constexpr int STAGES = DP >= 128 && NW == 4 && sizeof(T) == 2 ? 1 : 2, LDS = STAGES * STAGE;
   static constexpr int BYTES = KC * DP / NT, LB = BYTES / 2 < 16 ? BYTES / 2 : 16, NL = BYTES / LB;  // codes of a thread: NL loads of LB bytes, half of keys
   static constexpr int UPR = DP / 2 / LB;                                                    // loads of a row
   static_assert(LDS <= 160 * 1024, "LDS");
@@ -924,16 +960,25 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 256 ? 1 : 2) void 
   for (int qt = 0; qt < QT; ++qt) sm[qt].init();
   if (c0 < c1) {
     load(c0);
-    store(0);
-    if (c0 + 1 < c1) load(c0 + 1);
+    if constexpr (C::STAGES == 2) {
+      store(0);
+      if (c0 + 1 < c1) load(c0 + 1);
+    }
   }
   int stage = 0;
   for (int c = c0; c < c1; ++c) {
-    lds_barrier();  // chunk c is written, and every wave has read chunk c - 1, whose place is filled next
+    if constexpr (C::STAGES == 2) {
+      lds_barrier();  // chunk c is written, and every wave has read chunk c - 1, whose place is filled next
+      if (c + 1 < c1) store(stage ^ 1);
+      if (c + 2 < c1) load(c + 2);
+    } else {
+      if (c > c0) lds_barrier();  // every wave has read chunk c - 1
+      store(0);
+      lds_barrier();
+      if (c + 1 < c1) load(c + 1);
+    }
     const char *Ks = smem + stage * C::STAGE, *Vs = Ks + C::TILE;
-    stage ^= 1;
-    if (c + 1 < c1) store(stage);
-    if (c + 2 < c1) load(c + 2);
+    if constexpr (C::STAGES == 2) stage ^= 1;
     if (w * QT * 16 >= tr) continue;
     f32x4 s[QT][NM];
     qk_pieces<K, DP, QT, NM, N>(Ks, fr, s, g, p);
@@ -1088,7 +1133,8 @@ static Plan4 plan4(const fbsa_attn4_desc *d) {
     // against 29.9). Sequences round theirs up.
     const int64_t each = std::max<int64_t>(1, kCUs * (p.qt > 1 || p.DP >= 192 ? 4 : 8) / d->Hkv), nc = cdiv(d->S, 64);
     p.want = each * d->Hkv;
-    p.np = d->B == 1 ? std::min(each, nc) : std::min(each + d->B, nc * d->B);
+    // (so many sequences that the card goes through them several times need no shares)
+    p.np = d->B == 1 ? std::min(each, nc) : seqs >= 4 * p.want ? d->B : std::min(each + d->B, nc * d->B);
     p.rows = d->Hkv * p.np * TG;
     // (kernels of one wave to a SIMD have no such form)
     // One launch against two, where the waves have few chunks each, or the card many
@@ -1100,7 +1146,7 @@ static Plan4 plan4(const fbsa_attn4_desc *d) {
   } else {
     // As many as a CU holds (48 rows, d 128, 16 sequences: two to a CU 36.1 us, four
     // 41.0; d 64: 29.6 and 27.8), of 128 keys at least
-    const int64_t room = kCUs * (p.DP <= 64 ? (f32 ? 3 : 4) : p.DP == 128 ? 2 : 1);
+    const int64_t room = kCUs * (p.DP <= 64 ? (f32 ? 3 : 4) : p.DP == 128 ? (f32 || p.tr > 64 ? 2 : 3) : f32 || p.tr > 64 ? 1 : 2);
     if (p.rt == 1) {
       const int64_t each = std::max<int64_t>(1, room / d->Hkv), nc = cdiv(d->S, 128);
       p.want = each * d->Hkv;
@@ -1126,7 +1172,7 @@ template <typename T, int DP, int SUB, int QT, int W> static int launch_part4(co
   static_assert(lds <= 160 * 1024, "LDS");
   const int e = lds_optin((const void *)cache4_part_kernel<T, DP, SUB, QT, W>, lds, "hipFuncSetAttribute(cache4_part)");
   if (e) return e;
-  hipLaunchKernelGGL((cache4_part_kernel<T, DP, SUB, QT, W>), dim3((unsigned)c.a.Hkv, (unsigned)(W > 1 ? c.a.B : pl.np)), dim3(64 * W), lds, s, c);
+  hipLaunchKernelGGL((cache4_part_kernel<T, DP, SUB, QT, W>), dim3((unsigned)(W > 1 ? c.a.B : pl.np), (unsigned)c.a.Hkv), dim3(64 * W), lds, s, c);
   return hip_check(hipGetLastError(), "cache4_part_kernel launch");
 }
 template <typename T, int DP, int SUB> static int launch_few4(const Cache4Args &c, const Plan4 &pl, hipStream_t s) {
@@ -1249,9 +1295,10 @@ static int check_attn4(const fbsa_attn4_desc *d) {
   for (int x = 0; x < 3; ++x)
     if (d->sq[x] < 0 || d->so[x] < 0 || d->sq[x] * es % 16 || d->so[x] * es % 16)
       return fail(FBSA_EINVAL, "%s: strides of q and o must be non-negative multiples of 16 bytes", fn);
-  // (fewer than 2^32 threads: up to 512 a tile and share, 64 or 256 a row that is joined)
+  if (d->B * cdiv(d->S, 64) > lim) return fail(FBSA_EUNSUPPORTED, "%s: more than 2^31 chunks of 64 rows in all", fn);
+  // (fewer than 2^32 threads along an axis: up to 512 a tile and share, 64 or 256 a row that is joined)
   const Plan4 pl = plan4(d);
-  if (pl.rows > lim || d->B * d->Hq * d->T > 0x3ff0000LL || (pl.qt ? pl.np > 65535 : (pl.want ? 1 : d->B * pl.rt) * d->Hkv * pl.np > 0x7f0000LL))
+  if (pl.rows > lim || d->B * d->Hq * d->T > 0x3ff0000LL || (!pl.qt && (pl.want ? 1 : d->B * pl.rt) * d->Hkv * pl.np > 0x7f0000LL))
     return fail(FBSA_EUNSUPPORTED, "%s: grid too large", fn);
   return FBSA_OK;
 }

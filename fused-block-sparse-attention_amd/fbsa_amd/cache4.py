@@ -210,7 +210,8 @@ def cache_attention(q, k4, v4, step, lens=None, *, count=None, scale=None, out_g
     _aligned(what, pk | pv)
     lens = torch.full(p.shape[:1], p.S, dtype=torch.int32, device=p.device) if lens is None else _int32(lens)
     count = _int32(count)
-    ws = torch.empty(p.nbytes, dtype=torch.uint8, device=p.device)
+    # (256 bytes: the call joins no parts and touches no workspace, so any address does)
+    ws = o if p.nbytes == 256 else torch.empty(p.nbytes, dtype=torch.uint8, device=p.device)
     _launch(p, _lib.load().fbsa_cache4_attn, what, q.data_ptr(), pk, pv, step.data_ptr(), lens.data_ptr(), _ptr(count), _ptr(out_gate),
             o.data_ptr(), _ptr(lse), ws.data_ptr(), p.nbytes)
     return (o, lse) if need_lse else o

@@ -75,11 +75,17 @@ def check_attend(got, held, q, lens, count=None, scale=None, gate=None):
     (at most 1, the row's sum at least 1) may lose 2^-126 there, its product with the step
     the same twice (steps here are above 2^-4, so at most 2^-122 of v), and each piece of
     that as much, three of them: less than 2^-120 of sum |v| in all. Added to the `a`
-    of the bounds, which counts 2 * 2^-20 of it or more, as 2^-101 of sum |v|."""
+    of the bounds, which counts 2 * 2^-20 of it or more, as 2^-101 of sum |v|.
+    fp16 results below 2^-14 are multiples of 2^-24, off by up to 2^-25 whatever their size:
+    the bounds have that for an element but not for the L2 error, whose square it makes
+    2^-50 / 3 larger for each element. They take h^2 / 3 = 2^-22 / 3 of sum p^2 v^2, to
+    which 2^-28 is added. (6144 such results: sqrt(6144 / 3) 2^-25 = 1.35e-6.)"""
     k, v = values(held)
     r = tight.attend(q, k, v, lens, count, None, None, scale, gate, None)
     D = q.shape[-1]
     r["big"] *= (D + 17) / (D + 4)
     r["a"] = r["a"] + 2.0 ** -101 * r["v1"]
+    if q.dtype == torch.float16:
+        r["a2"] = r["a2"] + 2.0 ** -28
     rounded = q.shape[2] * (q.shape[1] // k.shape[1]) > 16
     tight.check((*got, None), r, q, k.shape[2], rounded and q.dtype != torch.float32, gate is not None)

@@ -216,6 +216,52 @@ def test_many_shares(dt, Hq, Hkv, T, S, D):
     _attend(dt, 2, Hq, Hkv, T, S, D, [S, S // 3], gated=True)
 
 
+@pytest.mark.parametrize("dt,B,Hq,Hkv,T,S,D", [("bf16", 70, 2, 2, 1, 900, 64), ("fp16", 150, 4, 1, 2, 700, 32), ("fp32", 65, 1, 1, 1, 6000, 64),
+                                               ("bf16", 200, 8, 1, 3, 300, 128), ("fp16", 67, 16, 1, 4, 400, 64), ("bf16", 1100, 8, 8, 1, 90, 32),
+                                               ("bf16", 8300, 1, 1, 1, 66, 32)])
+def test_many_sequences(dt, B, Hq, Hkv, T, S, D):
+    """More sequences than a wave has lanes, of all lengths, some without new tokens."""
+    lens = [(37 * b * b) % (S + 1) for b in range(B)]
+    count = [(b * 7) % (T + 1) if b % 3 == 0 else T for b in range(B)]
+    _attend(dt, B, Hq, Hkv, T, S, D, lens, count, seed=B)
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("Hq,T", [(1, 1), (8, 1), (16, 1), (8, 3), (8, 12), (8, 30)])
+def test_small_and_large_rows(dt, Hq, T):
+    """Steps near the ends of what a type holds (fp16: subnormal values)."""
+    g, t = _gen(T), DT[dt]
+    held = _held(g, t, 1, 1, 200, 64)
+    # (32-bit pieces are exact down to 2^-126, 24 bits below a probability times a step)
+    small, big = (2.0 ** -23, 512.0) if t == torch.float16 else (2.0 ** -60, 2.0 ** 100)
+    q = _randn(g, 1, Hq, T, 64, dtype=t)
+    for size in (small, big):
+        step = held[2].clone()
+        step[:, :, :, 1] = (step[:, :, :, 1].float() * 32).round().to(step.dtype) * size   # (of few bits: exact)
+        got = cache4.cache_attention(q, held[0], held[1], step, _ints([190]), need_lse=True)
+        ref.check_attend(got, (held[0], held[1], step), q, [190])
+
+
+def test_rows_beyond_4_gib():
+    """Codes of more than 2^32 bytes: rows behind them are written, read and attended."""
+    S, D = (1 << 26) + 1000, 128
+    held = cache4.empty(1, 1, S, D)
+    g = _gen(0)
+    k, v = (_randn(g, 1, 1, 5, D, dtype=torch.bfloat16) for _ in range(2))
+    k[0, 0, 4] = 4.0
+    for at in (S - 5, S - 1003):
+        cache4.append(*held, k, v, _ints([at]))
+        want = ref.held(k, v)
+        assert all(torch.equal(x.cpu().double(), y) for x, y in zip(cache4.read(*held, _ints([at]), 5), want))
+    # (the others' keys are zeros: a query along the last row's key has all its weight there)
+    q = torch.full((1, 1, 1, D), 2.0, dtype=torch.bfloat16, device=DEV)
+    o = cache4.cache_attention(q, *held, _ints([S]))
+    both = want[1][0, 0, 4]   # two such rows, of the same value
+    assert (o[0, 0, 0].cpu().double() - both).abs().max() <= 2.0 ** -8 * both.abs().max() + 1e-6
+    many = cache4.cache_attention(q.expand(1, 1, 40, D).contiguous(), *held, _ints([S]))
+    assert (many[0, 0, -1].cpu().double() - both).abs().max() <= 2.0 ** -7 * both.abs().max() + 1e-6
+
+
 @pytest.mark.parametrize("dt", list(DT))
 @pytest.mark.parametrize("Hq,T", [(1, 1), (8, 1), (2, 12)])
 def test_heavy_keys(dt, Hq, T):
