@@ -279,10 +279,6 @@ __device__ __forceinline__ void pv_tile(const char *tile, const float (&x)[QT][K
   }
 }
 
-// Adds up the parts of a call's rows in a fixed order (fbsa_cache.hip): a.part's rows
-// hold dp floats, dp one of 32, 64, 128, 256.
-int launch_cache_join(const CacheArgs &a, int dtype, int64_t dp, hipStream_t s);
-
 static inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 static inline size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 

@@ -1081,17 +1081,6 @@ template <typename T, int DP> static int launch_join(const CacheArgs &a, hipStre
     hipLaunchKernelGGL((cache_combine_kernel<T, DP, false>), dim3((unsigned)rows), dim3(256), 0, s, a);
   return hip_check(hipGetLastError(), "cache_combine_kernel launch");
 }
-template <typename T> static int join_of(const CacheArgs &a, int64_t dp, hipStream_t s) {
-  switch (dp) {
-    case 32: return launch_join<T, 32>(a, s);
-    case 64: return launch_join<T, 64>(a, s);
-    case 128: return launch_join<T, 128>(a, s);
-    default: return launch_join<T, 256>(a, s);
-  }
-}
-int launch_cache_join(const CacheArgs &a, int dtype, int64_t dp, hipStream_t s) {
-  return dtype == FBSA_BF16 ? join_of<bf16>(a, dp, s) : dtype == FBSA_F16 ? join_of<f16>(a, dp, s) : join_of<float>(a, dp, s);
-}
 
 template <typename T, int DP> static int launch_cache(const CacheArgs &a, int64_t nz, hipStream_t s) {
   using C = CacheCfg<T, DP>;

@@ -10,8 +10,8 @@
 // So rows are read back without rounding, products of values are the matrix cores' own,
 // and attention over the cache is attention over the rows read back.
 //
-// Attention: rows, tiles and shares as in the cache of 16 and 32 bits (fbsa_cache.hip),
-// whose join adds up the parts.
+// Attention: rows and tiles as in the cache of 16 and 32 bits (fbsa_cache.hip); the shares
+// of the keys are formed on the device from the sequences' lengths.
 #include <algorithm>
 
 #include "fbsa_cache.h"
@@ -249,9 +249,8 @@ struct Cache4Args {
   const uint16_t *step;
   int64_t ss[2];
   int32_t ng;            // steps of a key or value row
-  int32_t want;          // one tile a (sequence, KV head): shares that the call's chunks are cut into; 0: several tiles
-  int32_t least;         // chunks of a share
-  int2 *used;            // a sequence's first share and its number of them (want, several sequences)
+  int32_t want;          // shares that a KV head's chunks are cut into
+  int2 *used;            // a tile's first share and its number of them (several tiles to a KV head)
 };
 
 // An address that is the same on every lane, in scalar registers from here on: without the
@@ -263,13 +262,15 @@ __device__ __forceinline__ const char *uniform(const char *x) {
   asm("" : "+s"(hi));
   return (const char *)(uintptr_t)((uint64_t)hi << 32 | lo);
 }
-__device__ __forceinline__ int wave_sum(int x) {
-  x += __builtin_amdgcn_update_dpp(0, x, 0xb1, 0xf, 0xf, false);   // lane ^ 1
-  x += __builtin_amdgcn_update_dpp(0, x, 0x4e, 0xf, 0xf, false);   // lane ^ 2
-  x += __builtin_amdgcn_update_dpp(0, x, 0x141, 0xf, 0xf, false);  // 7 - lane of eight
-  x += __builtin_amdgcn_update_dpp(0, x, 0x140, 0xf, 0xf, false);  // 15 - lane of sixteen
+template <typename N> __device__ __forceinline__ N wave_sum(N x) {
+  auto with = [&](auto CTRL) { x += __builtin_bit_cast(N, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(CTRL)::value, 0xf, 0xf, false)); };
+  with(std::integral_constant<int, 0xb1>{});   // lane ^ 1
+  with(std::integral_constant<int, 0x4e>{});   // lane ^ 2
+  with(std::integral_constant<int, 0x141>{});  // 7 - lane of eight
+  with(std::integral_constant<int, 0x140>{});  // 15 - lane of sixteen
   x += __shfl_xor(x, 16, 64);
-  return x + __shfl_xor(x, 32, 64);
+  x += __shfl_xor(x, 32, 64);
+  return __builtin_bit_cast(N, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
 }
 // sums of lanes 0 .. lane
 __device__ __forceinline__ int wave_scan(int x) {
@@ -280,37 +281,62 @@ __device__ __forceinline__ int wave_scan(int x) {
   x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // the last of sixteen to the next sixteen
   return x + __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
 }
-// Share i of the sequences' chunks, which are cut into pieces of about the same number
-// (want of them over all KV heads, and one more for each sequence at most): sequence,
-// piece and number of pieces of it. The lengths are on the device, so every wave counts
-// (pieces by the capacity leave the longest sequence's to end last: 16 sequences of 1000
-// to 16301 rows). False: there is none.
-__device__ __forceinline__ int chunks4(const CacheArgs &a, int b) {
-  return b < a.B && seq_count(a, b) > 0 ? (int)(((uint32_t)seq_len(a, b) + 63u) / 64u) : 0;
+// Share i of a KV head's chunks, which are cut into pieces of about the same number: tile
+// (numbered from the one that sees the most keys on, the sequences of a place side by
+// side), piece, number of pieces and of the tile's first one. The lengths are on the
+// device, so every wave counts (the same number of pieces for each leaves the longest
+// sequence's to end last: 3 sequences of 2000 to 30000 rows, 200 tokens, 2 heads over 1, d
+// 256: 58.7 us against 43.7; 4 of 1000 to 16000, 128 tokens, 16 over 2, d 128: 78 against
+// 72). False: there is none.
+__device__ __forceinline__ int chunks4(const CacheArgs &a, int u) {
+  if (u >= a.B * a.rt_own) return 0;
+  const int tile = a.rt_own - 1 - u / a.B, b = a.rt_own == 1 ? u : u % a.B;
+  const int n = seq_len(a, b), c = seq_count(a, b);
+  if (a.rt_own == 1) return c > 0 ? (int)(((uint32_t)n + 63u) / 64u) : 0;
+  const int real = min(tile * a.tr_own + a.tr_own, c * a.G);
+  if (tile * a.tr_own >= real) return 0;
+  const int64_t keys = (int64_t)n - c + (real - 1) / a.G + 1;  // (own_bounds)
+  return keys < 0 ? 0 : (int)((keys + 63) / 64);
 }
-__device__ __forceinline__ bool share4(const Cache4Args &c4, int i, int lane, int &b, int &split, int &np, int &before) {
+// FIT: in `want` pieces at most, which run at a time, of LEAST chunks or more; otherwise
+// each tile may round its own up.
+template <bool FIT, int LEAST> __device__ __forceinline__ bool share4(const Cache4Args &c4, int i, int lane, int &u, int &split, int &np, int &before) {
   const CacheArgs &a = c4.a;
-  if (a.B == 1) {
-    b = 0; split = i; np = a.np_own; before = 0;
+  const int units = a.B * a.rt_own;
+  if (units == 1) {
+    u = 0; split = i; np = a.np_own; before = 0;
     return i < np;
   }
   if (a.direct) {
-    b = i; split = 0; np = 1; before = i;
-    return i < a.B;
+    u = i; split = 0; np = 1; before = i;
+    return i < units;
   }
-  int total = 0;  // (below 2^31: check_attn4)
+  const int one = chunks4(a, lane);  // (of most calls, all there are)
+  auto chunks = [&](int u0) { return u0 ? chunks4(a, u0 + lane) : one; };
+  int each;
+  if constexpr (FIT) {
+    float total = 0.f;  // (near enough, as is half a piece a tile for the rounding: the count below tells)
+    for (int u0 = 0; u0 < units; u0 += 64) total += (float)chunks(u0);
+    each = max(LEAST, (int)(wave_sum(total) / ((float)c4.want - 0.5f * (float)units)));
+    for (;; each += 1 + each / 16) {  // (ends: one piece a tile is no more than `want`)
+      int pieces = 0;
+      for (int u0 = 0; u0 < units; u0 += 64) pieces += u0 + lane < units ? max(1, (chunks(u0) + each - 1) / each) : 0;
+      if (wave_sum(pieces) <= c4.want) break;
+    }
+  } else {
+    int total = 0;  // (below 2^31: check_attn4)
 #pragma unroll 4
-  for (int b0 = lane; b0 < a.B; b0 += 64) total += chunks4(a, b0);
-  total = wave_sum(total);
-  const int most = c4.want / a.Hkv, each = max(c4.least, (total + most - 1) / most);
+    for (int u0 = 0; u0 < units; u0 += 64) total += chunks(u0);
+    each = max(LEAST, (wave_sum(total) + c4.want - 1) / c4.want);
+  }
   before = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int mine = b0 + lane < a.B ? max(1, (chunks4(a, b0 + lane) + each - 1) / each) : 0;
+  for (int u0 = 0; u0 < units; u0 += 64) {
+    const int mine = u0 + lane < units ? max(1, (chunks(u0) + each - 1) / each) : 0;
     const int upto = wave_scan(mine);
     const uint64_t past = __ballot(before + upto > i);
     if (past) {
       const int l = __builtin_ctzll(past);
-      b = b0 + l;
+      u = u0 + l;
       np = __builtin_amdgcn_readlane(mine, l);
       before += __builtin_amdgcn_readlane(upto, l) - np;
       split = i - before;
@@ -437,12 +463,13 @@ __global__ __launch_bounds__(64 * W, part4_waves(sizeof(T) == 4, DP, SUB, QT)) v
   const int wave = W == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   char *smem = smem_all + wave * C::LDS;
   const int lane = threadIdx.x & 63, g = lane >> 4, p = lane & 15, sub = p / ROWS;
-  const int hk = blockIdx.y;
+  // (a share's heads side by side: 32 sequences, 16 heads over 2, d 256: 29.4 us against 32.6)
+  const int share = (int)(blockIdx.x / (uint32_t)a.Hkv), hk = (int)(blockIdx.x - (uint32_t)share * a.Hkv);
   int b, split, np, before;
   if constexpr (W > 1) {
-    b = blockIdx.x; split = wave; np = W;
+    b = share; split = wave; np = W;
   } else {
-    if (!share4(c4, blockIdx.x, lane, b, split, np, before)) return;
+    if (!share4<false, 1>(c4, share, lane, b, split, np, before)) return;
     if (split == 0 && hk == 0 && lane == 0 && !a.direct) c4.used[b] = int2{before, np};
   }
   const int n = __builtin_amdgcn_readfirstlane(seq_len(a, b)), count = __builtin_amdgcn_readfirstlane(seq_count(a, b));
@@ -747,7 +774,7 @@ __global__ __launch_bounds__(64 * W, part4_waves(sizeof(T) == 4, DP, SUB, QT)) v
       if (g == 0 && a.lse) a.lse[((int64_t)b * a.Hq + head[qt]) * a.T + tok[qt]] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
       continue;
     }
-    const int64_t at = ((int64_t)hk * gridDim.x + blockIdx.x) * a.TG + rho;
+    const int64_t at = ((int64_t)hk * a.np_own + share) * a.TG + rho;
     if (g == 0) a.stat[at] = float2{m, lt};
     if (valid[qt] && lt != 0.f) {  // (a NaN sum is kept)
       float *dst = a.part + at * PITCH;
@@ -834,24 +861,12 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 256 ? 1 : 2) void 
   const CacheArgs &a = c4.a;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, p = lane & 15;
   const int tr = a.tr_own;
-  // (the last tokens' tiles see the most keys: they start first)
-  int b, hk, tile = 0, split, np = a.np_own;
-  int64_t slot;
-  if (c4.want) {
-    const int i = (int)(blockIdx.x / (uint32_t)a.Hkv);
-    int before;
-    hk = (int)(blockIdx.x - (uint32_t)i * a.Hkv);
-    if (!share4(c4, i, lane, b, split, np, before)) return;
-    if (split == 0 && hk == 0 && tid == 0 && !a.direct) c4.used[b] = int2{before, np};
-    slot = ((int64_t)hk * a.np_own + i) * tr;
-  } else {
-    const uint32_t per = (uint32_t)(a.Hkv * a.B), u0 = blockIdx.x % per, u1 = blockIdx.x / per;
-    hk = u0 % a.Hkv;
-    b = u0 / a.Hkv;
-    tile = a.rt_own - 1 - (int)(u1 % a.rt_own);
-    split = (int)(u1 / a.rt_own);
-    slot = ((((int64_t)b * a.Hkv + hk) * a.rt_own + tile) * np + split) * tr;
-  }
+  const int i = (int)(blockIdx.x / (uint32_t)a.Hkv), hk = (int)(blockIdx.x - (uint32_t)i * a.Hkv);
+  int u, split, np, before;
+  if (!share4<true, 2>(c4, i, lane, u, split, np, before)) return;
+  if (split == 0 && hk == 0 && tid == 0 && !a.direct) c4.used[u] = int2{before, np};
+  const int tile = a.rt_own - 1 - u / a.B, b = u % a.B;
+  const int64_t slot = ((int64_t)hk * a.np_own + i) * tr;
   RowInfo ri[QT];
 #pragma unroll
   for (int qt = 0; qt < QT; ++qt) {
@@ -1021,7 +1036,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 256 ? 1 : 2) void 
 // A row's parts added up: 8 threads to a part's 32 columns (a block has CW columns of a
 // row), so NG parts at a time, each thread with a running maximum of its own parts; then
 // across the threads in a fixed order.
-template <typename T, int TEAM, int CW> __global__ __launch_bounds__(256) void cache4_join_kernel(Cache4Args c4, int pitch, int shares) {
+template <typename T, int TEAM, int CW> __global__ __launch_bounds__(256) void cache4_join_kernel(Cache4Args c4, int pitch) {
   constexpr int LG = CW / 4, NG = TEAM / LG, U = 4;
   __shared__ f32x4 s_acc[256];
   __shared__ float2 s_ml[256];
@@ -1034,16 +1049,10 @@ template <typename T, int TEAM, int CW> __global__ __launch_bounds__(256) void c
   const RowInfo ri = row_info(a, b, hk, rho);
   const int col = blockIdx.y * CW + 4 * e;
   // part i of the row: first + i * tr_own
-  int64_t first;
-  int n = a.np_own;
-  if (c4.want) {
-    const int2 u = a.B > 1 ? c4.used[b] : int2{0, n};
-    first = ((int64_t)hk * shares + u.x) * a.tr_own + rho;
-    n = u.y;
-  } else {
-    const int tile = rho / a.tr_own;
-    first = ((int64_t)seq * a.rt_own + tile) * n * a.tr_own + (rho - tile * a.tr_own);
-  }
+  const int tile = rho / a.tr_own;
+  const int2 u = a.B * a.rt_own > 1 ? c4.used[(a.rt_own - 1 - tile) * a.B + b] : int2{0, a.np_own};
+  const int64_t first = ((int64_t)hk * a.np_own + u.x) * a.tr_own + (rho - tile * a.tr_own);
+  int n = u.y;
   if (!ri.valid) n = 0;
   float m = -INFINITY, l = 0.f;
   f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1124,7 +1133,6 @@ static Plan4 plan4(const fbsa_attn4_desc *d) {
   p.qt = few ? (int)cdiv(TG, 16) : 0;
   p.tr = few ? TG : tile_rows(d->dtype, TG);
   p.rt = cdiv(TG, p.tr);
-  const int64_t tiles = seqs * p.rt;
   p.joined = false;
   if (few) {
     // Shares of the chunks: as many as run at a time with two waves to a SIMD, or one
@@ -1132,9 +1140,9 @@ static Plan4 plan4(const fbsa_attn4_desc *d) {
     // 28.9 us against 30.3; one of 131072 rows 27.8 against 31.4; d 64, 262144 rows: 40.0
     // against 29.9). Sequences round theirs up.
     const int64_t each = std::max<int64_t>(1, kCUs * (p.qt > 1 || p.DP >= 192 ? 4 : 8) / d->Hkv), nc = cdiv(d->S, 64);
-    p.want = each * d->Hkv;
+    p.want = each;
     // (so many sequences that the card goes through them several times need no shares)
-    p.np = d->B == 1 ? std::min(each, nc) : seqs >= 4 * p.want ? d->B : std::min(each + d->B, nc * d->B);
+    p.np = d->B == 1 ? std::min(each, nc) : d->B >= 4 * each ? d->B : std::min(each + d->B, nc * d->B);
     p.rows = d->Hkv * p.np * TG;
     // (kernels of one wave to a SIMD have no such form)
     // One launch against two, where the waves have few chunks each, or the card many
@@ -1147,21 +1155,16 @@ static Plan4 plan4(const fbsa_attn4_desc *d) {
     // As many as a CU holds (48 rows, d 128, 16 sequences: two to a CU 36.1 us, four
     // 41.0; d 64: 29.6 and 27.8), of 128 keys at least
     const int64_t room = kCUs * (p.DP <= 64 ? (f32 ? 3 : 4) : p.DP == 128 ? (f32 || p.tr > 64 ? 2 : 3) : f32 || p.tr > 64 ? 1 : 2);
-    if (p.rt == 1) {
-      const int64_t each = std::max<int64_t>(1, room / d->Hkv), nc = cdiv(d->S, 128);
-      p.want = each * d->Hkv;
-      p.np = d->B == 1 ? std::min(each, nc) : std::min(each + d->B, nc * d->B);
-      p.rows = d->Hkv * p.np * p.tr;
-    } else {
-      p.want = 0;
-      p.np = std::max<int64_t>(1, std::min({room / tiles, cdiv(d->S, 128), (int64_t)256}));
-      p.rows = tiles * p.np * p.tr;
-    }
+    // Many tiles have one share each, several to a sequence as soon as they are half of that.
+    const int64_t each = std::max<int64_t>(1, room / d->Hkv), units = d->B * p.rt, nc = cdiv(d->S, 128);
+    p.want = 2 * units <= each || units == 1 ? each : each + units;
+    p.np = units >= 4 * each || (p.rt > 1 && 2 * units > each) ? units : std::min(p.want, nc * units);
+    p.rows = d->Hkv * p.np * p.tr;
   }
-  p.direct = p.joined || p.np == (p.want ? d->B : 1);
+  p.direct = p.joined || p.np == d->B * p.rt;
   const size_t parts = p.direct ? 0 : (size_t)p.rows;
   p.used = up256(parts * 8);
-  p.part = p.used + (p.direct || !p.want ? 0 : up256((size_t)d->B * 8));
+  p.part = p.used + (p.direct ? 0 : up256((size_t)(d->B * p.rt) * 8));
   p.total = p.part + up256(parts * p.pitch * 4);
   if (p.total == 0) p.total = 256;  // (0 says that a descriptor is refused)
   return p;
@@ -1172,7 +1175,7 @@ template <typename T, int DP, int SUB, int QT, int W> static int launch_part4(co
   static_assert(lds <= 160 * 1024, "LDS");
   const int e = lds_optin((const void *)cache4_part_kernel<T, DP, SUB, QT, W>, lds, "hipFuncSetAttribute(cache4_part)");
   if (e) return e;
-  hipLaunchKernelGGL((cache4_part_kernel<T, DP, SUB, QT, W>), dim3((unsigned)(W > 1 ? c.a.B : pl.np), (unsigned)c.a.Hkv), dim3(64 * W), lds, s, c);
+  hipLaunchKernelGGL((cache4_part_kernel<T, DP, SUB, QT, W>), dim3((unsigned)((W > 1 ? c.a.B : pl.np) * c.a.Hkv)), dim3(64 * W), lds, s, c);
   return hip_check(hipGetLastError(), "cache4_part_kernel launch");
 }
 template <typename T, int DP, int SUB> static int launch_few4(const Cache4Args &c, const Plan4 &pl, hipStream_t s) {
@@ -1183,17 +1186,17 @@ template <typename T, int DP, int SUB> static int launch_few4(const Cache4Args &
 }
 template <typename T> static int launch_join4(const Cache4Args &c, const Plan4 &pl, hipStream_t s) {
   const int64_t rows = (int64_t)c.a.B * c.a.Hkv * c.a.TG;
-  const int pitch = (int)pl.pitch, np = (int)pl.np;
+  const int pitch = (int)pl.pitch;
   // many rows: a wave each (of up to 128 columns); few: a workgroup for 128 or 32 columns
   if (rows >= 2048) {
     const unsigned wgs = (unsigned)cdiv(rows, 4);
-    if (pitch == 32) hipLaunchKernelGGL((cache4_join_kernel<T, 64, 32>), dim3(wgs), dim3(256), 0, s, c, pitch, np);
-    else if (pitch == 64) hipLaunchKernelGGL((cache4_join_kernel<T, 64, 64>), dim3(wgs), dim3(256), 0, s, c, pitch, np);
-    else hipLaunchKernelGGL((cache4_join_kernel<T, 64, 128>), dim3(wgs, (unsigned)(pitch / 128)), dim3(256), 0, s, c, pitch, np);
+    if (pitch == 32) hipLaunchKernelGGL((cache4_join_kernel<T, 64, 32>), dim3(wgs), dim3(256), 0, s, c, pitch);
+    else if (pitch == 64) hipLaunchKernelGGL((cache4_join_kernel<T, 64, 64>), dim3(wgs), dim3(256), 0, s, c, pitch);
+    else hipLaunchKernelGGL((cache4_join_kernel<T, 64, 128>), dim3(wgs, (unsigned)(pitch / 128)), dim3(256), 0, s, c, pitch);
   } else if (pitch >= 128 && rows * pitch >= 32 * 4 * kCUs) {
-    hipLaunchKernelGGL((cache4_join_kernel<T, 256, 128>), dim3((unsigned)rows, (unsigned)(pitch / 128)), dim3(256), 0, s, c, pitch, np);
+    hipLaunchKernelGGL((cache4_join_kernel<T, 256, 128>), dim3((unsigned)rows, (unsigned)(pitch / 128)), dim3(256), 0, s, c, pitch);
   } else {
-    hipLaunchKernelGGL((cache4_join_kernel<T, 256, 32>), dim3((unsigned)rows, (unsigned)cdiv(c.a.D, 32)), dim3(256), 0, s, c, pitch, np);
+    hipLaunchKernelGGL((cache4_join_kernel<T, 256, 32>), dim3((unsigned)rows, (unsigned)cdiv(c.a.D, 32)), dim3(256), 0, s, c, pitch);
   }
   return hip_check(hipGetLastError(), "cache4_join_kernel launch");
 }
@@ -1205,7 +1208,7 @@ template <typename T, int DP, int NW, int QT> static int launch_tile4(const Cach
   return hip_check(hipGetLastError(), "cache4_tile_kernel launch");
 }
 template <typename T, int DP> static int launch_attn4(const Cache4Args &c, const Plan4 &pl, hipStream_t s) {
-  const int64_t wgs = (pl.want ? 1 : (int64_t)c.a.B * pl.rt) * c.a.Hkv * pl.np;
+  const int64_t wgs = c.a.Hkv * pl.np;
   constexpr int MOST = most_sub4(sizeof(T) == 4, DP);
   if constexpr (MOST >= 4) {
     if (pl.sub == 4) return launch_few4<T, DP, 4>(c, pl, s);
@@ -1298,7 +1301,7 @@ static int check_attn4(const fbsa_attn4_desc *d) {
   if (d->B * cdiv(d->S, 64) > lim) return fail(FBSA_EUNSUPPORTED, "%s: more than 2^31 chunks of 64 rows in all", fn);
   // (fewer than 2^32 threads along an axis: up to 512 a tile and share, 64 or 256 a row that is joined)
   const Plan4 pl = plan4(d);
-  if (pl.rows > lim || d->B * d->Hq * d->T > 0x3ff0000LL || (!pl.qt && (pl.want ? 1 : d->B * pl.rt) * d->Hkv * pl.np > 0x7f0000LL))
+  if (pl.rows > lim || d->B * d->Hq * d->T > 0x3ff0000LL || (!pl.qt && d->Hkv * pl.np > 0x7f0000LL))
     return fail(FBSA_EUNSUPPORTED, "%s: grid too large", fn);
   return FBSA_OK;
 }
@@ -1391,7 +1394,6 @@ int fbsa_cache4_attn(const fbsa_attn4_desc *d, const void *q, const void *k4, co
   a.tr_own = (int)pl.tr; a.tr_pre = 16; a.rt_own = (int)pl.rt; a.np_own = (int)pl.np;
   a.direct = pl.direct;
   c.want = (int)pl.want;
-  c.least = pl.qt ? 1 : 2;
   c.used = (int2 *)((char *)workspace + pl.used);
   a.scale2 = d->scale == 0.f ? 1.f : fabsf(d->scale) * kLog2e;
   a.qand = d->scale == 0.f ? 0u : 0xffffffffu;
