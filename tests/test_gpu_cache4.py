@@ -226,6 +226,17 @@ def test_many_sequences(dt, B, Hq, Hkv, T, S, D):
     _attend(dt, B, Hq, Hkv, T, S, D, lens, count, seed=B)
 
 
+@pytest.mark.parametrize("dt,B,Hq,Hkv,T,S,D", [("bf16", 2, 8, 1, 900, 5000, 64), ("fp32", 2, 8, 1, 700, 3000, 32), ("fp16", 3, 4, 1, 500, 9000, 128),
+                                               ("bf16", 3, 2, 1, 300, 4000, 256), ("fp32", 3, 2, 2, 200, 2500, 160), ("bf16", 100, 8, 1, 5, 1500, 256),
+                                               ("fp16", 200, 8, 1, 6, 700, 192), ("bf16", 1100, 8, 1, 4, 200, 256)])
+def test_many_tiles(dt, B, Hq, Hkv, T, S, D):
+    """Tiles of many rows, more of them than a wave has lanes or than the card runs, whose
+    sequences differ in length and whose last tiles may be padding."""
+    lens = [S, 40, (S * 2) // 3][:B] + [(53 * b * b) % (S + 1) for b in range(3, B)]
+    count = [T, T // 3, T - 1][:B] + [(b * 5) % (T + 1) for b in range(3, B)]
+    _attend(dt, B, Hq, Hkv, T, S, D, lens, count, seed=T)
+
+
 @pytest.mark.parametrize("dt", list(DT))
 @pytest.mark.parametrize("Hq,T", [(1, 1), (8, 1), (16, 1), (8, 3), (8, 12), (8, 30)])
 def test_small_and_large_rows(dt, Hq, T):
