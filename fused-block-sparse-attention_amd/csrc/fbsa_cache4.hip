@@ -262,6 +262,19 @@ __device__ __forceinline__ const char *uniform(const char *x) {
   asm("" : "+s"(hi));
   return (const char *)(uintptr_t)((uint64_t)hi << 32 | lo);
 }
+// 4 bytes a lane to LDS, as g2lds16_s its 16 (the asm has m0 as a register it writes)
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void g2lds4_s(const void *sbase, unsigned voff, void *lds_wave_base) {
+  const unsigned m = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)lds_wave_base);
+  const uint64_t bp = (uint64_t)(uintptr_t)sbase;
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((unsigned)(bp >> 32));
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((unsigned)bp);
+  const uint64_t sb = ((uint64_t)hi << 32) | (uint64_t)lo;
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" : : "v"(voff), "s"(sb), "s"(m) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
 template <typename N> __device__ __forceinline__ N wave_sum(N x) {
   auto with = [&](auto CTRL) { x += __builtin_bit_cast(N, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), decltype(CTRL)::value, 0xf, 0xf, false)); };
   with(std::integral_constant<int, 0xb1>{});   // lane ^ 1

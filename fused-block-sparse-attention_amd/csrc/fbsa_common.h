@@ -95,14 +95,6 @@ __device__ __forceinline__ void g2lds4(const void *gsrc, void *lds_wave_base) {
   const unsigned m = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)lds_wave_base);
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" : : "v"(gsrc), "s"(m) : "memory", "m0");
 }
-__device__ __forceinline__ void g2lds4_s(const void *sbase, unsigned voff, void *lds_wave_base) {
-  const unsigned m = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)lds_wave_base);
-  const uint64_t bp = (uint64_t)(uintptr_t)sbase;
-  const uint32_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((unsigned)(bp >> 32));
-  const uint32_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((unsigned)bp);
-  const uint64_t sb = ((uint64_t)hi << 32) | (uint64_t)lo;
-  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" : : "v"(voff), "s"(sb), "s"(m) : "memory", "m0");
-}
 #pragma clang diagnostic pop
 
 // s_waitcnt with only the vector-memory counter constrained (gfx9 encoding:

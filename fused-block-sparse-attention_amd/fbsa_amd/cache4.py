@@ -108,10 +108,10 @@ def append(k4, v4, step, k_new, v_new, start, *, count=None):
     p = _plan("cache4.append", _plan_rows, (k_new.shape[2], k_new.dtype), (k4, v4, step, k_new, v_new, start, count))
     if p.empty:
         return
-    if (k_new.data_ptr() | v_new.data_ptr()) & 15 or not (p.ok[0] and p.ok[1]):
+    at = (k4.data_ptr(), v4.data_ptr(), step.data_ptr(), k_new.data_ptr(), v_new.data_ptr())
+    if (at[3] | at[4]) & 15 or not (p.ok[0] and p.ok[1]):
         k_new, v_new = (t.clone(memory_format=torch.contiguous_format) for t in (k_new, v_new))
         return append(k4, v4, step, k_new, v_new, start, count=count)
-    at = tuple(t.data_ptr() for t in (k4, v4, step, k_new, v_new))
     _aligned("cache4.append", at[0] | at[1])
     spans = tuple(zip(at, p.bytes))
     _apart("cache4.append", spans[:3], spans[3:])
@@ -137,10 +137,10 @@ def read(k4, v4, step, first, rows, *, count=None, dtype=None, out=None):
         raise ValueError("fbsa.cache4.read: out must be (k, v)")
     p = _plan("cache4.read", _plan_rows, (rows, dtype), (k4, v4, step, k, v, first, count))
     if k is None:
-        k, v = (torch.empty(p.shape, dtype=dtype, device=p.device) for _ in range(2))
+        k, v = torch.empty(p.shape, dtype=dtype, device=p.device), torch.empty(p.shape, dtype=dtype, device=p.device)
     if p.empty:
         return (k.zero_(), v.zero_())
-    at = tuple(t.data_ptr() for t in (k4, v4, step, k, v))
+    at = (k4.data_ptr(), v4.data_ptr(), step.data_ptr(), k.data_ptr(), v.data_ptr())
     _aligned("cache4.read", at[0] | at[1] | at[3] | at[4])
     if out is not None:
         spans = tuple(zip(at, p.bytes))
