@@ -311,8 +311,11 @@ __device__ __forceinline__ int chunks4(const CacheArgs &a, int u) {
   const int64_t keys = (int64_t)n - c + (real - 1) / a.G + 1;  // (own_bounds)
   return keys < 0 ? 0 : (int)((keys + 63) / 64);
 }
-// FIT: in `want` pieces at most, which run at a time, of LEAST chunks or more; otherwise
-// each tile may round its own up.
+// FIT: pieces of LEAST chunks or more, in `want` of them, which run at a time. Where there
+// are more tiles than half of that, what is a quarter longer than a place's share of the
+// chunks is cut, the others stay whole (16 sequences, 512 tokens, 8 heads over 1, d 128: one
+// of 30000 rows and 15 of 1000 211 us against 1205 uncut, all of 4000 210 against 184).
+// Otherwise each tile may round its own up.
 template <bool FIT, int LEAST> __device__ __forceinline__ bool share4(const Cache4Args &c4, int i, int lane, int &u, int &split, int &np, int &before) {
   const CacheArgs &a = c4.a;
   const int units = a.B * a.rt_own;
@@ -330,11 +333,13 @@ template <bool FIT, int LEAST> __device__ __forceinline__ bool share4(const Cach
   if constexpr (FIT) {
     float total = 0.f;  // (near enough, as is half a piece a tile for the rounding: the count below tells)
     for (int u0 = 0; u0 < units; u0 += 64) total += (float)chunks(u0);
-    each = max(LEAST, (int)(wave_sum(total) / ((float)c4.want - 0.5f * (float)units)));
-    for (;; each += 1 + each / 16) {  // (ends: one piece a tile is no more than `want`)
+    const bool fit = 2 * units <= c4.want;
+    const int most = fit ? c4.want : c4.want + units;
+    each = max(LEAST, (int)(wave_sum(total) / (fit ? (float)c4.want - 0.5f * (float)units : 0.8f * (float)c4.want)));
+    for (;; each += 1 + each / 16) {  // (ends: one piece a tile is no more than `most`)
       int pieces = 0;
       for (int u0 = 0; u0 < units; u0 += 64) pieces += u0 + lane < units ? max(1, (chunks(u0) + each - 1) / each) : 0;
-      if (wave_sum(pieces) <= c4.want) break;
+      if (wave_sum(pieces) <= most) break;
     }
   } else {
     int total = 0;  // (below 2^31: check_attn4)
@@ -453,6 +458,8 @@ template <typename T, int NG> struct Steps4 {
 // SUB-th of the chunk and zero outside the lanes that hold its keys, so a product has the
 // scores of 16 SUB keys and no lane holds one twice: a SUB-th of the exponentials and
 // splits. For the value product the first part's columns take the others' probabilities.
+// One token over 262144 rows, 8 heads, d 64: 25 us, 5.7 TB/s; 32 sequences, 16 heads over
+// 2, d 256: 23 us, 3.4 TB/s, one wave's chain from load to product.
 // W > 1: a workgroup's waves share a sequence's chunks and join their parts in LDS, where
 // that spares short caches the second launch.
 // QT > 1: that many 16-row tiles, for which the codes are made numbers once; 16-bit P is
@@ -778,7 +785,7 @@ __global__ __launch_bounds__(64 * W, part4_waves(sizeof(T) == 4, DP, SUB, QT)) v
     }
     const int rho = qt * 16 + p;
     if (rho >= a.TG) continue;
-    if (a.direct) {
+    if (a.direct || np == 1) {
       RowInfo ri;
       ri.b = b; ri.t = tok[qt]; ri.hq = head[qt];
       const float l = valid[qt] ? lt : 0.f, inv = l == 0.f ? 0.f : 1.f / l;
@@ -798,8 +805,9 @@ __global__ __launch_bounds__(64 * W, part4_waves(sizeof(T) == 4, DP, SUB, QT)) v
 }
 
 // Many rows: a workgroup per (tile of NW x 16 QT rows, share of the keys). Its threads
-// make 16-bit numbers of the codes, steps and all (exact), into two stages of LDS, and
-// from there it is the tile of a 16-bit cache. 32-bit rows are three bf16 pieces of
+// make 16-bit numbers of the codes, steps and all (exact), in LDS, and from there it is
+// the tile of a 16-bit cache. 2048 tokens over 16301 rows, 16 heads over 2, d 256: 541 us,
+// 0.98 PFLOP/s, matrix units 39% busy, LDS 49%, vector issue 51%, eight waves in step. 32-bit rows are three bf16 pieces of
 // queries and of probabilities: six products of the matrix units' fastest type cost less
 // than two of the slow 32-bit one.
 template <typename K, int DP, int QT, int NM, int N>
@@ -859,6 +867,8 @@ __device__ __forceinline__ void pv_pieces(const char *tile, const float (&x)[KC 
 template <typename T, int DP, int NW> struct Tile4 {
   using K = typename Pieces<T>::K;
   static constexpr int KC = 64, NT = NW * 64, CPR = DP / 8, TILE = KC * DP * 2, STAGE = 2 * TILE;
+  // One stage where two leave a CU fewer workgroups of four waves, which hide each other's
+  // barriers (16 sequences of 2000 to 16384 rows, 64 rows a head, d 256: 87 us with two, 50 with one)
   static constexpr int STAGES = DP >= 128 && NW == 4 && sizeof(T) == 2 ? 1 : 2, LDS = STAGES * STAGE;
   static constexpr int BYTES = KC * DP / NT, LB = BYTES / 2 < 16 ? BYTES / 2 : 16, NL = BYTES / LB;  // codes of a thread: NL loads of LB bytes, half of keys
   static constexpr int UPR = DP / 2 / LB;                                                    // loads of a row
@@ -1029,7 +1039,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 256 ? 1 : 2) void 
     const int i = (w * QT + qt) * 16 + p;
     if (i >= tr) continue;
     const float lt = sm[qt].total();
-    if (a.direct) {
+    if (a.direct || np == 1) {
       if (tile * tr + i >= a.TG) continue;
       const float l = ri[qt].valid ? lt : 0.f, inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
@@ -1066,6 +1076,7 @@ template <typename T, int TEAM, int CW> __global__ __launch_bounds__(256) void c
   const int2 u = a.B * a.rt_own > 1 ? c4.used[(a.rt_own - 1 - tile) * a.B + b] : int2{0, a.np_own};
   const int64_t first = ((int64_t)hk * a.np_own + u.x) * a.tr_own + (rho - tile * a.tr_own);
   int n = u.y;
+  if (n == 1) return;  // (written by the one that had it all)
   if (!ri.valid) n = 0;
   float m = -INFINITY, l = 0.f;
   f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1154,8 +1165,11 @@ static Plan4 plan4(const fbsa_attn4_desc *d) {
     // against 29.9). Sequences round theirs up.
     const int64_t each = std::max<int64_t>(1, kCUs * (p.qt > 1 || p.DP >= 192 ? 4 : 8) / d->Hkv), nc = cdiv(d->S, 64);
     p.want = each;
-    // (so many sequences that the card goes through them several times need no shares)
-    p.np = d->B == 1 ? std::min(each, nc) : d->B >= 4 * each ? d->B : std::min(each + d->B, nc * d->B);
+    // One share a sequence where the card goes through them several times and a wave with
+    // the longest is soon done beside the counting that shares take (30000 sequences of up
+    // to 130 rows, 24 heads over 1: 107 us against 3702; 1024 of up to 1024, 8 heads, fp32 d
+    // 256: 351 against 426; but 1099 of 64 rows and one of 16384, 8 heads, d 64: 213 against 47)
+    p.np = d->B == 1 ? std::min(each, nc) : d->B >= std::max(4 * each, 8 * nc) ? d->B : std::min(each + d->B, nc * d->B);
     p.rows = d->Hkv * p.np * TG;
     // (kernels of one wave to a SIMD have no such form)
     // One launch against two, where the waves have few chunks each, or the card many
@@ -1168,10 +1182,11 @@ static Plan4 plan4(const fbsa_attn4_desc *d) {
     // As many as a CU holds (48 rows, d 128, 16 sequences: two to a CU 36.1 us, four
     // 41.0; d 64: 29.6 and 27.8), of 128 keys at least
     const int64_t room = kCUs * (p.DP <= 64 ? (f32 ? 3 : 4) : p.DP == 128 ? (f32 || p.tr > 64 ? 2 : 3) : f32 || p.tr > 64 ? 1 : 2);
-    // Many tiles have one share each, several to a sequence as soon as they are half of that.
+    // One share a tile where the card goes through them several times (see above), and for
+    // one sequence's tiles, which see about the same, as soon as they are half of that.
     const int64_t each = std::max<int64_t>(1, room / d->Hkv), units = d->B * p.rt, nc = cdiv(d->S, 128);
-    p.want = 2 * units <= each || units == 1 ? each : each + units;
-    p.np = units >= 4 * each || (p.rt > 1 && 2 * units > each) ? units : std::min(p.want, nc * units);
+    p.want = each;
+    p.np = units >= std::max(4 * each, 16 * nc) || (d->B == 1 && p.rt > 1 && 2 * units > each) ? units : std::min(2 * units <= each || units == 1 ? each : each + units, nc * units);
     p.rows = d->Hkv * p.np * p.tr;
   }
   p.direct = p.joined || p.np == d->B * p.rt;

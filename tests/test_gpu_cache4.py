@@ -237,6 +237,16 @@ def test_many_tiles(dt, B, Hq, Hkv, T, S, D):
     _attend(dt, B, Hq, Hkv, T, S, D, lens, count, seed=T)
 
 
+@pytest.mark.parametrize("dt,B,Hq,Hkv,T,S,D", [("bf16", 16, 8, 1, 300, 9000, 128), ("fp16", 5, 8, 1, 450, 6000, 256), ("fp32", 40, 4, 2, 300, 3000, 32),
+                                               ("bf16", 3, 16, 4, 520, 5000, 64), ("fp32", 9, 2, 1, 900, 2500, 224)])
+def test_one_long_sequence(dt, B, Hq, Hkv, T, S, D):
+    """Tiles in several pieces beside tiles in one, and tiles that see nothing."""
+    lens = [(29 * b) % 200 for b in range(B)]
+    count = [T if b % 4 else T // 2 for b in range(B)]
+    lens[1], count[1] = S, T
+    _attend(dt, B, Hq, Hkv, T, S, D, lens, count, seed=B, gated=dt != "fp32")
+
+
 @pytest.mark.parametrize("dt", list(DT))
 @pytest.mark.parametrize("Hq,T", [(1, 1), (8, 1), (16, 1), (8, 3), (8, 12), (8, 30)])
 def test_small_and_large_rows(dt, Hq, T):
