@@ -247,6 +247,15 @@ def test_one_long_sequence(dt, B, Hq, Hkv, T, S, D):
     _attend(dt, B, Hq, Hkv, T, S, D, lens, count, seed=B, gated=dt != "fp32")
 
 
+@pytest.mark.parametrize("dt,B,H,T,S,D", [("bf16", 40, 256, 20, 600, 32), ("fp16", 18, 256, 40, 300, 32), ("fp32", 20, 256, 4, 250, 160)])
+def test_one_long_sequence_of_more_than_run_at_a_time(dt, B, H, T, S, D):
+    """So many heads that the card goes through the sequences several times, which are cut all the same."""
+    lens = [(29 * b) % 100 for b in range(B)]
+    count = [T if b % 4 else T // 2 for b in range(B)]
+    lens[1], count[1] = S, T
+    _attend(dt, B, H, H, T, S, D, lens, count, seed=B)
+
+
 @pytest.mark.parametrize("dt", list(DT))
 @pytest.mark.parametrize("Hq,T", [(1, 1), (8, 1), (16, 1), (8, 3), (8, 12), (8, 30)])
 def test_small_and_large_rows(dt, Hq, T):
