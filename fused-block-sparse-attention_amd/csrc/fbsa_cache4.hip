@@ -374,8 +374,10 @@ template <typename T> struct Pieces {
 template <> struct Pieces<f16> { using K = f16; static constexpr int Q = 1, P = 2; };
 template <> struct Pieces<float> { using K = bf16; static constexpr int Q = 3, P = 3; };
 
-// x as N bf16 numbers, each what the ones before leave (the last rounded, the others cut)
-template <int N> __device__ __forceinline__ void split8(const float *x, s16x8 *out) {
+// x as N bf16 numbers, each what the ones before leave (the last rounded, the others cut).
+// INF: numbers that may be infinite, which leave nothing (inf - inf is NaN, and made
+// queries NaN whose every score is -inf)
+template <int N, bool INF = false> __device__ __forceinline__ void split8(const float *x, s16x8 *out) {
   float r[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) r[e] = x[e];
@@ -386,8 +388,9 @@ template <int N> __device__ __forceinline__ void split8(const float *x, s16x8 *o
     for (int j = 0; j < 4; ++j) {
       const uint32_t a = __float_as_uint(r[2 * j]), b = __float_as_uint(r[2 * j + 1]);
       hw[j] = __builtin_amdgcn_perm(b, a, 0x07060302u);
-      r[2 * j] -= __uint_as_float(a & 0xffff0000u);
-      r[2 * j + 1] -= __uint_as_float(b & 0xffff0000u);
+      const bool ia = INF && fabsf(r[2 * j]) == INFINITY, ib = INF && fabsf(r[2 * j + 1]) == INFINITY;
+      r[2 * j] = ia ? 0.f : r[2 * j] - __uint_as_float(a & 0xffff0000u);
+      r[2 * j + 1] = ib ? 0.f : r[2 * j + 1] - __uint_as_float(b & 0xffff0000u);
     }
     out[n] = __builtin_bit_cast(s16x8, hw);
   }
@@ -409,7 +412,7 @@ template <typename T> __device__ __forceinline__ void load_q8(const CacheArgs &a
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(w[e / 4][e % 4]);
-    split8<3>(x, out);
+    split8<3, true>(x, out);
   } else {
     out[0] = __builtin_bit_cast(s16x8, w[0]);
   }
