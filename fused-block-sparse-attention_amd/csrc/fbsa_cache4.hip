@@ -397,7 +397,8 @@ template <int N, bool INF = false> __device__ __forceinline__ void split8(const 
   out[N - 1] = pack8<bf16>(r);
 }
 // elements d .. d + 7 of a query row (zeros past the head dim, or where `in` says), the scale's sign applied
-template <typename T> __device__ __forceinline__ void load_q8(const CacheArgs &a, const T *row, int d, bool in, s16x8 *out) {
+// and of 32-bit ones the largest magnitude so far
+template <typename T, bool INF> __device__ __forceinline__ void load_q8(const CacheArgs &a, const T *row, int d, bool in, s16x8 *out, float &top) {
   u32x4 w[sizeof(T) / 2];
 #pragma unroll
   for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
@@ -412,9 +413,20 @@ template <typename T> __device__ __forceinline__ void load_q8(const CacheArgs &a
     float x[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(w[e / 4][e % 4]);
-    split8<3, true>(x, out);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+    split8<3, INF>(x, out);
   } else {
     out[0] = __builtin_bit_cast(s16x8, w[0]);
+  }
+}
+// A wave's queries by `load`; 32-bit ones among which one is infinite a second time, with
+// its pieces looked at (each looked at from the start costs short caches 12% of a call)
+template <typename T, typename F> __device__ __forceinline__ void load_queries(F load) {
+  float top = 0.f;
+  load(std::false_type{}, top);
+  if constexpr (sizeof(T) == 4) {
+    if (__ballot(top == INFINITY)) load(std::true_type{}, top);
   }
 }
 
@@ -574,13 +586,15 @@ __global__ __launch_bounds__(64 * W, part4_waves(sizeof(T) == 4, DP, SUB, QT)) v
   }
 
   s16x8 fr[QT][NF][NQ];
+  load_queries<T>([&](auto INF, float &top) {
 #pragma unroll
-  for (int qt = 0; qt < QT; ++qt)
+    for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
-    for (int f = 0; f < NF; ++f) {
-      // product f of the group's FG: elements 8 f .. of this lane's, a LPS-th of the group
-      load_q8<T>(a, qrow[qt], (DP == 32 ? 0 : 64 * (f / FG)) + (g % LPS) * 8 * FG + 8 * (f % FG), SUB == 1 || g / LPS == sub, fr[qt][f]);
-    }
+      for (int f = 0; f < NF; ++f) {
+        // product f of the group's FG: elements 8 f .. of this lane's, a LPS-th of the group
+        load_q8<T, decltype(INF)::value>(a, qrow[qt], (DP == 32 ? 0 : 64 * (f / FG)) + (g % LPS) * 8 * FG + 8 * (f % FG), SUB == 1 || g / LPS == sub, fr[qt][f], top);
+      }
+  });
   // this lane's scores: keys 16 (sub NM + m) + 4 g + r; the row that it reads of 16-row tile m
   const int key0 = 16 * sub * NM + 4 * g, krow = 16 * (g / LPS) * NM + p, kswz = C::swk(p);
   const int vrow = 16 * (p >> 2) + 4 * g + (p & 3), vswz = C::swv(vrow);
@@ -912,15 +926,17 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 256 ? 1 : 2) void 
 
   static_assert(N == 1 || QT == 1, "pieces of one fragment");
   RowFrag<K, DP> fr[N * QT];
+  load_queries<T>([&](auto INF, float &top) {
 #pragma unroll
-  for (int qt = 0; qt < QT; ++qt)
+    for (int qt = 0; qt < QT; ++qt)
 #pragma unroll
-    for (int ks = 0; ks < DP / 32; ++ks) {
-      s16x8 x[N];
-      load_q8<T>(a, (const T *)a.q + ri[qt].b * a.sq[0] + ri[qt].hq * a.sq[1] + ri[qt].t * a.sq[2], 32 * ks + 8 * g, true, x);
+      for (int ks = 0; ks < DP / 32; ++ks) {
+        s16x8 x[N];
+        load_q8<T, decltype(INF)::value>(a, (const T *)a.q + ri[qt].b * a.sq[0] + ri[qt].hq * a.sq[1] + ri[qt].t * a.sq[2], 32 * ks + 8 * g, true, x, top);
 #pragma unroll
-      for (int n = 0; n < N; ++n) fr[n * QT + qt].h[ks] = x[n];
-    }
+        for (int n = 0; n < N; ++n) fr[n * QT + qt].h[ks] = x[n];
+      }
+  });
 
   // this thread's loads: half of keys, half of values, at the same rows and places
   constexpr int NH = C::NL / 2;
