@@ -106,8 +106,7 @@ template <int DP> struct SoftmaxState {
     for (int t = 0; t < DP / 16; ++t) o[t] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   // s: raw products (scaled by scale2 > 0 here), masked ones -inf; out: exponentials.
-  // ROWS < 16: a row's scores are in lane columns ROWS apart too, and share its reference
-  template <int NM, int ROWS = 16> __device__ __forceinline__ void step(const f32x4 (&s)[NM], float scale2, float (&x)[NM][4]) {
+  template <int NM> __device__ __forceinline__ void step(const f32x4 (&s)[NM], float scale2, float (&x)[NM][4]) {
     float mx = -INFINITY;
 #pragma unroll
     for (int k = 0; k < NM; ++k) mx = fmaxf(mx, fmaxf(fmaxf(s[k][0], s[k][1]), fmaxf(s[k][2], s[k][3])));
@@ -115,8 +114,6 @@ template <int DP> struct SoftmaxState {
     if (__ballot(mx > m + TAU)) {
       float mc = fmaxf(mx, shfl_xor_f(mx, 16));
       mc = fmaxf(mc, shfl_xor_f(mc, 32));
-#pragma unroll
-      for (int y = ROWS; y < 16; y <<= 1) mc = fmaxf(mc, shfl_xor_f(mc, y));
       if (mc > m + TAU) {
         const float alpha = __builtin_amdgcn_exp2f(m - mc);
         l *= alpha;

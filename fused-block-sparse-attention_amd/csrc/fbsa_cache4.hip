@@ -365,6 +365,54 @@ template <bool FIT, int LEAST> __device__ __forceinline__ bool share4(const Cach
   return false;
 }
 
+// ---- softmax -----------------------------------------------------------------
+// SoftmaxState's step for scores of any size. The largest of a row is a rounded product
+// with the scale, and the product within an fma is not: from 2^27 on the two are 8 and
+// more apart, which is more than exponentials in fp16 have room for, and from 2^31 on more
+// than 32-bit ones do (all of a row were 0 or infinite). There neighbouring scores are 8
+// apart or more, too, and no softmax tells what their sums' roundings hide; so such a row's
+// scale is the next power of two, whose products are exact: its largest is the reference.
+constexpr float kFar4 = 0x1p27f;
+__device__ __forceinline__ float far_scale(float scale2) { return __uint_as_float((__float_as_uint(scale2) + 0x7fffffu) & 0xff800000u); }
+// ROWS < 16: a row's scores are in lane columns ROWS apart too, and share its reference.
+// scale: the row's, scale2 at first
+template <int NM, int ROWS, int DP> __device__ __forceinline__ void softmax4(SoftmaxState<DP> &sm, float &scale, const f32x4 (&s)[NM], float scale2, float (&x)[NM][4]) {
+  constexpr float TAU = SoftmaxState<DP>::TAU;
+  float mx = -INFINITY;
+#pragma unroll
+  for (int k = 0; k < NM; ++k) mx = fmaxf(mx, fmaxf(fmaxf(s[k][0], s[k][1]), fmaxf(s[k][2], s[k][3])));
+  if (__ballot(mx * scale - sm.m > TAU)) {
+    float mc = fmaxf(mx, shfl_xor_f(mx, 16));
+    mc = fmaxf(mc, shfl_xor_f(mc, 32));
+#pragma unroll
+    for (int y = ROWS; y < 16; y <<= 1) mc = fmaxf(mc, shfl_xor_f(mc, y));
+    if (mc * scale - sm.m > TAU) {
+      scale = fabsf(mc * scale2) >= kFar4 ? far_scale(scale2) : scale2;
+      mc *= scale;
+      const float alpha = __builtin_amdgcn_exp2f(sm.m - mc);
+      sm.l *= alpha;
+#pragma unroll
+      for (int t = 0; t < DP / 16; ++t) sm.o[t] *= alpha;
+      sm.m = mc;
+    }
+  }
+  const float ref = sm.m == -INFINITY ? 0.f : sm.m;
+  float sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < NM; ++k)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      x[k][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[k][r], scale, -ref));
+      sum += x[k][r];
+    }
+  sm.l += sum;
+}
+// a row's normaliser in natural logarithms, of its reference and sum
+__device__ __forceinline__ float lse4(float scale2, float m, float l) {
+  if (fabsf(m) >= kFar4) m *= scale2 / far_scale(scale2);
+  return l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
+}
+
 // Queries and probabilities enter the products as sums of 16-bit numbers: a 32-bit number
 // is three bf16 exactly (8 bits each).
 template <typename T> struct Pieces {
@@ -600,8 +648,12 @@ __global__ __launch_bounds__(64 * W, part4_waves(sizeof(T) == 4, DP, SUB, QT)) v
   const int vrow = 16 * (p >> 2) + 4 * g + (p & 3), vswz = C::swv(vrow);
 
   SoftmaxState<DP> sm[QT];
+  float scale[QT];
 #pragma unroll
-  for (int qt = 0; qt < QT; ++qt) sm[qt].init();
+  for (int qt = 0; qt < QT; ++qt) {
+    sm[qt].init();
+    scale[qt] = a.scale2;
+  }
   for (int c = c0; c < c1; ++c) {
     wait_vmcnt<C::CPR>();  // keys and steps are here, the values may be under way
     lds_wait_all();
@@ -671,7 +723,7 @@ __global__ __launch_bounds__(64 * W, part4_waves(sizeof(T) == 4, DP, SUB, QT)) v
     }
     float x[QT][NM][4];
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt) sm[qt].template step<NM, ROWS>(s[qt], a.scale2, x[qt]);
+    for (int qt = 0; qt < QT; ++qt) softmax4<NM, ROWS>(sm[qt], scale[qt], s[qt], a.scale2, x[qt]);
 
     if (more) wait_vmcnt<C::CPR + NG>();
     else wait_vmcnt<0>();
@@ -787,7 +839,7 @@ __global__ __launch_bounds__(64 * W, part4_waves(sizeof(T) == 4, DP, SUB, QT)) v
       ri.hq = hk * a.G + row - ri.t * a.G;
       if (ri.t >= count) l = 0.f;
       store_row<T>(a, ri, acc, l == 0.f ? 0.f : 1.f / l, d);
-      if (d == 0 && a.lse) a.lse[((int64_t)b * a.Hq + ri.hq) * a.T + ri.t] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
+      if (d == 0 && a.lse) a.lse[((int64_t)b * a.Hq + ri.hq) * a.T + ri.t] = lse4(a.scale2, m, l);
     }
     return;
   }
@@ -808,7 +860,7 @@ __global__ __launch_bounds__(64 * W, part4_waves(sizeof(T) == 4, DP, SUB, QT)) v
       const float l = valid[qt] ? lt : 0.f, inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
       for (int t = 0; t < NT; ++t) store_row<T>(a, ri, sm[qt].o[t], inv, 16 * t + 4 * g);
-      if (g == 0 && a.lse) a.lse[((int64_t)b * a.Hq + head[qt]) * a.T + tok[qt]] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
+      if (g == 0 && a.lse) a.lse[((int64_t)b * a.Hq + head[qt]) * a.T + tok[qt]] = lse4(a.scale2, m, l);
       continue;
     }
     const int64_t at = ((int64_t)hk * a.np_own + share) * a.TG + rho;
@@ -1013,8 +1065,12 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 256 ? 1 : 2) void 
   };
 
   SoftmaxState<DP> sm[QT];
+  float scale[QT];
 #pragma unroll
-  for (int qt = 0; qt < QT; ++qt) sm[qt].init();
+  for (int qt = 0; qt < QT; ++qt) {
+    sm[qt].init();
+    scale[qt] = a.scale2;
+  }
   if (c0 < c1) {
     load(c0);
     if constexpr (C::STAGES == 2) {
@@ -1045,7 +1101,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 256 ? 1 : 2) void 
     }
     float x[QT][NM][4];
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt) sm[qt].template step<NM>(s[qt], a.scale2, x[qt]);
+    for (int qt = 0; qt < QT; ++qt) softmax4<NM, 16>(sm[qt], scale[qt], s[qt], a.scale2, x[qt]);
     if constexpr (N == 1) {
       pv_tile<K, DP, KC, QT>(Vs, x, sm, g, p);
     } else {
@@ -1063,7 +1119,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 256 ? 1 : 2) void 
       const float l = ri[qt].valid ? lt : 0.f, inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
       for (int t = 0; t < DP / 16; ++t) store_row<T>(a, ri[qt], sm[qt].o[t], inv, 16 * t + 4 * g);
-      if (g == 0 && a.lse) a.lse[((int64_t)ri[qt].b * a.Hq + ri[qt].hq) * a.T + ri[qt].t] = l == 0.f ? -INFINITY : (sm[qt].m + __log2f(l)) * kLn2;
+      if (g == 0 && a.lse) a.lse[((int64_t)ri[qt].b * a.Hq + ri[qt].hq) * a.T + ri[qt].t] = lse4(a.scale2, sm[qt].m, l);
       continue;
     }
     if (g == 0) a.stat[slot + i] = float2{sm[qt].m, lt};
@@ -1146,7 +1202,7 @@ template <typename T, int TEAM, int CW> __global__ __launch_bounds__(256) void c
     return;
   }
   store_row<T>(a, ri, acc, l == 0.f ? 0.f : 1.f / l, col);
-  if (col == 0 && a.lse) a.lse[((int64_t)b * a.Hq + ri.hq) * a.T + ri.t] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
+  if (col == 0 && a.lse) a.lse[((int64_t)b * a.Hq + ri.hq) * a.T + ri.t] = lse4(a.scale2, m, l);
 }
 
 // ---- host ---------------------------------------------------------------------
