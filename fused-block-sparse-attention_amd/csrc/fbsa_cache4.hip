@@ -367,17 +367,22 @@ template <bool FIT, int LEAST> __device__ __forceinline__ bool share4(const Cach
 
 // ---- softmax -----------------------------------------------------------------
 // SoftmaxState's step for scores of any size. The largest of a row is a rounded product
-// with the scale, and the product within an fma is not: from 2^27 on the two are 8 and
-// more apart, which is more than exponentials in fp16 have room for, and from 2^31 on more
-// than 32-bit ones do (all of a row were 0 or infinite). There neighbouring scores are 8
-// apart or more, too, and no softmax tells what their sums' roundings hide; so such a row's
-// scale is the next power of two, whose products are exact: its largest is the reference.
-constexpr float kFar4 = 0x1p27f;
+// with the scale, and the product within an fma is not: from 2^28 on the two are up to 16
+// apart, which is more than exponentials in fp16 have room for, and from 2^31 on more than
+// 32-bit ones do (all of a row were 0 or infinite). There neighbouring scores are 16 apart
+// or more, too, so all the weight is the largest's; such a row's scale is the next power
+// of two, whose products are exact: its largest is the reference.
+constexpr float kFar4 = 0x1p28f;
 __device__ __forceinline__ float far_scale(float scale2) { return __uint_as_float((__float_as_uint(scale2) + 0x7fffffu) & 0xff800000u); }
 // ROWS < 16: a row's scores are in lane columns ROWS apart too, and share its reference.
-// scale: the row's, scale2 at first
-template <int NM, int ROWS, int DP> __device__ __forceinline__ void softmax4(SoftmaxState<DP> &sm, float &scale, const f32x4 (&s)[NM], float scale2, float (&x)[NM][4]) {
-  constexpr float TAU = SoftmaxState<DP>::TAU;
+// scale: the row's, scale2 at first. UP: the reference is 2^UP below the largest, for
+// exponentials that fp16 is to hold: at UP = 7 a probability loses bits from 2^-21 on and
+// is 0 from 2^-32 on (2^-14 and 2^-25 at 0, which many small ones beside a large one came
+// to). They reach 2^14, and with the products' roundings 2^15 (a rounding of 4 or 8 goes
+// with scores and references that are multiples of 8 or 16), below fp16's 2^16.
+template <int NM, int ROWS, int UP, int DP>
+__device__ __forceinline__ void softmax4(SoftmaxState<DP> &sm, float &scale, const f32x4 (&s)[NM], float scale2, float (&x)[NM][4]) {
+  constexpr float TAU = UP ? 14.f : SoftmaxState<DP>::TAU;
   float mx = -INFINITY;
 #pragma unroll
   for (int k = 0; k < NM; ++k) mx = fmaxf(mx, fmaxf(fmaxf(s[k][0], s[k][1]), fmaxf(s[k][2], s[k][3])));
@@ -388,7 +393,7 @@ template <int NM, int ROWS, int DP> __device__ __forceinline__ void softmax4(Sof
     for (int y = ROWS; y < 16; y <<= 1) mc = fmaxf(mc, shfl_xor_f(mc, y));
     if (mc * scale - sm.m > TAU) {
       scale = fabsf(mc * scale2) >= kFar4 ? far_scale(scale2) : scale2;
-      mc *= scale;
+      mc = mc * scale - (float)UP;
       const float alpha = __builtin_amdgcn_exp2f(sm.m - mc);
       sm.l *= alpha;
 #pragma unroll
@@ -723,7 +728,7 @@ __global__ __launch_bounds__(64 * W, part4_waves(sizeof(T) == 4, DP, SUB, QT)) v
     }
     float x[QT][NM][4];
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt) softmax4<NM, ROWS>(sm[qt], scale[qt], s[qt], a.scale2, x[qt]);
+    for (int qt = 0; qt < QT; ++qt) softmax4<NM, ROWS, 0>(sm[qt], scale[qt], s[qt], a.scale2, x[qt]);
 
     if (more) wait_vmcnt<C::CPR + NG>();
     else wait_vmcnt<0>();
@@ -948,7 +953,7 @@ template <typename T, int DP, int NW, int QT>
 __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 256 ? 1 : 2) void cache4_tile_kernel(Cache4Args c4) {
   using C = Tile4<T, DP, NW>;
   using K = typename C::K;
-  constexpr int KC = C::KC, NM = KC / 16, N = Pieces<T>::Q;
+  constexpr int KC = C::KC, NM = KC / 16, N = Pieces<T>::Q, UP = __is_same(T, f16) ? 7 : 0;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   const CacheArgs &a = c4.a;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, p = lane & 15;
@@ -1101,7 +1106,7 @@ __global__ __launch_bounds__(NW * 64, sizeof(T) == 4 && DP == 256 ? 1 : 2) void 
     }
     float x[QT][NM][4];
 #pragma unroll
-    for (int qt = 0; qt < QT; ++qt) softmax4<NM, 16>(sm[qt], scale[qt], s[qt], a.scale2, x[qt]);
+    for (int qt = 0; qt < QT; ++qt) softmax4<NM, 16, UP>(sm[qt], scale[qt], s[qt], a.scale2, x[qt]);
     if constexpr (N == 1) {
       pv_tile<K, DP, KC, QT>(Vs, x, sm, g, p);
     } else {

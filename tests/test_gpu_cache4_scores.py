@@ -1,11 +1,11 @@
-"""Attention over a cache in 4 bits where scores are infinite or very large: every path, against the formula."""
+"""Attention over a cache in 4 bits where scores are infinite, very large or far apart: every path, against the formula."""
 import math
 
 import pytest
 import torch
 
 import _cache4ref as ref
-from fbsa_amd import cache4
+from fbsa_amd import cache, cache4
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -60,6 +60,36 @@ def _uniform(dt, S, D, keys, values):
         c = torch.tensor([code[abs(y)] + 8 * (y < 0) for y in x], dtype=torch.uint8, device=DEV)
         return (c * 17).view(1, 1, S, 1).expand(1, 1, S, D // 2).contiguous()
     return codes(keys), codes(values), torch.ones(1, 1, S, 2, -(-D // 64), dtype=ref.step_type(dt), device=DEV)
+
+
+@pytest.mark.parametrize("D,T,H", [(64, 300, 256), (128, 300, 256), (256, 130, 256), (256, 60, 512)])
+@pytest.mark.parametrize("first", [True, False])
+def test_many_small_probabilities_in_fp16(D, T, H, first):
+    """131072 keys 2^-25.3 below one that holds nearly all of a query's weight, in one share:
+    their 0.3% arrives (P in fp16 with 7 of its binades below: 0.3% of the row sum and
+    none of the result without them). With scale 1 / D and keys of 0 and 1 a query of
+    17.53125 has that score. Each p is off by h = 2^-11 of itself or, below 2^-14, by half
+    an fp16 step 2^-24 over 2^7, the row sum being at least 1: 2^-32. So o is off by h for P,
+    h for its storage, and 2^-32 sum |v|. Sums: a lane's row sum takes a step a chunk of 64
+    keys, an element of O two, each off by up to 2^-24 of what is there (the largest key's
+    weight, 1, and less than 2^-6 more), and the small terms being equal the roundings can go one way:
+    S / 64 2^-24 of the row sum, twice that of o; 2^-20 for the exponentials of either."""
+    S, h, a = 131072 + T, 2.0 ** -11, 17.53125
+    top = 0 if first else S - T - 1
+    keys, values = [0.0] * S, [6.0] * S
+    keys[top], values[top] = 1.0, 1.0
+    held = [x.expand(1, H, *x.shape[2:]) for x in _uniform(torch.float16, S, D, keys, values)]
+    q = torch.full((1, H, T, D), a, dtype=torch.float16, device=DEV)
+    o, lse = cache4.cache_attention(q, *held, scale=1.0 / D, need_lse=True)
+    assert next(reversed(cache._plans.values())).nbytes == 256   # one share a tile
+    seen = torch.arange(S - T + 1, S + 1, dtype=torch.float64).view(1, 1, T, 1)
+    w = (seen - 1) * math.exp(-a)
+    want = (1 + 6 * w) / (1 + w)
+    err = (o.cpu().double() - want).abs()
+    steps = (S / 64 + 1) * 2.0 ** -24
+    assert (err <= (2 * h + 3 * steps + 2.0 ** -19) * want + 2.0 ** -32 * 6 * seen).all(), f"{float(err.max()):.2e}"
+    # (the numbers near 17.5 are 2^-19 apart)
+    assert (lse.cpu().double() - (a + w.log1p()).squeeze(-1)).abs().max() <= steps + 2.0 ** -20 + 2.0 ** -19
 
 
 @pytest.mark.parametrize("dt", list(DT))
