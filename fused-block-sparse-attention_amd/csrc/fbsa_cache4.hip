@@ -1381,8 +1381,9 @@ static int check_rows4(const char *fn, const fbsa_rows4_desc *d) {
   for (int x = 0; x < 3; ++x)
     if (d->sk[x] < 0 || d->sv[x] < 0 || d->sk[x] * es % 16 || d->sv[x] * es % 16)
       return fail(FBSA_EINVAL, "%s: strides of the rows must be non-negative multiples of 16 bytes", fn);
-  // (a launch has fewer than 2^32 threads along an axis: at least 8 rows to 256 here)
-  if (d->B * d->H * d->T > 0x3ff0000LL) return fail(FBSA_EUNSUPPORTED, "%s: grid too large", fn);
+  // (a launch has fewer than 2^32 threads along an axis, the first of which holds T alone, at
+  // least 8 rows to 256; a call's rows in all stay below what one axis takes of them)
+  if (d->B * d->H * d->T > 0x7ff0000LL) return fail(FBSA_EUNSUPPORTED, "%s: grid too large", fn);
   return FBSA_OK;
 }
 

@@ -433,7 +433,8 @@ int fbsa_cache_evict(const fbsa_evict_desc *d, const void *k, const void *v, con
  * code x / step rounded to the nearest, ties to the even code, 6 at most. Every
  * value is then a bf16 number (F16: an fp16 number). A (sequence, head)'s row with a
  * NaN or an infinity among its key or value elements has NaN for all of its steps.
- * lens, start, first and count as above. No counterpart in the reference. */
+ * lens, start, first and count as above. A call takes up to 65535 (sequence, KV head)
+ * pairs; an append or read up to 134152192 rows (B H T). No counterpart in the reference. */
 typedef struct fbsa_rows4_desc {
   int32_t dtype, flags;                     /* flags: 0 */
   int64_t B, H, T, S, D;
