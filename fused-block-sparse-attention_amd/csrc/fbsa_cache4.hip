@@ -314,7 +314,9 @@ __device__ __forceinline__ int chunks4(const CacheArgs &a, int u) {
 // FIT: pieces of LEAST chunks or more, in `want` of them, which run at a time. Where there
 // are more tiles than half of that, what is a quarter longer than a place's share of the
 // chunks is cut, the others stay whole (16 sequences, 512 tokens, 8 heads over 1, d 128: one
-// of 30000 rows and 15 of 1000 211 us against 1205 uncut, all of 4000 210 against 184).
+// of 30000 rows and 15 of 1000 211 us against 1205 uncut, all of 4000 210 against 184). A
+// quarter is between the two: at none (1.0 for 0.8) those of 4000 take 244, lengths of 1000
+// to 30000 889 us in place of 937; at two thirds (0.6) 206 and 1063.
 // Otherwise each tile may round its own up.
 template <bool FIT, int LEAST> __device__ __forceinline__ bool share4(const Cache4Args &c4, int i, int lane, int &u, int &split, int &np, int &before) {
   const CacheArgs &a = c4.a;
@@ -530,8 +532,10 @@ template <typename T, int NG> struct Steps4 {
 // 2, d 256: 23 us, 3.4 TB/s, one wave's chain from load to product.
 // W > 1: a workgroup's waves share a sequence's chunks and join their parts in LDS, where
 // that spares short caches the second launch.
-// QT > 1: that many 16-row tiles, for which the codes are made numbers once; 16-bit P is
-// then rounded once (bf16), as in the kernel of many rows.
+// QT > 1: that many 16-row tiles, for which the codes are made numbers once; P times the
+// step is then rounded once in bf16, to half a step of what the result is rounded to (two
+// pieces: 16 sequences of 8192 to 16384 rows, 24 rows a head, d 128 34.7 us against 31.2, d
+// 64 25.0 against 23.5; one of 65536, d 128 37.0 against 32.9).
 // waves to a SIMD: one where 256 registers are too few
 constexpr int part4_waves(bool f32, int dp, int sub, int qt) {
   const int regs = qt * (dp / 4 + dp / 8 * sub * (f32 ? 3 : 1) + 32 / sub) + 64 + dp / 4;
@@ -881,9 +885,13 @@ __global__ __launch_bounds__(64 * W, part4_waves(sizeof(T) == 4, DP, SUB, QT)) v
 // Many rows: a workgroup per (tile of NW x 16 QT rows, share of the keys). Its threads
 // make 16-bit numbers of the codes, steps and all (exact), in LDS, and from there it is
 // the tile of a 16-bit cache. 2048 tokens over 16301 rows, 16 heads over 2, d 256: 541 us,
-// 0.98 PFLOP/s, matrix units 39% busy, LDS 49%, vector issue 51%, eight waves in step. 32-bit rows are three bf16 pieces of
-// queries and of probabilities: six products of the matrix units' fastest type cost less
-// than two of the slow 32-bit one.
+// 0.95 PFLOP/s, matrix units 39% busy, LDS 49%, vector issue 51%, eight waves in step. P is
+// rounded to the operand type once: a second piece is another product for each of the value
+// ones (that case 25% longer, 512 tokens of 2 sequences, d 128 18%, 48 rows a head, d 64
+// 5%), and one rounding of P and one of the result make 0.0023 of the result where the
+// second alone is 0.0017. 32-bit rows are three bf16 pieces of queries and of
+// probabilities: six products of the matrix units' fastest type cost less than two of the
+// slow 32-bit one.
 template <typename K, int DP, int QT, int NM, int N>
 __device__ __forceinline__ void qk_pieces(const char *tile, const RowFrag<K, DP> (&fr)[N * QT], f32x4 (&s)[QT][NM], int g, int p) {
   if constexpr (N == 1) {
@@ -1218,9 +1226,13 @@ struct Plan4 {
   bool joined;  // the waves of a workgroup share a sequence's chunks
   size_t used, part, total;
 };
-// (queries take D SUB / 2 registers, 32-bit ones three times as many; O D / 4 for each 16 rows)
+// (queries take D SUB / 8 registers, 32-bit ones three times as many; O D / 4 for each 16 rows)
 constexpr int most_sub4(bool f32, int64_t dp) { return f32 ? (dp <= 64 ? 4 : dp == 128 ? 2 : 1) : dp <= 128 ? 4 : 2; }
-constexpr int kJoined4 = 8;  // waves of a workgroup that joins its own parts
+// Waves of a workgroup that joins its own parts: with four, which take half as much LDS and
+// so many short sequences better, more calls are left to two launches (8 heads, d 128: 64
+// sequences of 2048 to 4096 rows 43.9 us against 55.8, of 256 to 512 14.1 against 10.0; fp32
+// d 64, 4 heads: 32 of 512 to 1024 9.2 and 9.3; over 100 shapes within 2% in the mean)
+constexpr int kJoined4 = 8;
 constexpr int most_tiles4(bool f32, int64_t dp) { return dp <= (f32 ? 64 : 128) ? 2 : 1; }
 static Plan4 plan4(const fbsa_attn4_desc *d) {
   Plan4 p;
@@ -1255,7 +1267,10 @@ static Plan4 plan4(const fbsa_attn4_desc *d) {
     // One launch against two, where the waves have few chunks each, or the card many
     // workgroups (8 heads, d 64, 1024 rows 6.8 us against 7.7, 4096 10.8 against 8.0; 32
     // sequences of those 15.5 against 18.5, of 8192 rows 24.1 against 25.9; 32 x 2 heads, d
-    // 256, 256 rows 9.9 against 12.6, 2048 22.3 against 19.3)
+    // 256, 256 rows 9.9 against 12.6, 2048 22.3 against 19.3). Twice the chunks for a lone
+    // sequence lose up to half (fp32, 4096 rows 9.2 against 14.1); 256 and more (sequence,
+    // head) pairs take four times as many (64 x 8 heads, d 64, 4096 rows 22.3 against 28.8 with
+    // as few; more than four times: 64 x 8 heads, d 128, 8192 rows 88 against 118, others alike)
     const int64_t chunks = std::max<int64_t>(1, 256 / p.DP) * std::min<int64_t>(4, std::max<int64_t>(1, seqs / 64));
     p.joined = TG <= 16 && part4_waves(f32, (int)p.DP, p.sub, 1) == 2 && nc > 1 && nc <= kJoined4 * chunks;
   } else {
@@ -1263,7 +1278,12 @@ static Plan4 plan4(const fbsa_attn4_desc *d) {
     // 41.0; d 64: 29.6 and 27.8), of 128 keys at least
     const int64_t room = kCUs * (p.DP <= 64 ? (f32 ? 3 : 4) : p.DP == 128 ? (f32 || p.tr > 64 ? 2 : 3) : f32 || p.tr > 64 ? 1 : 2);
     // One share a tile where the card goes through them several times (see above), and for
-    // one sequence's tiles, which see about the same, as soon as they are half of that.
+    // one sequence's tiles as soon as they are half of what runs at a time: those that see the
+    // most start first, and shares join through memory (16 heads over 2, d 256: 1040 tokens
+    // over 16301 rows 499 us against 530 cut as share4 does, 2048 571 against 581; 2048 tokens
+    // that see themselves alone, tiles of few keys to all, 75 against 89, 32 heads over 8, d
+    // 128 58 against 89). The last round of workgroups may be all but empty: 1040 tokens over
+    // 16301 rows take nearly as long as 2048, 2064 926 us.
     const int64_t each = std::max<int64_t>(1, room / d->Hkv), units = d->B * p.rt, nc = cdiv(d->S, 128);
     p.want = each;
     p.np = units >= std::max(4 * each, 16 * nc) || (d->B == 1 && p.rt > 1 && 2 * units > each) ? units : std::min(2 * units <= each || units == 1 ? each : each + units, nc * units);
@@ -1295,7 +1315,10 @@ template <typename T, int DP, int SUB> static int launch_few4(const Cache4Args &
 template <typename T> static int launch_join4(const Cache4Args &c, const Plan4 &pl, hipStream_t s) {
   const int64_t rows = (int64_t)c.a.B * c.a.Hkv * c.a.TG;
   const int pitch = (int)pl.pitch;
-  // many rows: a wave each (of up to 128 columns); few: a workgroup for 128 or 32 columns
+  // many rows: a wave each (of up to 128 columns); few: a workgroup for 128 or 32 columns, as
+  // many workgroups as there are CUs or more. (By waves and workgroups, a call: 4 sequences of
+  // 32 heads, d 128, 32768 rows 33.2 us and 27.5; 64 of 5 x 16, d 256 91 and 100. By 128 columns
+  // and 32: one of 16 heads, d 128, 131072 rows 42.1 and 22.1; 32 of 16, d 256 36.7 and 46.2.)
   if (rows >= 2048) {
     const unsigned wgs = (unsigned)cdiv(rows, 4);
     if (pitch == 32) hipLaunchKernelGGL((cache4_join_kernel<T, 64, 32>), dim3(wgs), dim3(256), 0, s, c, pitch);

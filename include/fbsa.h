@@ -454,9 +454,11 @@ int fbsa_cache4_read(const fbsa_rows4_desc *d, const void *k4, const void *v4, c
                      const int32_t *count, void *k, void *v, void *stream);
 
 /* fbsa_cache_attn over a cache in 4 bits (no prefix, no weights): the softmax and
- * products of the values above, in 32 bits; with more than 16 rows (tokens x heads of a
- * group) 16-bit types round each probability once. A row held as NaN makes the queries
- * that see it NaN, no others. 256 bytes of workspace say that the call touches none. */
+ * products of the values above, in 32 bits. With more than 16 rows (tokens x heads of a
+ * group) bf16 rounds each probability once, with its value's step or without; fp16 with more
+ * than 32, or more than 16 where D > 128 (below 2^-21 of a query's largest to a multiple of
+ * 2^-31). A row held as NaN makes the queries that see it NaN, no others. 256 bytes of
+ * workspace say that the call touches none. */
 typedef struct fbsa_attn4_desc {
   int32_t dtype, flags;                     /* flags: 0 */
   int64_t B, Hq, Hkv, T, S, D;
