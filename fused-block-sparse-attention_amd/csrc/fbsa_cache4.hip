@@ -1419,7 +1419,8 @@ static int check_attn4(const fbsa_attn4_desc *d) {
     return fail(FBSA_EINVAL, "%s: sizes must be positive (B=%lld Hq=%lld Hkv=%lld T=%lld S=%lld)", fn, (long long)d->B, (long long)d->Hq,
                 (long long)d->Hkv, (long long)d->T, (long long)d->S);
   if (d->Hq % d->Hkv) return fail(FBSA_EINVAL, "%s: Hq=%lld not a multiple of Hkv=%lld", fn, (long long)d->Hq, (long long)d->Hkv);
-  if (!isfinite(d->scale * kLog2e)) return fail(FBSA_EINVAL, "%s: scale times log2(e) is not finite", fn);
+  // (up to 2^127: the power of two above it is a number, far_scale)
+  if (!(fabsf(d->scale * kLog2e) <= 0x1p127f)) return fail(FBSA_EINVAL, "%s: scale times log2(e) is beyond 2^127", fn);
   const int64_t lim = 0x7fff0000LL;
   if (d->S > lim || d->B > lim || d->Hq > 65535 || d->T > lim || d->T * (d->Hq / d->Hkv) > lim || d->B > lim / d->Hq ||
       d->B * d->Hq > lim / d->T || d->B * d->Hkv > 65535)
