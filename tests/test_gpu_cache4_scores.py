@@ -117,3 +117,39 @@ def test_scores_of_any_size(dt, D, Hq, T, S):
         assert off.max() <= (2.0 ** -20 if dt == torch.float32 else 0.0), f"scale {scale}"
         score = D * scale * torch.where(sign > 0, 6.0, -0.5).double()
         assert ((lse.cpu().double() - score.view(1, Hq, 1)) / score.view(1, Hq, 1)).abs().max() <= 2.0 ** -21, f"scale {scale}"
+
+
+@pytest.mark.parametrize("dt", list(DT))
+@pytest.mark.parametrize("D", [64, 256])
+@pytest.mark.parametrize("Hq,T", ROWS)
+@pytest.mark.parametrize("S", [200, 3000])
+def test_very_large_scores_beside_small_ones(dt, D, Hq, T, S):
+    """Scores of 0 and, in some rows, 2^20 to 2^110: where those are positive (even heads) the
+    one of them at the end of what all queries see has all the weight, where negative the zeros share it
+    and nothing else adds. Their mean: sums of values that are multiples of 0.5, exact in 32 bits but for the
+    probabilities' 2^-20 (16-bit ones exact: they are 1), the division and the storage."""
+    g = torch.Generator().manual_seed(S + T)
+    values = [(-6.0, -3.0, 1.5, 4.0)[i] for i in torch.randint(0, 4, (S,), generator=g)]
+    keys = [0.0] * S
+    for s in (*range(3, S - T, 71), S - T - 1):
+        keys[s] = 4.0
+    keys[S - T - 1] = 6.0
+    dt = DT[dt]
+    held = _uniform(dt, S, D, keys, values)
+    sign = torch.ones(Hq)
+    sign[1::2] = -1
+    q = sign.view(1, Hq, 1, 1).expand(1, Hq, T, D).to(DEV, dt).contiguous()
+    zero, v = torch.tensor(keys) == 0, torch.tensor(values, dtype=torch.float64)
+    seen = torch.arange(S).view(1, S) <= torch.arange(S - T, S).view(T, 1)
+    n = (seen & zero).sum(1)
+    mean = ((seen & zero).double() @ v) / n
+    h = 0.0 if dt == torch.float32 else torch.finfo(dt).eps / 2
+    for scale in (12345.6789, 3.1e5, 3.3e7, 5.4321e20, 9.87e30):
+        o, lse = (x.cpu().double() for x in cache4.cache_attention(q, *held, scale=scale, need_lse=True))
+        for head in range(Hq):
+            if head % 2:
+                assert ((o[0, head] - mean.view(T, 1)).abs() <= (h + 2.0 ** -18) * mean.abs().view(T, 1) + 2.0 ** -18).all(), f"scale {scale}"
+                assert (lse[0, head] - n.double().log()).abs().max() <= 2.0 ** -18, f"scale {scale}"
+            else:
+                assert (o[0, head] - values[S - T - 1]).abs().max() <= 2.0 ** -18, f"scale {scale}"
+                assert (lse[0, head] / (6.0 * D * scale) - 1).abs().max() <= 2.0 ** -21, f"scale {scale}"
